@@ -485,6 +485,68 @@ int mxq_w4a8_quantize_weight(const void* w, int w_dtype, int64_t N, int64_t K, i
                              void* stream);
 
 /*
+ * ---- 8-bit floating point in blocks of 128 ----
+ * e4m3 codes with one E8M0 byte b per block: the values are code * 2^(b - 127). A block is 1 x 128 of an activation
+ * or a gradient, 128 x 128 of a weight. The quantizers take the smallest exponent e = b - 127 >= -117 with
+ * absmax <= 448 * 2^e (a block of zeros: b = 127) and round x / 2^e once, to nearest even; NaN and infinities become
+ * the NaN code in their own place, absmax being that of the finite elements. Rows of codes are zero-padded to whole
+ * blocks: row strides (in elements) are multiples of 16 and at least ceil(K / 128) * 128. Rows of scale bytes hold
+ * ceil(K / 128) of them; the matrix products read them four at a time (row strides multiples of 4, 4-byte aligned).
+ * No counterpart in the reference.
+ */
+
+/* Codes [M, ldq] and scales [M, lds] of x [M, K] (bf16, fp16 or fp32; row stride ldx). */
+int mxq_fp8_quantize_rows(const void* x, int x_dtype, int64_t ldx, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds,
+                          int64_t M, int64_t K, void* stream);
+
+/* The way back: out [M, K] contiguous of out_dtype. Any strides ldq >= K and lds >= ceil(K / 128). */
+int mxq_fp8_dequantize_rows(const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds, void* out, int out_dtype,
+                            int64_t M, int64_t K, void* stream);
+
+/*
+ * A weight [N, K] by 128 x 128 tiles: codes q [N, ldq], scale [ceil(N / 128), lds]; with qt not NULL also the
+ * transposed codes qt [K, ldqt] and scale_t [ceil(K / 128), ldst], which the input's gradient multiplies by.
+ */
+int mxq_fp8_quantize_tiles(const void* w, int w_dtype, int64_t ldw, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds,
+                           uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst, int64_t N, int64_t K, void* stream);
+
+/* Bytes of workspace mxq_fp8_gemm needs at this size on the current device (0: none). */
+int mxq_fp8_gemm_workspace(int64_t M, int64_t N, int64_t K, int64_t* bytes);
+
+/*
+ * d [M, N] = out(a b^T + bias): a codes [M, lda] with scales [M, ldsa] (1 x 128), b codes [N, ldb] with scales
+ * [ceil(N / 128), ldsb] (128 x 128), both zero behind column K; bias [N] of out_dtype or NULL. Sums are float32.
+ * bf16 and fp16 outputs use the e4m3 matrix instructions, which cut addends below 2^-13 of the largest of 64;
+ * fp32 outputs keep every addend.
+ */
+int mxq_fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa, const uint8_t* b, int64_t ldb,
+                 const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd, int out_dtype, int64_t M,
+                 int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The same for few rows. x_dtype MXQ_DTYPE_E4M3: x holds codes, sx their scales, M <= 64. Otherwise x [M, ldx] is
+ * quantized on the way, with the codes mxq_fp8_quantize_rows gives: M <= 16, K % 8 == 0, rows 16-byte aligned.
+ */
+int mxq_fp8_linear_rows(const void* x, int x_dtype, int64_t ldx, const uint8_t* sx, int64_t ldsx, const uint8_t* b,
+                        int64_t ldb, const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd, int out_dtype,
+                        int64_t M, int64_t N, int64_t K, void* stream);
+
+/* Row strips of mxq_fp8_grad_pass at this size on the current device. */
+int mxq_fp8_grad_strips(int64_t M, int64_t N, int64_t* strips);
+
+/*
+ * One pass over an output's gradient dy [M, N] (row stride ldy) for what the layer's gradients need of it, each part
+ * optional: its codes q and scales (q NULL: none), n_parts bfloat16 parts [n_parts, M, ldp] whose sum is dy (0, or
+ * 1 for bf16, 2 for fp16, 3 for fp32), and the column sums of each strip of rows, sums fp32 [strips, N] (NULL: none).
+ */
+int mxq_fp8_grad_pass(const void* dy, int dy_dtype, int64_t ldy, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds,
+                      void* parts, int n_parts, int64_t ldp, float* sums, int64_t strips, int64_t M, int64_t N,
+                      void* stream);
+
+/* out [n] = column sums of in [parts, n] (fp32), in a fixed order. */
+int mxq_column_join(const float* in, int64_t parts, int64_t n, void* out, int out_dtype, void* stream);
+
+/*
  * Measurement helper (no counterpart in the reference; it calibrates the roofline): runs
  * `workgroups` x 256 threads, each lane cycling eight v_mfma_i32_32x32x32_i8 accumulators over
  * four A and two B 16-byte fragments read from a / b (wrapping within a_bytes / b_bytes), for

@@ -1,0 +1,119 @@
+"""8-bit floating point layer without a GPU: the oracle's closed forms and the refusals, on the host before any launch."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from oracle import fp8_block as ob
+
+
+def _mx():
+    import mx_qlinear
+
+    return mx_qlinear
+
+
+def test_oracle_rounding_is_torchs():
+    v = torch.cat([torch.linspace(-448, 448, 20001, dtype=torch.float64), torch.linspace(-0.1, 0.1, 20001, dtype=torch.float64)])
+    v = v.float().double()
+    assert torch.equal(ob.round_e4m3(v), v.float().to(torch.float8_e4m3fn).double())
+    t = ob.e4m3_table()
+    codes = torch.arange(256).to(torch.uint8).view(torch.float8_e4m3fn).double()
+    assert torch.equal(t.nan_to_num(1e9), codes.nan_to_num(1e9))
+
+
+def test_oracle_exponents():
+    a = torch.tensor([0.0, 448.0, 448.0000001, 224.0, 2.0**-108, 448 * 2.0**-117, 2.0**-149, 3.4e38], dtype=torch.float64)
+    e = ob.exponent(a)
+    assert e.tolist() == [0, 0, 1, -1, -116, -117, -117, 120]
+    s = torch.ldexp(torch.ones((), dtype=torch.float64), e)
+    assert bool((a <= 448 * s).all())
+
+
+def test_cpu_tensors_are_refused():
+    mx = _mx()
+    x = torch.zeros(4, 256)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        mx.quantize_fp8_block128(x)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        mx.prepare_fp8_weight(x)
+    q, s = x.to(torch.float8_e4m3fn), torch.ones(4, 2).to(torch.float8_e8m0fnu)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        mx.dequantize_fp8_block128(q, s)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        mx.prepare_fp8_weight(torch.zeros(128, 256).to(torch.float8_e4m3fn), torch.ones(1, 2).to(torch.float8_e8m0fnu))
+
+
+def test_arguments_are_checked():
+    mx = _mx()
+    q, s = torch.zeros(4, 256).to(torch.float8_e4m3fn), torch.ones(4, 2).to(torch.float8_e8m0fnu)
+    p = mx.PreparedFp8Weight(q, s, None, None, 4, 256)
+    with pytest.raises(ValueError, match="unsupported input dtype"):
+        mx.quantize_fp8_block128(torch.zeros(4, 256, dtype=torch.int8, device="meta"))
+    with pytest.raises(ValueError, match="2D"):
+        mx.prepare_fp8_weight(torch.zeros(4))
+    with pytest.raises(ValueError, match="2D"):
+        mx.prepare_fp8_weight(torch.zeros(0, 4))
+    with pytest.raises(ValueError, match="scale of shape"):
+        mx.prepare_fp8_weight(torch.zeros(300, 256).to(torch.float8_e4m3fn), s)
+    with pytest.raises(ValueError, match="float8_e4m3fn"):
+        mx.prepare_fp8_weight(torch.zeros(4, 256), s)
+    with pytest.raises(TypeError, match="prepare_fp8_weight"):
+        mx.fp8_linear(torch.zeros(4, 256), torch.zeros(4, 256))
+    with pytest.raises(ValueError, match="K mismatch"):
+        mx.fp8_linear(torch.zeros(4, 128), p)
+    with pytest.raises(ValueError, match="non-empty"):
+        mx.fp8_linear(torch.zeros(4, 0), p)
+    with pytest.raises(ValueError, match="scale of shape"):
+        mx.fp8_linear_prequantized(q, torch.ones(4, 3).to(torch.float8_e8m0fnu), p)
+    with pytest.raises(ValueError, match="float8_e4m3fn"):
+        mx.fp8_linear_prequantized(q, torch.ones(4, 2), p)
+
+
+def _call(name, *args):
+    from mx_qlinear import _lib
+
+    return _lib.call(name, *args, None)
+
+
+def test_c_entries_refuse_before_any_launch():
+    """Sizes, strides, dtypes, pointers and workspaces (16 stands for an aligned pointer that is never read)."""
+    ok = 1 << 20
+    with pytest.raises(ValueError, match="dtype"):
+        _call("mxq_fp8_quantize_rows", ok, 3, 256, ok, 256, ok, 4, 8, 256)
+    for ldx, ldq, lds, k in ((255, 256, 4, 256), (256, 128, 4, 256), (256, 264, 4, 256), (256, 256, 1, 256), (256, 256, 4, 0)):
+        with pytest.raises(ValueError):
+            _call("mxq_fp8_quantize_rows", ok, 0, ldx, ok, ldq, ok, lds, 8, k)
+    with pytest.raises(ValueError, match="misaligned"):
+        _call("mxq_fp8_quantize_rows", ok, 0, 256, ok + 8, 256, ok, 4, 8, 256)
+    with pytest.raises(ValueError, match="null"):
+        _call("mxq_fp8_dequantize_rows", None, 256, ok, 2, ok, 0, 8, 256)
+    with pytest.raises(ValueError):
+        _call("mxq_fp8_quantize_tiles", ok, 0, 256, ok, 256, ok, 4, ok, 128, ok, 0, 8, 256)
+    with pytest.raises(ValueError, match="activations"):
+        _call("mxq_fp8_gemm", ok, 200, ok, 4, ok, 256, ok, 4, None, ok, 128, 2, 100, 128, 256, None, 0)
+    with pytest.raises(ValueError, match="weight"):
+        _call("mxq_fp8_gemm", ok, 256, ok, 4, ok, 256, ok, 2, None, ok, 128, 2, 100, 128, 256, None, 0)
+    with pytest.raises(ValueError, match="weight"):
+        _call("mxq_fp8_gemm", ok, 256, ok, 4, ok, 256, ok, 4, None, ok, 127, 2, 100, 128, 256, None, 0)
+    with pytest.raises(ValueError, match="misaligned"):
+        _call("mxq_fp8_gemm", ok + 1, 256, ok, 4, ok, 256, ok, 4, None, ok, 128, 2, 100, 128, 256, None, 0)
+    need = ctypes.c_int64()
+    from mx_qlinear import _lib
+
+    _lib.call("mxq_fp8_gemm_workspace", 128, 256, 16384, ctypes.byref(need))
+    assert need.value > 0  # two tiles: K is split
+    with pytest.raises(ValueError, match="workspace"):
+        _call("mxq_fp8_gemm", ok, 16384, ok, 128, ok, 16384, ok, 128, None, ok, 256, 2, 128, 256, 16384, ok, need.value - 16)
+    with pytest.raises(_lib.MxqError, match="rows"):
+        _call("mxq_fp8_linear_rows", ok, 2, 256, None, 0, ok, 256, ok, 4, None, ok, 128, 2, 17, 128, 256)
+    with pytest.raises(ValueError, match="activations"):
+        _call("mxq_fp8_linear_rows", ok, 2, 260, None, 0, ok, 256, ok, 4, None, ok, 128, 2, 4, 128, 250)
+    with pytest.raises(ValueError):
+        _call("mxq_fp8_grad_pass", ok, 2, 256, ok, 256, ok, 4, ok, 2, 256, None, 0, 8, 256)
+    # no rows: nothing to do, no pointer needed
+    _call("mxq_fp8_quantize_rows", None, 0, 256, None, 256, None, 4, 0, 256)
+    _call("mxq_fp8_gemm", None, 256, None, 4, None, 256, None, 4, None, None, 128, 2, 0, 128, 256, None, 0)

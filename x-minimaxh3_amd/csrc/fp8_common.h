@@ -1,0 +1,207 @@
+// 8-bit floating point in blocks of 128: the number format that the fp8 kernels share.
+//
+// A block (1 x 128 of an activation or a gradient, 128 x 128 of a weight) holds e4m3 codes q and one E8M0 byte b:
+// the values are q * 2^(b - 127). The exponent e = b - 127 is the smallest one with absmax <= 448 * 2^e (448 is
+// e4m3's largest value), so x / 2^e is exact in float32 and the only rounding of the quantizer is the one to e4m3
+// (to nearest, ties to even). A power of two is what the matrix instructions of gfx950 apply by themselves, and a
+// value q * 2^e is exact in bfloat16 and float32: e is at least -117, so that the smallest one, 2^-9 * 2^e, is not
+// subnormal there. A block of zeros has b = 127. NaN and infinities become e4m3's NaN code in their own place, and
+// absmax is that of the finite elements.
+#pragma once
+
+#include "mxq_common.h"
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v2s __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+
+namespace mxq {
+
+constexpr int kFp8Block = 128;
+constexpr int kFp8MinByte = 10;  // 2^-117
+
+// The scale byte of a block from the bits of its (finite) absmax: 448 = 1.75 * 2^8, so a significand above 1.75
+// takes the next exponent.
+MXQ_DEVICE uint32_t fp8_scale_byte(uint32_t amax_bits) {
+  const int b = (int)((amax_bits + 0x1FFFFFu) >> 23) - 8;
+  return amax_bits == 0 ? 127u : (uint32_t)max(b, kFp8MinByte);
+}
+
+MXQ_DEVICE float fp8_scale_f32(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// ---- 16 consecutive elements of one row, as loaded: 8 words of 16-bit types, 16 of float32 ----
+template <int kCode> struct Piece {
+  static constexpr int kWords = kCode == MXQ_DTYPE_F32 ? 16 : 8;
+  static constexpr int kBytes = kWords * 4;
+  uint32_t w[kWords];
+};
+
+template <int kCode>
+MXQ_DEVICE Piece<kCode> piece_load_vec(const void* p) {
+  Piece<kCode> r;
+#pragma unroll
+  for (int i = 0; i < Piece<kCode>::kWords / 4; ++i) {
+    const v4u v = reinterpret_cast<const v4u*>(p)[i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.w[4 * i + j] = v[j];
+  }
+  return r;
+}
+
+// The first `n` elements one by one, zeros behind them.
+template <int kCode>
+MXQ_DEVICE Piece<kCode> piece_load_some(const void* p, int n) {
+  Piece<kCode> r;
+  if constexpr (kCode == MXQ_DTYPE_F32) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r.w[i] = i < n ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
+  } else {
+    const uint16_t* s = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      r.w[i] = (2 * i < n ? (uint32_t)s[2 * i] : 0u) | ((2 * i + 1 < n ? (uint32_t)s[2 * i + 1] : 0u) << 16);
+  }
+  return r;
+}
+
+// `n` of 16 elements (n <= 0: none) from p; `vec`: p is 16-byte aligned.
+template <int kCode>
+MXQ_DEVICE Piece<kCode> piece_load(const void* p, int n, bool vec) {
+  if (vec && n >= 16) return piece_load_vec<kCode>(p);
+  return piece_load_some<kCode>(p, n);
+}
+
+template <int kCode>
+MXQ_DEVICE float piece_at(const Piece<kCode>& r, int i) {  // i is a constant once unrolled
+  if constexpr (kCode == MXQ_DTYPE_F32) return __uint_as_float(r.w[i]);
+  const uint32_t h = (i & 1) ? r.w[i >> 1] >> 16 : r.w[i >> 1] & 0xFFFFu;
+  return kCode == MXQ_DTYPE_F16 ? f16_to_f32(h) : bf16_to_f32(h);
+}
+
+// Bits of the float32 absmax of 16 elements, NaN and infinities above every finite value.
+template <int kCode>
+MXQ_DEVICE uint32_t piece_absmax(const Piece<kCode>& r) {
+  if constexpr (kCode == MXQ_DTYPE_F32) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, r.w[i] & 0x7FFFFFFFu);
+    return m;
+  } else {
+    uint32_t a = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = absmax_acc_bf16x2(a, r.w[i]);  // (16-bit magnitudes order as integers in both types)
+    const uint32_t h = max(a & 0xFFFFu, a >> 16);
+    return kCode == MXQ_DTYPE_F16 ? __float_as_uint(f16_to_f32(h)) & 0x7FFFFFFFu : h << 16;
+  }
+}
+
+// The same over the finite elements only.
+template <int kCode>
+MXQ_DEVICE uint32_t piece_absmax_finite(const Piece<kCode>& r) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t b = abs_bits(piece_at(r, i));
+    m = max(m, b < 0x7F800000u ? b : 0u);
+  }
+  return m;
+}
+
+// 16 elements divided by `scale` (a power of two) and rounded once to e4m3: v_cvt_scalef32_pk_fp8_* divides by the
+// scale's power of two, rounds to nearest even and gives the NaN code beyond 448, which only NaN and infinities are.
+template <int kCode>
+MXQ_DEVICE v4u piece_encode(const Piece<kCode>& r, float scale) {
+  v4u o;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v2s h = {0, 0};
+    if constexpr (kCode == MXQ_DTYPE_F32) {
+      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, __uint_as_float(r.w[4 * j]), __uint_as_float(r.w[4 * j + 1]), scale,
+                                                   false);
+      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, __uint_as_float(r.w[4 * j + 2]), __uint_as_float(r.w[4 * j + 3]),
+                                                   scale, true);
+    } else if constexpr (kCode == MXQ_DTYPE_F16) {
+      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(h, __builtin_bit_cast(v2h, r.w[2 * j]), scale, false);
+      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(h, __builtin_bit_cast(v2h, r.w[2 * j + 1]), scale, true);
+    } else {
+      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(v2bf, r.w[2 * j]), scale, false);
+      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(v2bf, r.w[2 * j + 1]), scale, true);
+    }
+    o[j] = __builtin_bit_cast(uint32_t, h);
+  }
+  return o;
+}
+
+// Four codes times a power of two as two bfloat16 pairs (exact).
+MXQ_DEVICE v2u fp8x4_to_bf16(uint32_t q, float scale) {
+  v2u o;
+  o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q, scale, false));
+  o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q, scale, true));
+  return o;
+}
+MXQ_DEVICE v8bf fp8x8_to_bf16(uint32_t q0, uint32_t q1, float scale) {
+  const v2u a = fp8x4_to_bf16(q0, scale), b = fp8x4_to_bf16(q1, scale);
+  return __builtin_bit_cast(v8bf, v4u{a[0], a[1], b[0], b[1]});
+}
+// ... and as four float32 (exact).
+MXQ_DEVICE v4f fp8x4_to_f32(uint32_t q, float scale) {
+  const v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q, scale, false);
+  const v2f b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q, scale, true);
+  return v4f{a[0], a[1], b[0], b[1]};
+}
+
+// max over lanes i, i ^ 1, 2, 4 (eight lanes hold a row's block, 16 elements each)
+MXQ_DEVICE uint32_t max8(uint32_t v) {
+  v = max(v, dpp_lane<kDppQuadXor1>(v));
+  v = max(v, dpp_lane<kDppQuadXor2>(v));
+  return max(v, lane_xor4(v));
+}
+
+// Stores 4 float values from column `col` on, as kCode; `n` of them are inside the row; `vec`: aligned to the run.
+template <int kCode>
+MXQ_DEVICE void store_run4(void* row, int64_t col, int n, bool vec, const float* y) {
+  if constexpr (kCode == MXQ_DTYPE_F32) {
+    float* p = reinterpret_cast<float*>(row) + col;
+    if (vec && n >= 4) {
+      *reinterpret_cast<v4f*>(p) = v4f{y[0], y[1], y[2], y[3]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < n) p[e] = y[e];
+    }
+  } else {
+    uint16_t* p = reinterpret_cast<uint16_t*>(row) + col;
+    uint32_t h[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = kCode == MXQ_DTYPE_F16 ? f32_to_f16_bits(y[e]) : f32_to_bf16_bits(y[e]);
+    if (vec && n >= 4) {
+      *reinterpret_cast<v2u*>(p) = v2u{h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < n) p[e] = (uint16_t)h[e];
+    }
+  }
+}
+
+MXQ_DEVICE float load_as_f32(const void* p, int64_t i, int code) {
+  if (code == MXQ_DTYPE_F32) return reinterpret_cast<const float*>(p)[i];
+  const uint32_t h = reinterpret_cast<const uint16_t*>(p)[i];
+  return code == MXQ_DTYPE_F16 ? f16_to_f32(h) : bf16_to_f32(h);
+}
+
+inline int dtype_bytes(int code) { return code == MXQ_DTYPE_F32 ? 4 : 2; }
+inline bool float_dtype(int code) { return code == MXQ_DTYPE_F32 || code == MXQ_DTYPE_F16 || code == MXQ_DTYPE_BF16; }
+
+// f.operator()<code>() for the run-time dtype code.
+template <class F>
+inline auto with_dtype(int code, F&& f) {
+  if (code == MXQ_DTYPE_F32) return f(std::integral_constant<int, MXQ_DTYPE_F32>{});
+  if (code == MXQ_DTYPE_F16) return f(std::integral_constant<int, MXQ_DTYPE_F16>{});
+  return f(std::integral_constant<int, MXQ_DTYPE_BF16>{});
+}
+
+}  // namespace mxq

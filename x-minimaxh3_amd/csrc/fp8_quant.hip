@@ -1,0 +1,361 @@
+// Quantizers of the block-128 e4m3 format (fp8_common.h), the way back, and the pass over an output's gradient.
+#include "fp8_common.h"
+
+namespace mxq {
+
+// ---- rows: one scale per 1 x 128 block ----
+// Eight lanes hold a block, 16 elements each, so a wave's loads cover whole lines, a block's maximum stays inside
+// eight lanes and every lane stores 16 codes. HBM-bound.
+template <int kCode>
+MXQ_DEVICE uint32_t block_scale_byte(const Piece<kCode>& p) {
+  uint32_t m = max8(piece_absmax(p));
+  if (m >= 0x7F800000u) m = max8(piece_absmax_finite(p));  // (the same for the eight lanes of a block)
+  return fp8_scale_byte(m);
+}
+
+constexpr int kRowUnroll = 4;
+
+template <int kCode>
+__global__ __launch_bounds__(256) void fp8_rows_quant_kernel(const char* x, int64_t ldx, uint8_t* q, int64_t ldq,
+                                                             uint8_t* s, int64_t lds, uint32_t M, uint32_t K, uint32_t kb,
+                                                             int vec) {
+  constexpr int kElem = kCode == MXQ_DTYPE_F32 ? 4 : 2;
+  const uint32_t total = M * kb;  // below 2^31 (checked by the launcher)
+  const uint32_t piece = threadIdx.x & 7, first = blockIdx.x * (32 * kRowUnroll) + (threadIdx.x >> 3);
+  Piece<kCode> p[kRowUnroll];
+  uint32_t row[kRowUnroll], b[kRowUnroll];
+#pragma unroll
+  for (int u = 0; u < kRowUnroll; ++u) {
+    const uint32_t g = min(first + u * 32, total - 1);
+    row[u] = g / kb;
+    b[u] = g - row[u] * kb;
+    const uint32_t col = b[u] * 128 + piece * 16;
+    p[u] = piece_load<kCode>(x + ((int64_t)row[u] * ldx + col) * kElem, (int)K - (int)col, vec);
+  }
+#pragma unroll
+  for (int u = 0; u < kRowUnroll; ++u) {
+    const uint32_t byte = block_scale_byte(p[u]);
+    const v4u codes = piece_encode(p[u], fp8_scale_f32(byte));
+    if (first + u * 32 < total) {
+      *reinterpret_cast<v4u*>(q + (int64_t)row[u] * ldq + b[u] * 128 + piece * 16) = codes;
+      if (piece == 0) s[(int64_t)row[u] * lds + b[u]] = (uint8_t)byte;
+    }
+  }
+}
+
+// ---- the way back ----
+template <int kCode>
+__global__ __launch_bounds__(256) void fp8_rows_dequant_kernel(const uint8_t* q, int64_t ldq, const uint8_t* s, int64_t lds,
+                                                               char* out, uint32_t M, uint32_t K, uint32_t pieces, int vec) {
+  constexpr int kElem = kCode == MXQ_DTYPE_F32 ? 4 : 2;
+  const uint32_t total = M * pieces;
+#pragma unroll
+  for (int u = 0; u < kRowUnroll; ++u) {
+    const uint32_t g = blockIdx.x * (256 * kRowUnroll) + u * 256 + threadIdx.x;
+    if (g >= total) return;
+    const uint32_t row = g / pieces, col = (g - row * pieces) * 16;
+    const int n = min(16, (int)(K - col));
+    const uint8_t* src = q + (int64_t)row * ldq + col;
+    v4u c = {0, 0, 0, 0};
+    if ((vec & 1) && n == 16) {
+      c = *reinterpret_cast<const v4u*>(src);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (i < n) c[i >> 2] |= (uint32_t)src[i] << (8 * (i & 3));
+    }
+    const float scale = fp8_scale_f32(s[(int64_t)row * lds + (col >> 7)]);
+    char* dst = out + (int64_t)row * K * kElem;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const v4f v = fp8x4_to_f32(c[j], scale);
+      const float y[4] = {v[0], v[1], v[2], v[3]};
+      store_run4<kCode>(dst, col + 4 * j, n - 4 * j, vec & 2, y);
+    }
+  }
+}
+
+// ---- weights: one scale per 128 x 128 tile, and the transposed codes that the input's gradient reads ----
+// One workgroup per tile: row t / 8 + 32 i, piece t % 8. The transposed copy goes through a 16 KB byte tile in LDS.
+template <int kCode>
+__global__ __launch_bounds__(256) void fp8_tiles_quant_kernel(const char* w, int64_t ldw, uint8_t* q, int64_t ldq, uint8_t* s,
+                                                              int64_t lds, uint8_t* qt, int64_t ldqt, uint8_t* st,
+                                                              int64_t ldst, int64_t N, int64_t K, int vec) {
+  constexpr int kElem = kCode == MXQ_DTYPE_F32 ? 4 : 2;
+  __shared__ uint32_t wave_max[4];
+  __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 132];  // rows of 132: a column's bytes spread over the banks
+  const int t = threadIdx.x, piece = t & 7;
+  const int64_t n0 = (int64_t)blockIdx.y * 128, k0 = (int64_t)blockIdx.x * 128, col = k0 + piece * 16;
+  Piece<kCode> p[4];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = n0 + (t >> 3) + 32 * i;
+    p[i] = piece_load<kCode>(w + (min(row, N - 1) * ldw + col) * kElem, row < N ? (int)(K - col) : 0, vec);
+    m = max(m, piece_absmax(p[i]));
+  }
+  m = wave_max_u32(m);
+  if ((t & 63) == 0) wave_max[t >> 6] = m;
+  __syncthreads();
+  m = max(max(wave_max[0], wave_max[1]), max(wave_max[2], wave_max[3]));
+  if (m >= 0x7F800000u) {  // (the whole workgroup)
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, piece_absmax_finite(p[i]));
+    m = wave_max_u32(m);
+    __syncthreads();
+    if ((t & 63) == 0) wave_max[t >> 6] = m;
+    __syncthreads();
+    m = max(max(wave_max[0], wave_max[1]), max(wave_max[2], wave_max[3]));
+  }
+  const uint32_t byte = fp8_scale_byte(m);
+  const float scale = fp8_scale_f32(byte);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = (t >> 3) + 32 * i;
+    const v4u c = piece_encode(p[i], scale);
+    if (n0 + r < N) *reinterpret_cast<v4u*>(q + (n0 + r) * ldq + col) = c;
+    if (qt) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<uint32_t*>(tile + r * 132 + piece * 16 + 4 * j) = c[j];
+    }
+  }
+  if (t == 0) s[blockIdx.y * lds + blockIdx.x] = (uint8_t)byte;
+  if (!qt) return;
+  if (t == 0) st[blockIdx.x * ldst + blockIdx.y] = (uint8_t)byte;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int k = (t >> 3) + 32 * i;  // row of the transposed tile
+    if (k0 + k < K) {
+      v4u c;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t v = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v |= (uint32_t)tile[(piece * 16 + 4 * j + e) * 132 + k] << (8 * e);
+        c[j] = v;
+      }
+      *reinterpret_cast<v4u*>(qt + (k0 + k) * ldqt + n0 + piece * 16) = c;
+    }
+  }
+}
+
+// ---- the pass over an output's gradient dY [M, N] ----
+// One read of dY makes all that the three gradients need of it: its e4m3 rows (the input's gradient), bfloat16 parts
+// of it where the weight's gradient cannot read dY itself (kParts: bf16 rows that are not 16-byte aligned 1, float16
+// 2, float32 3: parts p0 = bf16(x), p1 = bf16(x - p0), p2 = bf16(x - p0 - p1), whose sum is x to 16 and 24 bits), and
+// the column sums (the bias's gradient) of a strip of rows, in float32.
+// A workgroup takes 512 columns x `strip` rows: 32 lanes across, 8 rows at a time.
+template <int kCode, int kParts>
+__global__ __launch_bounds__(256) void fp8_grad_pass_kernel(const char* x, int64_t ldx, uint8_t* q, int64_t ldq, uint8_t* s,
+                                                            int64_t lds, uint16_t* parts, int64_t ldp, float* sums,
+                                                            int64_t M, int64_t N, int64_t nb, int64_t strip, int vec) {
+  constexpr int kElem = kCode == MXQ_DTYPE_F32 ? 4 : 2;
+  __shared__ float part_sum[8][512];
+  const int t = threadIdx.x, lane = t & 31, r = t >> 5;
+  const int64_t col = (int64_t)blockIdx.x * 512 + lane * 16, block = col >> 7;
+  const bool in = block < nb;  // (the same for the eight lanes of a block)
+  const int64_t first = (int64_t)blockIdx.y * strip, last = min(first + strip, M);
+  float acc[16] = {};
+  for (int64_t row = first + r; row < last; row += 8) {
+    const int n = in ? (int)(N - col) : 0;
+    const Piece<kCode> p = piece_load<kCode>(x + (row * ldx + (n > 0 ? col : 0)) * kElem, n, vec);
+    if (sums) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[i] += piece_at(p, i);
+    }
+    if (q) {
+      const uint32_t byte = block_scale_byte(p);
+      const v4u c = piece_encode(p, fp8_scale_f32(byte));
+      if (in) {
+        *reinterpret_cast<v4u*>(q + row * ldq + col) = c;
+        if ((lane & 7) == 0) s[row * lds + block] = (uint8_t)byte;
+      }
+    }
+    if constexpr (kParts > 0) {
+      if (in) {
+        uint32_t w[kParts][8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float a = piece_at(p, 2 * i), b = piece_at(p, 2 * i + 1);
+#pragma unroll
+          for (int k = 0; k < kParts; ++k) {
+            w[k][i] = pack_bf16x2(a, b);
+            // (NaN, an infinity, and a value that bfloat16 rounds to one leave no remainder)
+            const float ra = a - bf16_lo(w[k][i]), rb = b - bf16_hi(w[k][i]);
+            a = __builtin_fabsf(ra) < __builtin_inff() ? ra : 0.0f;
+            b = __builtin_fabsf(rb) < __builtin_inff() ? rb : 0.0f;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+          uint16_t* d = parts + ((int64_t)k * M + row) * ldp + col;
+          *reinterpret_cast<v4u*>(d) = v4u{w[k][0], w[k][1], w[k][2], w[k][3]};
+          *reinterpret_cast<v4u*>(d + 8) = v4u{w[k][4], w[k][5], w[k][6], w[k][7]};
+        }
+      }
+    }
+  }
+  if (!sums) return;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) part_sum[r][lane * 16 + i] = acc[i];
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int c = t + 256 * h;
+    const int64_t g = (int64_t)blockIdx.x * 512 + c;
+    if (g < N) {
+      float v = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v += part_sum[k][c];
+      sums[blockIdx.y * N + g] = v;
+    }
+  }
+}
+
+// out[c] = sum over `parts` rows of a float32 [parts, n] table, in row order by eighths: the columns' last sum.
+template <int kCode>
+__global__ __launch_bounds__(256) void column_join_kernel(const float* in, int64_t parts, int64_t n, void* out) {
+  __shared__ float sm[8][32];
+  const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
+  const int64_t col = (int64_t)blockIdx.x * 32 + c;
+  float v = 0.0f;
+  if (col < n) {
+#pragma unroll 8
+    for (int64_t i = r; i < parts; i += 8) v += in[i * n + col];
+  }
+  sm[r][c] = v;
+  __syncthreads();
+  if (r == 0 && col < n) {
+    v = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v += sm[k][c];
+    store_out<kCode>(reinterpret_cast<typename OutT<kCode>::T*>(out) + col, v);
+  }
+}
+
+}  // namespace mxq
+
+using namespace mxq;
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+extern "C" int mxq_fp8_quantize_rows(const void* x, int x_dtype, int64_t ldx, uint8_t* q, int64_t ldq, uint8_t* scale,
+                                     int64_t lds, int64_t M, int64_t K, void* stream) {
+  if (!float_dtype(x_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported input dtype code %d", x_dtype);
+  if (M < 0 || K < 1) return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld K=%lld", (long long)M, (long long)K);
+  const int64_t kb = (K + 127) / 128;
+  if (K >= (1ll << 30) || ldx < K || ldq < kb * 128 || ldq % 16 || lds < kb)
+    return mxq_set_error(MXQ_ERR_INVALID, "bad row strides ldx=%lld ldq=%lld lds=%lld for K=%lld", (long long)ldx,
+                         (long long)ldq, (long long)lds, (long long)K);
+  if (M == 0) return MXQ_OK;
+  if (!x || !q || !scale || !aligned16(q)) return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
+  if (M >= (1ll << 31) / kb - 65536 / kb - 1) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^31 blocks");
+  const int vec = aligned16(x) && ldx * dtype_bytes(x_dtype) % 16 == 0;
+  const unsigned grid = (unsigned)((M * kb + 32 * kRowUnroll - 1) / (32 * kRowUnroll));
+  with_dtype(x_dtype, [&](auto C) {
+    hipLaunchKernelGGL((fp8_rows_quant_kernel<decltype(C)::value>), dim3(grid), dim3(256), 0, (hipStream_t)stream,
+                       (const char*)x, ldx, q, ldq, scale, lds, (uint32_t)M, (uint32_t)K, (uint32_t)kb, vec);
+  });
+  return mxq_check_launch("fp8_rows_quant_kernel");
+}
+
+extern "C" int mxq_fp8_dequantize_rows(const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds, void* out,
+                                       int out_dtype, int64_t M, int64_t K, void* stream) {
+  if (!float_dtype(out_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported output dtype code %d", out_dtype);
+  if (M < 0 || K < 1) return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld K=%lld", (long long)M, (long long)K);
+  if (K >= (1ll << 30) || ldq < K || lds < (K + 127) / 128)
+    return mxq_set_error(MXQ_ERR_INVALID, "bad row strides ldq=%lld lds=%lld for K=%lld", (long long)ldq, (long long)lds,
+                         (long long)K);
+  if (M == 0) return MXQ_OK;
+  if (!q || !scale || !out) return mxq_set_error(MXQ_ERR_INVALID, "null pointer");
+  const int64_t pieces = (K + 15) / 16;
+  if (M >= (1ll << 31) / pieces - 65536 / pieces - 1) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^31 pieces");
+  const int run = 4 * dtype_bytes(out_dtype);
+  const int vec = (aligned16(q) && ldq % 16 == 0 ? 1 : 0) |
+                  (reinterpret_cast<uintptr_t>(out) % run == 0 && K % 4 == 0 ? 2 : 0);
+  const unsigned grid = (unsigned)((M * pieces + 256 * kRowUnroll - 1) / (256 * kRowUnroll));
+  with_dtype(out_dtype, [&](auto C) {
+    hipLaunchKernelGGL((fp8_rows_dequant_kernel<decltype(C)::value>), dim3(grid), dim3(256), 0, (hipStream_t)stream, q, ldq,
+                       scale, lds, (char*)out, (uint32_t)M, (uint32_t)K, (uint32_t)pieces, vec);
+  });
+  return mxq_check_launch("fp8_rows_dequant_kernel");
+}
+
+extern "C" int mxq_fp8_quantize_tiles(const void* w, int w_dtype, int64_t ldw, uint8_t* q, int64_t ldq, uint8_t* scale,
+                                      int64_t lds, uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst, int64_t N,
+                                      int64_t K, void* stream) {
+  if (!float_dtype(w_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported weight dtype code %d", w_dtype);
+  if (N < 1 || K < 1) return mxq_set_error(MXQ_ERR_INVALID, "bad size N=%lld K=%lld", (long long)N, (long long)K);
+  const int64_t kb = (K + 127) / 128, nb = (N + 127) / 128;
+  if (ldw < K || ldq < kb * 128 || ldq % 16 || lds < kb || (qt && (ldqt < nb * 128 || ldqt % 16 || ldst < nb)))
+    return mxq_set_error(MXQ_ERR_INVALID, "bad row strides for N=%lld K=%lld", (long long)N, (long long)K);
+  if (!w || !q || !scale || !aligned16(q) || (qt && (!scale_t || !aligned16(qt))))
+    return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
+  if (nb > 65535 || kb >= (1ll << 31)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 65535 tile rows");
+  const int vec = aligned16(w) && ldw * dtype_bytes(w_dtype) % 16 == 0;
+  with_dtype(w_dtype, [&](auto C) {
+    hipLaunchKernelGGL((fp8_tiles_quant_kernel<decltype(C)::value>), dim3((unsigned)kb, (unsigned)nb), dim3(256), 0,
+                       (hipStream_t)stream, (const char*)w, ldw, q, ldq, scale, lds, qt, ldqt, scale_t, ldst, N, K, vec);
+  });
+  return mxq_check_launch("fp8_tiles_quant_kernel");
+}
+
+// Rows per strip of the gradient pass: whole eights, about four workgroups per CU in all, at least 32 rows.
+static int64_t grad_strip(int64_t M, int64_t N) {
+  const int64_t panels = (N + 511) / 512;
+  const int64_t want = panels >= 4 * mxq_cu_count() ? 1 : 4 * mxq_cu_count() / panels;
+  int64_t strip = ((M + want - 1) / want + 7) / 8 * 8;
+  if (strip < 32) strip = 32;
+  const int64_t least = ((M + 65534) / 65535 + 7) / 8 * 8;  // grid.y
+  return strip < least ? least : strip;
+}
+
+extern "C" int mxq_fp8_grad_strips(int64_t M, int64_t N, int64_t* strips) {
+  if (M < 0 || N < 1 || !strips) return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld N=%lld", (long long)M, (long long)N);
+  const int64_t strip = grad_strip(M, N);
+  *strips = M == 0 ? 0 : (M + strip - 1) / strip;
+  return MXQ_OK;
+}
+
+extern "C" int mxq_fp8_grad_pass(const void* dy, int dy_dtype, int64_t ldy, uint8_t* q, int64_t ldq, uint8_t* scale,
+                                 int64_t lds, void* parts, int n_parts, int64_t ldp, float* sums, int64_t strips,
+                                 int64_t M, int64_t N, void* stream) {
+  if (!float_dtype(dy_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported gradient dtype code %d", dy_dtype);
+  if (M < 0 || N < 1) return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld N=%lld", (long long)M, (long long)N);
+  const int64_t nb = (N + 127) / 128, strip = grad_strip(M, N);
+  const int most = dy_dtype == MXQ_DTYPE_BF16 ? 1 : dy_dtype == MXQ_DTYPE_F16 ? 2 : 3;
+  if (ldy < N || (q && (ldq < nb * 128 || ldq % 16 || lds < nb)) ||
+      (n_parts != 0 && (n_parts != most || ldp < nb * 128 || ldp % 8)))
+    return mxq_set_error(MXQ_ERR_INVALID, "bad row strides or parts for N=%lld", (long long)N);
+  if (M == 0) return MXQ_OK;
+  if (!dy || (q && (!scale || !aligned16(q))) || (n_parts && (!parts || !aligned16(parts))))
+    return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
+  if (sums && strips != (M + strip - 1) / strip)
+    return mxq_set_error(MXQ_ERR_INVALID, "room for %lld strips, %lld needed", (long long)strips,
+                         (long long)((M + strip - 1) / strip));
+  const int vec = aligned16(dy) && ldy * dtype_bytes(dy_dtype) % 16 == 0;
+  const dim3 grid((unsigned)((N + 511) / 512), (unsigned)((M + strip - 1) / strip));
+  with_dtype(dy_dtype, [&](auto C) {
+    constexpr int kCode = decltype(C)::value;
+    constexpr int kMost = kCode == MXQ_DTYPE_BF16 ? 1 : kCode == MXQ_DTYPE_F16 ? 2 : 3;
+    if (n_parts)
+      hipLaunchKernelGGL((fp8_grad_pass_kernel<kCode, kMost>), grid, dim3(256), 0, (hipStream_t)stream, (const char*)dy, ldy,
+                         q, ldq, scale, lds, (uint16_t*)parts, ldp, sums, M, N, nb, strip, vec);
+    else
+      hipLaunchKernelGGL((fp8_grad_pass_kernel<kCode, 0>), grid, dim3(256), 0, (hipStream_t)stream, (const char*)dy, ldy, q,
+                         ldq, scale, lds, (uint16_t*)nullptr, (int64_t)0, sums, M, N, nb, strip, vec);
+  });
+  return mxq_check_launch("fp8_grad_pass_kernel");
+}
+
+extern "C" int mxq_column_join(const float* in, int64_t parts, int64_t n, void* out, int out_dtype, void* stream) {
+  if (!float_dtype(out_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported output dtype code %d", out_dtype);
+  if (parts < 0 || n < 1 || n >= (1ll << 36) || !out || (parts && !in)) return mxq_set_error(MXQ_ERR_INVALID, "bad argument");
+  with_dtype(out_dtype, [&](auto C) {
+    hipLaunchKernelGGL((column_join_kernel<decltype(C)::value>), dim3((unsigned)((n + 31) / 32)), dim3(256), 0,
+                       (hipStream_t)stream, in, parts, n, out);
+  });
+  return mxq_check_launch("column_join_kernel");
+}

@@ -1,0 +1,718 @@
+// Matrix product of block-128 e4m3 operands (fp8_common.h) on gfx950 matrix cores:
+//
+//   D[m, n] = out( sum_b 2^(ea[m, b] + eb[n / 128, b]) * sum_{k in block b} A[m, k] * B[n, k]  +  bias[n] )
+//
+// A [M, K] activations (or output gradients) with one scale per row and block, B [N, K] a weight (or its transposed
+// copy) with one per 128 x 128 tile; both K-contiguous, rows zero-padded to whole blocks. Sums are float32.
+//
+// Main loop: a workgroup of eight waves (two per SIMD) owns a 256 x 256 (or 128 x 256) output tile, a wave 128 x 64 (or
+// 64 x 64) of it. A stage is one block of 128 K-bytes; its A and B chunks are fetched by direct-to-LDS loads into a
+// ring of five 32 KB slots, one to two stages ahead. The two waves of a SIMD take turns: one issues the matrix
+// instructions of a half stage while the other reads its next fragments and issues loads. v_mfma_scale_f32_32x32x64_
+// f8f6f4 applies the scales itself: each lane gives one byte for its row, so a block's scale costs the loop nothing but
+// four words per four stages and wave (a byte per stage, shifted out of a word).
+//
+// Precision of that instruction, measured: within one 64-long product sum, addends below 2^-13 of the largest are
+// cut, and the sum is added to a float32. On the layers' data that is 5e-5 to 2e-4 of the result's root mean square,
+// below bfloat16's and float16's own rounding (1.7e-3, 2.1e-4). For float32 results (kWide) the fragments are
+// converted to bfloat16 with their scales, exactly, and the sums run on v_mfma_f32_32x32x16_bf16, which keeps every
+// addend to float32's precision at half the rate.
+//
+// Problems of few tiles split K over workgroups, which write float32 sums that fp8_join_kernel adds in order.
+
+#include "fp8_common.h"
+
+namespace mxq {
+
+constexpr int kTileN = 256, kStageK = 128;
+constexpr int kRing = 5, kSlot = 256 * kStageK;
+constexpr int kGemmLds = kRing * kSlot;
+static_assert(kGemmLds <= 160 * 1024, "LDS of a CU");
+constexpr int kGroupRows = 4;  // tile-rows per group of the tile order
+
+struct Fp8Gemm {
+  const uint8_t* a;
+  const uint8_t* b;
+  const uint8_t* sa;
+  const uint8_t* sb;
+  const void* bias;
+  void* d;  // split: float32 sums, slice s at s * M * N
+  int64_t M, N, lda, ldb, ldsa, ldsb, ldd;
+  int kb;                  // blocks of K
+  int tiles_m, tiles_n;
+  int splits, split_kb;    // K slices of split_kb blocks (a multiple of 4)
+  int vec;                 // whole rows of d are 16-byte aligned (and bias to 4 elements)
+};
+
+template <int kTM>
+struct Tile {
+  static constexpr int kBM = kTM, kWaveM = kTM / 2, kBI = kWaveM / 32, kBJ = 2;
+  static constexpr int kLoadsA = kTM / 64, kLoadsB = 4;  // 1 KB loads per wave and chunk
+};
+
+// ---- operand loads ----
+// Chunk rows are 128 bytes; 16-byte piece c of row r sits at piece c ^ ((r >> 1) & 7), so that the sixteen lanes a
+// ds_read_b128 serves at once (sixteen rows, one piece) touch every bank once. One load fills 1 KB: eight rows.
+MXQ_DEVICE int swizzle(int r) { return (r >> 1) & 7; }
+
+template <int kLoads>
+struct Chunk {
+  const uint8_t* base;  // row 0 of the tile
+  int bytes;            // the tile's rows in memory: rows behind the operand's last are the last one again
+  uint32_t off[kLoads];
+  int wave;
+};
+
+// (Rows are counted in 32 bits: a buffer resource has to be in scalar registers, and there is no scalar 64-bit minimum.
+// Computed in vector registers, it made every access loop over the lanes' resources.)
+template <int kLoads>
+MXQ_DEVICE Chunk<kLoads> make_chunk(const uint8_t* p, int64_t ld, int row0, int rows, int wave, int lane) {
+  Chunk<kLoads> c;
+  const int valid = min(rows - row0, kLoads * 64);
+  c.base = p + row0 * ld;
+  c.bytes = valid * (int)ld;
+  c.wave = wave;
+#pragma unroll
+  for (int t = 0; t < kLoads; ++t) {
+    const int r = (wave * kLoads + t) * 8 + (lane >> 3);
+    c.off[t] = (uint32_t)(min(r, valid - 1) * (int)ld + (((lane & 7) ^ swizzle(r)) << 4));
+  }
+  return c;
+}
+
+template <int kLoads>
+MXQ_DEVICE void issue_chunk(const Chunk<kLoads>& c, char* slot, int stage, bool on) {
+  if (on) {
+#pragma unroll
+    for (int t = 0; t < kLoads; ++t)
+      buffer_load_lds16(c.base, c.bytes, (lptr_t)(slot + (c.wave * kLoads + t) * 1024), c.off[t], stage * kStageK);
+  }
+}
+
+MXQ_DEVICE v8i join8(v4i a, v4i b) { return v8i{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
+
+// The 32 bytes of each of kCount 32-row blocks that a lane feeds the matrix instruction of half stage `half`: row
+// l % 32, pieces 4 half + l / 32 and 4 half + 2 + l / 32. (Both operands take the same bytes of K, in any order: a
+// block has one scale.)
+template <int kCount>
+MXQ_DEVICE void read_frags(uint32_t slot, int row, int lane, int half, v8i (&f)[kCount]) {
+  const int lr = lane & 31, c = half * 4 + (lane >> 5);
+  const uint32_t at = slot + (uint32_t)((row + lr) * kStageK);
+  const uint32_t x0 = at + (uint32_t)((c ^ swizzle(lr)) << 4), x1 = at + (uint32_t)(((c + 2) ^ swizzle(lr)) << 4);
+  static_for<kCount>([&](auto I) {
+    constexpr int i = decltype(I)::value;
+    f[i] = join8(lds_read_b128<i * 32 * kStageK>(x0), lds_read_b128<i * 32 * kStageK>(x1));
+  });
+}
+
+// acc += (b * 2^(sb - 127)) (a * 2^(sa - 127))^T over 64 bytes of K; the scales are the low bytes. Written as assembly
+// with the sum in place: the builtin's result may be another register tuple than its addend, and the 256-row tile then
+// spilled its accumulators (660 registers). What the compiler would look after is done here: two wait states between a
+// vector instruction's write of an operand and its read (s_nop), and mfma_drain before the sums are read.
+MXQ_DEVICE void mfma_scaled(v16f& acc, v8i b, v8i a, uint32_t sb, uint32_t sa) {
+  __asm__ volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]"
+                   : "+v"(acc)
+                   : "v"(b), "v"(a), "v"(sb), "v"(sa));
+}
+// Waits out the 16 passes of the last matrix instruction (19 wait states) before its sums are read.
+MXQ_DEVICE void mfma_drain() {
+  __builtin_amdgcn_sched_barrier(0);
+  __asm__ volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The matrix instructions of a half stage. They compute D^T blocks (B first): lane l holds row l % 32 of D and, in
+// register r, column (r / 4) * 8 + (l / 32) * 4 + r % 4.
+template <class C, bool kWide>
+MXQ_DEVICE void half_stage(const v8i (&fa)[C::kBI], const v8i (&fb)[C::kBJ], const uint32_t (&sa)[C::kBI], uint32_t sb,
+                           v16f (&acc)[C::kBI][C::kBJ]) {
+  if constexpr (!kWide) {
+#pragma unroll
+    for (int i = 0; i < C::kBI; ++i)
+#pragma unroll
+      for (int j = 0; j < C::kBJ; ++j)
+        mfma_scaled(acc[i][j], fb[j], fa[i], sb, sa[i]);
+  } else {
+    const float fsb = fp8_scale_f32(sb & 0xFFu);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      v8bf wb[C::kBJ];
+#pragma unroll
+      for (int j = 0; j < C::kBJ; ++j) wb[j] = fp8x8_to_bf16((uint32_t)fb[j][2 * q], (uint32_t)fb[j][2 * q + 1], fsb);
+#pragma unroll
+      for (int i = 0; i < C::kBI; ++i) {
+        const v8bf xa = fp8x8_to_bf16((uint32_t)fa[i][2 * q], (uint32_t)fa[i][2 * q + 1], fp8_scale_f32(sa[i] & 0xFFu));
+#pragma unroll
+        for (int j = 0; j < C::kBJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[j], xa, acc[i][j], 0, 0, 0);
+      }
+    }
+  }
+}
+
+MXQ_DEVICE void phase_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  barrier_no_drain();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// A wave's scale words for the four stages from `stage` on (a multiple of 4): its rows' and its columns'.
+template <class C>
+struct Scales {
+  uint32_t a[C::kBI], b;
+};
+template <class C>
+struct ScaleSource {
+  const uint8_t *a, *b;
+  int bytes_a, bytes_b;
+  uint32_t off[C::kBI];
+};
+MXQ_DEVICE uint32_t buffer_load_x1(const void* base, int bytes, uint32_t voff, int soff) {
+  return __builtin_amdgcn_raw_buffer_load_b32(
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, kRawBufferWord3), (int)voff, soff, 0);
+}
+template <class C>
+MXQ_DEVICE void load_scales(const ScaleSource<C>& s, int stage, Scales<C>& w) {
+#pragma unroll
+  for (int i = 0; i < C::kBI; ++i) w.a[i] = buffer_load_x1(s.a, s.bytes_a, s.off[i], stage);
+  w.b = buffer_load_x1(s.b, s.bytes_b, 0, stage);
+}
+
+// One group's whole main loop over stages [0, n) (kG = 0: waves 0-3, 1: waves 4-7). The operand chunks A_0 B_0 A_1
+// B_1 ... go to slot (chunk index) % 5. Iteration kt has four phases, a workgroup barrier behind each; group g computes
+// in phases 2 q + g and reads in the others:
+//   P0  g0: first half of kt      g1: reads (kt, 0), loads A_kt+2 into B_kt-1's slot
+//   P1  g1: first half            g0: reads (kt, 1), loads A_kt+2
+//   P2  g0: second half           g1: reads (kt, 1)          both then wait for stage kt+1
+//   P3  g1: second half + loads   g0: reads (kt+1, 0), loads B_kt+2 into A_kt's slot
+//       of B_kt+2
+// The scale words of stages 4 g .. 4 g + 3 are requested with the B loads of iteration 4 g - 2, so the next
+// iteration's wait covers them.
+template <class C, int kG, bool kWide>
+MXQ_DEVICE void main_loop(char* lds, const Chunk<C::kLoadsA>& ca, const Chunk<C::kLoadsB>& cb, const ScaleSource<C>& ss,
+                          int n, int wrow, int wcol, int lane, v16f (&acc)[C::kBI][C::kBJ]) {
+  const uint32_t base = lds_addr(lds);
+  auto slot_addr = [&](int s) { return base + (uint32_t)(s * kSlot); };
+  Scales<C> cur, next;
+  load_scales(ss, 0, cur);
+  __builtin_amdgcn_sched_barrier(0);
+  issue_chunk(ca, lds, 0, true);
+  issue_chunk(cb, lds + kSlot, 0, true);
+  issue_chunk(ca, lds + 2 * kSlot, 1, n > 1);
+  issue_chunk(cb, lds + 3 * kSlot, 1, n > 1);
+  if (n > 1)
+    wait_vmcnt<C::kLoadsA + C::kLoadsB>();
+  else
+    wait_vmcnt<0>();
+#pragma unroll
+  for (int i = 0; i < C::kBI; ++i) __asm__ volatile("" : "+v"(cur.a[i]));
+  __asm__ volatile("" : "+v"(cur.b));
+  next = cur;
+  phase_barrier();
+  v8i fa[C::kBI], fb[C::kBJ];
+  if constexpr (kG == 0) {
+    read_frags<C::kBI>(slot_addr(0), wrow, lane, 0, fa);
+    read_frags<C::kBJ>(slot_addr(1), wcol, lane, 0, fb);
+    wait_lgkm<0>();
+  }
+  phase_barrier();
+
+  int sa = 0;  // slot of A_kt; B_kt is in the next one
+  auto iteration = [&](int kt, auto SteadyC) {
+    constexpr bool kSteady = decltype(SteadyC)::value;  // stage kt + 2 exists
+    const int sb = sa == kRing - 1 ? 0 : sa + 1;
+    const int na = sb == kRing - 1 ? 0 : sb + 1;
+    const int nb = na == kRing - 1 ? 0 : na + 1;
+    const int pa = sa == 0 ? kRing - 1 : sa - 1;
+    const bool more = kSteady || kt + 2 < n;
+    char* slot_pa = lds + pa * kSlot;
+    char* slot_sa = lds + sa * kSlot;
+    auto next_scales = [&] {
+      if ((kt & 3) == 2 && more) load_scales(ss, kt + 2, next);
+    };
+    if constexpr (kG == 0) {
+      half_stage<C, kWide>(fa, fb, cur.a, cur.b, acc);  // P0
+      phase_barrier();
+      read_frags<C::kBI>(slot_addr(sa), wrow, lane, 1, fa);  // P1
+      read_frags<C::kBJ>(slot_addr(sb), wcol, lane, 1, fb);
+      issue_chunk(ca, slot_pa, kt + 2, more);
+      wait_lgkm<0>();
+      phase_barrier();
+      half_stage<C, kWide>(fa, fb, cur.a, cur.b, acc);  // P2
+    } else {
+      read_frags<C::kBI>(slot_addr(sa), wrow, lane, 0, fa);  // P0
+      read_frags<C::kBJ>(slot_addr(sb), wcol, lane, 0, fb);
+      issue_chunk(ca, slot_pa, kt + 2, more);
+      wait_lgkm<0>();
+      phase_barrier();
+      half_stage<C, kWide>(fa, fb, cur.a, cur.b, acc);  // P1
+      phase_barrier();
+      read_frags<C::kBI>(slot_addr(sa), wrow, lane, 1, fa);  // P2
+      read_frags<C::kBJ>(slot_addr(sb), wcol, lane, 1, fb);
+      wait_lgkm<0>();
+    }
+    // stage kt + 1 has landed: only A_kt+2 (when it exists) was issued after it
+    if (more)
+      wait_vmcnt<C::kLoadsA>();
+    else
+      wait_vmcnt<0>();
+    // The scale words requested an iteration ago have landed with it: the next stage's scales are taken here, ahead of
+    // the next request (behind it, the compiler would wait for that one).
+    Scales<C> after;
+    const bool whole = (kt & 3) == 3;
+#pragma unroll
+    for (int i = 0; i < C::kBI; ++i) {
+      after.a[i] = whole ? next.a[i] : cur.a[i] >> 8;
+      __asm__ volatile("" : "+v"(after.a[i]));
+    }
+    after.b = whole ? next.b : cur.b >> 8;
+    __asm__ volatile("" : "+v"(after.b));
+    phase_barrier();
+    if constexpr (kG == 0) {
+      // P3 (at the last stage these reads fetch slots nobody uses)
+      read_frags<C::kBI>(slot_addr(na), wrow, lane, 0, fa);
+      read_frags<C::kBJ>(slot_addr(nb), wcol, lane, 0, fb);
+      next_scales();
+      issue_chunk(cb, slot_sa, kt + 2, more);
+      wait_lgkm<0>();
+    } else {
+      next_scales();
+      issue_chunk(cb, slot_sa, kt + 2, more);
+      half_stage<C, kWide>(fa, fb, cur.a, cur.b, acc);  // P3
+    }
+    phase_barrier();
+    cur = after;
+    sa = na;
+  };
+  int kt = 0;
+  for (; kt + 2 < n; ++kt) iteration(kt, std::true_type{});
+  do {
+    iteration(kt, std::false_type{});
+  } while (++kt < n);
+  mfma_drain();
+}
+
+// ---- epilogue ----
+// A wave passes its output through 4 KB of LDS in pieces of 32 rows x 128 bytes (32-row block i, one or two column
+// blocks), so that eight lanes store a whole line.
+MXQ_DEVICE char* out_stage_at(char* buf, int r, int c) { return buf + r * 128 + ((c ^ ((r >> 1) & 7)) << 4); }
+
+MXQ_DEVICE void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+template <int kOut>
+MXQ_DEVICE uint32_t out_pair(float a, float b) {  // two 16-bit values
+  if constexpr (kOut == MXQ_DTYPE_BF16) return pack_bf16x2(a, b);
+  return f32_to_f16_bits(a) | (f32_to_f16_bits(b) << 16);
+}
+
+// Bias of the four columns from col on (behind the last: the last one's).
+template <int kOut>
+MXQ_DEVICE v4f bias_run(const void* bias, int col, int N) {
+  v4f b = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (bias) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = OutT<kOut>::load(reinterpret_cast<const typename OutT<kOut>::T*>(bias) + min(col + e, N - 1));
+  }
+  return b;
+}
+
+template <class C, int kOut, bool kSplit>
+MXQ_DEVICE void epilogue(const Fp8Gemm& p, char* lds, const v16f (&acc)[C::kBI][C::kBJ], int m0, int n0, int wrow,
+                         int wcol, int wave, int lane, void* d) {
+  constexpr int kElem = kOut == MXQ_DTYPE_F32 ? 4 : 2;
+  char* buf = lds + wave * 4096;
+  const int M = (int)p.M, N = (int)p.N;
+  const bool lines = p.vec && M - m0 >= C::kBM && N - n0 >= kTileN;
+  const int lr = lane & 31, lh = lane >> 5;
+  char* out = reinterpret_cast<char*>(d);
+#pragma unroll
+  for (int i = 0; i < C::kBI; ++i) {
+    const int row0 = m0 + wrow + i * 32;
+#pragma unroll
+    for (int j = 0; j < C::kBJ; ++j) {
+      const int col0 = n0 + wcol + j * 32;
+      if (kElem == 4 || j == 0) wave_lds_fence();  // the piece before has been read
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int col = col0 + q * 8 + lh * 4;
+        const v4f b = kSplit ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : bias_run<kOut>(p.bias, col, N);
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = kSplit ? acc[i][j][q * 4 + e] : acc[i][j][q * 4 + e] + b[e];
+        if (!lines) {
+          const int row = row0 + lr;
+          if (row < M) store_run4<kOut>(out + row * p.ldd * kElem, col, N - col, p.vec, y);
+        } else if constexpr (kElem == 4) {
+          *reinterpret_cast<v4f*>(out_stage_at(buf, lr, 2 * q + lh)) = v4f{y[0], y[1], y[2], y[3]};
+        } else {
+          *reinterpret_cast<v2u*>(out_stage_at(buf, lr, j * 4 + q) + lh * 8) =
+              v2u{out_pair<kOut>(y[0], y[1]), out_pair<kOut>(y[2], y[3])};
+        }
+      }
+      if (lines && (kElem == 4 || j == C::kBJ - 1)) {
+        wave_lds_fence();
+        const int64_t byte0 = (int64_t)(kElem == 4 ? col0 : n0 + wcol) * kElem;
+        v4u v[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) v[t] = *reinterpret_cast<const v4u*>(out_stage_at(buf, t * 8 + (lane >> 3), lane & 7));
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          __builtin_nontemporal_store(
+              v[t], reinterpret_cast<v4u*>(out + (row0 + t * 8 + (lane >> 3)) * p.ldd * kElem + byte0 + (lane & 7) * 16));
+      }
+    }
+  }
+}
+
+// Tile order: contiguous ranges over the 8 XCDs (workgroup ids are dealt to them in turn), each walked in groups of
+// kGroupRows tile-rows, so that an XCD's workgroups share operand panels in its L2.
+MXQ_DEVICE void tile_of(int bid, const Fp8Gemm& p, int& tm, int& tn, int& slice) {
+  const int tiles = p.tiles_m * p.tiles_n, num = tiles * p.splits, per = num / 8;
+  int t = bid < per * 8 ? (bid % 8) * per + bid / 8 : bid;
+  slice = t / tiles;
+  t -= slice * tiles;
+  const int group = kGroupRows * p.tiles_n, g = t / group, first = g * kGroupRows, rows = min(p.tiles_m - first, kGroupRows);
+  const int in = t - g * group;
+  tn = in / rows;
+  tm = first + in - tn * rows;
+}
+
+template <int kTM, int kOut, bool kSplit, bool kWide>
+__global__ __launch_bounds__(512, 2) void gemm_fp8_kernel(Fp8Gemm p) {
+  typedef Tile<kTM> C;
+  __shared__ __attribute__((aligned(1024))) char lds[kGemmLds];
+  int tm, tn, slice;
+  tile_of(blockIdx.x, p, tm, tn, slice);
+  const int M = (int)p.M, N = (int)p.N, m0 = tm * kTM, n0 = tn * kTileN;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  // waves w and w + 4 share a SIMD: the two 64-column halves of quadrant w % 4
+  const int wrow = ((wave & 3) >> 1) * C::kWaveM, wcol = (wave & 1) * 128 + (wave >> 2) * 64;
+  const int kb0 = slice * p.split_kb, n = min(p.split_kb, p.kb - kb0);
+  const auto ca = make_chunk<C::kLoadsA>(p.a + (int64_t)kb0 * kStageK, p.lda, m0, M, wave, lane);
+  const auto cb = make_chunk<C::kLoadsB>(p.b + (int64_t)kb0 * kStageK, p.ldb, n0, N, wave, lane);
+  ScaleSource<C> ss;
+  const int rows = min(M - m0, kTM);
+  ss.a = p.sa + m0 * p.ldsa + kb0;
+  ss.bytes_a = rows * (int)p.ldsa - kb0;
+#pragma unroll
+  for (int i = 0; i < C::kBI; ++i) ss.off[i] = (uint32_t)(min(wrow + i * 32 + (lane & 31), rows - 1) * (int)p.ldsa);
+  ss.b = p.sb + min((n0 + wcol) >> 7, (N - 1) >> 7) * p.ldsb + kb0;
+  ss.bytes_b = (int)p.ldsb - kb0;
+  v16f acc[C::kBI][C::kBJ] = {};
+  if (wave < 4)
+    main_loop<C, 0, kWide>(lds, ca, cb, ss, n, wrow, wcol, lane, acc);
+  else
+    main_loop<C, 1, kWide>(lds, ca, cb, ss, n, wrow, wcol, lane, acc);
+  void* d = p.d;
+  if constexpr (kSplit) d = reinterpret_cast<float*>(p.d) + slice * p.M * p.ldd;
+  epilogue<C, kOut, kSplit>(p, lds, acc, m0, n0, wrow, wcol, wave, lane, d);
+}
+
+// D = out(sum over slices + bias), four columns per thread; the slices' rows are padded to whole fours.
+template <int kOut>
+__global__ __launch_bounds__(256) void fp8_join_kernel(const float* part, int splits, int64_t M, int64_t N, int64_t ldp,
+                                                       const void* bias, char* d, int64_t ldd, int vec) {
+  constexpr int kElem = kOut == MXQ_DTYPE_F32 ? 4 : 2;
+  const int64_t runs = ldp / 4, g = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (g >= M * runs) return;
+  const int64_t row = g / runs;
+  const int col = (int)(g - row * runs) * 4;
+  v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < splits; ++s) y += *reinterpret_cast<const v4f*>(part + (s * M + row) * ldp + col);
+  y += bias_run<kOut>(bias, col, (int)N);
+  const float v[4] = {y[0], y[1], y[2], y[3]};
+  store_run4<kOut>(d + row * ldd * kElem, col, (int)N - col, vec, v);
+}
+
+// ---- few rows (up to 64): a stream of the weight ----
+// A workgroup's four waves take 16 kRT weight rows and share K. Fragments go from memory straight to registers
+// (a lane: row l % 16, bytes 16 (l / 16) + {0..15} and + 64 of a block), are converted to bfloat16 with their scales,
+// exactly, and multiplied by v_mfma_f32_16x16x32_bf16, so the sums keep float32's precision at no cost: the weight's
+// bytes bound this kernel. kFused: the activations come in their own type and each wave quantizes its own K range
+// of them in registers (up to 16 rows: the 16 columns of the instruction), which saves the quantizer's launch.
+struct Fp8Rows {
+  const void* x;  // kFused: [M, ldx] of the input type; else e4m3 codes [M, ldx]
+  const uint8_t* sx;
+  const uint8_t* b;
+  const uint8_t* sb;
+  const void* bias;
+  void* d;
+  int64_t M, N, K, ldx, ldsx, ldb, ldsb, ldd;
+  int kb, vec;
+};
+
+template <int kIn>
+MXQ_DEVICE void quantize_in_registers(const char* row, bool on, int64_t k0, int64_t K, int g, v8bf (&f)[4]) {
+  constexpr int kElem = kIn == MXQ_DTYPE_F32 ? 4 : 2;
+  Piece<kIn> p[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int64_t k = k0 + h * 64 + g * 16;
+    // (K is a multiple of 8 elements and rows are 16-byte aligned: halves of a piece are whole vectors)
+    const int n = on ? (int)(K - k) : 0;  // (K is at most 2^22)
+    p[h] = piece_load<kIn>(row + (n > 0 ? k : 0) * kElem, n, true);
+  }
+  auto across = [](uint32_t m) {  // lanes l, l ^ 16, l ^ 32, l ^ 48
+    const auto r = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+    m = max(r[0], r[1]);
+    const auto s = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    return max(s[0], s[1]);
+  };
+  uint32_t m = across(max(piece_absmax(p[0]), piece_absmax(p[1])));
+  if (__builtin_amdgcn_ballot_w64(m >= 0x7F800000u) != 0)  // (every lane takes part in the exchange)
+    m = across(max(piece_absmax_finite(p[0]), piece_absmax_finite(p[1])));
+  const float scale = fp8_scale_f32(fp8_scale_byte(m));
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const v4u c = piece_encode(p[h], scale);
+    f[2 * h] = fp8x8_to_bf16(c[0], c[1], scale);
+    f[2 * h + 1] = fp8x8_to_bf16(c[2], c[3], scale);
+  }
+}
+
+template <int kIn, int kOut, int kMT, int kRT, bool kFused>
+__global__ __launch_bounds__(256) void fp8_rows_kernel(Fp8Rows p) {
+  constexpr int kAhead = 4 / kRT > 1 ? 4 / kRT : 2;  // blocks whose weight loads are issued together
+  __shared__ v4f part[4][kRT][kMT][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
+  const int N = (int)p.N, n0 = blockIdx.x * (16 * kRT);
+  const int per = (p.kb + 3) / 4, first = wave * per, last = min(first + per, p.kb);
+  const int rows = min(N - n0, 16 * kRT);
+  const uint8_t* wb = p.b + n0 * p.ldb;
+  const int wbytes = (int)(rows * p.ldb);
+  uint32_t woff[kRT];
+#pragma unroll
+  for (int r = 0; r < kRT; ++r) {
+    const int row = r * 16 + lr;
+    woff[r] = row < rows ? (uint32_t)(row * (int)p.ldb + g * 16) : kBufferOff;
+  }
+  const uint8_t* sw = p.sb + (n0 >> 7) * p.ldsb;
+  v4f acc[kRT][kMT] = {};
+  for (int kb = first; kb < last; kb += kAhead) {
+    v4u w[kAhead][kRT][2];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int r = 0; r < kRT; ++r)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          w[u][r][h] = buffer_load_x4(wb, wbytes, kb + u < last ? woff[r] + (uint32_t)((kb + u) * 128 + h * 64) : kBufferOff);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (kb + u >= last) break;
+      v8bf xf[kMT][4];
+#pragma unroll
+      for (int m = 0; m < kMT; ++m) {
+        const int64_t row = m * 16 + lr;
+        const bool on = row < p.M;
+        if constexpr (kFused) {
+          constexpr int kElem = kIn == MXQ_DTYPE_F32 ? 4 : 2;
+          quantize_in_registers<kIn>(reinterpret_cast<const char*>(p.x) + (on ? row : 0) * p.ldx * kElem, on,
+                                     (int64_t)(kb + u) * 128, p.K, g, xf[m]);
+        } else {
+          const uint8_t* xq = reinterpret_cast<const uint8_t*>(p.x) + row * p.ldx + (kb + u) * 128 + g * 16;
+          v4u c[2] = {};
+          float scale = 1.0f;
+          if (on) {
+            c[0] = *reinterpret_cast<const v4u*>(xq);
+            c[1] = *reinterpret_cast<const v4u*>(xq + 64);
+            scale = fp8_scale_f32(p.sx[row * p.ldsx + kb + u]);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            xf[m][2 * h] = fp8x8_to_bf16(c[h][0], c[h][1], scale);
+            xf[m][2 * h + 1] = fp8x8_to_bf16(c[h][2], c[h][3], scale);
+          }
+        }
+      }
+      const float ws = fp8_scale_f32(sw[kb + u]);
+#pragma unroll
+      for (int r = 0; r < kRT; ++r)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const v8bf wf = fp8x8_to_bf16(w[u][r][q >> 1][2 * (q & 1)], w[u][r][q >> 1][2 * (q & 1) + 1], ws);
+#pragma unroll
+          for (int m = 0; m < kMT; ++m) acc[r][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, xf[m][q], acc[r][m], 0, 0, 0);
+        }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kRT; ++r)
+#pragma unroll
+    for (int m = 0; m < kMT; ++m) part[wave][r][m][lane] = acc[r][m];
+  __syncthreads();
+  // the four waves' sums in order; (r, m) pairs are dealt to the waves
+  constexpr int kElem = kOut == MXQ_DTYPE_F32 ? 4 : 2;
+  for (int t = wave; t < kRT * kMT; t += 4) {
+    const int r = t / kMT, m = t - r * kMT;
+    const int row = m * 16 + lr, col = n0 + r * 16 + g * 4;
+    v4f y = part[0][r][m][lane];
+#pragma unroll
+    for (int k = 1; k < 4; ++k) y += part[k][r][m][lane];
+    if (row < p.M && col < N) {
+      y += bias_run<kOut>(p.bias, col, N);
+      const float v[4] = {y[0], y[1], y[2], y[3]};
+      store_run4<kOut>(reinterpret_cast<char*>(p.d) + row * p.ldd * kElem, col, N - col, p.vec, v);
+    }
+  }
+}
+
+// ---- host side ----
+
+struct Fp8Plan {
+  int tile, splits, split_kb;
+};
+
+// Tile rows and K slices. A round of workgroups takes the time of one slice: its stages, and a fixed part (first
+// loads, epilogue) worth about eight of them at 256 rows; 128 rows halve the stage but not the fixed part. Slices also
+// write and read their float32 sums.
+static Fp8Plan plan_fp8(int64_t M, int64_t N, int64_t kb, int cus) {
+  Fp8Plan best = {256, 1, (int)((kb + 3) / 4 * 4)};
+  double best_cost = 1e300;
+  for (int tile = 256; tile >= 128; tile /= 2) {
+    const int64_t tiles = (M + tile - 1) / tile * ((N + kTileN - 1) / kTileN);
+    for (int64_t s = 1; s <= 32; ++s) {
+      const int64_t per = ((kb + s - 1) / s + 3) / 4 * 4, splits = (kb + per - 1) / per;
+      if (splits != s || (s > 1 && tiles * s > 4 * cus)) continue;
+      const double rounds = (double)((tiles * s + cus - 1) / cus);
+      const double stages = (double)(per < kb ? per : kb);
+      double cost = rounds * (stages * (tile == 256 ? 1.0 : 0.56) + 8.0);
+      if (s > 1) cost += 6.0 + (double)(M * N) * (double)(s + 1) / 2.0e6;  // the join: its launch and its traffic
+      if (cost < best_cost) {
+        best_cost = cost;
+        best = {tile, (int)s, (int)per};
+      }
+    }
+  }
+  return best;
+}
+
+}  // namespace mxq
+
+using namespace mxq;
+
+static bool aligned(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+
+template <int kTM, int kOut, bool kSplit, bool kWide>
+static int launch_gemm(const Fp8Gemm& p, void* stream) {
+  hipLaunchKernelGGL((gemm_fp8_kernel<kTM, kOut, kSplit, kWide>), dim3((unsigned)(p.tiles_m * p.tiles_n * p.splits)), dim3(512),
+                     0, (hipStream_t)stream, p);
+  return mxq_check_launch("gemm_fp8_kernel");
+}
+
+static int64_t split_bytes(const Fp8Plan& plan, int64_t M, int64_t N) {
+  return plan.splits > 1 ? plan.splits * M * ((N + 3) / 4 * 4) * 4 : 0;
+}
+
+static int check_product(int64_t M, int64_t N, int64_t K, int64_t ldb, int64_t ldsb, int64_t ldd, int out_dtype) {
+  if (!float_dtype(out_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported output dtype code %d", out_dtype);
+  if (M < 0 || N < 1 || K < 1 || M > (1ll << 31) - 1024 || N > (1ll << 31) - 1024 || K > (1ll << 22))
+    return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
+  const int64_t kb = (K + 127) / 128;
+  if (ldb < kb * 128 || ldb % 16 || ldb > (1ll << 22) + 4096 || ldsb < (kb + 3) / 4 * 4 || ldsb % 4 || ldsb > (1ll << 20) ||
+      ldd < N)
+    return mxq_set_error(MXQ_ERR_INVALID, "bad row strides of the weight or the output for N=%lld K=%lld", (long long)N,
+                         (long long)K);
+  return MXQ_OK;
+}
+
+extern "C" int mxq_fp8_gemm_workspace(int64_t M, int64_t N, int64_t K, int64_t* bytes) {
+  if (M < 0 || N < 1 || K < 1 || !bytes) return mxq_set_error(MXQ_ERR_INVALID, "bad argument");
+  *bytes = M == 0 ? 0 : split_bytes(plan_fp8(M, N, (K + 127) / 128, mxq_cu_count()), M, N);
+  return MXQ_OK;
+}
+
+extern "C" int mxq_fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa, const uint8_t* b, int64_t ldb,
+                            const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd, int out_dtype,
+                            int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (const int rc = check_product(M, N, K, ldb, ldsb, ldd, out_dtype)) return rc;
+  const int64_t kb = (K + 127) / 128;
+  if (lda < kb * 128 || lda % 16 || lda > (1ll << 22) + 4096 || ldsa < (kb + 3) / 4 * 4 || ldsa % 4 || ldsa > (1ll << 20))
+    return mxq_set_error(MXQ_ERR_INVALID, "bad row strides of the activations for K=%lld", (long long)K);
+  if (M == 0) return MXQ_OK;
+  if (!a || !sa || !b || !sb || !d || !aligned(a, 16) || !aligned(b, 16) || !aligned(sa, 4) || !aligned(sb, 4))
+    return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
+  const Fp8Plan plan = plan_fp8(M, N, kb, mxq_cu_count());
+  const int64_t tiles_m = (M + plan.tile - 1) / plan.tile, tiles_n = (N + kTileN - 1) / kTileN;
+  if (tiles_m * tiles_n * plan.splits >= (1ll << 31)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^31 tiles");
+  const int64_t need = split_bytes(plan, M, N);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return mxq_set_error(MXQ_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  Fp8Gemm p = {a, b, sa, sb, bias, d, M, N, lda, ldb, ldsa, ldsb, ldd, (int)kb, (int)tiles_m, (int)tiles_n, plan.splits,
+               plan.split_kb, 0};
+  const bool wide = out_dtype == MXQ_DTYPE_F32;
+  if (plan.splits > 1) {
+    const int64_t ldp = (N + 3) / 4 * 4;
+    p.d = workspace;
+    p.ldd = ldp;
+    p.vec = 1;
+    p.bias = nullptr;
+    int rc;
+    if (plan.tile == 256)
+      rc = wide ? launch_gemm<256, 0, true, true>(p, stream) : launch_gemm<256, 0, true, false>(p, stream);
+    else
+      rc = wide ? launch_gemm<128, 0, true, true>(p, stream) : launch_gemm<128, 0, true, false>(p, stream);
+    if (rc) return rc;
+    const int64_t blocks = (M * (ldp / 4) + 255) / 256;
+    if (blocks >= (1ll << 31)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "output too large");
+    with_dtype(out_dtype, [&](auto O) {
+      constexpr int kOut = decltype(O)::value;
+      const int vec = aligned(d, kOut == MXQ_DTYPE_F32 ? 16 : 8) && ldd % 4 == 0;
+      hipLaunchKernelGGL((fp8_join_kernel<kOut>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream,
+                         (const float*)workspace, plan.splits, M, N, ldp, bias, (char*)d, ldd, vec);
+    });
+    return mxq_check_launch("fp8_join_kernel");
+  }
+  p.vec = aligned(d, 16) && ldd * dtype_bytes(out_dtype) % 16 == 0;
+  return with_dtype(out_dtype, [&](auto O) {
+    constexpr int kOut = decltype(O)::value;
+    constexpr bool kWide = kOut == MXQ_DTYPE_F32;
+    return plan.tile == 256 ? launch_gemm<256, kOut, false, kWide>(p, stream) : launch_gemm<128, kOut, false, kWide>(p, stream);
+  });
+}
+
+template <int kIn, int kOut, int kMT, bool kFused>
+static void launch_rows(const Fp8Rows& p, void* stream) {
+  // 32 weight rows per workgroup where that leaves four workgroups per CU
+  const int64_t wide = (p.N + 31) / 32;
+  if (wide >= 2 * mxq_cu_count() || kMT > 1)
+    hipLaunchKernelGGL((fp8_rows_kernel<kIn, kOut, kMT, 2, kFused>), dim3((unsigned)wide), dim3(256), 0, (hipStream_t)stream, p);
+  else
+    hipLaunchKernelGGL((fp8_rows_kernel<kIn, kOut, kMT, 1, kFused>), dim3((unsigned)((p.N + 15) / 16)), dim3(256), 0,
+                       (hipStream_t)stream, p);
+}
+
+extern "C" int mxq_fp8_linear_rows(const void* x, int x_dtype, int64_t ldx, const uint8_t* sx, int64_t ldsx, const uint8_t* b,
+                                   int64_t ldb, const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd,
+                                   int out_dtype, int64_t M, int64_t N, int64_t K, void* stream) {
+  if (const int rc = check_product(M, N, K, ldb, ldsb, ldd, out_dtype)) return rc;
+  const bool fused = x_dtype != MXQ_DTYPE_E4M3;
+  const int64_t kb = (K + 127) / 128;
+  if (fused && !float_dtype(x_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported input dtype code %d", x_dtype);
+  if (M > (fused ? 16 : 64)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "%lld rows", (long long)M);
+  if (fused ? (ldx < K || ldx * dtype_bytes(x_dtype) % 16 || K % 8)
+            : (ldx < kb * 128 || ldx % 16 || ldsx < kb))
+    return mxq_set_error(MXQ_ERR_INVALID, "bad row strides of the activations for K=%lld", (long long)K);
+  if (M == 0) return MXQ_OK;
+  if (!x || !b || !sb || !d || (!fused && !sx) || !aligned(x, 16) || !aligned(b, 16))
+    return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
+  const Fp8Rows p = {x, sx, b, sb, bias, d, M, N, K, ldx, ldsx, ldb, ldsb, ldd, (int)kb,
+                     aligned(d, 4 * dtype_bytes(out_dtype)) && ldd % 4 == 0};
+  with_dtype(out_dtype, [&](auto O) {
+    constexpr int kOut = decltype(O)::value;
+    if (fused) {
+      with_dtype(x_dtype, [&](auto X) { launch_rows<decltype(X)::value, kOut, 1, true>(p, stream); });
+    } else if (M <= 16) {
+      launch_rows<MXQ_DTYPE_BF16, kOut, 1, false>(p, stream);
+    } else if (M <= 32) {
+      launch_rows<MXQ_DTYPE_BF16, kOut, 2, false>(p, stream);
+    } else {
+      launch_rows<MXQ_DTYPE_BF16, kOut, 4, false>(p, stream);
+    }
+  });
+  return mxq_check_launch("fp8_rows_kernel");
+}

@@ -41,6 +41,14 @@ from .ops import (  # noqa: F401
     prepare_w4a8_grouped,
     w4a8_int8_linear,
 )
+from .fp8 import (  # noqa: F401
+    PreparedFp8Weight,
+    dequantize_fp8_block128,
+    fp8_linear,
+    fp8_linear_prequantized,
+    prepare_fp8_weight,
+    quantize_fp8_block128,
+)
 from .checkpoint import (  # noqa: F401
     MappingTensorSource,
     SafeTensorSource,

@@ -71,6 +71,15 @@ SIGNATURES: dict[str, list] = {
     "mxq_probe_lane_exchange": [_P, _P, _P, _P, _P],
     "mxq_w4a8_quantize_weight": [_P, _I, _I64, _I64, _I64, _I64, _I, _P, _I, _P, _P, _P, _P, _P, _P],
     "mxq_int8_group_sums": [_P, _P, _P, _I64, _I64, _I64, _I, _P],
+    "mxq_fp8_quantize_rows": [_P, _I, _I64, _P, _I64, _P, _I64, _I64, _I64, _P],
+    "mxq_fp8_dequantize_rows": [_P, _I64, _P, _I64, _P, _I, _I64, _I64, _P],
+    "mxq_fp8_quantize_tiles": [_P, _I, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _P],
+    "mxq_fp8_gemm_workspace": [_I64, _I64, _I64, _P],
+    "mxq_fp8_gemm": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I, _I64, _I64, _I64, _P, _I64, _P],
+    "mxq_fp8_linear_rows": [_P, _I, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I, _I64, _I64, _I64, _P],
+    "mxq_fp8_grad_strips": [_I64, _I64, _P],
+    "mxq_fp8_grad_pass": [_P, _I, _I64, _P, _I64, _P, _I64, _P, _I, _I64, _P, _I64, _I64, _I64, _P],
+    "mxq_column_join": [_P, _I64, _I64, _P, _I, _P],
 }
 
 _lib = None

@@ -546,6 +546,38 @@ int mxq_fp8_grad_pass(const void* dy, int dy_dtype, int64_t ldy, uint8_t* q, int
 /* out [n] = column sums of in [parts, n] (fp32), in a fixed order. */
 int mxq_column_join(const float* in, int64_t parts, int64_t n, void* out, int out_dtype, void* stream);
 
+/* Bytes of workspace mxq_fp8_wgrad needs at this size on the current device (0: none). */
+int mxq_fp8_wgrad_workspace(int64_t M, int64_t N, int64_t K, int parts, int64_t* bytes);
+
+/*
+ * The weight's gradient dw [N, K] (contiguous, out_dtype) = sum over parts and rows m of dy[m, n] x[m, k]: dy bfloat16
+ * [parts, M, ldy] (ldy a multiple of 8 and at least N rounded up to 16; what lies behind column N is not used), x the
+ * values of codes [M, ldq] (ldq a multiple of 16, at least K rounded up to 16) and scales [M, lds]. Sums are float32.
+ */
+int mxq_fp8_wgrad(const void* dy, int parts, int64_t ldy, const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds,
+                  void* dw, int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                  void* stream);
+
+/*
+ * Layer norm of rows: y [M, D] (contiguous) = (x - mean) * rstd * w + b, rstd = 1 / sqrt(variance + eps), in float32,
+ * rounded once; x [M, ldx] and y of dtype, w and b [D] of param_dtype or NULL (1 and 0); mean and rstd fp32 [M] or NULL.
+ * D <= 24576. The norm under CK/backends/eager/adaln.py:11-14, with a learned weight.
+ */
+int mxq_layer_norm(const void* x, int dtype, int64_t ldx, const void* w, const void* b, int param_dtype, float eps, void* y,
+                   float* mean, float* rstd, int64_t M, int64_t D, void* stream);
+
+/* Row strips of mxq_layer_norm_backward at this size on the current device. */
+int mxq_layer_norm_backward_strips(int64_t M, int64_t D, int64_t* strips);
+
+/*
+ * Its gradients: dx [M, D] (contiguous, dtype) from dy [M, ldy] of dtype, x [M, ldx] of dtype, or codes with x_dtype
+ * MXQ_DTYPE_E4M3 and scales [M, ldxs], and the forward's mean and rstd. sums fp32 [strips, 2, D] (NULL: none) receives
+ * the strips' sums of dy * xh and of dy, whose column sums (mxq_column_join) are the weight's and the bias's gradients.
+ */
+int mxq_layer_norm_backward(const void* dy, int dtype, int64_t ldy, const void* x, int x_dtype, int64_t ldx,
+                            const uint8_t* x_scale, int64_t ldxs, const float* mean, const float* rstd, const void* w,
+                            int param_dtype, void* dx, float* sums, int64_t strips, int64_t M, int64_t D, void* stream);
+
 /*
  * Measurement helper (no counterpart in the reference; it calibrates the roofline): runs
  * `workgroups` x 256 threads, each lane cycling eight v_mfma_i32_32x32x32_i8 accumulators over

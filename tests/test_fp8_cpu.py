@@ -117,3 +117,66 @@ def test_c_entries_refuse_before_any_launch():
     # no rows: nothing to do, no pointer needed
     _call("mxq_fp8_quantize_rows", None, 0, 256, None, 256, None, 4, 0, 256)
     _call("mxq_fp8_gemm", None, 256, None, 4, None, 256, None, 4, None, None, 128, 2, 0, 128, 256, None, 0)
+
+
+def test_gradient_arguments_are_checked():
+    mx = _mx()
+    q, s = torch.zeros(4, 256).to(torch.float8_e4m3fn), torch.ones(4, 2).to(torch.float8_e8m0fnu)
+    p = mx.PreparedFp8Weight(q, s, None, None, 8, 256)
+    with pytest.raises(ValueError, match="transposed"):
+        mx.fp8_linear_backward(torch.zeros(4, 8), q, s, p)
+    with pytest.raises(ValueError, match="gradient of shape"):
+        mx.fp8_linear_backward(torch.zeros(4, 9), q, s, p)
+    with pytest.raises(ValueError, match="gradient dtype"):
+        mx.fp8_linear_backward(torch.zeros(4, 8, dtype=torch.int32), q, s, p)
+    with pytest.raises(ValueError, match="output dtype"):
+        mx.fp8_linear_backward(torch.zeros(4, 8), q, s, p, grad_dtype=torch.int8)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        mx.fp8_linear_backward(torch.zeros(4, 8), q, s, p, (False, True, True))
+    x, stat = torch.zeros(4, 256), torch.zeros(4)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        mx.layer_norm(x)
+    with pytest.raises(ValueError, match="eps"):
+        mx.layer_norm(x, eps=-1.0)
+    with pytest.raises(ValueError, match="non-empty"):
+        mx.layer_norm(x[:, :0])
+    with pytest.raises(ValueError, match="input dtype"):
+        mx.layer_norm(x.int())
+    with pytest.raises(ValueError, match="input of"):
+        mx.layer_norm_backward(x, x.bfloat16(), stat, stat)
+    with pytest.raises(ValueError, match="input of shape"):
+        mx.layer_norm_backward(x, (q[:, :128], s[:, :1]), stat, stat)
+    with pytest.raises(ValueError, match="mean"):
+        mx.layer_norm_backward(x, x, stat[:3], stat)
+    with pytest.raises(ValueError, match="rstd"):
+        mx.layer_norm_backward(x, x, stat, stat.double())
+    with pytest.raises(ValueError, match="input features"):
+        mx.Fp8Linear(128, 8)(x)
+    with pytest.raises(ValueError, match="features"):
+        mx.LayerNorm(128)(x)
+
+
+def test_c_gradient_entries_refuse_before_any_launch():
+    from mx_qlinear import _lib
+
+    ok = 1 << 20
+    for args in ((ok, 0, 256, ok, 256, ok, 2, ok, 0, 8, 256, 256), (ok, 1, 250, ok, 256, ok, 2, ok, 0, 8, 250, 256),
+                 (ok, 1, 256, ok, 248, ok, 2, ok, 0, 8, 256, 248), (ok, 1, 256, ok, 256, ok, 1, ok, 0, 8, 256, 256),
+                 (ok + 2, 1, 256, ok, 256, ok, 2, ok, 0, 8, 256, 256), (ok, 1, 256, ok, 256, ok, 2, ok, 5, 8, 256, 256)):
+        with pytest.raises(ValueError):
+            _call("mxq_fp8_wgrad", *args, None, 0)
+    need = ctypes.c_int64()
+    _lib.call("mxq_fp8_wgrad_workspace", 65536, 256, 256, 1, ctypes.byref(need))
+    assert need.value > 0
+    with pytest.raises(ValueError, match="workspace"):
+        _call("mxq_fp8_wgrad", ok, 1, 256, ok, 256, ok, 2, ok, 0, 65536, 256, 256, None, 0)
+    with pytest.raises(_lib.MxqError, match="24576"):
+        _call("mxq_layer_norm", ok, 2, 24577, None, None, 2, 1e-5, ok, None, None, 4, 24577)
+    with pytest.raises(ValueError):
+        _call("mxq_layer_norm", ok, 2, 127, None, None, 2, 1e-5, ok, None, None, 4, 128)
+    with pytest.raises(ValueError, match="strips"):
+        _call("mxq_layer_norm_backward", ok, 2, 128, ok, 2, 128, None, 0, ok, ok, None, 2, ok, ok, 9999, 4, 128)
+    with pytest.raises(ValueError, match="dtype code"):
+        _call("mxq_layer_norm_backward", ok, 2, 128, ok, 0, 128, None, 0, ok, ok, None, 2, ok, None, 0, 4, 128)
+    with pytest.raises(ValueError, match="null"):
+        _call("mxq_layer_norm_backward", ok, 2, 128, ok, 5, 128, None, 1, ok, ok, None, 2, ok, None, 0, 4, 128)

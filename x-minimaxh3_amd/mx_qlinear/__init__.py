@@ -42,10 +42,15 @@ from .ops import (  # noqa: F401
     w4a8_int8_linear,
 )
 from .fp8 import (  # noqa: F401
+    Fp8Linear,
+    LayerNorm,
     PreparedFp8Weight,
     dequantize_fp8_block128,
     fp8_linear,
+    fp8_linear_backward,
     fp8_linear_prequantized,
+    layer_norm,
+    layer_norm_backward,
     prepare_fp8_weight,
     quantize_fp8_block128,
 )

@@ -80,6 +80,11 @@ SIGNATURES: dict[str, list] = {
     "mxq_fp8_grad_strips": [_I64, _I64, _P],
     "mxq_fp8_grad_pass": [_P, _I, _I64, _P, _I64, _P, _I64, _P, _I, _I64, _P, _I64, _I64, _I64, _P],
     "mxq_column_join": [_P, _I64, _I64, _P, _I, _P],
+    "mxq_fp8_wgrad_workspace": [_I64, _I64, _I64, _I, _P],
+    "mxq_fp8_wgrad": [_P, _I, _I64, _P, _I64, _P, _I64, _P, _I, _I64, _I64, _I64, _P, _I64, _P],
+    "mxq_layer_norm": [_P, _I, _I64, _P, _P, _I, _F, _P, _P, _P, _I64, _I64, _P],
+    "mxq_layer_norm_backward_strips": [_I64, _I64, _P],
+    "mxq_layer_norm_backward": [_P, _I, _I64, _P, _I, _I64, _P, _I64, _P, _P, _P, _I, _P, _P, _I64, _I64, _I64, _P],
 }
 
 _lib = None

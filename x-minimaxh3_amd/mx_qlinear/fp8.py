@@ -270,3 +270,309 @@ def fp8_linear_prequantized(q: torch.Tensor, scale: torch.Tensor, weight: Prepar
         q, scale = _operand(q, scale, k)
     out = _product(dev, q, scale, m, k, weight.q, weight.scale, n, bias, out_dtype)
     return out if len(shape) == 2 else out.reshape(*shape[:-1], n)
+
+
+# ---------------------------------------------------------------------------------------
+# gradients
+# ---------------------------------------------------------------------------------------
+
+@functools.lru_cache(maxsize=4096)
+def _wgrad_bytes(m: int, n: int, k: int, parts: int, index: int) -> int:
+    out = ctypes.c_int64()
+    with torch.cuda.device(index):
+        _lib.call("mxq_fp8_wgrad_workspace", m, n, k, parts, ctypes.byref(out))
+    return out.value
+
+
+@functools.lru_cache(maxsize=4096)
+def _strips(name: str, m: int, n: int, index: int) -> int:
+    out = ctypes.c_int64()
+    with torch.cuda.device(index):
+        _lib.call(name, m, n, ctypes.byref(out))
+    return out.value
+
+
+def _column_join(dev, sums: torch.Tensor, n: int, dtype: torch.dtype) -> torch.Tensor:
+    out = torch.empty(n, dtype=dtype, device=dev)
+    _launch(dev, "mxq_column_join", sums.data_ptr(), sums.shape[0], n, out.data_ptr(), _OUT_CODES[dtype])
+    return out
+
+
+def _readable(t: torch.Tensor, width: int) -> bool:
+    """Whether every row of ``t`` (1-byte elements) can be read ``width`` wide from 16-byte boundaries."""
+    m, ld = t.shape[0], t.stride(0)
+    if t.data_ptr() % 16 or (m > 1 and (ld % 16 or ld < width)):
+        return False
+    return t.untyped_storage().nbytes() - t.storage_offset() >= (m - 1) * ld + width
+
+
+_PARTS = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}
+
+
+def fp8_linear_backward(dy: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, weight: PreparedFp8Weight,
+                        needs: tuple[bool, bool, bool] = (True, True, True), grad_dtype: torch.dtype = torch.float32):
+    """Gradients ``(dx, dweight, dbias)`` of :func:`fp8_linear` from the output's gradient ``dy [..., N]``, the input as it
+    was kept in 8 bits (the pair ``q [..., K]``, ``scale``) and the prepared weight; ``needs`` says which (``None`` for the
+    others). The quantizers pass gradients through unchanged.
+
+    ``dx = dY^ W^`` in ``dy``'s dtype, ``dY^`` being ``dy`` quantized as an activation is; ``dweight = dy^T X^`` and
+    ``dbias = sum dy`` in ``grad_dtype``, from ``dy`` itself: with float32 sums of exact products where ``dy`` is bf16,
+    fp16 or (to 24 bits) fp32, which go through the matrix instructions as one, two or three bfloat16 parts.
+    """
+    shape = q.shape
+    q, scale, m, k = _pair(q, scale)
+    _check_weight(weight, k)
+    code = _float_code(dy, "gradient")
+    gcode = _out_code(grad_dtype)
+    n = weight.out_features
+    if tuple(dy.shape) != (*shape[:-1], n):
+        raise ValueError(f"gradient of shape {tuple(dy.shape)}, expected {(*shape[:-1], n)}")
+    want_x, want_w, want_b = needs
+    if want_x and weight.qt is None:
+        raise ValueError("the input's gradient needs the transposed weight (prepare_fp8_weight(..., transposed=True))")
+    dev = _require_gpu(dy, q, scale, weight.q)
+    y = _rows_in_place(dy, n)
+    ldy = y.stride(0) if m > 1 else max(y.stride(0), n)
+    nb = -(-n // BLOCK)
+    parts, n_parts = None, 0
+    if want_w and m and not (dy.dtype == torch.bfloat16 and n % 16 == 0 and y.data_ptr() % 16 == 0 and ldy % 8 == 0):
+        n_parts = _PARTS[dy.dtype]
+        parts = torch.empty((n_parts, m, nb * BLOCK), dtype=torch.bfloat16, device=dev)
+    yq = ys = None
+    if want_x:
+        yq, ys = _new_pair(m, n, dev)
+    strips = _strips("mxq_fp8_grad_strips", m, n, dev.index) if want_b else 0
+    sums = torch.empty((strips, n), dtype=torch.float32, device=dev) if want_b else None
+    if m and (want_x or want_b or n_parts):
+        _launch(dev, "mxq_fp8_grad_pass", y.data_ptr(), code, ldy, _ptr(yq), nb * BLOCK, _ptr(ys), ys.shape[1] if want_x else 0,
+                _ptr(parts), n_parts, nb * BLOCK, _ptr(sums), strips, m, n)
+    dx = dw = db = None
+    if want_x:
+        dx = _product(dev, yq, ys, m, n, weight.qt, weight.scale_t, k, None, dy.dtype).reshape(shape)
+    if want_w:
+        if m and not _readable(q, _ceil(k, 16)):
+            q = _pad(q, _ceil(k, BLOCK))
+        need = _wgrad_bytes(m, n, k, n_parts or 1, dev.index)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        dw = torch.empty((n, k), dtype=grad_dtype, device=dev)
+        src, ld = (parts, nb * BLOCK) if n_parts else (y, ldy)
+        _launch(dev, "mxq_fp8_wgrad", src.data_ptr(), n_parts or 1, max(ld, _ceil(n, 16)), q.data_ptr(),
+                q.stride(0) if m > 1 else _ceil(k, 16), scale.data_ptr(), max(scale.stride(0), scale.shape[1]), dw.data_ptr(), gcode, m, n, k,
+                _ptr(ws), need)
+    if want_b:
+        db = _column_join(dev, sums, n, grad_dtype)
+    return dx, dw, db
+
+
+# ---------------------------------------------------------------------------------------
+# layer norm
+# ---------------------------------------------------------------------------------------
+
+def _norm_params(d: int, dev, dtype, weight, bias):
+    """Weight and bias as the kernels read them: both of x's dtype or both float32."""
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.numel() != d or t.dim() != 1):
+            raise ValueError(f"layer norm {name} of shape {tuple(t.shape)}, expected ({d},)")
+    given = [t for t in (weight, bias) if t is not None]
+    target = dtype if all(t.dtype == dtype for t in given) else torch.float32
+    out = [None if t is None else t.detach().to(device=dev, dtype=target).contiguous() for t in (weight, bias)]
+    return out[0], out[1], _OUT_CODES[target]
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
+               return_stats: bool = False):
+    """``(x - mean) * rstd * weight + bias`` over the last dimension (at most 24576), in float32 and rounded once to ``x``'s
+    dtype. ``return_stats`` adds the rows' float32 ``mean`` and ``rstd``, which :func:`layer_norm_backward` takes."""
+    code = _float_code(x, "input")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError("layer_norm needs a non-empty last dimension")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    dev = _require_gpu(x, weight, bias)
+    d = x.shape[-1]
+    w, b, pcode = _norm_params(d, dev, x.dtype, weight, bias)
+    x2 = _rows_in_place(x, d)
+    m = x2.shape[0]
+    y = torch.empty((m, d), dtype=x.dtype, device=dev)
+    mean = torch.empty(m, dtype=torch.float32, device=dev) if return_stats else None
+    rstd = torch.empty(m, dtype=torch.float32, device=dev) if return_stats else None
+    if m:
+        _launch(dev, "mxq_layer_norm", x2.data_ptr(), code, x2.stride(0) if m > 1 else max(x2.stride(0), d), _ptr(w), _ptr(b), pcode,
+                float(eps), y.data_ptr(), _ptr(mean), _ptr(rstd), m, d)
+    y = y if x.dim() == 2 else y.reshape(x.shape)
+    if not return_stats:
+        return y
+    if x.dim() != 2:
+        mean, rstd = mean.reshape(x.shape[:-1]), rstd.reshape(x.shape[:-1])
+    return y, mean, rstd
+
+
+def layer_norm_backward(dy: torch.Tensor, x, mean: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor | None = None,
+                        needs_params: bool = True):
+    """Gradients ``(dx, dweight, dbias)`` of :func:`layer_norm`: ``dx`` in ``dy``'s dtype, the other two in float32 (``None``
+    without ``needs_params``). ``x`` is the forward's input, or that input as it was kept in 8 bits, a ``(codes, scale)``
+    pair of :func:`quantize_fp8_block128`; ``mean`` and ``rstd`` are the forward's."""
+    code = _float_code(dy, "gradient")
+    if dy.dim() < 1 or dy.shape[-1] == 0:
+        raise ValueError("layer_norm_backward needs a non-empty last dimension")
+    d = dy.shape[-1]
+    if isinstance(x, (tuple, list)):
+        if tuple(x[0].shape) != tuple(dy.shape):
+            raise ValueError(f"input of shape {tuple(x[0].shape)} for a gradient of shape {tuple(dy.shape)}")
+        x2, xs, _, _ = _pair(*x)
+        xcode, ldxs = _lib.DTYPE_E4M3, max(xs.stride(0), xs.shape[1])
+    else:
+        if tuple(x.shape) != tuple(dy.shape):
+            raise ValueError(f"input of shape {tuple(x.shape)} for a gradient of shape {tuple(dy.shape)}")
+        if x.dtype != dy.dtype:
+            raise ValueError(f"input of {x.dtype} for a gradient of {dy.dtype}")
+        x2, xs, xcode, ldxs = _rows_in_place(x, d), None, code, 0
+    y2 = _rows_in_place(dy, d)
+    m = y2.shape[0]
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        if t.dtype != torch.float32 or t.numel() != m:
+            raise ValueError(f"{name} must be float32 with one entry per row ({m}), got {t.dtype} {tuple(t.shape)}")
+    dev = _require_gpu(dy, x2, xs, mean, rstd, weight)
+    w, _, pcode = _norm_params(d, dev, dy.dtype, weight, None)
+    dx = torch.empty((m, d), dtype=dy.dtype, device=dev)
+    strips = _strips("mxq_layer_norm_backward_strips", m, d, dev.index) if needs_params else 0
+    sums = torch.empty((strips, 2 * d), dtype=torch.float32, device=dev) if needs_params else None
+    if m:
+        mean, rstd = mean.contiguous(), rstd.contiguous()
+        _launch(dev, "mxq_layer_norm_backward", y2.data_ptr(), code, max(y2.stride(0), d), x2.data_ptr(), xcode, max(x2.stride(0), d),
+                _ptr(xs), ldxs, mean.data_ptr(), rstd.data_ptr(), _ptr(w), pcode, dx.data_ptr(), _ptr(sums), strips, m, d)
+    dx = dx if dy.dim() == 2 else dx.reshape(dy.shape)
+    if not needs_params:
+        return dx, None, None
+    both = _column_join(dev, sums, 2 * d, torch.float32)
+    return dx, both[:d], both[d:]
+
+
+# ---------------------------------------------------------------------------------------
+# modules
+# ---------------------------------------------------------------------------------------
+
+def _refuse_capture(device: torch.device) -> None:
+    """Autograd keeps one accumulation node per parameter, bound to the stream of its first use, for as long as any graph
+    holds it: a backward pass captured while an eager graph of the same parameters lives would join that stream and
+    end the process. A training step is captured through the functions, which own no such nodes."""
+    with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the autograd modules are not captured into graphs; capture fp8_linear, fp8_linear_backward, "
+                               "layer_norm and layer_norm_backward instead")
+
+
+class _Fp8LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, prepared):
+        dev = _require_gpu(x, prepared.q, bias)
+        _refuse_capture(dev)
+        q, s, m, k = _quantize_rows(x)
+        n = prepared.out_features
+        y = _product(dev, q, s, m, k, prepared.q, prepared.scale, n, _bias(bias, n, x.dtype, dev), x.dtype)
+        # the input leaves the graph in 8 bits: only the pair is kept
+        ctx.save_for_backward(q, s, prepared.qt, prepared.scale_t)
+        ctx.sizes = (x.shape, n, k)
+        ctx.dtypes = (None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+        return y.reshape(*x.shape[:-1], n)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        _refuse_capture(dy.device)
+        q, s, qt, st = ctx.saved_tensors
+        shape, n, k = ctx.sizes
+        wdtype, bdtype = ctx.dtypes
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        weight = PreparedFp8Weight(q, s, qt, st, n, k)  # (the gradients read the transposed copy only)
+        m = q.shape[0]
+        dx, dw, db = fp8_linear_backward(dy.reshape(m, n), q[:, :k], s[:, : -(-k // BLOCK)], weight, (want_x, want_w, want_b),
+                                         wdtype or bdtype or torch.float32)
+        return (dx.reshape(shape) if want_x else None, dw, db.to(bdtype) if want_b else None, None)
+
+
+class Fp8Linear(torch.nn.Module):
+    """A linear layer computed in 8-bit floating point, for serving and for training.
+
+    ``weight`` ``[out_features, in_features]`` and ``bias`` are ordinary parameters (bf16, fp16 or fp32). Without gradients
+    the layer runs :func:`fp8_linear` on the weight's 8-bit form, built by :meth:`prepare` (and again after a load or an
+    update, by calling it again); with gradients the form is built from the parameter in every forward, and what the
+    backward pass keeps of the input is its 8-bit pair (:func:`fp8_linear_backward`). The quantizers pass gradients
+    through unchanged. Activations are bf16, fp16 or fp32.
+    """
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None):
+        super().__init__()
+        self.in_features, self.out_features = in_features, out_features
+        self.weight = torch.nn.Parameter(torch.empty(out_features, in_features, device=device, dtype=dtype))
+        self.bias = torch.nn.Parameter(torch.zeros(out_features, device=device, dtype=dtype)) if bias else None
+        torch.nn.init.normal_(self.weight, std=in_features**-0.5)
+        self._prepared: PreparedFp8Weight | None = None
+
+    def prepare(self) -> "Fp8Linear":
+        """Builds the weight's 8-bit form from its present contents, for calls without weight gradients."""
+        self._prepared = prepare_fp8_weight(self.weight)
+        return self
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.dim() < 1 or x.shape[-1] != self.in_features:
+            raise ValueError(f"input of shape {tuple(x.shape)} for a layer of {self.in_features} input features")
+        params = [p for p in (self.weight, self.bias) if p is not None]
+        if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, *params))):
+            if self._prepared is None:
+                self.prepare()
+            return fp8_linear(x, self._prepared, self.bias)
+        if self.weight.requires_grad or self._prepared is None or self._prepared.qt is None:
+            prepared = prepare_fp8_weight(self.weight)
+            if not self.weight.requires_grad:
+                self._prepared = prepared
+        else:
+            prepared = self._prepared
+        return _Fp8LinearFn.apply(x, self.weight, self.bias, prepared)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, keep_fp8):
+        _refuse_capture(x.device)
+        y, mean, rstd = layer_norm(x, weight, bias, eps, return_stats=True)
+        kept = quantize_fp8_block128(x) if keep_fp8 else (x,)
+        ctx.save_for_backward(mean, rstd, weight, *kept)
+        ctx.dtypes = tuple(None if t is None else t.dtype for t in (weight, bias))
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        _refuse_capture(dy.device)
+        mean, rstd, weight, *kept = ctx.saved_tensors
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        x = tuple(kept) if len(kept) == 2 else kept[0]
+        dx, dw, db = layer_norm_backward(dy, x, mean, rstd, weight, needs_params=want_w or want_b)
+        return (dx if want_x else None, dw.to(ctx.dtypes[0]) if want_w else None, db.to(ctx.dtypes[1]) if want_b else None,
+                None, None)
+
+
+class LayerNorm(torch.nn.Module):
+    """Layer norm over the last dimension (:func:`layer_norm`) with a learned weight and bias. ``keep_fp8`` keeps the input
+    for the backward pass in 8 bits instead of as it is."""
+
+    def __init__(self, features: int, eps: float = 1e-5, bias: bool = True, keep_fp8: bool = False, device=None, dtype=None):
+        super().__init__()
+        self.features, self.eps, self.keep_fp8 = features, eps, keep_fp8
+        self.weight = torch.nn.Parameter(torch.ones(features, device=device, dtype=dtype))
+        self.bias = torch.nn.Parameter(torch.zeros(features, device=device, dtype=dtype)) if bias else None
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.dim() < 1 or x.shape[-1] != self.features:
+            raise ValueError(f"input of shape {tuple(x.shape)} for a norm of {self.features} features")
+        params = [p for p in (self.weight, self.bias) if p is not None]
+        if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, *params))):
+            return layer_norm(x, self.weight, self.bias, self.eps)
+        return _LayerNormFn.apply(x, self.weight, self.bias, self.eps, self.keep_fp8)
+
+    def extra_repr(self) -> str:
+        return f"{self.features}, eps={self.eps}, bias={self.bias is not None}, keep_fp8={self.keep_fp8}"

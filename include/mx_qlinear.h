@@ -525,7 +525,7 @@ int mxq_fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa,
 
 /*
  * The same for few rows. x_dtype MXQ_DTYPE_E4M3: x holds codes, sx their scales, M <= 64. Otherwise x [M, ldx] is
- * quantized on the way, with the codes mxq_fp8_quantize_rows gives: M <= 16, K % 8 == 0, rows 16-byte aligned.
+ * quantized on the way, with the codes mxq_fp8_quantize_rows gives: M <= 16.
  */
 int mxq_fp8_linear_rows(const void* x, int x_dtype, int64_t ldx, const uint8_t* sx, int64_t ldsx, const uint8_t* b,
                         int64_t ldb, const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd, int out_dtype,

@@ -111,7 +111,7 @@ def test_c_entries_refuse_before_any_launch():
     with pytest.raises(_lib.MxqError, match="rows"):
         _call("mxq_fp8_linear_rows", ok, 2, 256, None, 0, ok, 256, ok, 4, None, ok, 128, 2, 17, 128, 256)
     with pytest.raises(ValueError, match="activations"):
-        _call("mxq_fp8_linear_rows", ok, 2, 260, None, 0, ok, 256, ok, 4, None, ok, 128, 2, 4, 128, 250)
+        _call("mxq_fp8_linear_rows", ok, 2, 249, None, 0, ok, 256, ok, 4, None, ok, 128, 2, 4, 128, 250)
     with pytest.raises(ValueError):
         _call("mxq_fp8_grad_pass", ok, 2, 256, ok, 256, ok, 4, ok, 2, 256, None, 0, 8, 256)
     # no rows: nothing to do, no pointer needed

@@ -18,6 +18,12 @@ typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 
+// 16 and 8 bytes from any address: one access, gfx950 splits it where it crosses a boundary. Rows of odd widths are read and
+// written through these: element by element they cost an access and a wait for each.
+typedef unsigned int v4u_any __attribute__((ext_vector_type(4), aligned(1)));
+typedef unsigned int v2u_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(1)));
+
 namespace mxq {
 
 constexpr int kFp8Block = 128;
@@ -44,34 +50,40 @@ MXQ_DEVICE Piece<kCode> piece_load_vec(const void* p) {
   Piece<kCode> r;
 #pragma unroll
   for (int i = 0; i < Piece<kCode>::kWords / 4; ++i) {
-    const v4u v = reinterpret_cast<const v4u*>(p)[i];
+    const v4u v = *reinterpret_cast<const v4u_any*>(reinterpret_cast<const char*>(p) + 16 * i);
 #pragma unroll
     for (int j = 0; j < 4; ++j) r.w[4 * i + j] = v[j];
   }
   return r;
 }
 
-// The first `n` elements one by one, zeros behind them.
+// The first `n` elements (1 to 15), zeros behind them: each load made, of the last element where there is none.
 template <int kCode>
 MXQ_DEVICE Piece<kCode> piece_load_some(const void* p, int n) {
   Piece<kCode> r;
   if constexpr (kCode == MXQ_DTYPE_F32) {
+    const uint32_t* s = reinterpret_cast<const uint32_t*>(p);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) r.w[i] = i < n ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
+    for (int i = 0; i < 16; ++i) r.w[i] = s[min(i, n - 1)];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r.w[i] = i < n ? r.w[i] : 0u;
   } else {
     const uint16_t* s = reinterpret_cast<const uint16_t*>(p);
+    uint32_t h[16];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      r.w[i] = (2 * i < n ? (uint32_t)s[2 * i] : 0u) | ((2 * i + 1 < n ? (uint32_t)s[2 * i + 1] : 0u) << 16);
+    for (int i = 0; i < 16; ++i) h[i] = s[min(i, n - 1)];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.w[i] = (2 * i < n ? h[2 * i] : 0u) | ((2 * i + 1 < n ? h[2 * i + 1] : 0u) << 16);
   }
   return r;
 }
 
-// `n` of 16 elements (n <= 0: none) from p; `vec`: p is 16-byte aligned.
+// `n` of 16 elements from p (n <= 0: zeros, nothing is read).
 template <int kCode>
-MXQ_DEVICE Piece<kCode> piece_load(const void* p, int n, bool vec) {
-  if (vec && n >= 16) return piece_load_vec<kCode>(p);
-  return piece_load_some<kCode>(p, n);
+MXQ_DEVICE Piece<kCode> piece_load(const void* p, int n) {
+  if (n >= 16) return piece_load_vec<kCode>(p);
+  if (n > 0) return piece_load_some<kCode>(p, n);
+  return Piece<kCode>{};
 }
 
 template <int kCode>
@@ -160,13 +172,13 @@ MXQ_DEVICE uint32_t max8(uint32_t v) {
   return max(v, lane_xor4(v));
 }
 
-// Stores 4 float values from column `col` on, as kCode; `n` of them are inside the row; `vec`: aligned to the run.
+// Stores 4 float values from column `col` on, as kCode; `n` of them are inside the row.
 template <int kCode>
-MXQ_DEVICE void store_run4(void* row, int64_t col, int n, bool vec, const float* y) {
+MXQ_DEVICE void store_run4(void* row, int64_t col, int n, const float* y) {
   if constexpr (kCode == MXQ_DTYPE_F32) {
     float* p = reinterpret_cast<float*>(row) + col;
-    if (vec && n >= 4) {
-      *reinterpret_cast<v4f*>(p) = v4f{y[0], y[1], y[2], y[3]};
+    if (n >= 4) {
+      *reinterpret_cast<v4f_any*>(p) = v4f{y[0], y[1], y[2], y[3]};
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -177,8 +189,8 @@ MXQ_DEVICE void store_run4(void* row, int64_t col, int n, bool vec, const float*
     uint32_t h[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) h[e] = kCode == MXQ_DTYPE_F16 ? f32_to_f16_bits(y[e]) : f32_to_bf16_bits(y[e]);
-    if (vec && n >= 4) {
-      *reinterpret_cast<v2u*>(p) = v2u{h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
+    if (n >= 4) {
+      *reinterpret_cast<v2u_any*>(p) = v2u{h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)

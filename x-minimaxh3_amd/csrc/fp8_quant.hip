@@ -17,8 +17,7 @@ constexpr int kRowUnroll = 4;
 
 template <int kCode>
 __global__ __launch_bounds__(256) void fp8_rows_quant_kernel(const char* x, int64_t ldx, uint8_t* q, int64_t ldq,
-                                                             uint8_t* s, int64_t lds, uint32_t M, uint32_t K, uint32_t kb,
-                                                             int vec) {
+                                                             uint8_t* s, int64_t lds, uint32_t M, uint32_t K, uint32_t kb) {
   constexpr int kElem = kCode == MXQ_DTYPE_F32 ? 4 : 2;
   const uint32_t total = M * kb;  // below 2^31 (checked by the launcher)
   const uint32_t piece = threadIdx.x & 7, first = blockIdx.x * (32 * kRowUnroll) + (threadIdx.x >> 3);
@@ -30,7 +29,7 @@ __global__ __launch_bounds__(256) void fp8_rows_quant_kernel(const char* x, int6
     row[u] = g / kb;
     b[u] = g - row[u] * kb;
     const uint32_t col = b[u] * 128 + piece * 16;
-    p[u] = piece_load<kCode>(x + ((int64_t)row[u] * ldx + col) * kElem, (int)K - (int)col, vec);
+    p[u] = piece_load<kCode>(x + ((int64_t)row[u] * ldx + col) * kElem, (int)K - (int)col);
   }
 #pragma unroll
   for (int u = 0; u < kRowUnroll; ++u) {
@@ -44,33 +43,61 @@ __global__ __launch_bounds__(256) void fp8_rows_quant_kernel(const char* x, int6
 }
 
 // ---- the way back ----
+// A lane takes the codes whose values fill one 16-byte store, so that a wave's stores are whole lines.
 template <int kCode>
 __global__ __launch_bounds__(256) void fp8_rows_dequant_kernel(const uint8_t* q, int64_t ldq, const uint8_t* s, int64_t lds,
-                                                               char* out, uint32_t M, uint32_t K, uint32_t pieces, int vec) {
-  constexpr int kElem = kCode == MXQ_DTYPE_F32 ? 4 : 2;
+                                                               char* out, uint32_t M, uint32_t K, uint32_t pieces) {
+  constexpr int kElem = kCode == MXQ_DTYPE_F32 ? 4 : 2, kCodes = 16 / kElem;
   const uint32_t total = M * pieces;
+  uint32_t c[kRowUnroll][2], row[kRowUnroll], col[kRowUnroll], sc[kRowUnroll];
 #pragma unroll
   for (int u = 0; u < kRowUnroll; ++u) {
-    const uint32_t g = blockIdx.x * (256 * kRowUnroll) + u * 256 + threadIdx.x;
-    if (g >= total) return;
-    const uint32_t row = g / pieces, col = (g - row * pieces) * 16;
-    const int n = min(16, (int)(K - col));
-    const uint8_t* src = q + (int64_t)row * ldq + col;
-    v4u c = {0, 0, 0, 0};
-    if ((vec & 1) && n == 16) {
-      c = *reinterpret_cast<const v4u*>(src);
+    const uint32_t g = min(blockIdx.x * (256 * kRowUnroll) + u * 256 + threadIdx.x, total - 1);
+    row[u] = g / pieces;
+    col[u] = (g - row[u] * pieces) * kCodes;
+    const int n = (int)(K - col[u]);
+    const uint8_t* src = q + (int64_t)row[u] * ldq + col[u];
+    sc[u] = s[(int64_t)row[u] * lds + (col[u] >> 7)];
+    c[u][0] = c[u][1] = 0;
+    if (n >= kCodes) {
+      if constexpr (kCodes == 8) {
+        const v2u v = *reinterpret_cast<const v2u_any*>(src);
+        c[u][0] = v[0];
+        c[u][1] = v[1];
+      } else {
+        __builtin_memcpy(&c[u][0], src, 4);
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (i < n) c[i >> 2] |= (uint32_t)src[i] << (8 * (i & 3));
+      for (int i = 0; i < kCodes; ++i) {
+        const uint32_t v = src[min(i, n - 1)];
+        c[u][i >> 2] |= (i < n ? v : 0u) << (8 * (i & 3));
+      }
     }
-    const float scale = fp8_scale_f32(s[(int64_t)row * lds + (col >> 7)]);
-    char* dst = out + (int64_t)row * K * kElem;
+  }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const v4f v = fp8x4_to_f32(c[j], scale);
+  for (int u = 0; u < kRowUnroll; ++u) {
+    if (blockIdx.x * (256 * kRowUnroll) + u * 256 + threadIdx.x >= total) return;
+    char* dst = out + ((int64_t)row[u] * K + col[u]) * kElem;
+    const int n = (int)(K - col[u]);
+    const float scale = fp8_scale_f32(sc[u]);
+    if constexpr (kCodes == 4) {
+      const v4f v = fp8x4_to_f32(c[u][0], scale);
       const float y[4] = {v[0], v[1], v[2], v[3]};
-      store_run4<kCode>(dst, col + 4 * j, n - 4 * j, vec & 2, y);
+      store_run4<kCode>(dst, 0, n, y);
+    } else {
+      const v4f v = fp8x4_to_f32(c[u][0], scale), w = fp8x4_to_f32(c[u][1], scale);
+      auto pair = [](float a, float b) {
+        return kCode == MXQ_DTYPE_F16 ? f32_to_f16_bits(a) | (f32_to_f16_bits(b) << 16) : pack_bf16x2(a, b);
+      };
+      const v4u o = {pair(v[0], v[1]), pair(v[2], v[3]), pair(w[0], w[1]), pair(w[2], w[3])};
+      if (n >= 8) {
+        *reinterpret_cast<v4u_any*>(dst) = o;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < n) reinterpret_cast<uint16_t*>(dst)[i] = (uint16_t)(o[i >> 1] >> (16 * (i & 1)));
+      }
     }
   }
 }
@@ -80,7 +107,7 @@ __global__ __launch_bounds__(256) void fp8_rows_dequant_kernel(const uint8_t* q,
 template <int kCode>
 __global__ __launch_bounds__(256) void fp8_tiles_quant_kernel(const char* w, int64_t ldw, uint8_t* q, int64_t ldq, uint8_t* s,
                                                               int64_t lds, uint8_t* qt, int64_t ldqt, uint8_t* st,
-                                                              int64_t ldst, int64_t N, int64_t K, int vec) {
+                                                              int64_t ldst, int64_t N, int64_t K) {
   constexpr int kElem = kCode == MXQ_DTYPE_F32 ? 4 : 2;
   __shared__ uint32_t wave_max[4];
   __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 132];  // rows of 132: a column's bytes spread over the banks
@@ -91,7 +118,7 @@ __global__ __launch_bounds__(256) void fp8_tiles_quant_kernel(const char* w, int
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t row = n0 + (t >> 3) + 32 * i;
-    p[i] = piece_load<kCode>(w + (min(row, N - 1) * ldw + col) * kElem, row < N ? (int)(K - col) : 0, vec);
+    p[i] = piece_load<kCode>(w + (min(row, N - 1) * ldw + col) * kElem, row < N ? (int)(K - col) : 0);
     m = max(m, piece_absmax(p[i]));
   }
   m = wave_max_u32(m);
@@ -150,7 +177,7 @@ __global__ __launch_bounds__(256) void fp8_tiles_quant_kernel(const char* w, int
 template <int kCode, int kParts>
 __global__ __launch_bounds__(256) void fp8_grad_pass_kernel(const char* x, int64_t ldx, uint8_t* q, int64_t ldq, uint8_t* s,
                                                             int64_t lds, uint16_t* parts, int64_t ldp, float* sums,
-                                                            int64_t M, int64_t N, int64_t nb, int64_t strip, int vec) {
+                                                            int64_t M, int64_t N, int64_t nb, int64_t strip) {
   constexpr int kElem = kCode == MXQ_DTYPE_F32 ? 4 : 2;
   __shared__ float part_sum[8][512];
   const int t = threadIdx.x, lane = t & 31, r = t >> 5;
@@ -160,7 +187,7 @@ __global__ __launch_bounds__(256) void fp8_grad_pass_kernel(const char* x, int64
   float acc[16] = {};
   for (int64_t row = first + r; row < last; row += 8) {
     const int n = in ? (int)(N - col) : 0;
-    const Piece<kCode> p = piece_load<kCode>(x + (row * ldx + (n > 0 ? col : 0)) * kElem, n, vec);
+    const Piece<kCode> p = piece_load<kCode>(x + (row * ldx + (n > 0 ? col : 0)) * kElem, n);
     if (sums) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[i] += piece_at(p, i);
@@ -252,11 +279,10 @@ extern "C" int mxq_fp8_quantize_rows(const void* x, int x_dtype, int64_t ldx, ui
   if (M == 0) return MXQ_OK;
   if (!x || !q || !scale || !aligned16(q)) return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
   if (M >= (1ll << 31) / kb - 65536 / kb - 1) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^31 blocks");
-  const int vec = aligned16(x) && ldx * dtype_bytes(x_dtype) % 16 == 0;
   const unsigned grid = (unsigned)((M * kb + 32 * kRowUnroll - 1) / (32 * kRowUnroll));
   with_dtype(x_dtype, [&](auto C) {
     hipLaunchKernelGGL((fp8_rows_quant_kernel<decltype(C)::value>), dim3(grid), dim3(256), 0, (hipStream_t)stream,
-                       (const char*)x, ldx, q, ldq, scale, lds, (uint32_t)M, (uint32_t)K, (uint32_t)kb, vec);
+                       (const char*)x, ldx, q, ldq, scale, lds, (uint32_t)M, (uint32_t)K, (uint32_t)kb);
   });
   return mxq_check_launch("fp8_rows_quant_kernel");
 }
@@ -270,15 +296,13 @@ extern "C" int mxq_fp8_dequantize_rows(const uint8_t* q, int64_t ldq, const uint
                          (long long)K);
   if (M == 0) return MXQ_OK;
   if (!q || !scale || !out) return mxq_set_error(MXQ_ERR_INVALID, "null pointer");
-  const int64_t pieces = (K + 15) / 16;
+  const int codes = 16 / dtype_bytes(out_dtype);
+  const int64_t pieces = (K + codes - 1) / codes;
   if (M >= (1ll << 31) / pieces - 65536 / pieces - 1) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^31 pieces");
-  const int run = 4 * dtype_bytes(out_dtype);
-  const int vec = (aligned16(q) && ldq % 16 == 0 ? 1 : 0) |
-                  (reinterpret_cast<uintptr_t>(out) % run == 0 && K % 4 == 0 ? 2 : 0);
   const unsigned grid = (unsigned)((M * pieces + 256 * kRowUnroll - 1) / (256 * kRowUnroll));
   with_dtype(out_dtype, [&](auto C) {
     hipLaunchKernelGGL((fp8_rows_dequant_kernel<decltype(C)::value>), dim3(grid), dim3(256), 0, (hipStream_t)stream, q, ldq,
-                       scale, lds, (char*)out, (uint32_t)M, (uint32_t)K, (uint32_t)pieces, vec);
+                       scale, lds, (char*)out, (uint32_t)M, (uint32_t)K, (uint32_t)pieces);
   });
   return mxq_check_launch("fp8_rows_dequant_kernel");
 }
@@ -294,10 +318,9 @@ extern "C" int mxq_fp8_quantize_tiles(const void* w, int w_dtype, int64_t ldw, u
   if (!w || !q || !scale || !aligned16(q) || (qt && (!scale_t || !aligned16(qt))))
     return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
   if (nb > 65535 || kb >= (1ll << 31)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 65535 tile rows");
-  const int vec = aligned16(w) && ldw * dtype_bytes(w_dtype) % 16 == 0;
   with_dtype(w_dtype, [&](auto C) {
     hipLaunchKernelGGL((fp8_tiles_quant_kernel<decltype(C)::value>), dim3((unsigned)kb, (unsigned)nb), dim3(256), 0,
-                       (hipStream_t)stream, (const char*)w, ldw, q, ldq, scale, lds, qt, ldqt, scale_t, ldst, N, K, vec);
+                       (hipStream_t)stream, (const char*)w, ldw, q, ldq, scale, lds, qt, ldqt, scale_t, ldst, N, K);
   });
   return mxq_check_launch("fp8_tiles_quant_kernel");
 }
@@ -335,17 +358,16 @@ extern "C" int mxq_fp8_grad_pass(const void* dy, int dy_dtype, int64_t ldy, uint
   if (sums && strips != (M + strip - 1) / strip)
     return mxq_set_error(MXQ_ERR_INVALID, "room for %lld strips, %lld needed", (long long)strips,
                          (long long)((M + strip - 1) / strip));
-  const int vec = aligned16(dy) && ldy * dtype_bytes(dy_dtype) % 16 == 0;
   const dim3 grid((unsigned)((N + 511) / 512), (unsigned)((M + strip - 1) / strip));
   with_dtype(dy_dtype, [&](auto C) {
     constexpr int kCode = decltype(C)::value;
     constexpr int kMost = kCode == MXQ_DTYPE_BF16 ? 1 : kCode == MXQ_DTYPE_F16 ? 2 : 3;
     if (n_parts)
       hipLaunchKernelGGL((fp8_grad_pass_kernel<kCode, kMost>), grid, dim3(256), 0, (hipStream_t)stream, (const char*)dy, ldy,
-                         q, ldq, scale, lds, (uint16_t*)parts, ldp, sums, M, N, nb, strip, vec);
+                         q, ldq, scale, lds, (uint16_t*)parts, ldp, sums, M, N, nb, strip);
     else
       hipLaunchKernelGGL((fp8_grad_pass_kernel<kCode, 0>), grid, dim3(256), 0, (hipStream_t)stream, (const char*)dy, ldy, q,
-                         ldq, scale, lds, (uint16_t*)nullptr, (int64_t)0, sums, M, N, nb, strip, vec);
+                         ldq, scale, lds, (uint16_t*)nullptr, (int64_t)0, sums, M, N, nb, strip);
   });
   return mxq_check_launch("fp8_grad_pass_kernel");
 }

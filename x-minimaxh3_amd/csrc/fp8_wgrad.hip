@@ -32,7 +32,6 @@ struct Wgrad {
   void* d;  // split: float32 sums, slice i at i * N * ldd
   int64_t M, N, K, ldy, part_stride, ldq, lds, ldd;
   int parts, tiles_n, tiles_k, splits, split_rows;  // split_rows: a multiple of kWRows
-  int vec;  // rows of d aligned to four elements
 };
 
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -54,7 +53,7 @@ MXQ_DEVICE uint32_t fragment_base(uint32_t operand, int c0, int lane) {
 }
 template <int kRow>
 MXQ_DEVICE v4s read_transposed(uint32_t base) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)((lds_ptr)base + kRow * 512));
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)((lds_ptr)(uintptr_t)base + kRow * 512));
 }
 MXQ_DEVICE v8bf join_fragment(const v4s (&f)[2]) {
   typedef short v8s __attribute__((ext_vector_type(8)));
@@ -131,7 +130,7 @@ __global__ __launch_bounds__(kWThreads, 1) void fp8_wgrad_kernel(Wgrad p) {
     v4u v = kP == 0 ? ya[j] : yb[j];
     if constexpr (kP >= 2)
       v = __builtin_bit_cast(v4u, fp8x8_to_bf16(xq[j][2 * kP - 4], xq[j][2 * kP - 3], fp8_scale_f32(xs[j])));
-    *(lds_v4u)((lds_ptr)(at ^ buf) + kOff) = v;
+    *(lds_v4u)((lds_ptr)(uintptr_t)(at ^ buf) + kOff) = v;
   };
   v16f acc[kWNB][4] = {};  // [n block][k block]
   // A stage is four half steps of 16 rows, a half step 4 kWNB slots, each one matrix instruction and a part of the other
@@ -216,7 +215,7 @@ __global__ __launch_bounds__(kWThreads, 1) void fp8_wgrad_kernel(Wgrad p) {
       for (int e = 0; e < 4; ++e) {
         const int k = k0 + wk + b * 32 + e * 8 + (lane >> 5) * 4;
         const float v[4] = {acc[a][b][4 * e], acc[a][b][4 * e + 1], acc[a][b][4 * e + 2], acc[a][b][4 * e + 3]};
-        store_run4<kOut>(d + (int64_t)n * p.ldd * kElem, k, K - k, p.vec, v);
+        store_run4<kOut>(d + (int64_t)n * p.ldd * kElem, k, K - k, v);
       }
   }
 }
@@ -224,7 +223,7 @@ __global__ __launch_bounds__(kWThreads, 1) void fp8_wgrad_kernel(Wgrad p) {
 // D = out(sum over slices), four columns per thread.
 template <int kOut>
 __global__ __launch_bounds__(256) void wgrad_join_kernel(const float* part, int splits, int64_t N, int64_t K, int64_t ldp,
-                                                         char* d, int vec) {
+                                                         char* d) {
   constexpr int kElem = kOut == MXQ_DTYPE_F32 ? 4 : 2;
   const int64_t runs = ldp / 4, g = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (g >= N * runs) return;
@@ -233,7 +232,7 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const float* part, int 
   v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int s = 0; s < splits; ++s) y += *reinterpret_cast<const v4f*>(part + (s * N + row) * ldp + col);
   const float v[4] = {y[0], y[1], y[2], y[3]};
-  store_run4<kOut>(d + row * K * kElem, col, (int)K - col, vec, v);
+  store_run4<kOut>(d + row * K * kElem, col, (int)K - col, v);
 }
 
 struct WgradPlan {
@@ -296,23 +295,20 @@ extern "C" int mxq_fp8_wgrad(const void* dy, int parts, int64_t ldy, const uint8
   const int64_t need = wgrad_bytes(plan, N, K);
   if (need > 0 && (!workspace || workspace_bytes < need || !wg_aligned(workspace, 16)))
     return mxq_set_error(MXQ_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
-  const int run = 4 * dtype_bytes(out_dtype);
-  const int vec = wg_aligned(dw, run) && K % 4 == 0;
   Wgrad p = {(const uint16_t*)dy, q, scale, dw, M, N, K, ldy, M * ldy, ldq, lds, K, parts, (int)tiles_n, (int)tiles_k,
-             plan.splits, (int)plan.rows, vec};
+             plan.splits, (int)plan.rows};
   const unsigned grid = (unsigned)(tiles_n * tiles_k * plan.splits);
   if (plan.splits > 1) {
     const int64_t ldp = (K + 3) / 4 * 4;
     p.d = workspace;
     p.ldd = ldp;
-    p.vec = 1;
     const int64_t blocks = (N * (ldp / 4) + 255) / 256;
     if (blocks >= (1ll << 31)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "gradient too large");
     hipLaunchKernelGGL((fp8_wgrad_kernel<MXQ_DTYPE_F32, true>), dim3(grid), dim3(kWThreads), 0, (hipStream_t)stream, p);
     if (const int rc = mxq_check_launch("fp8_wgrad_kernel")) return rc;
     with_dtype(out_dtype, [&](auto O) {
       hipLaunchKernelGGL((wgrad_join_kernel<decltype(O)::value>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream,
-                         (const float*)workspace, plan.splits, N, K, ldp, (char*)dw, vec);
+                         (const float*)workspace, plan.splits, N, K, ldp, (char*)dw);
     });
     return mxq_check_launch("wgrad_join_kernel");
   }

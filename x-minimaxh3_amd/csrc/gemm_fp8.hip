@@ -344,7 +344,7 @@ MXQ_DEVICE void epilogue(const Fp8Gemm& p, char* lds, const v16f (&acc)[C::kBI][
         for (int e = 0; e < 4; ++e) y[e] = kSplit ? acc[i][j][q * 4 + e] : acc[i][j][q * 4 + e] + b[e];
         if (!lines) {
           const int row = row0 + lr;
-          if (row < M) store_run4<kOut>(out + row * p.ldd * kElem, col, N - col, p.vec, y);
+          if (row < M) store_run4<kOut>(out + row * p.ldd * kElem, col, N - col, y);
         } else if constexpr (kElem == 4) {
           *reinterpret_cast<v4f*>(out_stage_at(buf, lr, 2 * q + lh)) = v4f{y[0], y[1], y[2], y[3]};
         } else {
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_kernel(Fp8Gemm p) {
 // D = out(sum over slices + bias), four columns per thread; the slices' rows are padded to whole fours.
 template <int kOut>
 __global__ __launch_bounds__(256) void fp8_join_kernel(const float* part, int splits, int64_t M, int64_t N, int64_t ldp,
-                                                       const void* bias, char* d, int64_t ldd, int vec) {
+                                                       const void* bias, char* d, int64_t ldd) {
   constexpr int kElem = kOut == MXQ_DTYPE_F32 ? 4 : 2;
   const int64_t runs = ldp / 4, g = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (g >= M * runs) return;
@@ -424,7 +424,7 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const float* part, int sp
   for (int s = 0; s < splits; ++s) y += *reinterpret_cast<const v4f*>(part + (s * M + row) * ldp + col);
   y += bias_run<kOut>(bias, col, (int)N);
   const float v[4] = {y[0], y[1], y[2], y[3]};
-  store_run4<kOut>(d + row * ldd * kElem, col, (int)N - col, vec, v);
+  store_run4<kOut>(d + row * ldd * kElem, col, (int)N - col, v);
 }
 
 // ---- few rows (up to 64): a stream of the weight ----
@@ -441,7 +441,7 @@ struct Fp8Rows {
   const void* bias;
   void* d;
   int64_t M, N, K, ldx, ldsx, ldb, ldsb, ldd;
-  int kb, vec;
+  int kb;
 };
 
 template <int kIn>
@@ -451,9 +451,8 @@ MXQ_DEVICE void quantize_in_registers(const char* row, bool on, int64_t k0, int6
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int64_t k = k0 + h * 64 + g * 16;
-    // (K is a multiple of 8 elements and rows are 16-byte aligned: halves of a piece are whole vectors)
     const int n = on ? (int)(K - k) : 0;  // (K is at most 2^22)
-    p[h] = piece_load<kIn>(row + (n > 0 ? k : 0) * kElem, n, true);
+    p[h] = piece_load<kIn>(row + (n > 0 ? k : 0) * kElem, n);
   }
   auto across = [](uint32_t m) {  // lanes l, l ^ 16, l ^ 32, l ^ 48
     const auto r = __builtin_amdgcn_permlane16_swap(m, m, false, false);
@@ -555,7 +554,7 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(Fp8Rows p) {
     if (row < p.M && col < N) {
       y += bias_run<kOut>(p.bias, col, N);
       const float v[4] = {y[0], y[1], y[2], y[3]};
-      store_run4<kOut>(reinterpret_cast<char*>(p.d) + row * p.ldd * kElem, col, N - col, p.vec, v);
+      store_run4<kOut>(reinterpret_cast<char*>(p.d) + row * p.ldd * kElem, col, N - col, v);
     }
   }
 }
@@ -661,9 +660,8 @@ extern "C" int mxq_fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, in
     if (blocks >= (1ll << 31)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "output too large");
     with_dtype(out_dtype, [&](auto O) {
       constexpr int kOut = decltype(O)::value;
-      const int vec = aligned(d, kOut == MXQ_DTYPE_F32 ? 16 : 8) && ldd % 4 == 0;
       hipLaunchKernelGGL((fp8_join_kernel<kOut>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream,
-                         (const float*)workspace, plan.splits, M, N, ldp, bias, (char*)d, ldd, vec);
+                         (const float*)workspace, plan.splits, M, N, ldp, bias, (char*)d, ldd);
     });
     return mxq_check_launch("fp8_join_kernel");
   }
@@ -694,14 +692,12 @@ extern "C" int mxq_fp8_linear_rows(const void* x, int x_dtype, int64_t ldx, cons
   const int64_t kb = (K + 127) / 128;
   if (fused && !float_dtype(x_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported input dtype code %d", x_dtype);
   if (M > (fused ? 16 : 64)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "%lld rows", (long long)M);
-  if (fused ? (ldx < K || ldx * dtype_bytes(x_dtype) % 16 || K % 8)
-            : (ldx < kb * 128 || ldx % 16 || ldsx < kb))
+  if (fused ? ldx < K : (ldx < kb * 128 || ldx % 16 || ldsx < kb))
     return mxq_set_error(MXQ_ERR_INVALID, "bad row strides of the activations for K=%lld", (long long)K);
   if (M == 0) return MXQ_OK;
-  if (!x || !b || !sb || !d || (!fused && !sx) || !aligned(x, 16) || !aligned(b, 16))
+  if (!x || !b || !sb || !d || (!fused && (!sx || !aligned(x, 16))) || !aligned(b, 16))
     return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
-  const Fp8Rows p = {x, sx, b, sb, bias, d, M, N, K, ldx, ldsx, ldb, ldsb, ldd, (int)kb,
-                     aligned(d, 4 * dtype_bytes(out_dtype)) && ldd % 4 == 0};
+  const Fp8Rows p = {x, sx, b, sb, bias, d, M, N, K, ldx, ldsx, ldb, ldsb, ldd, (int)kb};
   with_dtype(out_dtype, [&](auto O) {
     constexpr int kOut = decltype(O)::value;
     if (fused) {

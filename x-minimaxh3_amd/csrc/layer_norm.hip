@@ -4,7 +4,8 @@
 //   dx = rstd * (g - E[g] - xh * E[g * xh]),  g = dy * w, xh = (x - mean) * rstd
 //   dw = sum over rows of dy * xh,  db = sum over rows of dy
 //
-// A row is held in registers by kWaves waves, chunks of eight elements per lane, so x (and dy) are read once; the
+// A row is held in registers by as many waves as it has chunks of 512 elements (up to sixteen), eight elements per lane and
+// chunk, so x (and dy) are read once; the
 // variance is that of the centred values, not a difference of large sums. HBM-bound. The backward pass also keeps its
 // lanes' columns of dw and db in registers over all the rows a workgroup takes, writes them once per workgroup, and
 // column_join_kernel adds the workgroups' sums in a fixed order: no atomics, the same bits on every run. Its x can be
@@ -23,30 +24,32 @@ template <int kCode> struct Eight {
   uint32_t w[kWords];
 };
 
-// `n` of eight elements (n <= 0: none, zeros) from p; `vec`: p is aligned to the eight.
-template <int kCode>
-MXQ_DEVICE Eight<kCode> load8(const char* p, int n, bool vec) {
-  Eight<kCode> r;
+// A lane's eight columns of a row of D: those from `col` on; the last lane with any of a row that is not whole eights takes
+// the row's last eight and counts those from `lo` on; a lane behind the row takes the first eight and counts none; of a
+// row below eight elements, lane 0 takes and counts them all. kVec: D % 8 == 0.
+struct Window {
+  int start, lo, hi;
+};
+template <bool kVec>
+MXQ_DEVICE Window window(int col, int D) {
+  if constexpr (kVec) return col < D ? Window{col, 0, 8} : Window{0, 8, 8};
+  if (D < 8) return col == 0 ? Window{0, 0, D} : Window{0, 8, 8};
+  const int n = D - col;
+  return n >= 8 ? Window{col, 0, 8} : n > 0 ? Window{D - 8, 8 - n, 8} : Window{0, 8, 8};
+}
+
+// The window's elements, from any address (one access each: a branch per element, or per load, would end in a wait).
+template <int kCode, bool kVec>
+MXQ_DEVICE Eight<kCode> load8(const char* row, const Window& at, int D) {
   constexpr int kWords = Eight<kCode>::kWords;
+  Eight<kCode> r;
+  const char* p = row + (int64_t)at.start * Eight<kCode>::kElem;
+  if (!kVec && D < 8) {
 #pragma unroll
-  for (int i = 0; i < kWords; ++i) r.w[i] = 0;
-  if (vec && n >= 8) {
-    if constexpr (kWords == 2) {
-      const v2u v = *reinterpret_cast<const v2u*>(p);
-      r.w[0] = v[0];
-      r.w[1] = v[1];
-    } else {
+    for (int i = 0; i < kWords; ++i) r.w[i] = 0;
 #pragma unroll
-      for (int i = 0; i < kWords / 4; ++i) {
-        const v4u v = reinterpret_cast<const v4u*>(p)[i];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r.w[4 * i + j] = v[j];
-      }
-    }
-  } else if (n > 0) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) {
+    for (int i = 0; i < 7; ++i)
+      if (i < D) {
         if constexpr (kCode == MXQ_DTYPE_F32)
           r.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
         else if constexpr (kCode == kCodeFp8)
@@ -54,8 +57,26 @@ MXQ_DEVICE Eight<kCode> load8(const char* p, int n, bool vec) {
         else
           r.w[i >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
       }
+  } else if constexpr (kWords == 2) {
+    const v2u v = *reinterpret_cast<const v2u_any*>(p);
+    r.w[0] = v[0];
+    r.w[1] = v[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < kWords / 4; ++i) {
+      const v4u v = *reinterpret_cast<const v4u_any*>(p + 16 * i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.w[4 * i + j] = v[j];
+    }
   }
   return r;
+}
+
+// v with the elements that the window does not count at zero.
+template <bool kVec>
+MXQ_DEVICE void counted(const Window& at, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (kVec ? at.lo == 0 : (e >= at.lo && e < at.hi)) ? v[e] : 0.0f;
 }
 
 template <int kCode>
@@ -79,60 +100,71 @@ MXQ_DEVICE void to_f32(const Eight<kCode>& r, float scale, float (&v)[8]) {
   }
 }
 
-template <int kCode>
-MXQ_DEVICE void store8(char* p, int n, bool vec, const float (&v)[8]) {
-  if (vec && n >= 8) {
-    if constexpr (kCode == MXQ_DTYPE_F32) {
-      reinterpret_cast<v4f*>(p)[0] = v4f{v[0], v[1], v[2], v[3]};
-      reinterpret_cast<v4f*>(p)[1] = v4f{v[4], v[5], v[6], v[7]};
-    } else {
-      v4u o;
+// Eight results at the window (two lanes of a row's end may store the same values twice).
+template <int kCode, bool kVec>
+MXQ_DEVICE void store8(char* row, const Window& at, int D, const float (&v)[8]) {
+  if (at.lo >= 8) return;
+  char* p = row + (int64_t)at.start * Eight<kCode>::kElem;
+  if (!kVec && D < 8) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        o[i] = kCode == MXQ_DTYPE_F16 ? f32_to_f16_bits(v[2 * i]) | (f32_to_f16_bits(v[2 * i + 1]) << 16)
-                                      : pack_bf16x2(v[2 * i], v[2 * i + 1]);
-      *reinterpret_cast<v4u*>(p) = o;
-    }
+    for (int i = 0; i < 7; ++i)
+      if (i < D) store_out<kCode>(reinterpret_cast<typename OutT<kCode>::T*>(p) + i, v[i]);
+  } else if constexpr (kCode == MXQ_DTYPE_F32) {
+    *reinterpret_cast<v4f_any*>(p) = v4f{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<v4f_any*>(p + 16) = v4f{v[4], v[5], v[6], v[7]};
   } else {
+    v4u o;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) store_out<kCode>(reinterpret_cast<typename OutT<kCode>::T*>(p) + i, v[i]);
+    for (int i = 0; i < 4; ++i)
+      o[i] = kCode == MXQ_DTYPE_F16 ? f32_to_f16_bits(v[2 * i]) | (f32_to_f16_bits(v[2 * i + 1]) << 16)
+                                    : pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<v4u_any*>(p) = o;
   }
 }
 
-// Eight values of a weight or bias vector of a run-time type (`none` where there is none).
-MXQ_DEVICE void param8(const char* p, int code, int col, int n, bool vec, float none, float (&v)[8]) {
+// The window's values of a weight or bias vector of a run-time type (`none` where there is none).
+template <bool kVec>
+MXQ_DEVICE void param8(const char* p, int code, const Window& at, int D, float none, float (&v)[8]) {
   if (!p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = none;
   } else if (code == MXQ_DTYPE_F32) {
-    to_f32(load8<MXQ_DTYPE_F32>(p + (int64_t)col * 4, n, vec), 1.0f, v);
+    to_f32(load8<MXQ_DTYPE_F32, kVec>(p, at, D), 1.0f, v);
   } else if (code == MXQ_DTYPE_F16) {
-    to_f32(load8<MXQ_DTYPE_F16>(p + (int64_t)col * 2, n, vec), 1.0f, v);
+    to_f32(load8<MXQ_DTYPE_F16, kVec>(p, at, D), 1.0f, v);
   } else {
-    to_f32(load8<MXQ_DTYPE_BF16>(p + (int64_t)col * 2, n, vec), 1.0f, v);
+    to_f32(load8<MXQ_DTYPE_BF16, kVec>(p, at, D), 1.0f, v);
   }
 }
 
-// Sums over the row's waves of one or two values; every lane gets them. `red`: a slot of kWaves x 2 floats of the row,
-// another one for every other call.
-template <int kWaves>
-MXQ_DEVICE void row_sum(float& a, float& b, float* red, int wave, int lane) {
-  a = wave_sum(a);
-  b = wave_sum(b);
-  if constexpr (kWaves > 1) {
-    if (lane == 0) {
-      red[2 * wave] = a;
-      red[2 * wave + 1] = b;
-    }
+MXQ_DEVICE float lane_value(float v, int lane) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
+}
+// v + v[i ^ 8], then ^ 4, 2, 1: the sum of sixteen lanes.
+MXQ_DEVICE float sum16(float v) {
+  v += __uint_as_float(dpp_lane<kDppRowRor8>(__float_as_uint(v)));
+  v += __uint_as_float(lane_xor4(__float_as_uint(v)));
+  v += __uint_as_float(dpp_lane<kDppQuadXor2>(__float_as_uint(v)));
+  return v + __uint_as_float(dpp_lane<kDppQuadXor1>(__float_as_uint(v)));
+}
+
+// Sums over the row's waves of two values at once: one exchange puts a's halves added up in lanes 0-31 and b's in lanes
+// 32-63, so the rest of the tree serves both. kOne: the row is one wave's. `red`: 2 x 16 floats of the row's workgroup,
+// others for every other call.
+template <bool kOne>
+MXQ_DEVICE void row_sum(float& a, float& b, float (&red)[2][16], int wave, int waves, int lane) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  float v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = sum16(__uint_as_float(q[0]) + __uint_as_float(q[1]));
+  if constexpr (!kOne) {
+    if ((lane & 31) == 0) red[lane >> 5][wave] = v;
     __syncthreads();
-    a = b = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      a += red[2 * i];
-      b += red[2 * i + 1];
-    }
+    v = red[lane >> 5][lane & 15];
+    v = sum16((lane & 15) < waves ? v : 0.0f);  // (lanes 16-31 the same as 0-15)
   }
+  a = lane_value(v, 0);
+  b = lane_value(v, 32);
 }
 
 struct Norm {
@@ -140,54 +172,48 @@ struct Norm {
   char* y;
   float *mean, *rstd;
   int64_t M, ldx;
-  int D, wcode, vec, pvec;
+  int D, wcode;
   float eps;
 };
 
-template <int kWaves> struct NormBlock {
-  static constexpr int kThreads = kWaves == 1 ? 256 : kWaves * 64;
-  static constexpr int kRows = kWaves == 1 ? 4 : 1;  // rows a workgroup holds at once
-};
-
-template <int kCode, int kChunks, int kWaves>
-__global__ __launch_bounds__(NormBlock<kWaves>::kThreads) void layer_norm_kernel(Norm p) {
+// kOne: a wave per row, four rows per workgroup; else a workgroup per row.
+template <int kCode, int kChunks, bool kOne, bool kVec>
+__global__ __launch_bounds__(kOne ? 256 : 1024) void layer_norm_kernel(Norm p) {
   constexpr int kElem = Eight<kCode>::kElem;
-  __shared__ float red[2][2 * kWaves];
-  const int wave = kWaves == 1 ? 0 : threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t row = kWaves == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  __shared__ float red[2][2][16];
+  const int waves = kOne ? 1 : blockDim.x >> 6, wave = kOne ? 0 : threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t row = kOne ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
   if (row >= p.M) return;  // (whole waves; with several per row, whole workgroups)
   const char* x = p.x + row * p.ldx * kElem;
   Eight<kCode> raw[kChunks];
+  auto at = [&](int i) { return window<kVec>(((i * waves + wave) * 64 + lane) * 8, p.D); };
 #pragma unroll
-  for (int i = 0; i < kChunks; ++i) {
-    const int col = ((i * kWaves + wave) * 64 + lane) * 8;
-    raw[i] = load8<kCode>(x + (int64_t)(col < p.D ? col : 0) * kElem, p.D - col, p.vec);
-  }
+  for (int i = 0; i < kChunks; ++i) raw[i] = load8<kCode, kVec>(x, at(i), p.D);
   const float inv = 1.0f / (float)p.D;
   float s = 0.0f, none = 0.0f;
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
     float v[8];
     to_f32(raw[i], 1.0f, v);
+    counted<kVec>(at(i), v);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s += v[e];
   }
-  row_sum<kWaves>(s, none, red[0], wave, lane);
+  row_sum<kOne>(s, none, red[0], wave, waves, lane);
   const float mean = s * inv;
   float s2 = 0.0f;
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
-    const int n = p.D - ((i * kWaves + wave) * 64 + lane) * 8;
     float v[8];
     to_f32(raw[i], 1.0f, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float d = e < n ? v[e] - mean : 0.0f;
-      s2 += d * d;
-    }
+    for (int e = 0; e < 8; ++e) v[e] -= mean;
+    counted<kVec>(at(i), v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s2 = fmaf(v[e], v[e], s2);
   }
   none = 0.0f;
-  row_sum<kWaves>(s2, none, red[1], wave, lane);
+  row_sum<kOne>(s2, none, red[1], wave, waves, lane);
   const float rstd = 1.0f / sqrtf(s2 * inv + p.eps);
   if (wave == 0 && lane == 0) {
     if (p.mean) p.mean[row] = mean;
@@ -196,15 +222,13 @@ __global__ __launch_bounds__(NormBlock<kWaves>::kThreads) void layer_norm_kernel
   char* y = p.y + row * p.D * kElem;
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
-    const int col = ((i * kWaves + wave) * 64 + lane) * 8, n = p.D - col;
-    if (n <= 0) continue;
     float v[8], w[8], b[8];
     to_f32(raw[i], 1.0f, v);
-    param8(p.w, p.wcode, col, n, p.pvec, 1.0f, w);
-    param8(p.b, p.wcode, col, n, p.pvec, 0.0f, b);
+    param8<kVec>(p.w, p.wcode, at(i), p.D, 1.0f, w);
+    param8<kVec>(p.b, p.wcode, at(i), p.D, 0.0f, b);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (v[e] - mean) * rstd * w[e] + b[e];
-    store8<kCode>(y + (int64_t)col * kElem, n, p.vec, v);
+    for (int e = 0; e < 8; ++e) v[e] = fmaf((v[e] - mean) * rstd, w[e], b[e]);
+    store8<kCode, kVec>(y, at(i), p.D, v);
   }
 }
 
@@ -215,123 +239,183 @@ struct NormGrad {
   char* dx;
   float* sums;  // [grid][2][D]: dw and db of the workgroup's rows
   int64_t M, ldy, ldx, ldxs;
-  int D, wcode, vec_y, vec_x, pvec;
+  int D, wcode;
 };
 
-template <int kCode, int kX, int kChunks, int kWaves>
-__global__ __launch_bounds__(NormBlock<kWaves>::kThreads) void layer_norm_grad_kernel(NormGrad p) {
-  constexpr int kElem = Eight<kCode>::kElem, kElemX = Eight<kX>::kElem, kRows = NormBlock<kWaves>::kRows;
-  __shared__ float red[2][2 * kWaves];
-  const int wave = kWaves == 1 ? 0 : threadIdx.x >> 6, lane = threadIdx.x & 63, sub = kWaves == 1 ? threadIdx.x >> 6 : 0;
+template <int kCode, int kX, int kChunks, int kThreads, bool kVec>
+__global__ __launch_bounds__(kThreads) void layer_norm_grad_kernel(NormGrad p) {
+  constexpr bool kOne = kThreads == 256;  // a wave per row, four rows per workgroup; else a workgroup per row
+  constexpr int kElem = Eight<kCode>::kElem, kElemX = Eight<kX>::kElem, kRows = kOne ? 4 : 1;
+  constexpr bool kAhead = kChunks == 1;  // (more chunks leave no registers for a second row at 1024 threads)
+  __shared__ float red[2][2][16];
+  const int waves = kOne ? 1 : blockDim.x >> 6, wave = kOne ? 0 : threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int sub = kOne ? threadIdx.x >> 6 : 0;
   const float inv = 1.0f / (float)p.D;
-  float dw[kChunks][8] = {}, db[kChunks][8] = {};
-  int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * kRows + sub; row < p.M; row += (int64_t)gridDim.x * kRows) {
-    Eight<kCode> ry[kChunks];
-    Eight<kX> rx[kChunks];
-    float sc[kChunks];
+  float dw[kChunks][8] = {}, db[kChunks][8] = {}, w[kChunks][8];
+  auto at = [&](int i) { return window<kVec>(((i * waves + wave) * 64 + lane) * 8, p.D); };
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) param8<kVec>(p.w, p.wcode, at(i), p.D, 1.0f, w[i]);
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t row = (int64_t)blockIdx.x * kRows + sub;
+  // The next row is requested ahead of the present one's arithmetic (kAhead); what a lane keeps of a row is its raw words, from
+  // which g and xh are formed again behind the row's sums (kept as float32 they took 60 registers more, a wave per SIMD).
+  Eight<kCode> ry[kChunks];
+  Eight<kX> rx[kChunks];
+  uint32_t rs[kChunks];
+  float mean = 0.0f, rstd = 0.0f;
+  auto load = [&](int64_t k) {
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      const int col = ((i * kWaves + wave) * 64 + lane) * 8, n = p.D - col, at = n > 0 ? col : 0;
-      ry[i] = load8<kCode>(p.dy + (row * p.ldy + at) * kElem, n, p.vec_y);
-      rx[i] = load8<kX>(p.x + (row * p.ldx + at) * kElemX, n, p.vec_x);
-      sc[i] = kX == kCodeFp8 ? fp8_scale_f32(p.xs[row * p.ldxs + (at >> 7)]) : 1.0f;
+      ry[i] = load8<kCode, kVec>(p.dy + k * p.ldy * kElem, at(i), p.D);
+      rx[i] = load8<kX, kVec>(p.x + k * p.ldx * kElemX, at(i), p.D);
+      if constexpr (kX == kCodeFp8) {
+        const uint8_t* xs = p.xs + k * p.ldxs;
+        const Window c = at(i);
+        // (a window that was moved to the row's end may reach back into the block before)
+        rs[i] = xs[c.start >> 7] | (kVec || p.D < 8 ? 0u : (uint32_t)xs[(c.start + 7) >> 7] << 8);
+      }
     }
-    const float mean = p.mean[row], rstd = p.rstd[row];
-    float s1 = 0.0f, s2 = 0.0f;
-    float g[kChunks][8], xh[kChunks][8];
+    mean = p.mean[k];
+    rstd = p.rstd[k];
+  };
+  auto x_values = [&](const Eight<kX>& t, uint32_t scales, int i, float (&v)[8]) {
+    to_f32(t, fp8_scale_f32(scales & 0xFFu), v);
+    if constexpr (kX == kCodeFp8 && !kVec) {
+      if (p.D >= 8) {
+        float u[8];
+        to_f32(t, fp8_scale_f32(scales >> 8), u);
+        const int c = at(i).start & 127;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = c + e < 128 ? v[e] : u[e];
+      }
+    }
+  };
+  if (kAhead && row < p.M) load(row);
+  for (int turn = 0; row < p.M; row += step, turn ^= 1) {
+    Eight<kCode> ty[kChunks];
+    Eight<kX> tx[kChunks];
+    uint32_t ts[kChunks];
+    if constexpr (!kAhead) load(row);
+    const float m = mean, r = rstd;
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      const int col = ((i * kWaves + wave) * 64 + lane) * 8, n = p.D - col;
-      float w[8], y[8];
-      to_f32(ry[i], 1.0f, y);
-      to_f32(rx[i], sc[i], xh[i]);
-      param8(p.w, p.wcode, n > 0 ? col : 0, n, p.pvec, 1.0f, w);
+      ty[i] = ry[i];
+      tx[i] = rx[i];
+      ts[i] = rs[i];
+    }
+    if (kAhead && row + step < p.M) load(row + step);
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      float y[8], x[8];
+      to_f32(ty[i], 1.0f, y);
+      counted<kVec>(at(i), y);  // (y = 0 adds nothing to any sum)
+      x_values(tx[i], ts[i], i, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        xh[i][e] = e < n ? (xh[i][e] - mean) * rstd : 0.0f;
-        g[i][e] = y[e] * w[e];
-        s1 += g[i][e];
-        s2 += g[i][e] * xh[i][e];
-        dw[i][e] += y[e] * xh[i][e];
+        const float xh = (x[e] - m) * r, g = y[e] * w[i][e];
+        s1 += g;
+        s2 = fmaf(g, xh, s2);
+        dw[i][e] = fmaf(y[e], xh, dw[i][e]);
         db[i][e] += y[e];
       }
     }
-    row_sum<kWaves>(s1, s2, red[turn], wave, lane);
-    turn ^= 1;
-    const float c1 = s1 * inv, c2 = s2 * inv;
+    row_sum<kOne>(s1, s2, red[turn], wave, waves, lane);
+    const float rc1 = r * (s1 * inv), a = r * r * (s2 * inv);  // dx = r g - r c1 - (x - m) r^2 c2
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      const int col = ((i * kWaves + wave) * 64 + lane) * 8, n = p.D - col;
-      if (n <= 0) continue;
-      float v[8];
+      float v[8], x[8];
+      // (formed again from the words: the statement keeps the compiler from holding the first pass's values instead)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = rstd * (g[i][e] - c1 - xh[i][e] * c2);
-      store8<kCode>(p.dx + (row * p.D + col) * kElem, n, p.vec_y && (p.D & 7) == 0, v);
+      for (int k = 0; k < Eight<kCode>::kWords; ++k) __asm__ volatile("" : "+v"(ty[i].w[k]));
+#pragma unroll
+      for (int k = 0; k < Eight<kX>::kWords; ++k) __asm__ volatile("" : "+v"(tx[i].w[k]));
+      to_f32(ty[i], 1.0f, v);
+      x_values(tx[i], ts[i], i, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e] * w[i][e], r, fmaf(x[e] - m, -a, -rc1));
+      store8<kCode, kVec>(p.dx + row * p.D * kElem, at(i), p.D, v);
     }
   }
   if (!p.sums) return;
   float* out = p.sums + (int64_t)blockIdx.x * 2 * p.D;
-  if constexpr (kWaves == 1) {  // the workgroup's four waves hold the same columns: their sums in order
+  if constexpr (kOne) {  // the workgroup's four waves hold the same columns: their sums in order
     __shared__ float part[4][64 * 8];
+    const Window c = at(0);
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i)
+    for (int k = 0; k < 2; ++k) {
+      __syncthreads();
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        __syncthreads();
+      for (int e = 0; e < 8; ++e) part[sub][e * 64 + lane] = k ? db[0][e] : dw[0][e];
+      __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) part[sub][e * 64 + lane] = k ? db[i][e] : dw[i][e];
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int j = sub * 2 + e, col = (i * 64 + lane) * 8 + j;
-          if (col < p.D)
-            out[k * p.D + col] = ((part[0][j * 64 + lane] + part[1][j * 64 + lane]) + part[2][j * 64 + lane]) + part[3][j * 64 + lane];
-        }
+      for (int e = 0; e < 2; ++e) {
+        const int j = sub * 2 + e;
+        if (j >= c.lo && j < c.hi)
+          out[k * p.D + c.start + j] =
+              ((part[0][j * 64 + lane] + part[1][j * 64 + lane]) + part[2][j * 64 + lane]) + part[3][j * 64 + lane];
       }
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      const int col = ((i * kWaves + wave) * 64 + lane) * 8;
+      const Window c = at(i);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (col + e < p.D) {
-          out[col + e] = dw[i][e];
-          out[p.D + col + e] = db[i][e];
+        if (e >= c.lo && e < c.hi) {
+          out[c.start + e] = dw[i][e];
+          out[p.D + c.start + e] = db[i][e];
         }
     }
   }
 }
 
-// Waves per row and chunks per lane: rows up to 1024 elements by one wave, up to 8192 by four, up to 24576 by sixteen.
+// Chunks per lane and waves per row of the backward pass: up to 512 elements one wave, up to 8192 a chunk per lane of as
+// many waves as it takes (hidden 5120: ten waves, every lane at work), beyond that two and three chunks of up to sixteen.
+template <class F>
+static void with_bool(bool v, F&& f) {
+  if (v)
+    f(std::true_type{});
+  else
+    f(std::false_type{});
+}
+
 constexpr int kNormMaxD = 24576;
 template <class F>
 static void with_shape(int D, F&& f) {
   using std::integral_constant;
-  const int n = (D + 511) / 512;  // chunks of one wave
-  if (n <= 1) f(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-  else if (n <= 2) f(integral_constant<int, 2>{}, integral_constant<int, 1>{});
-  else if (n <= 4) f(integral_constant<int, 1>{}, integral_constant<int, 4>{});
-  else if (n <= 8) f(integral_constant<int, 2>{}, integral_constant<int, 4>{});
-  else if (n <= 12) f(integral_constant<int, 3>{}, integral_constant<int, 4>{});
-  else if (n <= 16) f(integral_constant<int, 4>{}, integral_constant<int, 4>{});
-  else if (n <= 32) f(integral_constant<int, 2>{}, integral_constant<int, 16>{});
-  else f(integral_constant<int, 3>{}, integral_constant<int, 16>{});
+  const int n = (D + 511) / 512;
+  if (n <= 1) f(integral_constant<int, 1>{}, integral_constant<int, 256>{}, 256);
+  else if (n <= 16) f(integral_constant<int, 1>{}, integral_constant<int, 1024>{}, n * 64);
+  else if (n <= 32) f(integral_constant<int, 2>{}, integral_constant<int, 1024>{}, (n + 1) / 2 * 64);
+  else f(integral_constant<int, 3>{}, integral_constant<int, 1024>{}, (n + 2) / 3 * 64);
 }
 
-// Workgroups of the backward pass: resident ones, each with an equal share of the rows.
+// The forward pass holds a row from its loads to its stores, so rows under way per CU count: few waves of many chunks
+// (75600 x 5120: two waves of five chunks 297 us, four of three 326, five of two 380, ten of one 458).
+template <class F>
+static void with_forward_shape(int D, F&& f) {
+  using std::integral_constant;
+  const int n = (D + 511) / 512;
+  auto go = [&](auto N) { f(N, std::false_type{}, (n + decltype(N)::value - 1) / decltype(N)::value * 64); };
+  if (n <= 1) f(integral_constant<int, 1>{}, std::true_type{}, 256);
+  else if (n <= 4) go(integral_constant<int, 2>{});
+  else if (n <= 8) go(integral_constant<int, 4>{});
+  else if (n <= 10) go(integral_constant<int, 5>{});
+  else if (n <= 24) go(integral_constant<int, 6>{});
+  else go(integral_constant<int, 4>{});
+}
+
+// Workgroups of the backward pass: about twenty waves per CU (sixteen of the wide forms), each with an equal share of rows.
 static int64_t norm_grad_grid(int64_t M, int64_t D, int cus) {
-  const int64_t units = D <= 1024 ? (M + 3) / 4 : M, most = (int64_t)cus * (D <= 8192 ? 3 : 1);
+  const int64_t n = (D + 511) / 512, units = n <= 1 ? (M + 3) / 4 : M;
+  const int64_t most = cus * (n <= 1 ? 5 : n <= 16 ? (20 / n > 1 ? 20 / n : 1) : 1);
   return units < most ? units : most;
 }
 
 }  // namespace mxq
 
 using namespace mxq;
-
-static bool ln_aligned(const void* p, int64_t ld, int elem) {
-  return reinterpret_cast<uintptr_t>(p) % (8 * elem < 16 ? 8 * elem : 16) == 0 && ld % 8 == 0;
-}
 
 static int check_norm(int64_t M, int64_t D, int dtype, int wcode) {
   if (!float_dtype(dtype) || !float_dtype(wcode)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported dtype codes %d, %d", dtype, wcode);
@@ -347,15 +431,15 @@ extern "C" int mxq_layer_norm(const void* x, int dtype, int64_t ldx, const void*
   if (!(eps >= 0.0f)) return mxq_set_error(MXQ_ERR_INVALID, "eps %g", (double)eps);
   if (M == 0) return MXQ_OK;
   if (!x || !y) return mxq_set_error(MXQ_ERR_INVALID, "null pointer");
-  const int elem = dtype_bytes(dtype);
-  const Norm p = {(const char*)x, (const char*)w, (const char*)b, (char*)y, mean, rstd, M, ldx, (int)D, param_dtype,
-                  ln_aligned(x, ldx, elem) && ln_aligned(y, D, elem), ln_aligned(w, 8, 4) && ln_aligned(b, 8, 4), eps};
-  with_shape((int)D, [&](auto N, auto W) {
+  const Norm p = {(const char*)x, (const char*)w, (const char*)b, (char*)y, mean, rstd, M, ldx, (int)D, param_dtype, eps};
+  with_forward_shape((int)D, [&](auto N, auto One, int threads) {
     with_dtype(dtype, [&](auto C) {
-      constexpr int kWaves = decltype(W)::value;
-      const unsigned grid = (unsigned)(kWaves == 1 ? (M + 3) / 4 : M);
-      hipLaunchKernelGGL((layer_norm_kernel<decltype(C)::value, decltype(N)::value, kWaves>), dim3(grid),
-                         dim3(NormBlock<kWaves>::kThreads), 0, (hipStream_t)stream, p);
+      constexpr bool kOne = decltype(One)::value;
+      const unsigned grid = (unsigned)(kOne ? (M + 3) / 4 : M);
+      with_bool(D % 8 == 0, [&](auto V) {
+        hipLaunchKernelGGL((layer_norm_kernel<decltype(C)::value, decltype(N)::value, kOne, decltype(V)::value>), dim3(grid),
+                           dim3(threads), 0, (hipStream_t)stream, p);
+      });
     });
   });
   return mxq_check_launch("layer_norm_kernel");
@@ -381,19 +465,18 @@ extern "C" int mxq_layer_norm_backward(const void* dy, int dtype, int64_t ldy, c
   const int64_t grid = norm_grad_grid(M, D, mxq_cu_count());
   if (sums && strips != grid)
     return mxq_set_error(MXQ_ERR_INVALID, "room for %lld strips, %lld needed", (long long)strips, (long long)grid);
-  const int elem = dtype_bytes(dtype);
   const NormGrad p = {(const char*)dy, (const char*)x, (const char*)w, x_scale, mean, rstd, (char*)dx, sums, M, ldy, ldx, ldxs,
-                      (int)D, param_dtype, ln_aligned(dy, ldy, elem) && ln_aligned(dx, 8, elem),
-                      ln_aligned(x, ldx, kept ? 1 : elem), ln_aligned(w, 8, 4)};
-  with_shape((int)D, [&](auto N, auto W) {
+                      (int)D, param_dtype};
+  with_shape((int)D, [&](auto N, auto T, int threads) {
     with_dtype(dtype, [&](auto C) {
-      constexpr int kCode = decltype(C)::value, kWaves = decltype(W)::value, kChunks = decltype(N)::value;
-      if (kept)
-        hipLaunchKernelGGL((layer_norm_grad_kernel<kCode, kCodeFp8, kChunks, kWaves>), dim3((unsigned)grid),
-                           dim3(NormBlock<kWaves>::kThreads), 0, (hipStream_t)stream, p);
-      else
-        hipLaunchKernelGGL((layer_norm_grad_kernel<kCode, kCode, kChunks, kWaves>), dim3((unsigned)grid),
-                           dim3(NormBlock<kWaves>::kThreads), 0, (hipStream_t)stream, p);
+      constexpr int kCode = decltype(C)::value, kChunks = decltype(N)::value, kThreads = decltype(T)::value;
+      with_bool(D % 8 == 0, [&](auto V) {
+        with_bool(kept, [&](auto K) {
+          constexpr int kX = decltype(K)::value ? kCodeFp8 : kCode;
+          hipLaunchKernelGGL((layer_norm_grad_kernel<kCode, kX, kChunks, kThreads, decltype(V)::value>), dim3((unsigned)grid),
+                             dim3(threads), 0, (hipStream_t)stream, p);
+        });
+      });
     });
   });
   return mxq_check_launch("layer_norm_grad_kernel");

@@ -243,14 +243,12 @@ def fp8_linear(x: torch.Tensor, weight: PreparedFp8Weight, bias: torch.Tensor | 
     n, k = weight.out_features, weight.in_features
     bias = _bias(bias, n, out_dtype, dev)
     m = x.numel() // k
-    if 0 < m <= _FUSED_ROWS and k % 8 == 0:
+    if 0 < m <= _FUSED_ROWS:
         x2 = _rows_in_place(x, k)
-        ld = x2.stride(0) if m > 1 else k
-        if x2.data_ptr() % 16 == 0 and ld * x2.element_size() % 16 == 0:
-            out = torch.empty((m, n), dtype=out_dtype, device=dev)
-            _launch(dev, "mxq_fp8_linear_rows", x2.data_ptr(), xcode, ld, None, 0, weight.q.data_ptr(), weight.q.shape[1],
-                    weight.scale.data_ptr(), weight.scale.shape[1], _ptr(bias), out.data_ptr(), n, code, m, n, k)
-            return out if x.dim() == 2 else out.reshape(*x.shape[:-1], n)
+        out = torch.empty((m, n), dtype=out_dtype, device=dev)
+        _launch(dev, "mxq_fp8_linear_rows", x2.data_ptr(), xcode, x2.stride(0) if m > 1 else k, None, 0, weight.q.data_ptr(),
+                weight.q.shape[1], weight.scale.data_ptr(), weight.scale.shape[1], _ptr(bias), out.data_ptr(), n, code, m, n, k)
+        return out if x.dim() == 2 else out.reshape(*x.shape[:-1], n)
     q, s, m, k = _quantize_rows(x)
     out = _product(dev, q, s, m, k, weight.q, weight.scale, n, bias, out_dtype)
     return out if x.dim() == 2 else out.reshape(*x.shape[:-1], n)

@@ -566,17 +566,50 @@ int mxq_fp8_wgrad(const void* dy, int parts, int64_t ldy, const uint8_t* q, int6
 int mxq_layer_norm(const void* x, int dtype, int64_t ldx, const void* w, const void* b, int param_dtype, float eps, void* y,
                    float* mean, float* rstd, int64_t M, int64_t D, void* stream);
 
-/* Row strips of mxq_layer_norm_backward at this size on the current device. */
-int mxq_layer_norm_backward_strips(int64_t M, int64_t D, int64_t* strips);
+/* Bytes of workspace mxq_layer_norm_backward needs for dparams at this size on the current device. */
+int mxq_layer_norm_backward_workspace(int64_t M, int64_t D, int64_t* bytes);
 
 /*
  * Its gradients: dx [M, D] (contiguous, dtype) from dy [M, ldy] of dtype, x [M, ldx] of dtype, or codes with x_dtype
- * MXQ_DTYPE_E4M3 and scales [M, ldxs], and the forward's mean and rstd. sums fp32 [strips, 2, D] (NULL: none) receives
- * the strips' sums of dy * xh and of dy, whose column sums (mxq_column_join) are the weight's and the bias's gradients.
+ * MXQ_DTYPE_E4M3 and scales [M, ldxs], and the forward's mean and rstd. dparams fp32 [2, D] (NULL: none): the weight's
+ * gradient, the sums over rows of dy * xh, and the bias's, those of dy.
  */
 int mxq_layer_norm_backward(const void* dy, int dtype, int64_t ldy, const void* x, int x_dtype, int64_t ldx,
                             const uint8_t* x_scale, int64_t ldxs, const float* mean, const float* rstd, const void* w,
-                            int param_dtype, void* dx, float* sums, int64_t strips, int64_t M, int64_t D, void* stream);
+                            int param_dtype, void* dx, float* dparams, int64_t M, int64_t D, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
+/* Rows of `width` bytes, lds apart, copied to rows ldd apart (a multiple of 16), zeros behind them. */
+int mxq_pad_rows(const uint8_t* src, int64_t lds, int64_t width, uint8_t* dst, int64_t ldd, int64_t rows, void* stream);
+
+/* Bytes of workspace mxq_fp8_linear needs at this size on the current device (0 up to 16 rows). */
+int mxq_fp8_linear_workspace(int64_t M, int64_t N, int64_t K, int64_t* bytes);
+
+/*
+ * The layer's forward pass in one call: d [M, N] = out(quantize(x) b^T + bias), x [M, ldx] of x_dtype; the weight and
+ * the rest as in mxq_fp8_gemm. N and K up to 2^22.
+ */
+int mxq_fp8_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* b, int64_t ldb, const uint8_t* sb, int64_t ldsb,
+                   const void* bias, void* d, int64_t ldd, int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
+/*
+ * Bytes of workspace mxq_fp8_linear_backward needs at this size on the current device. needs: 1 dx, 2 dw, 4 db, added up;
+ * direct and readable as below.
+ */
+int mxq_fp8_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dy_dtype, int direct, int readable, int needs,
+                                      int64_t* bytes);
+
+/*
+ * The layer's backward pass in one call, from dy [M, ldy] of dy_dtype, the input's codes q [M, ldq] and scales [M, lds]
+ * and the transposed weight bt [K, ldbt], sbt: dx [M, K] (contiguous, dy_dtype), dw [N, K] and db [N] (grad_dtype), each
+ * NULL to leave it out. direct: the weight's gradient reads dy itself (bf16, N % 16 == 0, ldy % 8 == 0, 16-byte
+ * aligned) in place of parts of it. readable: q is as mxq_fp8_wgrad reads it, else its rows are copied.
+ */
+int mxq_fp8_linear_backward(const void* dy, int dy_dtype, int64_t ldy, int direct, const uint8_t* q, int64_t ldq,
+                            const uint8_t* scale, int64_t lds, int readable, const uint8_t* bt, int64_t ldbt,
+                            const uint8_t* sbt, int64_t ldsbt, void* dx, void* dw, void* db, int grad_dtype, int64_t M,
+                            int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Measurement helper (no counterpart in the reference; it calibrates the roofline): runs

@@ -174,9 +174,19 @@ def test_c_gradient_entries_refuse_before_any_launch():
         _call("mxq_layer_norm", ok, 2, 24577, None, None, 2, 1e-5, ok, None, None, 4, 24577)
     with pytest.raises(ValueError):
         _call("mxq_layer_norm", ok, 2, 127, None, None, 2, 1e-5, ok, None, None, 4, 128)
-    with pytest.raises(ValueError, match="strips"):
-        _call("mxq_layer_norm_backward", ok, 2, 128, ok, 2, 128, None, 0, ok, ok, None, 2, ok, ok, 9999, 4, 128)
+    with pytest.raises(ValueError, match="workspace"):
+        _call("mxq_layer_norm_backward", ok, 2, 128, ok, 2, 128, None, 0, ok, ok, None, 2, ok, ok, 4, 128, ok, 8)
     with pytest.raises(ValueError, match="dtype code"):
-        _call("mxq_layer_norm_backward", ok, 2, 128, ok, 0, 128, None, 0, ok, ok, None, 2, ok, None, 0, 4, 128)
+        _call("mxq_layer_norm_backward", ok, 2, 128, ok, 0, 128, None, 0, ok, ok, None, 2, ok, None, 4, 128, None, 0)
     with pytest.raises(ValueError, match="null"):
-        _call("mxq_layer_norm_backward", ok, 2, 128, ok, 5, 128, None, 1, ok, ok, None, 2, ok, None, 0, 4, 128)
+        _call("mxq_layer_norm_backward", ok, 2, 128, ok, 5, 128, None, 1, ok, ok, None, 2, ok, None, 4, 128, None, 0)
+    with pytest.raises(ValueError, match="directly"):
+        _call("mxq_fp8_linear_backward", ok, 1, 256, 1, ok, 256, ok, 2, 1, ok, 256, ok, 4, ok, ok, ok, 0, 8, 256, 256, ok, 1 << 30)
+    with pytest.raises(ValueError, match="workspace"):
+        _call("mxq_fp8_linear_backward", ok, 1, 256, 0, ok, 256, ok, 2, 1, ok, 256, ok, 4, ok, ok, ok, 0, 8, 256, 256, None, 0)
+    with pytest.raises(ValueError, match="workspace"):
+        _call("mxq_fp8_linear", ok, 2, 256, ok, 256, ok, 4, None, ok, 128, 2, 100, 128, 256, ok, 64)
+    with pytest.raises(ValueError, match="size"):
+        _call("mxq_fp8_linear", ok, 2, 256, ok, 256, ok, 4, None, ok, 128, 2, 100, 0, 256, ok, 64)
+    with pytest.raises(ValueError, match="strides"):
+        _call("mxq_pad_rows", ok, 100, 100, ok, 104, 4)

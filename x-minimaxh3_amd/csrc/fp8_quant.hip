@@ -241,6 +241,28 @@ __global__ __launch_bounds__(256) void fp8_grad_pass_kernel(const char* x, int64
   }
 }
 
+// Rows of bytes copied to 16-byte rows `ldd` apart, zeros behind their `width`: codes and scales whose own rows are not.
+__global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* src, int64_t lds, int width, uint8_t* dst, int ldd,
+                                                       int64_t total) {
+  const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (g >= total) return;
+  const int pieces = ldd / 16;
+  const int64_t row = g / pieces;
+  const int col = (int)(g - row * pieces) * 16, n = width - col;
+  const uint8_t* s = src + row * lds + col;
+  v4u v = {0, 0, 0, 0};
+  if (n >= 16) {
+    v = *reinterpret_cast<const v4u_any*>(s);
+  } else if (n > 0) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t b = s[min(i, n - 1)];
+      v[i >> 2] |= (i < n ? b : 0u) << (8 * (i & 3));
+    }
+  }
+  *reinterpret_cast<v4u*>(dst + row * ldd + col) = v;
+}
+
 // out[c] = sum over `parts` rows of a float32 [parts, n] table, in row order by eighths: the columns' last sum.
 template <int kCode>
 __global__ __launch_bounds__(256) void column_join_kernel(const float* in, int64_t parts, int64_t n, void* out) {
@@ -370,6 +392,20 @@ extern "C" int mxq_fp8_grad_pass(const void* dy, int dy_dtype, int64_t ldy, uint
                          ldq, scale, lds, (uint16_t*)nullptr, (int64_t)0, sums, M, N, nb, strip);
   });
   return mxq_check_launch("fp8_grad_pass_kernel");
+}
+
+extern "C" int mxq_pad_rows(const uint8_t* src, int64_t lds, int64_t width, uint8_t* dst, int64_t ldd, int64_t rows,
+                            void* stream) {
+  if (rows < 0 || width < 1 || lds < width || ldd < width || ldd % 16 || ldd >= (1ll << 31))
+    return mxq_set_error(MXQ_ERR_INVALID, "bad rows of %lld bytes, strides %lld and %lld", (long long)width, (long long)lds,
+                         (long long)ldd);
+  if (rows == 0) return MXQ_OK;
+  if (!src || !dst || !aligned16(dst)) return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
+  const int64_t total = rows * (ldd / 16);
+  if (total > (1ll << 38)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "too many rows");
+  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, (hipStream_t)stream, src, lds,
+                     (int)width, dst, (int)ldd, total);
+  return mxq_check_launch("pad_rows_kernel");
 }
 
 extern "C" int mxq_column_join(const float* in, int64_t parts, int64_t n, void* out, int out_dtype, void* stream) {

@@ -445,26 +445,28 @@ extern "C" int mxq_layer_norm(const void* x, int dtype, int64_t ldx, const void*
   return mxq_check_launch("layer_norm_kernel");
 }
 
-extern "C" int mxq_layer_norm_backward_strips(int64_t M, int64_t D, int64_t* strips) {
-  if (M < 0 || D < 1 || !strips) return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld D=%lld", (long long)M, (long long)D);
-  *strips = norm_grad_grid(M, D, mxq_cu_count());
+extern "C" int mxq_layer_norm_backward_workspace(int64_t M, int64_t D, int64_t* bytes) {
+  if (M < 0 || D < 1 || D > kNormMaxD || !bytes)
+    return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld D=%lld", (long long)M, (long long)D);
+  *bytes = norm_grad_grid(M, D, mxq_cu_count()) * 2 * D * 4;
   return MXQ_OK;
 }
 
 extern "C" int mxq_layer_norm_backward(const void* dy, int dtype, int64_t ldy, const void* x, int x_dtype, int64_t ldx,
                                        const uint8_t* x_scale, int64_t ldxs, const float* mean, const float* rstd,
-                                       const void* w, int param_dtype, void* dx, float* sums, int64_t strips, int64_t M,
-                                       int64_t D, void* stream) {
+                                       const void* w, int param_dtype, void* dx, float* dparams, int64_t M, int64_t D,
+                                       void* workspace, int64_t workspace_bytes, void* stream) {
   if (const int rc = check_norm(M, D, dtype, param_dtype)) return rc;
   const bool kept = x_dtype == MXQ_DTYPE_E4M3;
   if (!kept && x_dtype != dtype) return mxq_set_error(MXQ_ERR_INVALID, "x of dtype code %d for gradients of %d", x_dtype, dtype);
   if (ldy < D || ldx < D || (kept && ldxs < (D + 127) / 128))
     return mxq_set_error(MXQ_ERR_INVALID, "bad row strides for %lld columns", (long long)D);
-  if (M == 0) return MXQ_OK;
+  if (M == 0) return dparams ? mxq_column_join(nullptr, 0, 2 * D, dparams, MXQ_DTYPE_F32, stream) : MXQ_OK;
   if (!dy || !x || !mean || !rstd || !dx || (kept && !x_scale)) return mxq_set_error(MXQ_ERR_INVALID, "null pointer");
-  const int64_t grid = norm_grad_grid(M, D, mxq_cu_count());
-  if (sums && strips != grid)
-    return mxq_set_error(MXQ_ERR_INVALID, "room for %lld strips, %lld needed", (long long)strips, (long long)grid);
+  const int64_t grid = norm_grad_grid(M, D, mxq_cu_count()), need = grid * 2 * D * 4;
+  if (dparams && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 4))
+    return mxq_set_error(MXQ_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  float* sums = dparams ? (float*)workspace : nullptr;
   const NormGrad p = {(const char*)dy, (const char*)x, (const char*)w, x_scale, mean, rstd, (char*)dx, sums, M, ldy, ldx, ldxs,
                       (int)D, param_dtype};
   with_shape((int)D, [&](auto N, auto T, int threads) {
@@ -479,5 +481,6 @@ extern "C" int mxq_layer_norm_backward(const void* dy, int dtype, int64_t ldy, c
       });
     });
   });
-  return mxq_check_launch("layer_norm_grad_kernel");
+  if (const int rc = mxq_check_launch("layer_norm_grad_kernel")) return rc;
+  return dparams ? mxq_column_join(sums, grid, 2 * D, dparams, MXQ_DTYPE_F32, stream) : MXQ_OK;
 }

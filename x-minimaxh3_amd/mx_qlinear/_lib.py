@@ -83,8 +83,14 @@ SIGNATURES: dict[str, list] = {
     "mxq_fp8_wgrad_workspace": [_I64, _I64, _I64, _I, _P],
     "mxq_fp8_wgrad": [_P, _I, _I64, _P, _I64, _P, _I64, _P, _I, _I64, _I64, _I64, _P, _I64, _P],
     "mxq_layer_norm": [_P, _I, _I64, _P, _P, _I, _F, _P, _P, _P, _I64, _I64, _P],
-    "mxq_layer_norm_backward_strips": [_I64, _I64, _P],
-    "mxq_layer_norm_backward": [_P, _I, _I64, _P, _I, _I64, _P, _I64, _P, _P, _P, _I, _P, _P, _I64, _I64, _I64, _P],
+    "mxq_layer_norm_backward_workspace": [_I64, _I64, _P],
+    "mxq_layer_norm_backward": [_P, _I, _I64, _P, _I, _I64, _P, _I64, _P, _P, _P, _I, _P, _P, _I64, _I64, _P, _I64, _P],
+    "mxq_pad_rows": [_P, _I64, _I64, _P, _I64, _I64, _P],
+    "mxq_fp8_linear_workspace": [_I64, _I64, _I64, _P],
+    "mxq_fp8_linear": [_P, _I, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I, _I64, _I64, _I64, _P, _I64, _P],
+    "mxq_fp8_linear_backward_workspace": [_I64, _I64, _I64, _I, _I, _I, _I, _P],
+    "mxq_fp8_linear_backward": [_P, _I, _I64, _I, _P, _I64, _P, _I64, _I, _P, _I64, _P, _I64, _P, _P, _P, _I, _I64, _I64, _I64,
+                                _P, _I64, _P],
 }
 
 _lib = None

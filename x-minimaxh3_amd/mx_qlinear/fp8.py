@@ -82,10 +82,13 @@ def _pair(q: torch.Tensor, scale: torch.Tensor, what: str = "activation"):
 
 
 def _pad(t: torch.Tensor, ld: int) -> torch.Tensor:
-    """A copy of 1-byte rows with row stride ``ld``, zeros behind them."""
-    out = torch.zeros((t.shape[0], ld), dtype=torch.uint8, device=t.device)
-    out[:, : t.shape[1]] = t.view(torch.uint8)
-    return out.view(t.dtype)
+    """A copy of 1-byte rows with row stride ``ld`` (rounded up to 16), zeros behind them."""
+    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    m, width = t.shape
+    out = torch.empty((m, _ceil(ld, 16)), dtype=t.dtype, device=t.device)
+    _launch(t.device, "mxq_pad_rows", t.data_ptr(), t.stride(0) if m > 1 else width, width, out.data_ptr(), out.shape[1], m)
+    return out
 
 
 def _operand(q: torch.Tensor, scale: torch.Tensor, k: int):
@@ -198,11 +201,16 @@ def prepare_fp8_weight(weight: torch.Tensor, scale: torch.Tensor | None = None, 
 # ---------------------------------------------------------------------------------------
 
 @functools.lru_cache(maxsize=4096)
-def _gemm_bytes(m: int, n: int, k: int, index: int) -> int:
+def _workspace(name: str, index: int, *sizes: int) -> int:
+    """The library's answer to a workspace query ``name`` for device ``index``, asked with it current."""
     out = ctypes.c_int64()
     with torch.cuda.device(index):
-        _lib.call("mxq_fp8_gemm_workspace", m, n, k, ctypes.byref(out))
+        _lib.call(name, *sizes, ctypes.byref(out))
     return out.value
+
+
+def _room(need: int, dev) -> torch.Tensor | None:
+    return torch.empty(need, dtype=torch.uint8, device=dev) if need else None
 
 
 def _product(dev, a, sa, m: int, k: int, b, sb, n: int, bias, out_dtype) -> torch.Tensor:
@@ -215,8 +223,8 @@ def _product(dev, a, sa, m: int, k: int, b, sb, n: int, bias, out_dtype) -> torc
         _launch(dev, "mxq_fp8_linear_rows", a.data_ptr(), _lib.DTYPE_E4M3, a.stride(0), sa.data_ptr(), sa.stride(0), b.data_ptr(),
                 b.stride(0), sb.data_ptr(), sb.stride(0), _ptr(bias), out.data_ptr(), n, code, m, n, k)
         return out
-    need = _gemm_bytes(m, n, k, dev.index)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    need = _workspace("mxq_fp8_gemm_workspace", dev.index, m, n, k)
+    ws = _room(need, dev)
     _launch(dev, "mxq_fp8_gemm", a.data_ptr(), a.stride(0), sa.data_ptr(), sa.stride(0), b.data_ptr(), b.stride(0), sb.data_ptr(),
             sb.stride(0), _ptr(bias), out.data_ptr(), n, code, m, n, k, _ptr(ws), need)
     return out
@@ -242,15 +250,15 @@ def fp8_linear(x: torch.Tensor, weight: PreparedFp8Weight, bias: torch.Tensor | 
     code = _out_code(out_dtype)
     n, k = weight.out_features, weight.in_features
     bias = _bias(bias, n, out_dtype, dev)
-    m = x.numel() // k
-    if 0 < m <= _FUSED_ROWS:
-        x2 = _rows_in_place(x, k)
-        out = torch.empty((m, n), dtype=out_dtype, device=dev)
-        _launch(dev, "mxq_fp8_linear_rows", x2.data_ptr(), xcode, x2.stride(0) if m > 1 else k, None, 0, weight.q.data_ptr(),
-                weight.q.shape[1], weight.scale.data_ptr(), weight.scale.shape[1], _ptr(bias), out.data_ptr(), n, code, m, n, k)
-        return out if x.dim() == 2 else out.reshape(*x.shape[:-1], n)
-    q, s, m, k = _quantize_rows(x)
-    out = _product(dev, q, s, m, k, weight.q, weight.scale, n, bias, out_dtype)
+    x2 = _rows_in_place(x, k)
+    m = x2.shape[0]
+    out = torch.empty((m, n), dtype=out_dtype, device=dev)
+    if m:
+        q, s = weight.q, weight.scale
+        need = 0 if m <= _FUSED_ROWS else _workspace("mxq_fp8_linear_workspace", dev.index, m, n, k)
+        ws = _room(need, dev)
+        _launch(dev, "mxq_fp8_linear", x2.data_ptr(), xcode, x2.stride(0) if m > 1 else k, q.data_ptr(), q.shape[1], s.data_ptr(),
+                s.shape[1], _ptr(bias), out.data_ptr(), n, code, m, n, k, _ptr(ws), need)
     return out if x.dim() == 2 else out.reshape(*x.shape[:-1], n)
 
 
@@ -274,37 +282,12 @@ def fp8_linear_prequantized(q: torch.Tensor, scale: torch.Tensor, weight: Prepar
 # gradients
 # ---------------------------------------------------------------------------------------
 
-@functools.lru_cache(maxsize=4096)
-def _wgrad_bytes(m: int, n: int, k: int, parts: int, index: int) -> int:
-    out = ctypes.c_int64()
-    with torch.cuda.device(index):
-        _lib.call("mxq_fp8_wgrad_workspace", m, n, k, parts, ctypes.byref(out))
-    return out.value
-
-
-@functools.lru_cache(maxsize=4096)
-def _strips(name: str, m: int, n: int, index: int) -> int:
-    out = ctypes.c_int64()
-    with torch.cuda.device(index):
-        _lib.call(name, m, n, ctypes.byref(out))
-    return out.value
-
-
-def _column_join(dev, sums: torch.Tensor, n: int, dtype: torch.dtype) -> torch.Tensor:
-    out = torch.empty(n, dtype=dtype, device=dev)
-    _launch(dev, "mxq_column_join", sums.data_ptr(), sums.shape[0], n, out.data_ptr(), _OUT_CODES[dtype])
-    return out
-
-
 def _readable(t: torch.Tensor, width: int) -> bool:
     """Whether every row of ``t`` (1-byte elements) can be read ``width`` wide from 16-byte boundaries."""
     m, ld = t.shape[0], t.stride(0)
     if t.data_ptr() % 16 or (m > 1 and (ld % 16 or ld < width)):
         return False
     return t.untyped_storage().nbytes() - t.storage_offset() >= (m - 1) * ld + width
-
-
-_PARTS = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}
 
 
 def fp8_linear_backward(dy: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, weight: PreparedFp8Weight,
@@ -330,35 +313,24 @@ def fp8_linear_backward(dy: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, 
         raise ValueError("the input's gradient needs the transposed weight (prepare_fp8_weight(..., transposed=True))")
     dev = _require_gpu(dy, q, scale, weight.q)
     y = _rows_in_place(dy, n)
-    ldy = y.stride(0) if m > 1 else max(y.stride(0), n)
-    nb = -(-n // BLOCK)
-    parts, n_parts = None, 0
-    if want_w and m and not (dy.dtype == torch.bfloat16 and n % 16 == 0 and y.data_ptr() % 16 == 0 and ldy % 8 == 0):
-        n_parts = _PARTS[dy.dtype]
-        parts = torch.empty((n_parts, m, nb * BLOCK), dtype=torch.bfloat16, device=dev)
-    yq = ys = None
-    if want_x:
-        yq, ys = _new_pair(m, n, dev)
-    strips = _strips("mxq_fp8_grad_strips", m, n, dev.index) if want_b else 0
-    sums = torch.empty((strips, n), dtype=torch.float32, device=dev) if want_b else None
-    if m and (want_x or want_b or n_parts):
-        _launch(dev, "mxq_fp8_grad_pass", y.data_ptr(), code, ldy, _ptr(yq), nb * BLOCK, _ptr(ys), ys.shape[1] if want_x else 0,
-                _ptr(parts), n_parts, nb * BLOCK, _ptr(sums), strips, m, n)
-    dx = dw = db = None
-    if want_x:
-        dx = _product(dev, yq, ys, m, n, weight.qt, weight.scale_t, k, None, dy.dtype).reshape(shape)
-    if want_w:
-        if m and not _readable(q, _ceil(k, 16)):
-            q = _pad(q, _ceil(k, BLOCK))
-        need = _wgrad_bytes(m, n, k, n_parts or 1, dev.index)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        dw = torch.empty((n, k), dtype=grad_dtype, device=dev)
-        src, ld = (parts, nb * BLOCK) if n_parts else (y, ldy)
-        _launch(dev, "mxq_fp8_wgrad", src.data_ptr(), n_parts or 1, max(ld, _ceil(n, 16)), q.data_ptr(),
-                q.stride(0) if m > 1 else _ceil(k, 16), scale.data_ptr(), max(scale.stride(0), scale.shape[1]), dw.data_ptr(), gcode, m, n, k,
-                _ptr(ws), need)
-    if want_b:
-        db = _column_join(dev, sums, n, grad_dtype)
+    ldy = y.stride(0) if m > 1 else n
+    direct = dy.dtype == torch.bfloat16 and n % 16 == 0 and ldy % 8 == 0 and y.data_ptr() % 16 == 0
+    readable = _readable(q, _ceil(k, 16))
+    dx = torch.empty((m, k), dtype=dy.dtype, device=dev) if want_x else None
+    dw = torch.empty((n, k), dtype=grad_dtype, device=dev) if want_w else None
+    db = torch.empty(n, dtype=grad_dtype, device=dev) if want_b else None
+    # (without rows dx is empty, and its pointer may be null)
+    needs = (1 if want_x and m else 0) | (2 if want_w else 0) | (4 if want_b else 0)
+    if needs:
+        need = _workspace("mxq_fp8_linear_backward_workspace", dev.index, m, n, k, code, direct, readable, needs)
+        ws = _room(need, dev)
+        bt, st = weight.qt, weight.scale_t
+        _launch(dev, "mxq_fp8_linear_backward", y.data_ptr(), code, ldy, direct, q.data_ptr(),
+                q.stride(0) if m > 1 else _ceil(k, 16) if readable else k, scale.data_ptr(), max(scale.stride(0), scale.shape[1]),
+                readable, _ptr(bt), bt.shape[1] if want_x else 0, _ptr(st), st.shape[1] if want_x else 0,
+                dx.data_ptr() if want_x and m else None, _ptr(dw), _ptr(db), gcode, m, n, k, _ptr(ws), need)
+    if want_x and len(shape) != 2:
+        dx = dx.reshape(shape)
     return dx, dw, db
 
 
@@ -433,17 +405,17 @@ def layer_norm_backward(dy: torch.Tensor, x, mean: torch.Tensor, rstd: torch.Ten
     dev = _require_gpu(dy, x2, xs, mean, rstd, weight)
     w, _, pcode = _norm_params(d, dev, dy.dtype, weight, None)
     dx = torch.empty((m, d), dtype=dy.dtype, device=dev)
-    strips = _strips("mxq_layer_norm_backward_strips", m, d, dev.index) if needs_params else 0
-    sums = torch.empty((strips, 2 * d), dtype=torch.float32, device=dev) if needs_params else None
-    if m:
+    both = torch.empty((2, d), dtype=torch.float32, device=dev) if needs_params else None
+    need = _workspace("mxq_layer_norm_backward_workspace", dev.index, m, d) if needs_params else 0
+    ws = _room(need, dev)
+    if m or needs_params:
         mean, rstd = mean.contiguous(), rstd.contiguous()
         _launch(dev, "mxq_layer_norm_backward", y2.data_ptr(), code, max(y2.stride(0), d), x2.data_ptr(), xcode, max(x2.stride(0), d),
-                _ptr(xs), ldxs, mean.data_ptr(), rstd.data_ptr(), _ptr(w), pcode, dx.data_ptr(), _ptr(sums), strips, m, d)
+                _ptr(xs), ldxs, mean.data_ptr(), rstd.data_ptr(), _ptr(w), pcode, dx.data_ptr(), _ptr(both), m, d, _ptr(ws), need)
     dx = dx if dy.dim() == 2 else dx.reshape(dy.shape)
     if not needs_params:
         return dx, None, None
-    both = _column_join(dev, sums, 2 * d, torch.float32)
-    return dx, both[:d], both[d:]
+    return dx, both[0], both[1]
 
 
 # ---------------------------------------------------------------------------------------

@@ -524,7 +524,7 @@ int mxq_fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa,
                  int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
- * The same for few rows. x_dtype MXQ_DTYPE_E4M3: x holds codes, sx their scales, M <= 64. Otherwise x [M, ldx] is
+ * The same for few rows. x_dtype MXQ_DTYPE_E4M3: x holds codes, sx their scales, M <= 32. Otherwise x [M, ldx] is
  * quantized on the way, with the codes mxq_fp8_quantize_rows gives: M <= 16.
  */
 int mxq_fp8_linear_rows(const void* x, int x_dtype, int64_t ldx, const uint8_t* sx, int64_t ldsx, const uint8_t* b,

@@ -172,6 +172,27 @@ MXQ_DEVICE uint32_t max8(uint32_t v) {
   return max(v, lane_xor4(v));
 }
 
+// The scale byte of a block held by eight lanes.
+template <int kCode>
+MXQ_DEVICE uint32_t block_scale_byte(const Piece<kCode>& p) {
+  uint32_t m = max8(piece_absmax(p));
+  if (m >= 0x7F800000u) m = max8(piece_absmax_finite(p));  // (the same for the eight lanes of a block)
+  return fp8_scale_byte(m);
+}
+
+// The sum of `n` vectors, `stride` apart, in order; eight loads are in flight.
+MXQ_DEVICE v4f sum_slices(const v4f* p, int n, int64_t stride) {
+  v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < n; s += 8) {
+    v4f t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = s + i < n ? p[(s + i) * stride] : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y += t[i];
+  }
+  return y;
+}
+
 // Stores 4 float values from column `col` on, as kCode; `n` of them are inside the row.
 template <int kCode>
 MXQ_DEVICE void store_run4(void* row, int64_t col, int n, const float* y) {

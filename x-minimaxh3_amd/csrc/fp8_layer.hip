@@ -35,7 +35,7 @@ Pair take_pair(Carve& c, int64_t rows, int64_t cols) {
   return p;
 }
 
-constexpr int64_t kFused = 16, kFew = 64;  // rows that the few-row product quantizes itself, and takes at all
+constexpr int64_t kFused = 16, kFew = 32;  // rows that the few-row product quantizes itself, and takes at all
 
 struct ForwardSpace {
   Pair x;

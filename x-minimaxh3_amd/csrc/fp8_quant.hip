@@ -6,13 +6,6 @@ namespace mxq {
 // ---- rows: one scale per 1 x 128 block ----
 // Eight lanes hold a block, 16 elements each, so a wave's loads cover whole lines, a block's maximum stays inside
 // eight lanes and every lane stores 16 codes. HBM-bound.
-template <int kCode>
-MXQ_DEVICE uint32_t block_scale_byte(const Piece<kCode>& p) {
-  uint32_t m = max8(piece_absmax(p));
-  if (m >= 0x7F800000u) m = max8(piece_absmax_finite(p));  // (the same for the eight lanes of a block)
-  return fp8_scale_byte(m);
-}
-
 constexpr int kRowUnroll = 4;
 
 template <int kCode>
@@ -263,18 +256,27 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* src, int64
   *reinterpret_cast<v4u*>(dst + row * ldd + col) = v;
 }
 
-// out[c] = sum over `parts` rows of a float32 [parts, n] table, in row order by eighths: the columns' last sum.
+// out[c] = sum over `parts` rows of a float32 [parts, n] table: the columns' last sum. 32 columns (a line) and 32
+// shares of the rows per workgroup: a share's loads go out eight at a time, so there are many shares.
 template <int kCode>
-__global__ __launch_bounds__(256) void column_join_kernel(const float* in, int64_t parts, int64_t n, void* out) {
-  __shared__ float sm[8][32];
+__global__ __launch_bounds__(1024) void column_join_kernel(const float* in, int64_t parts, int64_t n, void* out) {
+  __shared__ float sm[32][32];
   const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
   const int64_t col = (int64_t)blockIdx.x * 32 + c;
   float v = 0.0f;
   if (col < n) {
 #pragma unroll 8
-    for (int64_t i = r; i < parts; i += 8) v += in[i * n + col];
+    for (int64_t i = r; i < parts; i += 32) v += in[i * n + col];
   }
   sm[r][c] = v;
+  __syncthreads();
+  if (r < 8) {
+    v = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v += sm[r * 4 + k][c];
+  }
+  __syncthreads();
+  if (r < 8) sm[r][c] = v;
   __syncthreads();
   if (r == 0 && col < n) {
     v = 0.0f;
@@ -412,7 +414,7 @@ extern "C" int mxq_column_join(const float* in, int64_t parts, int64_t n, void* 
   if (!float_dtype(out_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported output dtype code %d", out_dtype);
   if (parts < 0 || n < 1 || n >= (1ll << 36) || !out || (parts && !in)) return mxq_set_error(MXQ_ERR_INVALID, "bad argument");
   with_dtype(out_dtype, [&](auto C) {
-    hipLaunchKernelGGL((column_join_kernel<decltype(C)::value>), dim3((unsigned)((n + 31) / 32)), dim3(256), 0,
+    hipLaunchKernelGGL((column_join_kernel<decltype(C)::value>), dim3((unsigned)((n + 31) / 32)), dim3(1024), 0,
                        (hipStream_t)stream, in, parts, n, out);
   });
   return mxq_check_launch("column_join_kernel");

@@ -410,7 +410,8 @@ static void with_forward_shape(int D, F&& f) {
 static int64_t norm_grad_grid(int64_t M, int64_t D, int cus) {
   const int64_t n = (D + 511) / 512, units = n <= 1 ? (M + 3) / 4 : M;
   const int64_t most = cus * (n <= 1 ? 5 : n <= 16 ? (20 / n > 1 ? 20 / n : 1) : 1);
-  return units < most ? units : most;
+  const int64_t few = units < cus ? units : units / 4 > cus ? units / 4 : cus;
+  return few < most ? few : most;
 }
 
 }  // namespace mxq

@@ -19,12 +19,12 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .ops import _OUT_CODES, _bias, _launch, _out_code, _ptr, _require_gpu, _rows
+from .ops import _OUT_CODES, _bias, _launch, _out_code, _ptr, _require_gpu, _rows, _vector
 
 BLOCK = 128
 _CODES, _SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
 # rows up to which a product streams the weight (mxq_fp8_linear_rows), and those it quantizes on the way
-_FEW_ROWS, _FUSED_ROWS = 64, 16
+_FEW_ROWS, _FUSED_ROWS = 32, 16
 
 
 def _ceil(n: int, to: int) -> int:
@@ -345,8 +345,8 @@ def _norm_params(d: int, dev, dtype, weight, bias):
             raise ValueError(f"layer norm {name} of shape {tuple(t.shape)}, expected ({d},)")
     given = [t for t in (weight, bias) if t is not None]
     target = dtype if all(t.dtype == dtype for t in given) else torch.float32
-    out = [None if t is None else t.detach().to(device=dev, dtype=target).contiguous() for t in (weight, bias)]
-    return out[0], out[1], _OUT_CODES[target]
+    return (None if weight is None else _vector(weight, target, dev), None if bias is None else _vector(bias, target, dev),
+            _OUT_CODES[target])
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
@@ -409,7 +409,7 @@ def layer_norm_backward(dy: torch.Tensor, x, mean: torch.Tensor, rstd: torch.Ten
     need = _workspace("mxq_layer_norm_backward_workspace", dev.index, m, d) if needs_params else 0
     ws = _room(need, dev)
     if m or needs_params:
-        mean, rstd = mean.contiguous(), rstd.contiguous()
+        mean, rstd = _vector(mean, torch.float32, dev), _vector(rstd, torch.float32, dev)
         _launch(dev, "mxq_layer_norm_backward", y2.data_ptr(), code, max(y2.stride(0), d), x2.data_ptr(), xcode, max(x2.stride(0), d),
                 _ptr(xs), ldxs, mean.data_ptr(), rstd.data_ptr(), _ptr(w), pcode, dx.data_ptr(), _ptr(both), m, d, _ptr(ws), need)
     dx = dx if dy.dim() == 2 else dx.reshape(dy.shape)

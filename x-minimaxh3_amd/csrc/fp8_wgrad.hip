@@ -251,7 +251,7 @@ static WgradPlan plan_wgrad(int64_t M, int64_t N, int64_t K, int parts, int cus)
     if (rows == 0 || (M + rows - 1) / rows != s || (s > 1 && tiles * s > 4 * cus)) continue;
     const double rounds = (double)((tiles * s + cus - 1) / cus);
     double cost = rounds * ((double)(rows / kWRows) * parts * 1.5 + 4.5);
-    if (s > 1) cost += 4.0 + (double)(N * K) * (double)(s + 1) / 1.3e6;
+    if (s > 1) cost += 4.0 + (double)(N * K) * (double)(s + 1) / 1.0e6;
     if (cost < best_cost) {
       best_cost = cost;
       best = {(int)s, rows};

@@ -312,9 +312,20 @@ MXQ_DEVICE uint32_t out_pair(float a, float b) {  // two 16-bit values
 template <int kOut>
 MXQ_DEVICE v4f bias_run(const void* bias, int col, int N) {
   v4f b = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (bias) {
+  if (!bias) return b;
+  const typename OutT<kOut>::T* p = reinterpret_cast<const typename OutT<kOut>::T*>(bias);
+  if (col + 4 > N) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) b[e] = OutT<kOut>::load(reinterpret_cast<const typename OutT<kOut>::T*>(bias) + min(col + e, N - 1));
+    for (int e = 0; e < 4; ++e) b[e] = OutT<kOut>::load(p + min(col + e, N - 1));
+  } else if constexpr (kOut == MXQ_DTYPE_F32) {
+    b = *reinterpret_cast<const v4f_any*>(p + col);
+  } else {
+    const v2u w = *reinterpret_cast<const v2u_any*>(p + col);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t h = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
+      b[e] = kOut == MXQ_DTYPE_F16 ? f16_to_f32(h) : bf16_to_f32(h);
+    }
   }
   return b;
 }
@@ -328,6 +339,13 @@ MXQ_DEVICE void epilogue(const Fp8Gemm& p, char* lds, const v16f (&acc)[C::kBI][
   const bool lines = p.vec && M - m0 >= C::kBM && N - n0 >= kTileN;
   const int lr = lane & 31, lh = lane >> 5;
   char* out = reinterpret_cast<char*>(d);
+  v4f bias[kSplit ? 1 : C::kBJ][4];  // (read once, ahead of the first piece's stores)
+  if constexpr (!kSplit) {
+#pragma unroll
+    for (int j = 0; j < C::kBJ; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) bias[j][q] = bias_run<kOut>(p.bias, n0 + wcol + j * 32 + q * 8 + lh * 4, N);
+  }
 #pragma unroll
   for (int i = 0; i < C::kBI; ++i) {
     const int row0 = m0 + wrow + i * 32;
@@ -338,10 +356,9 @@ MXQ_DEVICE void epilogue(const Fp8Gemm& p, char* lds, const v16f (&acc)[C::kBI][
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int col = col0 + q * 8 + lh * 4;
-        const v4f b = kSplit ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : bias_run<kOut>(p.bias, col, N);
         float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = kSplit ? acc[i][j][q * 4 + e] : acc[i][j][q * 4 + e] + b[e];
+        for (int e = 0; e < 4; ++e) y[e] = kSplit ? acc[i][j][q * 4 + e] : acc[i][j][q * 4 + e] + bias[kSplit ? 0 : j][q][e];
         if (!lines) {
           const int row = row0 + lr;
           if (row < M) store_run4<kOut>(out + row * p.ldd * kElem, col, N - col, y);
@@ -628,7 +645,7 @@ static Fp8Plan plan_fp8(int64_t M, int64_t N, int64_t kb, int cus) {
       const double rounds = (double)((tiles * s + cus - 1) / cus);
       const double stages = (double)(per < kb ? per : kb);
       double cost = rounds * (stages * (tile == 256 ? 1.35 : 0.72) + 5.0);
-      if (s > 1) cost += 4.0 + (double)(M * N) * (double)(s + 1) / 1.3e6;
+      if (s > 1) cost += 4.0 + (double)(M * N) * (double)(s + 1) / 1.0e6;
       if (cost < best_cost) {
         best_cost = cost;
         best = {tile, (int)s, (int)per};

@@ -25,6 +25,7 @@ BLOCK = 128
 _CODES, _SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
 # rows up to which a product streams the weight (mxq_fp8_linear_rows), and those it quantizes on the way
 _FEW_ROWS, _FUSED_ROWS = 32, 16
+_MAX_STRIDE = 1 << 22  # of an operand's rows; wider ones are copied
 
 
 def _ceil(n: int, to: int) -> int:
@@ -95,9 +96,9 @@ def _operand(q: torch.Tensor, scale: torch.Tensor, k: int):
     """A pair as the matrix products read it: code rows of whole, zero-padded blocks from 16-byte boundaries, scale rows
     of whole words. Pairs of this module's quantizers of whole blocks pass as they are; others are copied."""
     kb = -(-k // BLOCK)
-    if k % BLOCK or q.stride(0) % 16 or q.data_ptr() % 16 or q.stride(0) < k:
+    if k % BLOCK or q.stride(0) % 16 or q.data_ptr() % 16 or not k <= q.stride(0) <= _MAX_STRIDE:
         q = _pad(q, kb * BLOCK)
-    if scale.stride(0) % 4 or scale.data_ptr() % 4 or scale.stride(0) < _ceil(kb, 4):
+    if scale.stride(0) % 4 or scale.data_ptr() % 4 or not _ceil(kb, 4) <= scale.stride(0) <= _MAX_STRIDE // 4:
         scale = _pad(scale, _ceil(kb, 4))
     return q, scale
 
@@ -340,11 +341,13 @@ def fp8_linear_backward(dy: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, 
 
 def _norm_params(d: int, dev, dtype, weight, bias):
     """Weight and bias as the kernels read them: both of x's dtype or both float32."""
+    target = dtype
     for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and (t.numel() != d or t.dim() != 1):
-            raise ValueError(f"layer norm {name} of shape {tuple(t.shape)}, expected ({d},)")
-    given = [t for t in (weight, bias) if t is not None]
-    target = dtype if all(t.dtype == dtype for t in given) else torch.float32
+        if t is not None:
+            if t.shape != (d,):
+                raise ValueError(f"layer norm {name} of shape {tuple(t.shape)}, expected ({d},)")
+            if t.dtype != dtype:
+                target = torch.float32
     return (None if weight is None else _vector(weight, target, dev), None if bias is None else _vector(bias, target, dev),
             _OUT_CODES[target])
 
@@ -415,7 +418,8 @@ def layer_norm_backward(dy: torch.Tensor, x, mean: torch.Tensor, rstd: torch.Ten
     dx = dx if dy.dim() == 2 else dx.reshape(dy.shape)
     if not needs_params:
         return dx, None, None
-    return dx, both[0], both[1]
+    dw, db = both.unbind(0)
+    return dx, dw, db
 
 
 # ---------------------------------------------------------------------------------------

@@ -375,3 +375,70 @@ def test_modules_are_not_captured(dev):
         torch.cuda.synchronize()
         with torch.no_grad():
             assert torch.equal(y, module(x))
+
+
+def test_views_that_end_their_storage(dev):
+    """Operands that are the last columns of wider tensors: nothing behind their last row is read (the guard values would
+    show in no result; the reads' bounds are the kernel's), and the results are those of copies."""
+    mx = _mx()
+    m, n, k = 150, 272, 384
+    x, w = _acts(m, 2 * k, torch.bfloat16, 1), _acts(n, k, torch.float32, 2) * 0.05
+    p = mx.prepare_fp8_weight(w.to(dev))
+    q, s = mx.quantize_fp8_block128(x.to(dev))
+    dy = (_acts(m, 2 * n, torch.bfloat16, 3) * 0.01).to(dev)
+    dv, qv, sv = dy[:, n:], q[:, k:], s[:, 3:]
+    got = mx.fp8_linear_backward(dv, qv, sv, p)
+    want = mx.fp8_linear_backward(dv.contiguous(), qv.contiguous(), sv.contiguous(), p)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(mx.fp8_linear_prequantized(qv, sv, p), mx.fp8_linear_prequantized(qv.contiguous(), sv.contiguous(), p))
+    xv, d = ob.rows(x[:, k:])[0], dv.double().cpu()
+    _check_sum(got[1], d.t() @ xv, d.abs().t() @ xv.abs(), 216)
+    # rows further apart than the products take: copied
+    far = torch.zeros(2, 5_000_000, dtype=torch.float8_e4m3fn, device=dev)
+    far[:, :k] = q[:2, :k]
+    y = mx.fp8_linear_prequantized(far[:, :k], s[:2, :3], p)
+    assert torch.equal(y, mx.fp8_linear_prequantized(q[:2, :k].contiguous(), s[:2, :3].contiguous(), p))
+    # a gradient that is one value, expanded
+    ones = torch.ones((), dtype=torch.bfloat16, device=dev).expand(m, n)
+    a, b = mx.fp8_linear_backward(ones, qv, sv, p), mx.fp8_linear_backward(ones.contiguous(), qv, sv, p)
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_layer_norm_of_more_rows_than_a_grid_axis(dev):
+    """2^26 rows and some: a row per wave is more than 2^32 threads."""
+    mx = _mx()
+    m = 2**26 + 5
+    x = torch.zeros(m, 2, dtype=torch.bfloat16, device=dev)
+    x[:, 0] = 1.0
+    x[-3:, 1] = 3.0
+    y = mx.layer_norm(x, eps=0.0)
+    assert bool((y[: m - 3, 0] == 1).all()) and bool((y[: m - 3, 1] == -1).all())
+    assert bool((y[m - 3 :, 0] == -1).all()) and bool((y[m - 3 :, 1] == 1).all())
+
+
+def test_quantizers_from_a_replayed_graph(dev):
+    """Each replay gives what an eager call on the same input gives, with eager work between."""
+    mx = _mx()
+    inputs = [_acts(70, 333, torch.float16, i).to(dev) for i in range(4)]
+    w = _acts(200, 333, torch.float32, 9).to(dev)
+    static = inputs[0].clone()
+
+    def step(x):
+        q, s = mx.quantize_fp8_block128(x)
+        p = mx.prepare_fp8_weight(w)
+        return (q.view(torch.uint8), s.view(torch.uint8), mx.dequantize_fp8_block128(q, s, torch.float32),
+                mx.fp8_linear_prequantized(q, s, p), mx.fp8_linear(x[:9], p), *mx.fp8_linear_backward(mx.fp8_linear(x, p), q, s, p))
+
+    step(static)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for x in (inputs[1], inputs[2], inputs[3], inputs[1]):
+        static.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        want = step(x)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -237,23 +237,23 @@ __global__ __launch_bounds__(256) void fp8_grad_pass_kernel(const char* x, int64
 // Rows of bytes copied to 16-byte rows `ldd` apart, zeros behind their `width`: codes and scales whose own rows are not.
 __global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* src, int64_t lds, int width, uint8_t* dst, int ldd,
                                                        int64_t total) {
-  const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (g >= total) return;
   const int pieces = ldd / 16;
-  const int64_t row = g / pieces;
-  const int col = (int)(g - row * pieces) * 16, n = width - col;
-  const uint8_t* s = src + row * lds + col;
-  v4u v = {0, 0, 0, 0};
-  if (n >= 16) {
-    v = *reinterpret_cast<const v4u_any*>(s);
-  } else if (n > 0) {
+  for (int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x; g < total; g += (int64_t)gridDim.x * 256) {
+    const int64_t row = g / pieces;
+    const int col = (int)(g - row * pieces) * 16, n = width - col;
+    const uint8_t* s = src + row * lds + col;
+    v4u v = {0, 0, 0, 0};
+    if (n >= 16) {
+      v = *reinterpret_cast<const v4u_any*>(s);
+    } else if (n > 0) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t b = s[min(i, n - 1)];
-      v[i >> 2] |= (i < n ? b : 0u) << (8 * (i & 3));
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t b = s[min(i, n - 1)];
+        v[i >> 2] |= (i < n ? b : 0u) << (8 * (i & 3));
+      }
     }
+    *reinterpret_cast<v4u*>(dst + row * ldd + col) = v;
   }
-  *reinterpret_cast<v4u*>(dst + row * ldd + col) = v;
 }
 
 // out[c] = sum over `parts` rows of a float32 [parts, n] table: the columns' last sum. 32 columns (a line) and 32
@@ -403,16 +403,16 @@ extern "C" int mxq_pad_rows(const uint8_t* src, int64_t lds, int64_t width, uint
                          (long long)ldd);
   if (rows == 0) return MXQ_OK;
   if (!src || !dst || !aligned16(dst)) return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
-  const int64_t total = rows * (ldd / 16);
-  if (total > (1ll << 38)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "too many rows");
-  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, (hipStream_t)stream, src, lds,
+  if (rows >= (1ll << 40)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "too many rows");
+  const int64_t total = rows * (ldd / 16), blocks = (total + 255) / 256;
+  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, (hipStream_t)stream, src, lds,
                      (int)width, dst, (int)ldd, total);
   return mxq_check_launch("pad_rows_kernel");
 }
 
 extern "C" int mxq_column_join(const float* in, int64_t parts, int64_t n, void* out, int out_dtype, void* stream) {
   if (!float_dtype(out_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported output dtype code %d", out_dtype);
-  if (parts < 0 || n < 1 || n >= (1ll << 36) || !out || (parts && !in)) return mxq_set_error(MXQ_ERR_INVALID, "bad argument");
+  if (parts < 0 || n < 1 || n >= (1ll << 27) || !out || (parts && !in)) return mxq_set_error(MXQ_ERR_INVALID, "bad argument");
   with_dtype(out_dtype, [&](auto C) {
     hipLaunchKernelGGL((column_join_kernel<decltype(C)::value>), dim3((unsigned)((n + 31) / 32)), dim3(1024), 0,
                        (hipStream_t)stream, in, parts, n, out);

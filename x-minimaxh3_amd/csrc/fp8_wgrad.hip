@@ -83,14 +83,15 @@ __global__ __launch_bounds__(kWThreads, 1) void fp8_wgrad_kernel(Wgrad p) {
   const int stages = (m_last - m_first + kWRows - 1) / kWRows, total = stages * p.parts;
 
   // A thread's share of a stage: rows tid / 16 + kStep j, columns 16 (tid % 16) .. + 15 of both operands, by buffer loads
-  // whose offsets point outside for what lies behind the slice's last row or the last column (they read zeros; columns of
-  // dY behind N hold another column's values, whose sums are not stored).
+  // whose offsets point outside for what lies behind the slice's last row or the last column (they read zeros). Nothing is
+  // read behind column N rounded up to 16 of dY or the last scale, where a view's last row may end its storage: the
+  // columns behind hold other columns' values, whose sums are not stored.
   constexpr int kStep = kWThreads / 16, kShare = kWRows / kStep;
   const int r = tid >> 4, c = (tid & 15) * 16;
   const int ldy = (int)p.ldy, ldq = (int)p.ldq, lds_ = (int)p.lds;
-  const uint32_t oy = (uint32_t)(r * ldy + min(n0 + c, max(ldy - 16, 0))) * 2;
+  const uint32_t oy = (uint32_t)(r * ldy + min(n0 + c, ((int)p.N + 15) / 16 * 16 - 16)) * 2;
   const uint32_t oq = k0 + c < (int)p.K ? (uint32_t)(r * ldq + k0 + c) : kBufferOff;
-  const uint32_t os = (uint32_t)(r * lds_ + min((k0 + c) >> 7, lds_ - 1));
+  const uint32_t os = (uint32_t)(r * lds_ + (min(k0 + c, (int)p.K - 1) >> 7));
   v4u ya[kShare], yb[kShare], xq[kShare];
   uint32_t xs[kShare];
   // (the position of the next load: rows left in the slice and the operands' rows; offsets of lanes with a row stay inside
@@ -291,7 +292,7 @@ extern "C" int mxq_fp8_wgrad(const void* dy, int parts, int64_t ldy, const uint8
     return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
   const WgradPlan plan = plan_wgrad(M, N, K, parts, mxq_cu_count());
   const int64_t tiles_n = (N + kWTile - 1) / kWTile, tiles_k = (K + kWTile - 1) / kWTile;
-  if (tiles_n * tiles_k * plan.splits >= (1ll << 31)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^31 tiles");
+  if (tiles_n * tiles_k * plan.splits >= (1ll << 23)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^23 tiles");
   const int64_t need = wgrad_bytes(plan, N, K);
   if (need > 0 && (!workspace || workspace_bytes < need || !wg_aligned(workspace, 16)))
     return mxq_set_error(MXQ_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
@@ -303,7 +304,6 @@ extern "C" int mxq_fp8_wgrad(const void* dy, int parts, int64_t ldy, const uint8
     p.d = workspace;
     p.ldd = ldp;
     const int64_t blocks = (N * (ldp / 4) + 255) / 256;
-    if (blocks >= (1ll << 31)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "gradient too large");
     hipLaunchKernelGGL((fp8_wgrad_kernel<MXQ_DTYPE_F32, true>), dim3(grid), dim3(kWThreads), 0, (hipStream_t)stream, p);
     if (const int rc = mxq_check_launch("fp8_wgrad_kernel")) return rc;
     with_dtype(out_dtype, [&](auto O) {

@@ -661,7 +661,6 @@ using namespace mxq;
 
 static bool aligned(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-
 template <int kTM, int kOut, bool kSplit, bool kWide>
 static int launch_gemm(const Fp8Gemm& p, void* stream) {
   hipLaunchKernelGGL((gemm_fp8_kernel<kTM, kOut, kSplit, kWide>), dim3((unsigned)(p.tiles_m * p.tiles_n * p.splits)), dim3(512),
@@ -675,7 +674,7 @@ static int64_t split_bytes(const Fp8Plan& plan, int64_t M, int64_t N) {
 
 static int check_product(int64_t M, int64_t N, int64_t K, int64_t ldb, int64_t ldsb, int64_t ldd, int out_dtype) {
   if (!float_dtype(out_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported output dtype code %d", out_dtype);
-  if (M < 0 || N < 1 || K < 1 || M > (1ll << 31) - 1024 || N > (1ll << 31) - 1024 || K > (1ll << 22))
+  if (M < 0 || N < 1 || K < 1 || M > (1ll << 31) - 1024 || N > (1ll << 27) || K > (1ll << 22))
     return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
   const int64_t kb = (K + 127) / 128;
   if (ldb < kb * 128 || ldb % 16 || ldb > (1ll << 22) + 4096 || ldsb < (kb + 3) / 4 * 4 || ldsb % 4 || ldsb > (1ll << 20) ||
@@ -703,7 +702,7 @@ extern "C" int mxq_fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, in
     return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
   const Fp8Plan plan = plan_fp8(M, N, kb, mxq_cu_count());
   const int64_t tiles_m = (M + plan.tile - 1) / plan.tile, tiles_n = (N + kTileN - 1) / kTileN;
-  if (tiles_m * tiles_n * plan.splits >= (1ll << 31)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^31 tiles");
+  if (tiles_m * tiles_n * plan.splits >= (1ll << 23)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^23 tiles");
   const int64_t need = split_bytes(plan, M, N);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return mxq_set_error(MXQ_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
@@ -722,8 +721,7 @@ extern "C" int mxq_fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, in
     else
       rc = wide ? launch_gemm<128, 0, true, true>(p, stream) : launch_gemm<128, 0, true, false>(p, stream);
     if (rc) return rc;
-    const int64_t blocks = (M * (ldp / 4) + 255) / 256;
-    if (blocks >= (1ll << 31)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "output too large");
+    const int64_t blocks = (M * (ldp / 4) + 255) / 256;  // (slices are for few tiles: far below 2^24)
     with_dtype(out_dtype, [&](auto O) {
       constexpr int kOut = decltype(O)::value;
       hipLaunchKernelGGL((fp8_join_kernel<kOut>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream,

@@ -182,7 +182,7 @@ __global__ __launch_bounds__(kOne ? 256 : 1024) void layer_norm_kernel(Norm p) {
   constexpr int kElem = Eight<kCode>::kElem;
   __shared__ float red[2][2][16];
   const int waves = kOne ? 1 : blockDim.x >> 6, wave = kOne ? 0 : threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t row = kOne ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, row = kOne ? block * 4 + (threadIdx.x >> 6) : block;
   if (row >= p.M) return;  // (whole waves; with several per row, whole workgroups)
   const char* x = p.x + row * p.ldx * kElem;
   Eight<kCode> raw[kChunks];
@@ -418,6 +418,9 @@ static int64_t norm_grad_grid(int64_t M, int64_t D, int cus) {
 
 using namespace mxq;
 
+// Workgroups across: a launch takes less than 2^32 threads along an axis.
+constexpr int64_t kNormGridX = 1 << 20;
+
 static int check_norm(int64_t M, int64_t D, int dtype, int wcode) {
   if (!float_dtype(dtype) || !float_dtype(wcode)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported dtype codes %d, %d", dtype, wcode);
   if (M < 0 || D < 1 || M >= (1ll << 31)) return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld D=%lld", (long long)M, (long long)D);
@@ -436,10 +439,11 @@ extern "C" int mxq_layer_norm(const void* x, int dtype, int64_t ldx, const void*
   with_forward_shape((int)D, [&](auto N, auto One, int threads) {
     with_dtype(dtype, [&](auto C) {
       constexpr bool kOne = decltype(One)::value;
-      const unsigned grid = (unsigned)(kOne ? (M + 3) / 4 : M);
+      const int64_t blocks = kOne ? (M + 3) / 4 : M;
+      const unsigned wide = (unsigned)(blocks < kNormGridX ? blocks : kNormGridX);
       with_bool(D % 8 == 0, [&](auto V) {
-        hipLaunchKernelGGL((layer_norm_kernel<decltype(C)::value, decltype(N)::value, kOne, decltype(V)::value>), dim3(grid),
-                           dim3(threads), 0, (hipStream_t)stream, p);
+        hipLaunchKernelGGL((layer_norm_kernel<decltype(C)::value, decltype(N)::value, kOne, decltype(V)::value>),
+                           dim3(wide, (unsigned)((blocks + wide - 1) / wide)), dim3(threads), 0, (hipStream_t)stream, p);
       });
     });
   });

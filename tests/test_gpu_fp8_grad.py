@@ -10,6 +10,8 @@ behind; 96 * 2^-24 where two such sums meet.
 
 from __future__ import annotations
 
+import copy
+
 import pytest
 import torch
 
@@ -339,9 +341,10 @@ def test_norm_and_layer_trained_together(dev, dtype, keep):
     with torch.no_grad():
         assert torch.equal(layer(norm(x)), out)
         layer.weight.mul_(2.0)
-        assert torch.equal(layer(norm(x)), out)  # (the form that was prepared)
+        changed = layer(norm(x))  # (the form follows the parameter)
+        assert not torch.equal(changed, out)
         layer.prepare()
-        assert not torch.equal(layer(norm(x)), out)
+        assert torch.equal(layer(norm(x)), changed)
 
 
 def test_frozen_layer_gives_the_inputs_gradient_only(dev):
@@ -442,3 +445,46 @@ def test_quantizers_from_a_replayed_graph(dev):
         want = step(x)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_the_module_follows_its_weight(dev):
+    """Without gradients the layer reads the parameter's present contents: after a step, a load, a move to another type, and
+    in a graph that was captured before any eager call."""
+    mx = _mx()
+    g = _gen(5)
+    x = torch.randn(40, 256, generator=g).to(torch.bfloat16).to(dev)
+    layer = mx.Fp8Linear(256, 96, device=dev, dtype=torch.float32)
+
+    def fresh():
+        return mx.fp8_linear(x, mx.prepare_fp8_weight(layer.weight.detach()), layer.bias.detach())
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad():
+        mx.fp8_linear(x, mx.prepare_fp8_weight(layer.weight), layer.bias)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            captured = layer(x)
+        assert torch.equal(layer(x), fresh())
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, fresh())
+    before = fresh()
+    opt = torch.optim.SGD(layer.parameters(), lr=0.5)
+    layer(x).float().sum().backward()
+    opt.step()
+    with torch.no_grad():
+        assert torch.equal(layer(x), fresh()) and not torch.equal(fresh(), before)
+        layer.load_state_dict({k: v * 2 for k, v in layer.state_dict().items()})
+        assert torch.equal(layer(x), fresh())
+        layer.bfloat16()
+        assert torch.equal(layer(x), fresh())
+        assert layer._form() is layer._form()
+        layer.weight = torch.nn.Parameter(layer.weight.detach() * 3)
+        assert torch.equal(layer(x), fresh())
+        assert torch.equal(copy.deepcopy(layer)(x), fresh())
+    layer.weight.requires_grad_(False)
+    xg = x.clone().requires_grad_()
+    layer(xg).float().sum().backward()
+    q, s = mx.quantize_fp8_block128(x)
+    want = mx.fp8_linear_backward(torch.ones(40, 96, device=dev, dtype=torch.bfloat16), q, s, mx.prepare_fp8_weight(layer.weight))
+    assert torch.equal(xg.grad, want[0])

@@ -468,11 +468,12 @@ class _Fp8LinearFn(torch.autograd.Function):
 class Fp8Linear(torch.nn.Module):
     """A linear layer computed in 8-bit floating point, for serving and for training.
 
-    ``weight`` ``[out_features, in_features]`` and ``bias`` are ordinary parameters (bf16, fp16 or fp32). Without gradients
-    the layer runs :func:`fp8_linear` on the weight's 8-bit form, built by :meth:`prepare` (and again after a load or an
-    update, by calling it again); with gradients the form is built from the parameter in every forward, and what the
-    backward pass keeps of the input is its 8-bit pair (:func:`fp8_linear_backward`). The quantizers pass gradients
-    through unchanged. Activations are bf16, fp16 or fp32.
+    ``weight`` ``[out_features, in_features]`` and ``bias`` are ordinary parameters (bf16, fp16 or fp32). A weight that needs
+    no gradient is read in its 8-bit form, built by :meth:`prepare` or the first call, and again once the parameter was
+    moved, loaded or changed in place (changes through ``.data`` are not seen: call :meth:`prepare`). One that needs a
+    gradient has the form built from the parameter in every forward, and what the backward pass keeps of the input is its
+    8-bit pair (:func:`fp8_linear_backward`). The quantizers pass gradients through unchanged. Activations are bf16, fp16
+    or fp32.
     """
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None):
@@ -482,26 +483,33 @@ class Fp8Linear(torch.nn.Module):
         self.bias = torch.nn.Parameter(torch.zeros(out_features, device=device, dtype=dtype)) if bias else None
         torch.nn.init.normal_(self.weight, std=in_features**-0.5)
         self._prepared: PreparedFp8Weight | None = None
+        self._prepared_of = None
+
+    def _state(self):
+        """What changes with the parameter's contents: the parameter, its storage and its count of changes in place."""
+        w = self.weight
+        return (w,), w.data_ptr(), w.dtype, w.device, None if w.is_inference() else w._version
 
     def prepare(self) -> "Fp8Linear":
         """Builds the weight's 8-bit form from its present contents, for calls without weight gradients."""
-        self._prepared = prepare_fp8_weight(self.weight)
+        self._prepared, self._prepared_of = prepare_fp8_weight(self.weight), self._state()
         return self
+
+    def _form(self) -> PreparedFp8Weight:
+        now, then = self._state(), self._prepared_of
+        if then is not None and then[0][0] is now[0][0] and then[1:] == now[1:]:
+            return self._prepared
+        if self.weight.is_cuda and torch.cuda.is_current_stream_capturing():
+            return prepare_fp8_weight(self.weight)  # (part of the graph, filled by its replays only: not kept)
+        return self.prepare()._prepared
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dim() < 1 or x.shape[-1] != self.in_features:
             raise ValueError(f"input of shape {tuple(x.shape)} for a layer of {self.in_features} input features")
         params = [p for p in (self.weight, self.bias) if p is not None]
         if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, *params))):
-            if self._prepared is None:
-                self.prepare()
-            return fp8_linear(x, self._prepared, self.bias)
-        if self.weight.requires_grad or self._prepared is None or self._prepared.qt is None:
-            prepared = prepare_fp8_weight(self.weight)
-            if not self.weight.requires_grad:
-                self._prepared = prepared
-        else:
-            prepared = self._prepared
+            return fp8_linear(x, self._form(), self.bias)
+        prepared = prepare_fp8_weight(self.weight) if self.weight.requires_grad else self._form()
         return _Fp8LinearFn.apply(x, self.weight, self.bias, prepared)
 
     def extra_repr(self) -> str:

@@ -33,6 +33,19 @@ def test_oracle_exponents():
     assert bool((a <= 448 * s).all())
 
 
+def test_oracle_layer_norm_is_autograds():
+    g = torch.Generator().manual_seed(4)
+    x, w, b, dy = (torch.randn(n, 37, generator=g, dtype=torch.float64) for n in (6, 1, 1, 6))
+    w, b = w[0], b[0]
+    xs = [t.clone().requires_grad_() for t in (x, w, b)]
+    y = torch.nn.functional.layer_norm(xs[0], (37,), xs[1], xs[2], 1e-5)
+    y.backward(dy)
+    got, mean, rstd = ob.layer_norm(x, w, b, 1e-5)
+    torch.testing.assert_close(got, y.detach(), rtol=1e-12, atol=1e-12)
+    for a, t in zip(ob.layer_norm_backward(dy, x, mean, rstd, w), xs):
+        torch.testing.assert_close(a, t.grad, rtol=1e-11, atol=1e-11)
+
+
 def test_cpu_tensors_are_refused():
     mx = _mx()
     x = torch.zeros(4, 256)

@@ -18,6 +18,9 @@
 // converted to bfloat16 with their scales, exactly, and the sums run on v_mfma_f32_32x32x16_bf16, which keeps every
 // addend to float32's precision at half the rate.
 //
+// 75600 x 5120 of K 5120 takes 1.57 to 1.63 ms (2.5 PFLOP/s; 2.67 in the loop, from K 5120 against 10240 at 16384 x 4096):
+// the clock falls to about 1.85 GHz, power bounds it (a library's product 2.81).
+//
 // Problems of few tiles split K over workgroups, which write float32 sums that fp8_join_kernel adds in order.
 
 #include "fp8_common.h"

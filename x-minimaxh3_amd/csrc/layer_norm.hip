@@ -5,11 +5,11 @@
 //   dw = sum over rows of dy * xh,  db = sum over rows of dy
 //
 // A row is held in registers by as many waves as it has chunks of 512 elements (up to sixteen), eight elements per lane and
-// chunk, so x (and dy) are read once; the
-// variance is that of the centred values, not a difference of large sums. HBM-bound. The backward pass also keeps its
-// lanes' columns of dw and db in registers over all the rows a workgroup takes, writes them once per workgroup, and
-// column_join_kernel adds the workgroups' sums in a fixed order: no atomics, the same bits on every run. Its x can be
-// the input as it was kept in 8 bits (fp8_common.h), decoded as it is read.
+// chunk, so x (and dy) are read once; the variance is that of the centred values, not a difference of large sums.
+// HBM-bound: 75600 x 5120 bf16 forward 292 us (5.3 TB/s), backward from the input in 8 bits 384 + 8 us (4.9 TB/s). The
+// backward pass also keeps its lanes' columns of dw and db in registers over all the rows a workgroup takes, writes them
+// once per workgroup, and column_join_kernel adds the workgroups' sums in a fixed order: no atomics, the same bits on
+// every run. Its x can be the input as it was kept in 8 bits (fp8_common.h), decoded as it is read.
 
 #include "fp8_common.h"
 
@@ -406,7 +406,9 @@ static void with_forward_shape(int D, F&& f) {
   else go(integral_constant<int, 4>{});
 }
 
-// Workgroups of the backward pass: about twenty waves per CU (sixteen of the wide forms), each with an equal share of rows.
+// Workgroups of the backward pass: about twenty waves per CU (sixteen of the wide forms), each with an equal share of rows; four rows
+// at least once every CU has a workgroup, since each writes 2 D sums (777 x 1003: 256 workgroups 8.2 us and a join of 3.4,
+// one per row 10.6 and 6.0).
 static int64_t norm_grad_grid(int64_t M, int64_t D, int cus) {
   const int64_t n = (D + 511) / 512, units = n <= 1 ? (M + 3) / 4 : M;
   const int64_t most = cus * (n <= 1 ? 5 : n <= 16 ? (20 / n > 1 ? 20 / n : 1) : 1);

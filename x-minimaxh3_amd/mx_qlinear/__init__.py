@@ -4,7 +4,8 @@ Per-token INT8 activation quantization (optionally fused with adaLN), INT8 x INT
 GEMMs on CDNA4 matrix cores with fused dequant / bias / tanh-GELU / re-quant epilogues, and
 W4A8 GEMMs, with the ConvRot (regular Hadamard) rotation and the GELU / SwiGLU input
 activations folded into the quantizer, behind the reference's Comfy-Kitchen function names and its quantized-linear
-module contract. All compute runs in hand-written HIP kernels (libmx_qlinear.so, C ABI in
+module contract; and the 8-bit floating point layer (e4m3 with a power of two per block of 128) with its
+gradients, 8-bit activation checkpoints and the layer norm. All compute runs in hand-written HIP kernels (libmx_qlinear.so, C ABI in
 include/mx_qlinear.h); there is no CPU path.
 """
 

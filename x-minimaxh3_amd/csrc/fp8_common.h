@@ -180,6 +180,13 @@ MXQ_DEVICE uint32_t block_scale_byte(const Piece<kCode>& p) {
   return fp8_scale_byte(m);
 }
 
+// Orders a wave's LDS accesses: what its lanes wrote, its lanes read.
+MXQ_DEVICE void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // The sum of `n` vectors, `stride` apart, in order; eight loads are in flight.
 MXQ_DEVICE v4f sum_slices(const v4f* p, int n, int64_t stride) {
   v4f y = {0.0f, 0.0f, 0.0f, 0.0f};

@@ -62,6 +62,7 @@ MXQ_DEVICE v8bf join_fragment(const v4s (&f)[2]) {
   return __builtin_bit_cast(v8bf, v8s{f[0][0], f[0][1], f[0][2], f[0][3], f[1][0], f[1][1], f[1][2], f[1][3]});
 }
 
+static_assert(2 * 2 * kWStage / kWWaves >= 32 * 512, "LDS of a wave's block of results");
 static_assert(kWRows == 64, "a stage is four half steps, written in two parts");
 MXQ_DEVICE uint32_t buffer_load_u8(const void* base, int bytes, uint32_t voff) {
   return __builtin_amdgcn_raw_buffer_load_b8(
@@ -203,23 +204,34 @@ __global__ __launch_bounds__(kWThreads, 1) void fp8_wgrad_kernel(Wgrad p) {
   publish();
   static_for<kReads>([&](auto I) { read(0, std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{}, I); });
   for (int i = 0; i < total; ++i) stage();
-  // lane l holds row n = l % 32 of a block and, in register e, column (e / 4) * 8 + (l / 32) * 4 + e % 4
+  // Lane l holds row n = l % 32 of a block and, in register e, column (e / 4) * 8 + (l / 32) * 4 + e % 4. Stored from there, an
+  // instruction would touch 32 bytes of 32 rows; through the wave's 16 KB of LDS (no wave reads a stage any more: the last
+  // barrier is behind the last half step's reads) 32 lanes store a row's 128 columns. 16-byte piece c of row r sits at
+  // piece c ^ r.
   constexpr int kElem = kOut == MXQ_DTYPE_F32 ? 4 : 2;
   char* d = reinterpret_cast<char*>(p.d);
   if constexpr (kSplit) d += (int64_t)slice * p.N * p.ldd * 4;
   const int N = (int)p.N, K = (int)p.K;
+  char* turn = lds + wave * (2 * 2 * kWStage / kWWaves);
 #pragma unroll
   for (int a = 0; a < kWNB; ++a) {
-    const int n = n0 + wn + a * 32 + (lane & 31);
-    if (n >= N) continue;
+    wave_lds_fence();
+    const int r = lane & 31;
 #pragma unroll
     for (int b = 0; b < 4; ++b)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int k = k0 + wk + b * 32 + e * 8 + (lane >> 5) * 4;
-        const float v[4] = {acc[a][b][4 * e], acc[a][b][4 * e + 1], acc[a][b][4 * e + 2], acc[a][b][4 * e + 3]};
-        store_run4<kOut>(d + (int64_t)n * p.ldd * kElem, k, K - k, v);
-      }
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<v4f*>(turn + r * 512 + (((b * 8 + e * 2 + (lane >> 5)) ^ r) << 4)) =
+            v4f{acc[a][b][4 * e], acc[a][b][4 * e + 1], acc[a][b][4 * e + 2], acc[a][b][4 * e + 3]};
+    wave_lds_fence();
+    const int k = k0 + wk + (lane & 31) * 4;
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+      const int row = t * 2 + (lane >> 5), n = n0 + wn + a * 32 + row;
+      const v4f y = *reinterpret_cast<const v4f*>(turn + row * 512 + (((lane & 31) ^ row) << 4));
+      const float v[4] = {y[0], y[1], y[2], y[3]};
+      if (n < N) store_run4<kOut>(d + (int64_t)n * p.ldd * kElem, k, K - k, v);
+    }
   }
 }
 

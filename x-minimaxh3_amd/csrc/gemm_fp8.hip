@@ -299,12 +299,6 @@ MXQ_DEVICE void main_loop(char* lds, const Chunk<C::kLoadsA>& ca, const Chunk<C:
 // blocks), so that eight lanes store a whole line.
 MXQ_DEVICE char* out_stage_at(char* buf, int r, int c) { return buf + r * 128 + ((c ^ ((r >> 1) & 7)) << 4); }
 
-MXQ_DEVICE void wave_lds_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 template <int kOut>
 MXQ_DEVICE uint32_t out_pair(float a, float b) {  // two 16-bit values
   if constexpr (kOut == MXQ_DTYPE_BF16) return pack_bf16x2(a, b);

@@ -517,19 +517,11 @@ int mxq_fp8_gemm_workspace(int64_t M, int64_t N, int64_t K, int64_t* bytes);
  * d [M, N] = out(a b^T + bias): a codes [M, lda] with scales [M, ldsa] (1 x 128), b codes [N, ldb] with scales
  * [ceil(N / 128), ldsb] (128 x 128), both zero behind column K; bias [N] of out_dtype or NULL. Sums are float32.
  * bf16 and fp16 outputs use the e4m3 matrix instructions, which cut addends below 2^-13 of the largest of 64;
- * fp32 outputs keep every addend.
+ * fp32 outputs and up to 16 rows keep every addend.
  */
 int mxq_fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa, const uint8_t* b, int64_t ldb,
                  const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd, int out_dtype, int64_t M,
                  int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
-
-/*
- * The same for few rows. x_dtype MXQ_DTYPE_E4M3: x holds codes, sx their scales, M <= 32. Otherwise x [M, ldx] is
- * quantized on the way, with the codes mxq_fp8_quantize_rows gives: M <= 16.
- */
-int mxq_fp8_linear_rows(const void* x, int x_dtype, int64_t ldx, const uint8_t* sx, int64_t ldsx, const uint8_t* b,
-                        int64_t ldb, const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd, int out_dtype,
-                        int64_t M, int64_t N, int64_t K, void* stream);
 
 /* Row strips of mxq_fp8_grad_pass at this size on the current device. */
 int mxq_fp8_grad_strips(int64_t M, int64_t N, int64_t* strips);

@@ -121,10 +121,8 @@ def test_c_entries_refuse_before_any_launch():
     assert need.value > 0  # two tiles: K is split
     with pytest.raises(ValueError, match="workspace"):
         _call("mxq_fp8_gemm", ok, 16384, ok, 128, ok, 16384, ok, 128, None, ok, 256, 2, 128, 256, 16384, ok, need.value - 16)
-    with pytest.raises(_lib.MxqError, match="rows"):
-        _call("mxq_fp8_linear_rows", ok, 2, 256, None, 0, ok, 256, ok, 4, None, ok, 128, 2, 17, 128, 256)
     with pytest.raises(ValueError, match="activations"):
-        _call("mxq_fp8_linear_rows", ok, 2, 249, None, 0, ok, 256, ok, 4, None, ok, 128, 2, 4, 128, 250)
+        _call("mxq_fp8_linear", ok, 2, 249, ok, 256, ok, 4, None, ok, 128, 2, 4, 128, 250, None, 0)
     with pytest.raises(ValueError):
         _call("mxq_fp8_grad_pass", ok, 2, 256, ok, 256, ok, 4, ok, 2, 256, None, 0, 8, 256)
     # no rows: nothing to do, no pointer needed

@@ -2,7 +2,7 @@
 products within bounds derived from the arithmetic.
 
 Bounds. u(t) is half a step of the output type (bf16 2^-8 / 2 ..., i.e. torch.finfo(t).eps / 2), the last rounding. In
-front of it, float32 outputs (and all of up to 32 rows) sum exact bf16 x bf16 products in float32: at most one rounding
+front of it, float32 outputs (and all of up to 16 rows) sum exact bf16 x bf16 products in float32: at most one rounding
 of 2^-24 per addend, so |error| <= 2^-24 (K + 2) sum|p|. bf16 and fp16 outputs of more rows go through the e4m3
 instruction, which cuts each addend of a 64-long sum below 2^-13 of the largest: |error| <= 64 * 2^-13 max|p| per 64.
 Those are worst cases; the norms are held to (u + 2^-10) |y|, with cuts of independent sign (rms of a cut 2^-13 max|p|,
@@ -183,7 +183,9 @@ def test_strided_and_many_dimensional_inputs(dev):
 PRODUCTS = [(1, 1, 1), (1, 128, 128), (1, 100, 1000), (2, 33, 8), (16, 2049, 1280), (5, 700, 5000), (17, 96, 130), (33, 300, 1000),
             (64, 513, 640), (65, 300, 130), (128, 256, 128), (200, 256, 384), (256, 512, 1024), (333, 515, 2500),
             (700, 1000, 2048), (1025, 1300, 1152), (4100, 700, 520), (1, 40, 40000), (3, 17000, 300), (9, 70, 9001), (12, 50, 4608),
-            (16, 40, 2600), (32, 129, 3100)]
+            (16, 40, 2600), (32, 129, 3100), (5, 5000, 300), (16, 8000, 520), (1, 8200, 300), (16, 12200, 130), (9, 15300, 260),
+            (27, 15360, 130), (16, 20470, 300), (30, 20480, 200), (13, 21500, 300), (20, 24000, 130), (16, 32760, 130),
+            (31, 30000, 130), (1, 32768, 200), (16, 2000, 14336), (29, 2000, 14336), (1, 50000, 130)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -195,7 +197,7 @@ def test_linear(dev, dtype, m, n, k):
     p = mx.prepare_fp8_weight(w.to(dev))
     xv, wv = ob.rows(x)[0], ob.tiles(w)[0]
     b = None if bias is None else bias.to(dev)
-    wide = m <= 32 or dtype == torch.float32
+    wide = m <= 16 or dtype == torch.float32
     y = mx.fp8_linear(x.to(dev), p, b)
     assert y.dtype == dtype
     check_product(y, xv, wv, bias, wide)
@@ -213,7 +215,7 @@ def test_linear_output_types_and_shapes(dev, out, m):
     w = _acts(130, 520, torch.float32, 9) * 0.05
     y = mx.fp8_linear(x.to(dev), mx.prepare_fp8_weight(w.to(dev)), out_dtype=out)
     assert y.shape == (2, m, 130) and y.dtype == out
-    check_product(y.view(2 * m, 130), ob.rows(x.view(2 * m, 520))[0], ob.tiles(w)[0], None, 2 * m <= 32 or out == torch.float32)
+    check_product(y.view(2 * m, 130), ob.rows(x.view(2 * m, 520))[0], ob.tiles(w)[0], None, 2 * m <= 16 or out == torch.float32)
 
 
 def test_linear_of_no_rows(dev):

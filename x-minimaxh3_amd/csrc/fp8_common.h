@@ -27,6 +27,15 @@ typedef float v4f_any __attribute__((ext_vector_type(4), aligned(1)));
 namespace mxq {
 
 constexpr int kFp8Block = 128;
+
+// The few-row product (gemm_fp8.hip): rows that it takes as codes, and those it quantizes itself; whether it is the form to
+// take; and the product (M within those bounds, arguments as mxq_fp8_gemm's, x of x_dtype where it is not MXQ_DTYPE_E4M3).
+constexpr int64_t kFp8FewRows = 32, kFp8FusedRows = 16;
+bool fp8_rows_pays(int64_t M, int64_t N, int64_t K);
+int fp8_linear_rows(const void* x, int x_dtype, int64_t ldx, const uint8_t* sx, int64_t ldsx, const uint8_t* b, int64_t ldb,
+                    const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd, int out_dtype, int64_t M, int64_t N,
+                    int64_t K, void* stream);
+
 constexpr int kFp8MinByte = 10;  // 2^-117
 
 // The scale byte of a block from the bits of its (finite) absmax: 448 = 1.75 * 2^8, so a significand above 1.75

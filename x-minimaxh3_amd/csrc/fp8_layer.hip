@@ -35,8 +35,6 @@ Pair take_pair(Carve& c, int64_t rows, int64_t cols) {
   return p;
 }
 
-constexpr int64_t kFused = 16, kFew = 32;  // rows that the few-row product quantizes itself, and takes at all
-
 struct ForwardSpace {
   Pair x;
   void* gemm;
@@ -44,22 +42,13 @@ struct ForwardSpace {
 };
 int forward_space(uint8_t* base, int64_t M, int64_t N, int64_t K, ForwardSpace& f) {
   f = {};
-  if (M <= kFused) return MXQ_OK;
+  if (M <= kFp8FusedRows) return MXQ_OK;
   Carve c{base};
   f.x = take_pair(c, M, K);
-  if (M > kFew) {
-    if (const int rc = mxq_fp8_gemm_workspace(M, N, K, &f.gemm_bytes)) return rc;
-    f.gemm = c.take<void>(f.gemm_bytes);
-  }
+  if (const int rc = mxq_fp8_gemm_workspace(M, N, K, &f.gemm_bytes)) return rc;
+  f.gemm = c.take<void>(f.gemm_bytes);
   f.total = c.used;
   return MXQ_OK;
-}
-
-int product(const Pair& x, const uint8_t* b, int64_t ldb, const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd,
-            int out_dtype, int64_t M, int64_t N, int64_t K, void* ws, int64_t ws_bytes, void* stream) {
-  if (M <= kFew)
-    return mxq_fp8_linear_rows(x.q, MXQ_DTYPE_E4M3, x.ldq, x.s, x.lds, b, ldb, sb, ldsb, bias, d, ldd, out_dtype, M, N, K, stream);
-  return mxq_fp8_gemm(x.q, x.ldq, x.s, x.lds, b, ldb, sb, ldsb, bias, d, ldd, out_dtype, M, N, K, ws, ws_bytes, stream);
 }
 
 bool sizes_ok(int64_t M, int64_t N, int64_t K) {
@@ -81,10 +70,8 @@ int backward_space(uint8_t* base, int64_t M, int64_t N, int64_t K, int dy_dtype,
   const int most = dy_dtype == MXQ_DTYPE_BF16 ? 1 : dy_dtype == MXQ_DTYPE_F16 ? 2 : 3;
   if (needs & 1) {
     s.dy = take_pair(c, M, N);
-    if (M > kFew) {
-      if (const int rc = mxq_fp8_gemm_workspace(M, K, N, &s.gemm_bytes)) return rc;
-      s.gemm = c.take<void>(s.gemm_bytes);
-    }
+    if (const int rc = mxq_fp8_gemm_workspace(M, K, N, &s.gemm_bytes)) return rc;
+    s.gemm = c.take<void>(s.gemm_bytes);
   }
   if (needs & 2) {
     s.n_parts = direct || M == 0 ? 0 : most;
@@ -121,16 +108,15 @@ extern "C" int mxq_fp8_linear(const void* x, int x_dtype, int64_t ldx, const uin
   if (!sizes_ok(M, N, K))
     return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
   if (M == 0) return MXQ_OK;
-  if (M <= kFused) {
-    if (x_dtype == MXQ_DTYPE_E4M3) return mxq_set_error(MXQ_ERR_INVALID, "unsupported input dtype code %d", x_dtype);
-    return mxq_fp8_linear_rows(x, x_dtype, ldx, nullptr, 0, b, ldb, sb, ldsb, bias, d, ldd, out_dtype, M, N, K, stream);
-  }
+  if (!float_dtype(x_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported input dtype code %d", x_dtype);
+  if (M <= kFp8FusedRows)
+    return fp8_linear_rows(x, x_dtype, ldx, nullptr, 0, b, ldb, sb, ldsb, bias, d, ldd, out_dtype, M, N, K, stream);
   ForwardSpace f;
   if (const int rc = forward_space((uint8_t*)workspace, M, N, K, f)) return rc;
   if (!workspace || workspace_bytes < f.total || reinterpret_cast<uintptr_t>(workspace) % 16)
     return mxq_set_error(MXQ_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)f.total);
   if (const int rc = mxq_fp8_quantize_rows(x, x_dtype, ldx, f.x.q, f.x.ldq, f.x.s, f.x.lds, M, K, stream)) return rc;
-  return product(f.x, b, ldb, sb, ldsb, bias, d, ldd, out_dtype, M, N, K, f.gemm, f.gemm_bytes, stream);
+  return mxq_fp8_gemm(f.x.q, f.x.ldq, f.x.s, f.x.lds, b, ldb, sb, ldsb, bias, d, ldd, out_dtype, M, N, K, f.gemm, f.gemm_bytes, stream);
 }
 
 extern "C" int mxq_fp8_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dy_dtype, int direct, int readable,
@@ -164,7 +150,9 @@ extern "C" int mxq_fp8_linear_backward(const void* dy, int dy_dtype, int64_t ldy
       return rc;
   }
   if (dx && M > 0) {
-    if (const int rc = product(s.dy, bt, ldbt, sbt, ldsbt, nullptr, dx, K, dy_dtype, M, K, N, s.gemm, s.gemm_bytes, stream)) return rc;
+    if (const int rc = mxq_fp8_gemm(s.dy.q, s.dy.ldq, s.dy.s, s.dy.lds, bt, ldbt, sbt, ldsbt, nullptr, dx, K, dy_dtype, M, K, N, s.gemm,
+                                    s.gemm_bytes, stream))
+      return rc;
   }
   if (dw) {
     if (M > 0 && !readable) {

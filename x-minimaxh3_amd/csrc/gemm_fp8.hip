@@ -23,6 +23,9 @@
 //
 // Problems of few tiles split K over workgroups, which write float32 sums that fp8_join_kernel adds in order.
 
+#include <algorithm>
+#include <cmath>
+
 #include "fp8_common.h"
 
 namespace mxq {
@@ -441,16 +444,15 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const float* part, int sp
 }
 
 // ---- few rows (up to 32): a stream of the weight ----
-// A workgroup's four waves take 16 kRT weight rows and share K. Fragments go from memory straight to registers
+// A workgroup's four or eight waves take 16 kRT weight rows and share K. Fragments go from memory straight to registers
 // (a lane: row l % 16, bytes 16 (l / 16) + {0..15} and + 64 of a block), a group of kG blocks ahead of the one at work,
 // are converted to bfloat16 with their scales, exactly, and multiplied by v_mfma_f32_16x16x32_bf16, so the sums keep
 // float32's precision at no cost: the weight's bytes bound this kernel. kFused: the activations come in their own type
 // and each wave quantizes its own K range of them, a chunk of blocks at a time, into its part of LDS (up to 16 rows:
-// the 16 columns of the instruction), which saves the quantizer's launch.
-// Measured (bf16 in and out): 1 row, K 5120, N 20480 in 20.4 us (5.1 TB/s), 16 rows, K 5376, N 21504 in 32.3 us; there
-// 28.2 us go to the product from codes and 4.4 us would go to the quantizer's own launch. From 17 rows on the rows' own
-// traffic from the caches grows with each workgroup: 32 rows, K 5120, N 5120 take 12.6 us against 16.5 us as 128-row
-// tiles, 64 rows took 20.7 us, and N 20480 53.9 us against 30.2 us.
+// the 16 columns of the instruction), which saves the quantizer's launch. How many weight rows a workgroup takes
+// decides (plan_rows): each workgroup quantizes, or reads, all of x again, and what counts is the CU with the most
+// weight rows. Measured (bf16 in and out): K 5120, N 20480 (80 weight rows: a workgroup per CU) 1 row 19.6 us (5.4 TB/s),
+// 16 rows 23.2; with 32 weight rows a workgroup 20.4 and 32.0.
 struct Fp8Rows {
   const void* x;  // kFused: [M, ldx] of the input type; else e4m3 codes [M, ldx]
   const uint8_t* sx;
@@ -460,7 +462,7 @@ struct Fp8Rows {
   void* d;
   int64_t M, N, K, ldx, ldsx, ldb, ldsb, ldd;
   int kb;
-  int chunk_log2;  // kFused: blocks per chunk
+  int chunk_log2, x_code;  // kFused: blocks per chunk, x's type
 };
 
 // LDS of a wave's chunk: rows of codes, 16 bytes apart in banks, then a scale byte per row and block.
@@ -496,21 +498,25 @@ MXQ_DEVICE void quantize_chunk(const Fp8Rows& p, uint8_t* lds, int kb0, int last
   wave_lds_fence();
 }
 
+// Blocks per group; a chunk holds two groups.
+constexpr int rows_group(int mt, int rt) { return mt == 1 && rt <= 2 ? 2 : 1; }
+
 template <int kMT, int kRT, bool kFused>
 struct RowsBlock {  // one block's operands of a wave
   v4u w[kRT][2];
-  uint32_t ws;
+  uint32_t ws[2];  // of the weight rows in the first and the second 128-row tile
   v4u x[kFused ? 1 : kMT][2];
   uint32_t xs[kFused ? 1 : kMT];
 };
 
-template <int kIn, int kOut, int kMT, int kRT, bool kFused>
-__global__ __launch_bounds__(256) void fp8_rows_kernel(Fp8Rows p) {
-  constexpr int kG = kMT == 1 ? 2 : 1;  // (a chunk is four blocks at least: two groups)
+template <int kOut, int kMT, int kRT, bool kFused>
+__global__ __launch_bounds__(512) void fp8_rows_kernel(Fp8Rows p) {
+  constexpr int kG = rows_group(kMT, kRT);
+  const int kW = blockDim.x >> 6;
   extern __shared__ __align__(16) uint8_t rows_lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
   const int N = (int)p.N, M = (int)p.M, n0 = blockIdx.x * (16 * kRT);
-  const int per = (p.kb + 3) / 4, first = wave * per, last = min(first + per, p.kb);
+  const int per = (p.kb + kW - 1) / kW, first = wave * per, last = min(first + per, p.kb);
   const int rows = min(N - n0, 16 * kRT);
   const uint8_t* wb = p.b + n0 * p.ldb;
   const int wbytes = (int)(rows * p.ldb);
@@ -521,6 +527,7 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(Fp8Rows p) {
     woff[r] = row < rows ? (uint32_t)(row * (int)p.ldb + g * 16) : kBufferOff;
   }
   const uint8_t* sw = p.sb + (n0 >> 7) * p.ldsb;
+  const int64_t sw1 = ((n0 + rows - 1) >> 7) > (n0 >> 7) ? p.ldsb : 0;
   uint8_t* chunk = rows_lds + (kFused ? wave * chunk_bytes(M, p.chunk_log2) : 0);
   const int ld = chunk_row(p.chunk_log2), chunk_mask = (1 << p.chunk_log2) - 1;
   v4f acc[kRT][kMT] = {};
@@ -535,7 +542,8 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(Fp8Rows p) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           t[u].w[r][h] = buffer_load_x4(wb, wbytes, in ? woff[r] + (uint32_t)((kb + u) * 128 + h * 64) : kBufferOff);
-      t[u].ws = sw[min(at, p.kb - 1)];
+      t[u].ws[0] = sw[min(at, p.kb - 1)];
+      if constexpr (kRT > 2) t[u].ws[1] = sw[sw1 + min(at, p.kb - 1)];
       if constexpr (!kFused) {
 #pragma unroll
         for (int m = 0; m < kMT; ++m) {  // (rows behind the last are the last one again; their sums are not stored)
@@ -577,15 +585,16 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(Fp8Rows p) {
           xf[m][2 * h + 1] = fp8x8_to_bf16(c[h][2], c[h][3], scale);
         }
       }
-      const float ws = fp8_scale_f32(t[u].ws);
 #pragma unroll
-      for (int r = 0; r < kRT; ++r)
+      for (int r = 0; r < kRT; ++r) {
+        const float ws = fp8_scale_f32(kRT <= 2 || ((n0 + r * 16) >> 7) == (n0 >> 7) ? t[u].ws[0] : t[u].ws[1]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const v8bf wf = fp8x8_to_bf16(t[u].w[r][q >> 1][2 * (q & 1)], t[u].w[r][q >> 1][2 * (q & 1) + 1], ws);
 #pragma unroll
           for (int m = 0; m < kMT; ++m) acc[r][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, xf[m][q], acc[r][m], 0, 0, 0);
         }
+      }
     }
   };
   Block t0[kG], t1[kG];
@@ -593,26 +602,31 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(Fp8Rows p) {
   for (int kb = first; kb < last; kb += 2 * kG) {
     load(t1, kb + kG);
     if constexpr (kFused) {
-      if (((kb - first) & chunk_mask) == 0) quantize_chunk<kIn>(p, chunk, kb, min(last, kb + chunk_mask + 1), lane);
+      if (((kb - first) & chunk_mask) == 0) {
+        const int end = min(last, kb + chunk_mask + 1);
+        if (p.x_code == MXQ_DTYPE_BF16) quantize_chunk<MXQ_DTYPE_BF16>(p, chunk, kb, end, lane);
+        else if (p.x_code == MXQ_DTYPE_F16) quantize_chunk<MXQ_DTYPE_F16>(p, chunk, kb, end, lane);
+        else quantize_chunk<MXQ_DTYPE_F32>(p, chunk, kb, end, lane);
+      }
     }
     compute(t0, kb);
     load(t0, kb + 2 * kG);
     compute(t1, kb + kG);
   }
-  v4f* part = reinterpret_cast<v4f*>(rows_lds + (kFused ? 4 * chunk_bytes(M, p.chunk_log2) : 0));
+  if constexpr (kFused) __syncthreads();  // (the sums take the chunks' place)
+  v4f* part = reinterpret_cast<v4f*>(rows_lds);
 #pragma unroll
   for (int r = 0; r < kRT; ++r)
 #pragma unroll
     for (int m = 0; m < kMT; ++m) part[((wave * kRT + r) * kMT + m) * 64 + lane] = acc[r][m];
   __syncthreads();
-  // the four waves' sums in order; (r, m) pairs are dealt to the waves
+  // the waves' sums in order; (r, m) pairs are dealt to the waves
   constexpr int kElem = kOut == MXQ_DTYPE_F32 ? 4 : 2;
-  for (int t = wave; t < kRT * kMT; t += 4) {
+  for (int t = wave; t < kRT * kMT; t += kW) {
     const int r = t / kMT, m = t - r * kMT;
     const int row = m * 16 + lr, col = n0 + r * 16 + g * 4;
     v4f y = part[t * 64 + lane];
-#pragma unroll
-    for (int k = 1; k < 4; ++k) y += part[(k * kRT * kMT + t) * 64 + lane];
+    for (int k = 1; k < kW; ++k) y += part[(k * kRT * kMT + t) * 64 + lane];
     if (row < M && col < N) {
       y += bias_run<kOut>(p.bias, col, N);
       const float v[4] = {y[0], y[1], y[2], y[3]};
@@ -625,15 +639,16 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(Fp8Rows p) {
 
 struct Fp8Plan {
   int tile, splits, split_kb;
+  double cost;
 };
 
 // Tile rows and K slices, by an estimate in microseconds: a round of workgroups takes 5 for its first loads and its
-// epilogue and 1.35 (256 rows) or 0.72 (128 rows) per stage; slices cost a join, 4 and its traffic, which the last-level
+// epilogue and 1.35 (256 rows) or 0.72 (128 rows) per stage, all of them the weight's bytes; slices cost a join, 4 and its traffic, which the last-level
 // cache holds. Both sides measured: 1501 x 1000 of K = 3001 (48 tiles) takes 14.7 + 5.0 us in slices, 21.9 us whole; 1024 x 5120 of K = 5120 takes 38 us on 160
 // tiles of 128 rows, 2048 rows 60 us on 160 of 256.
 static Fp8Plan plan_fp8(int64_t M, int64_t N, int64_t kb, int cus) {
-  Fp8Plan best = {256, 1, (int)((kb + 3) / 4 * 4)};
-  double best_cost = 1e300;
+  Fp8Plan best = {256, 1, (int)((kb + 3) / 4 * 4), 1e300};
+  const double stream = (double)(N * kb) * 128.0 / 4.9e6 + 2.0;
   for (int tile = 256; tile >= 128; tile /= 2) {
     const int64_t tiles = (M + tile - 1) / tile * ((N + kTileN - 1) / kTileN);
     for (int64_t s = 1; s <= 32; ++s) {
@@ -642,14 +657,50 @@ static Fp8Plan plan_fp8(int64_t M, int64_t N, int64_t kb, int cus) {
       const double rounds = (double)((tiles * s + cus - 1) / cus);
       const double stages = (double)(per < kb ? per : kb);
       double cost = rounds * (stages * (tile == 256 ? 1.35 : 0.72) + 5.0);
+      if (cost < stream) cost = stream;
       if (s > 1) cost += 4.0 + (double)(M * N) * (double)(s + 1) / 1.0e6;
-      if (cost < best_cost) {
-        best_cost = cost;
-        best = {tile, (int)s, (int)per};
-      }
+      if (cost < best.cost) best = {tile, (int)s, (int)per, cost};
     }
   }
   return best;
+}
+
+// Weight rows (in sixteens) and waves of a workgroup of the few-row product, by an estimate in microseconds. The CU with
+// the most workgroups (rounds) streams its weight rows, 0.086 per sixteen and block with every CU at work (less where some
+// are idle), and reads x for each workgroup, 0.0052 per row and block where it quantizes them, 0.0023 from codes.
+// Workgroups of four waves share a CU, so that the last round counts half; those of eight take 1 us more to start and end
+// and reach more of a lone CU's rate. Measured, bf16, by 16 / 32 / 48 weight rows and four waves, 32 / 64 / 80 / 96 / 128 and
+// eight: one row, K 5120, N 5120: 8.1 8.8 11.0, 9.1 12.5 15.7 18.6 23.1; N 32768: 26.5 26.9 27.2, 34.8 27.8 33.8 39.9 28.4;
+// K 20480, N 5120: 25.9 24.0 33.2, 22.0 39.0 49.1 58.4 73.5; 16 rows, K 5120, N 15360: 27.6 24.3 26.2, 29.5 18.8 21.3 23.7
+// 27.7; N 32768: 49.7 41.8 35.2, 57.6 35.6 41.4 46.4 31.3.
+struct RowsPlan {
+  int rt, waves;
+  double cost;
+};
+static RowsPlan plan_rows(int64_t M, int64_t N, int64_t kb, int cus, bool fused) {
+  RowsPlan best = {1, 4, 1e300};
+  for (int waves = 4; waves <= 8; waves += 4) {
+    for (const int rt : {1, 2, 3, 4, 5, 6, 8}) {
+      if (waves == 4 && rt > 3) break;
+      const double groups = (double)((N + 16 * rt - 1) / (16 * rt)), share = groups / cus, rounds = std::ceil(share);
+      const double busy = std::min(1.0, std::max(share, waves == 4 ? 0.78 : 0.7));
+      const double turns = waves == 4 && rounds > 1.0 ? (rounds + share) / 2 : rounds;
+      const double cost = (waves == 4 ? 2.5 : 3.5) + turns * (double)kb * (rt * 0.086 * busy + (double)M * (fused ? 0.0052 : 0.0023));
+      if (cost < best.cost) best = {rt, waves, cost};
+    }
+  }
+  return best;
+}
+
+// Up to 16 rows always; up to 32 where the tiles would not be split or take longer (32 rows, bf16: K 5120, N 5120 13 us
+// against 11.2 + 4.1; K 20480, N 5120 48 against 24 + 4.1).
+bool fp8_rows_pays(int64_t M, int64_t N, int64_t K) {
+  if (M <= kFp8FusedRows) return true;
+  if (M > kFp8FewRows) return false;
+  const int64_t kb = (K + 127) / 128;
+  const int cus = mxq_cu_count();
+  const Fp8Plan tiles = plan_fp8(M, N, kb, cus);
+  return tiles.splits == 1 || plan_rows(M, N, kb, cus, false).cost <= tiles.cost;
 }
 
 }  // namespace mxq
@@ -683,7 +734,7 @@ static int check_product(int64_t M, int64_t N, int64_t K, int64_t ldb, int64_t l
 
 extern "C" int mxq_fp8_gemm_workspace(int64_t M, int64_t N, int64_t K, int64_t* bytes) {
   if (M < 0 || N < 1 || K < 1 || !bytes) return mxq_set_error(MXQ_ERR_INVALID, "bad argument");
-  *bytes = M == 0 ? 0 : split_bytes(plan_fp8(M, N, (K + 127) / 128, mxq_cu_count()), M, N);
+  *bytes = M == 0 || fp8_rows_pays(M, N, K) ? 0 : split_bytes(plan_fp8(M, N, (K + 127) / 128, mxq_cu_count()), M, N);
   return MXQ_OK;
 }
 
@@ -697,6 +748,8 @@ extern "C" int mxq_fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, in
   if (M == 0) return MXQ_OK;
   if (!a || !sa || !b || !sb || !d || !aligned(a, 16) || !aligned(b, 16) || !aligned(sa, 4) || !aligned(sb, 4))
     return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
+  if (fp8_rows_pays(M, N, K))
+    return fp8_linear_rows(a, MXQ_DTYPE_E4M3, lda, sa, ldsa, b, ldb, sb, ldsb, bias, d, ldd, out_dtype, M, N, K, stream);
   const Fp8Plan plan = plan_fp8(M, N, kb, mxq_cu_count());
   const int64_t tiles_m = (M + plan.tile - 1) / plan.tile, tiles_n = (N + kTileN - 1) / kTileN;
   if (tiles_m * tiles_n * plan.splits >= (1ll << 23)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^23 tiles");
@@ -734,54 +787,54 @@ extern "C" int mxq_fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, in
   });
 }
 
-template <int kIn, int kOut, int kMT, int kRT, bool kFused>
-static void launch_rows_of(Fp8Rows p, void* stream) {
-  int bytes = kRT * kMT * 4096;
+template <int kOut, int kMT, int kRT, bool kFused>
+static void launch_rows_of(Fp8Rows p, int waves, void* stream) {
+  int bytes = kRT * kMT * 1024 * waves;
   if constexpr (kFused) {
-    // chunks of a wave's whole K range, down to two groups of blocks where the rows would take more than 8 KB of LDS
-    const int per = (p.kb + 3) / 4;
-    p.chunk_log2 = 3;
-    while (p.chunk_log2 < 6 && (1 << p.chunk_log2) < per && chunk_bytes((int)p.M, p.chunk_log2 + 1) <= 9 * 1024) ++p.chunk_log2;
-    while (chunk_bytes((int)p.M, p.chunk_log2) > 9 * 1024) --p.chunk_log2;
-    bytes += 4 * chunk_bytes((int)p.M, p.chunk_log2);
+    // chunks of a wave's whole K range where all rows' take up to 36 KB of LDS, down to two groups of blocks
+    constexpr int kLeast = rows_group(kMT, kRT) == 2 ? 2 : 1;
+    const int per = (p.kb + waves - 1) / waves, M = (int)p.M;
+    p.chunk_log2 = kLeast;
+    while (p.chunk_log2 < 6 && (1 << p.chunk_log2) < per && waves * chunk_bytes(M, p.chunk_log2 + 1) <= 36 * 1024) ++p.chunk_log2;
+    bytes = std::max(bytes, waves * chunk_bytes(M, p.chunk_log2));
   }
-  hipLaunchKernelGGL((fp8_rows_kernel<kIn, kOut, kMT, kRT, kFused>), dim3((unsigned)((p.N + 16 * kRT - 1) / (16 * kRT))), dim3(256),
-                     bytes, (hipStream_t)stream, p);
+  hipLaunchKernelGGL((fp8_rows_kernel<kOut, kMT, kRT, kFused>), dim3((unsigned)((p.N + 16 * kRT - 1) / (16 * kRT))),
+                     dim3(64 * waves), bytes, (hipStream_t)stream, p);
 }
 
-template <int kIn, int kOut, int kMT, bool kFused>
+template <int kOut, int kMT, bool kFused>
 static void launch_rows(const Fp8Rows& p, void* stream) {
-  // 32 weight rows per workgroup where that leaves two workgroups per CU (N 20480: 1 row 20.0 us, 64 weight rows 22.9 us,
-  // 16 rows 28.2 and 27.1 us)
-  if ((p.N + 31) / 32 >= 2 * mxq_cu_count() || kMT > 1)
-    launch_rows_of<kIn, kOut, kMT, 2, kFused>(p, stream);
-  else
-    launch_rows_of<kIn, kOut, kMT, 1, kFused>(p, stream);
+  const RowsPlan plan = plan_rows(p.M, p.N, p.kb, mxq_cu_count(), kFused);
+  switch (plan.rt) {
+    case 1: return launch_rows_of<kOut, kMT, 1, kFused>(p, plan.waves, stream);
+    case 2: return launch_rows_of<kOut, kMT, 2, kFused>(p, plan.waves, stream);
+    case 3: return launch_rows_of<kOut, kMT, 3, kFused>(p, plan.waves, stream);
+    case 4: return launch_rows_of<kOut, kMT, 4, kFused>(p, plan.waves, stream);
+    case 5: return launch_rows_of<kOut, kMT, 5, kFused>(p, plan.waves, stream);
+    case 6: return launch_rows_of<kOut, kMT, 6, kFused>(p, plan.waves, stream);
+    default: return launch_rows_of<kOut, kMT, 8, kFused>(p, plan.waves, stream);
+  }
 }
 
-extern "C" int mxq_fp8_linear_rows(const void* x, int x_dtype, int64_t ldx, const uint8_t* sx, int64_t ldsx, const uint8_t* b,
-                                   int64_t ldb, const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd,
-                                   int out_dtype, int64_t M, int64_t N, int64_t K, void* stream) {
+int mxq::fp8_linear_rows(const void* x, int x_dtype, int64_t ldx, const uint8_t* sx, int64_t ldsx, const uint8_t* b, int64_t ldb,
+                         const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd, int out_dtype, int64_t M,
+                         int64_t N, int64_t K, void* stream) {
   if (const int rc = check_product(M, N, K, ldb, ldsb, ldd, out_dtype)) return rc;
   const bool fused = x_dtype != MXQ_DTYPE_E4M3;
   const int64_t kb = (K + 127) / 128;
   if (fused && !float_dtype(x_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported input dtype code %d", x_dtype);
-  if (M > (fused ? 16 : 32)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "%lld rows", (long long)M);
-  if (fused ? ldx < K : (ldx < kb * 128 || ldx % 16 || ldsx < kb))
+  if (fused && ldx < K)
     return mxq_set_error(MXQ_ERR_INVALID, "bad row strides of the activations for K=%lld", (long long)K);
-  if (M == 0) return MXQ_OK;
-  if (!x || !b || !sb || !d || (!fused && (!sx || !aligned(x, 16))) || !aligned(b, 16))
-    return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
-  const Fp8Rows p = {x, sx, b, sb, bias, d, M, N, K, ldx, ldsx, ldb, ldsb, ldd, (int)kb, 0};
+  if (!x || !b || !sb || !d || !aligned(b, 16)) return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
+  const Fp8Rows p = {x, sx, b, sb, bias, d, M, N, K, ldx, ldsx, ldb, ldsb, ldd, (int)kb, 0, x_dtype};
   with_dtype(out_dtype, [&](auto O) {
     constexpr int kOut = decltype(O)::value;
-    if (fused) {
-      with_dtype(x_dtype, [&](auto X) { launch_rows<decltype(X)::value, kOut, 1, true>(p, stream); });
-    } else if (M <= 16) {
-      launch_rows<MXQ_DTYPE_BF16, kOut, 1, false>(p, stream);
-    } else {
-      launch_rows<MXQ_DTYPE_BF16, kOut, 2, false>(p, stream);
-    }
+    if (fused)
+      launch_rows<kOut, 1, true>(p, stream);
+    else if (M <= 16)
+      launch_rows<kOut, 1, false>(p, stream);
+    else
+      launch_rows<kOut, 2, false>(p, stream);
   });
   return mxq_check_launch("fp8_rows_kernel");
 }

@@ -23,8 +23,6 @@ from .ops import _OUT_CODES, _bias, _launch, _out_code, _ptr, _require_gpu, _row
 
 BLOCK = 128
 _CODES, _SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
-# rows up to which a product streams the weight (mxq_fp8_linear_rows), and those it quantizes on the way
-_FEW_ROWS, _FUSED_ROWS = 32, 16
 _MAX_STRIDE = 1 << 22  # of an operand's rows; wider ones are copied
 
 
@@ -220,10 +218,6 @@ def _product(dev, a, sa, m: int, k: int, b, sb, n: int, bias, out_dtype) -> torc
     code = _out_code(out_dtype)
     if m == 0:
         return out
-    if m <= _FEW_ROWS:
-        _launch(dev, "mxq_fp8_linear_rows", a.data_ptr(), _lib.DTYPE_E4M3, a.stride(0), sa.data_ptr(), sa.stride(0), b.data_ptr(),
-                b.stride(0), sb.data_ptr(), sb.stride(0), _ptr(bias), out.data_ptr(), n, code, m, n, k)
-        return out
     need = _workspace("mxq_fp8_gemm_workspace", dev.index, m, n, k)
     ws = _room(need, dev)
     _launch(dev, "mxq_fp8_gemm", a.data_ptr(), a.stride(0), sa.data_ptr(), sa.stride(0), b.data_ptr(), b.stride(0), sb.data_ptr(),
@@ -256,7 +250,7 @@ def fp8_linear(x: torch.Tensor, weight: PreparedFp8Weight, bias: torch.Tensor | 
     out = torch.empty((m, n), dtype=out_dtype, device=dev)
     if m:
         q, s = weight.q, weight.scale
-        need = 0 if m <= _FUSED_ROWS else _workspace("mxq_fp8_linear_workspace", dev.index, m, n, k)
+        need = _workspace("mxq_fp8_linear_workspace", dev.index, m, n, k)
         ws = _room(need, dev)
         _launch(dev, "mxq_fp8_linear", x2.data_ptr(), xcode, x2.stride(0) if m > 1 else k, q.data_ptr(), q.shape[1], s.data_ptr(),
                 s.shape[1], _ptr(bias), out.data_ptr(), n, code, m, n, k, _ptr(ws), need)

@@ -47,14 +47,15 @@ def _rows_in_place(x: torch.Tensor, width: int) -> torch.Tensor:
 def _new_pair(m: int, k: int, dev) -> tuple[torch.Tensor, torch.Tensor]:
     """Storage for codes and scales of [m, k]: rows of whole blocks, scale rows of whole words."""
     kb = -(-k // BLOCK)
-    return (torch.empty((m, kb * BLOCK), dtype=_CODES, device=dev),
-            torch.empty((m, _ceil(kb, 4)), dtype=_SCALE, device=dev))
+    return (torch.empty(m, kb * BLOCK, dtype=_CODES, device=dev),
+            torch.empty(m, _ceil(kb, 4), dtype=_SCALE, device=dev))
 
 
 def _view(t: torch.Tensor, lead: tuple[int, ...], width: int) -> torch.Tensor:
     """The first ``width`` columns of ``t`` as ``[*lead, width]`` (a view)."""
-    if t.shape[1] != width:
-        t = t[:, :width]
+    m, ld = t.shape
+    if ld != width:
+        t = t.as_strided((m, width), (ld, 1))
     return t if len(lead) == 1 else t.unflatten(0, lead) if lead else t.squeeze(0)
 
 
@@ -85,7 +86,7 @@ def _pad(t: torch.Tensor, ld: int) -> torch.Tensor:
     if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         t = t.contiguous()
     m, width = t.shape
-    out = torch.empty((m, _ceil(ld, 16)), dtype=t.dtype, device=t.device)
+    out = torch.empty(m, _ceil(ld, 16), dtype=t.dtype, device=t.device)
     _launch(t.device, "mxq_pad_rows", t.data_ptr(), t.stride(0) if m > 1 else width, width, out.data_ptr(), out.shape[1], m)
     return out
 
@@ -186,7 +187,7 @@ def prepare_fp8_weight(weight: torch.Tensor, scale: torch.Tensor | None = None, 
     code = _float_code(weight, "weight")
     dev = _require_gpu(weight)
     w = _rows_in_place(weight, k)
-    q = torch.empty((n, kb * BLOCK), dtype=_CODES, device=dev)
+    q = torch.empty(n, kb * BLOCK, dtype=_CODES, device=dev)
     s = torch.empty((nb, _ceil(kb, 4)), dtype=_SCALE, device=dev)
     qt = torch.empty((k, nb * BLOCK), dtype=_CODES, device=dev) if transposed else None
     st = torch.empty((kb, _ceil(nb, 4)), dtype=_SCALE, device=dev) if transposed else None
@@ -214,7 +215,7 @@ def _room(need: int, dev) -> torch.Tensor | None:
 
 def _product(dev, a, sa, m: int, k: int, b, sb, n: int, bias, out_dtype) -> torch.Tensor:
     """``[m, n]`` of operands in the products' layout."""
-    out = torch.empty((m, n), dtype=out_dtype, device=dev)
+    out = torch.empty(m, n, dtype=out_dtype, device=dev)
     code = _out_code(out_dtype)
     if m == 0:
         return out
@@ -247,7 +248,7 @@ def fp8_linear(x: torch.Tensor, weight: PreparedFp8Weight, bias: torch.Tensor | 
     bias = _bias(bias, n, out_dtype, dev)
     x2 = _rows_in_place(x, k)
     m = x2.shape[0]
-    out = torch.empty((m, n), dtype=out_dtype, device=dev)
+    out = torch.empty(m, n, dtype=out_dtype, device=dev)
     if m:
         q, s = weight.q, weight.scale
         need = _workspace("mxq_fp8_linear_workspace", dev.index, m, n, k)
@@ -311,8 +312,8 @@ def fp8_linear_backward(dy: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, 
     ldy = y.stride(0) if m > 1 else n
     direct = dy.dtype == torch.bfloat16 and n % 16 == 0 and ldy % 8 == 0 and y.data_ptr() % 16 == 0
     readable = _readable(q, _ceil(k, 16))
-    dx = torch.empty((m, k), dtype=dy.dtype, device=dev) if want_x else None
-    dw = torch.empty((n, k), dtype=grad_dtype, device=dev) if want_w else None
+    dx = torch.empty(m, k, dtype=dy.dtype, device=dev) if want_x else None
+    dw = torch.empty(n, k, dtype=grad_dtype, device=dev) if want_w else None
     db = torch.empty(n, dtype=grad_dtype, device=dev) if want_b else None
     # (without rows dx is empty, and its pointer may be null)
     needs = (1 if want_x and m else 0) | (2 if want_w else 0) | (4 if want_b else 0)
@@ -360,7 +361,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     w, b, pcode = _norm_params(d, dev, x.dtype, weight, bias)
     x2 = _rows_in_place(x, d)
     m = x2.shape[0]
-    y = torch.empty((m, d), dtype=x.dtype, device=dev)
+    y = torch.empty(m, d, dtype=x.dtype, device=dev)
     mean = torch.empty(m, dtype=torch.float32, device=dev) if return_stats else None
     rstd = torch.empty(m, dtype=torch.float32, device=dev) if return_stats else None
     if m:
@@ -401,8 +402,8 @@ def layer_norm_backward(dy: torch.Tensor, x, mean: torch.Tensor, rstd: torch.Ten
             raise ValueError(f"{name} must be float32 with one entry per row ({m}), got {t.dtype} {tuple(t.shape)}")
     dev = _require_gpu(dy, x2, xs, mean, rstd, weight)
     w, _, pcode = _norm_params(d, dev, dy.dtype, weight, None)
-    dx = torch.empty((m, d), dtype=dy.dtype, device=dev)
-    both = torch.empty((2, d), dtype=torch.float32, device=dev) if needs_params else None
+    dx = torch.empty(m, d, dtype=dy.dtype, device=dev)
+    both = torch.empty(2, d, dtype=torch.float32, device=dev) if needs_params else None
     need = _workspace("mxq_layer_norm_backward_workspace", dev.index, m, d) if needs_params else 0
     ws = _room(need, dev)
     if m or needs_params:

@@ -11,8 +11,8 @@
 // waves owns a 256 (n) x 256 (k) tile, a wave 64 x 128 of it; a stage is 64 rows of m: dY's 64 x 256 bfloat16 (32 KB) and
 // X's 64 x 256 codes, decoded on the way from registers to LDS (32 KB). Problems of few tiles split M over workgroups,
 // which write float32 sums that wgrad_join_kernel adds in order. 8192 rows, N 5376, K 14336: 1.01 to 1.04 ms, 1.25 PFLOP/s
-// at 1.8 GHz, 64 % of the cycles matrix instructions (a library's plain bfloat16 product of row-major operands runs at 1.43 on the same card, with a transposed
-// left operand, which this is, at 0.96).
+// at 1.8 GHz, 64 % of the cycles matrix instructions (a library's plain bfloat16 product of row-major operands runs at
+// 1.43 on the same card, with a transposed left operand, which this is, at 0.96).
 
 #include "fp8_common.h"
 

@@ -281,3 +281,28 @@ def test_two_streams_and_a_replayed_graph(dev):
         torch.cuda.synchronize()
         for s, o in zip(static, out):
             assert torch.equal(o, mx.fp8_linear(s, p))
+
+
+def test_every_code_and_scale_byte(dev):
+    """Pairs of other making: the value of all 256 codes under all 256 scale bytes (255 is NaN), restored and multiplied."""
+    mx = _mx()
+    q = torch.arange(256, dtype=torch.uint8).repeat(256, 1).view(torch.float8_e4m3fn)
+    s = torch.arange(256, dtype=torch.uint8)[:, None].repeat(1, 2).view(torch.float8_e8m0fnu)
+    ref = q.float().double() * s.float().double().repeat_interleave(128, 1)
+    for dtype in DTYPES:
+        got = mx.dequantize_fp8_block128(q.to(dev), s.to(dev), dtype)
+        assert _same(got.cpu().double(), ref.to(dtype).double())
+    # without the NaN codes: a product's row is NaN where its scale is, and exact for the scales that the quantizers give
+    keep = torch.ones(256, dtype=torch.bool)
+    keep[[127, 255]] = False
+    z = q.view(torch.uint8).clone()
+    z[:, ~keep] = 0
+    p = mx.prepare_fp8_weight(torch.eye(256).to(dev))
+    for first, last in ((0, 256), (100, 109), (220, 247), (250, 256)):
+        rows = slice(first, last)
+        y = mx.fp8_linear_prequantized(z[rows].view(torch.float8_e4m3fn).to(dev), s[rows].contiguous().to(dev), p, out_dtype=torch.float32)
+        want = torch.where(keep[None, :], ref[rows], 0.0)
+        want[torch.arange(first, last) == 255] = float("nan")
+        byte = torch.arange(first, last)
+        fair = ((byte >= 10) & (byte < 247)) | (byte == 255)  # (448 * 2^120 is beyond float32)
+        assert _same(y.cpu().double()[fair], want.float().double()[fair])

@@ -47,7 +47,7 @@ struct Fp8Gemm {
   int kb;                  // blocks of K
   int tiles_m, tiles_n;
   int splits, split_kb;    // K slices of split_kb blocks (a multiple of 4)
-  int vec;                 // whole rows of d are 16-byte aligned (and bias to 4 elements)
+  int vec;                 // rows of d are 16-byte aligned
 };
 
 template <int kTM>

@@ -510,6 +510,11 @@ int mxq_fp8_dequantize_rows(const uint8_t* q, int64_t ldq, const uint8_t* scale,
 int mxq_fp8_quantize_tiles(const void* w, int w_dtype, int64_t ldw, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds,
                            uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst, int64_t N, int64_t K, void* stream);
 
+/* The same from codes w [N, ldw] and scales w_scale [ceil(N / 128), ldws] that are there already, of any alignment. */
+int mxq_fp8_prepare_tiles(const uint8_t* w, int64_t ldw, const uint8_t* w_scale, int64_t ldws, uint8_t* q, int64_t ldq,
+                          uint8_t* scale, int64_t lds, uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst, int64_t N,
+                          int64_t K, void* stream);
+
 /* Bytes of workspace mxq_fp8_gemm needs at this size on the current device (0: none). */
 int mxq_fp8_gemm_workspace(int64_t M, int64_t N, int64_t K, int64_t* bytes);
 

@@ -200,4 +200,8 @@ def test_c_gradient_entries_refuse_before_any_launch():
     with pytest.raises(ValueError, match="size"):
         _call("mxq_fp8_linear", ok, 2, 256, ok, 256, ok, 4, None, ok, 128, 2, 100, 0, 256, ok, 64)
     with pytest.raises(ValueError, match="strides"):
+        _call("mxq_fp8_prepare_tiles", ok, 99, ok, 1, ok, 128, ok, 4, None, 0, None, 0, 100, 100)
+    with pytest.raises(ValueError, match="scale"):
+        _call("mxq_fp8_prepare_tiles", ok, 300, ok, 2, ok, 384, ok, 4, None, 0, None, 0, 100, 300)
+    with pytest.raises(ValueError, match="strides"):
         _call("mxq_pad_rows", ok, 100, 100, ok, 104, 4)

@@ -306,3 +306,34 @@ def test_every_code_and_scale_byte(dev):
         byte = torch.arange(first, last)
         fair = ((byte >= 10) & (byte < 247)) | (byte == 255)  # (448 * 2^120 is beyond float32)
         assert _same(y.cpu().double()[fair], want.float().double()[fair])
+
+
+@pytest.mark.parametrize("n,k", [(1, 1), (130, 205), (513, 1152), (300, 77)])
+def test_weight_from_codes_of_any_layout(dev, n, k):
+    """Codes and scales inside larger tensors, at odd offsets and strides, and transposed: the same form as from copies."""
+    mx = _mx()
+    g = _gen(n + k)
+    nb, kb = -(-n // 128), -(-k // 128)
+    big = torch.randint(0, 127, (n + 2, k + 10), generator=g, dtype=torch.uint8)
+    sbig = torch.randint(100, 140, (nb + 1, kb + 3), generator=g, dtype=torch.uint8)
+    codes, scales = big[1 : n + 1, 3 : k + 3], sbig[:nb, 1 : kb + 1]
+    want_q = torch.zeros(n, kb * 128, dtype=torch.uint8)
+    want_q[:, :k] = codes
+    want_t = torch.zeros(k, nb * 128, dtype=torch.uint8)
+    want_t[:, :n] = codes.t()
+
+    def dev8(t, dtype):
+        return t.to(dev).view(dtype)
+
+    f8, e8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+    for w, s in ((dev8(big, f8)[1 : n + 1, 3 : k + 3], dev8(sbig, e8)[:nb, 1 : kb + 1]),
+                 (dev8(codes.t().contiguous(), f8).t(), dev8(scales.t().contiguous(), e8).t())):
+        for transposed in (True, False):
+            p = mx.prepare_fp8_weight(w, s, transposed)
+            assert torch.equal(p.q.cpu().view(torch.uint8), want_q)
+            assert torch.equal(p.scale.cpu().view(torch.uint8)[:, :kb], scales)
+            if transposed:
+                assert torch.equal(p.qt.cpu().view(torch.uint8), want_t)
+                assert torch.equal(p.scale_t.cpu().view(torch.uint8)[:, :nb], scales.t())
+            else:
+                assert p.qt is None and p.scale_t is None

@@ -26,8 +26,6 @@ typedef float v4f_any __attribute__((ext_vector_type(4), aligned(1)));
 
 namespace mxq {
 
-constexpr int kFp8Block = 128;
-
 // The few-row product (gemm_fp8.hip): rows that it takes as codes, and those it quantizes itself; whether it is the form to
 // take; and the product (M within those bounds, arguments as mxq_fp8_gemm's, x of x_dtype where it is not MXQ_DTYPE_E4M3).
 constexpr int64_t kFp8FewRows = 32, kFp8FusedRows = 16;
@@ -234,12 +232,6 @@ MXQ_DEVICE void store_run4(void* row, int64_t col, int n, const float* y) {
         if (e < n) p[e] = (uint16_t)h[e];
     }
   }
-}
-
-MXQ_DEVICE float load_as_f32(const void* p, int64_t i, int code) {
-  if (code == MXQ_DTYPE_F32) return reinterpret_cast<const float*>(p)[i];
-  const uint32_t h = reinterpret_cast<const uint16_t*>(p)[i];
-  return code == MXQ_DTYPE_F16 ? f16_to_f32(h) : bf16_to_f32(h);
 }
 
 inline int dtype_bytes(int code) { return code == MXQ_DTYPE_F32 ? 4 : 2; }

@@ -96,24 +96,75 @@ __global__ __launch_bounds__(256) void fp8_rows_dequant_kernel(const uint8_t* q,
   }
 }
 
+// `n` of 16 bytes from s, zeros behind them (n <= 0: nothing is read).
+MXQ_DEVICE v4u bytes_load(const uint8_t* s, int n) {
+  v4u v = {0, 0, 0, 0};
+  if (n >= 16) {
+    v = *reinterpret_cast<const v4u_any*>(s);
+  } else if (n > 0) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t b = s[min(i, n - 1)];
+      v[i >> 2] |= (i < n ? b : 0u) << (8 * (i & 3));
+    }
+  }
+  return v;
+}
+
 // ---- weights: one scale per 128 x 128 tile, and the transposed codes that the input's gradient reads ----
 // One workgroup per tile: row t / 8 + 32 i, piece t % 8. The transposed copy goes through a 16 KB byte tile in LDS.
 // HBM-bound: 21504 x 5376 bf16 in 90 us (5.1 TB/s) with the transposed copy, 65 without.
+// Writes a tile's codes (c[i]: row t / 8 + 32 i, piece t % 8) and scale byte, and those of the transposed copy.
+struct TileOut {
+  uint8_t *q, *s, *qt, *st;
+  int64_t ldq, lds, ldqt, ldst, N, K;
+};
+MXQ_DEVICE void store_tile(const TileOut& o, uint8_t* tile, const v4u (&c)[4], uint32_t byte) {
+  const int t = threadIdx.x, piece = t & 7;
+  const int64_t n0 = (int64_t)blockIdx.y * 128, k0 = (int64_t)blockIdx.x * 128, col = k0 + piece * 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = (t >> 3) + 32 * i;
+    if (n0 + r < o.N) *reinterpret_cast<v4u*>(o.q + (n0 + r) * o.ldq + col) = c[i];
+    if (o.qt) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<uint32_t*>(tile + r * 132 + piece * 16 + 4 * j) = c[i][j];
+    }
+  }
+  if (t == 0) o.s[blockIdx.y * o.lds + blockIdx.x] = (uint8_t)byte;
+  if (!o.qt) return;
+  if (t == 0) o.st[blockIdx.x * o.ldst + blockIdx.y] = (uint8_t)byte;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int k = (t >> 3) + 32 * i;  // row of the transposed tile
+    if (k0 + k < o.K) {
+      v4u v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t u = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u |= (uint32_t)tile[(piece * 16 + 4 * j + e) * 132 + k] << (8 * e);
+        v[j] = u;
+      }
+      *reinterpret_cast<v4u*>(o.qt + (k0 + k) * o.ldqt + n0 + piece * 16) = v;
+    }
+  }
+}
+
 template <int kCode>
-__global__ __launch_bounds__(256) void fp8_tiles_quant_kernel(const char* w, int64_t ldw, uint8_t* q, int64_t ldq, uint8_t* s,
-                                                              int64_t lds, uint8_t* qt, int64_t ldqt, uint8_t* st,
-                                                              int64_t ldst, int64_t N, int64_t K) {
+__global__ __launch_bounds__(256) void fp8_tiles_quant_kernel(const char* w, int64_t ldw, TileOut o) {
   constexpr int kElem = kCode == MXQ_DTYPE_F32 ? 4 : 2;
   __shared__ uint32_t wave_max[4];
   __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 132];  // rows of 132: a column's bytes spread over the banks
   const int t = threadIdx.x, piece = t & 7;
-  const int64_t n0 = (int64_t)blockIdx.y * 128, k0 = (int64_t)blockIdx.x * 128, col = k0 + piece * 16;
+  const int64_t n0 = (int64_t)blockIdx.y * 128, col = (int64_t)blockIdx.x * 128 + piece * 16;
   Piece<kCode> p[4];
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t row = n0 + (t >> 3) + 32 * i;
-    p[i] = piece_load<kCode>(w + (min(row, N - 1) * ldw + col) * kElem, row < N ? (int)(K - col) : 0);
+    p[i] = piece_load<kCode>(w + (min(row, o.N - 1) * ldw + col) * kElem, row < o.N ? (int)(o.K - col) : 0);
     m = max(m, piece_absmax(p[i]));
   }
   m = wave_max_u32(m);
@@ -132,35 +183,25 @@ __global__ __launch_bounds__(256) void fp8_tiles_quant_kernel(const char* w, int
   }
   const uint32_t byte = fp8_scale_byte(m);
   const float scale = fp8_scale_f32(byte);
+  v4u c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = piece_encode(p[i], scale);
+  store_tile(o, tile, c, byte);
+}
+
+// The same of codes that are there already, with their scales [ceil(N / 128), ldws]: 21504 x 5376 in 65 us (5.3 TB/s).
+__global__ __launch_bounds__(256) void fp8_tiles_copy_kernel(const uint8_t* w, int64_t ldw, const uint8_t* ws, int64_t ldws,
+                                                             TileOut o) {
+  __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 132];
+  const int t = threadIdx.x;
+  const int64_t n0 = (int64_t)blockIdx.y * 128, col = (int64_t)blockIdx.x * 128 + (t & 7) * 16;
+  v4u c[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = (t >> 3) + 32 * i;
-    const v4u c = piece_encode(p[i], scale);
-    if (n0 + r < N) *reinterpret_cast<v4u*>(q + (n0 + r) * ldq + col) = c;
-    if (qt) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) *reinterpret_cast<uint32_t*>(tile + r * 132 + piece * 16 + 4 * j) = c[j];
-    }
+    const int64_t row = n0 + (t >> 3) + 32 * i;
+    c[i] = bytes_load(w + min(row, o.N - 1) * ldw + col, row < o.N ? (int)(o.K - col) : 0);
   }
-  if (t == 0) s[blockIdx.y * lds + blockIdx.x] = (uint8_t)byte;
-  if (!qt) return;
-  if (t == 0) st[blockIdx.x * ldst + blockIdx.y] = (uint8_t)byte;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int k = (t >> 3) + 32 * i;  // row of the transposed tile
-    if (k0 + k < K) {
-      v4u c;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t v = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v |= (uint32_t)tile[(piece * 16 + 4 * j + e) * 132 + k] << (8 * e);
-        c[j] = v;
-      }
-      *reinterpret_cast<v4u*>(qt + (k0 + k) * ldqt + n0 + piece * 16) = c;
-    }
-  }
+  store_tile(o, tile, c, ws[blockIdx.y * ldws + blockIdx.x]);
 }
 
 // ---- the pass over an output's gradient dY [M, N] ----
@@ -245,17 +286,7 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* src, int64
     const int64_t row = g / pieces;
     const int col = (int)(g - row * pieces) * 16, n = width - col;
     const uint8_t* s = src + row * lds + col;
-    v4u v = {0, 0, 0, 0};
-    if (n >= 16) {
-      v = *reinterpret_cast<const v4u_any*>(s);
-    } else if (n > 0) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint32_t b = s[min(i, n - 1)];
-        v[i >> 2] |= (i < n ? b : 0u) << (8 * (i & 3));
-      }
-    }
-    *reinterpret_cast<v4u*>(dst + row * ldd + col) = v;
+    *reinterpret_cast<v4u*>(dst + row * ldd + col) = bytes_load(s, n);
   }
 }
 
@@ -334,22 +365,39 @@ extern "C" int mxq_fp8_dequantize_rows(const uint8_t* q, int64_t ldq, const uint
   return mxq_check_launch("fp8_rows_dequant_kernel");
 }
 
+static int check_tiles(const TileOut& o, const void* w, int64_t ldw) {
+  const int64_t kb = (o.K + 127) / 128, nb = (o.N + 127) / 128;
+  if (o.N < 1 || o.K < 1) return mxq_set_error(MXQ_ERR_INVALID, "bad size N=%lld K=%lld", (long long)o.N, (long long)o.K);
+  if (ldw < o.K || o.ldq < kb * 128 || o.ldq % 16 || o.lds < kb || (o.qt && (o.ldqt < nb * 128 || o.ldqt % 16 || o.ldst < nb)))
+    return mxq_set_error(MXQ_ERR_INVALID, "bad row strides for N=%lld K=%lld", (long long)o.N, (long long)o.K);
+  if (!w || !o.q || !o.s || !aligned16(o.q) || (o.qt && (!o.st || !aligned16(o.qt))))
+    return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
+  if (nb > 65535 || kb >= (1ll << 23)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 65535 tile rows or 2^23 columns");
+  return MXQ_OK;
+}
+
 extern "C" int mxq_fp8_quantize_tiles(const void* w, int w_dtype, int64_t ldw, uint8_t* q, int64_t ldq, uint8_t* scale,
                                       int64_t lds, uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst, int64_t N,
                                       int64_t K, void* stream) {
   if (!float_dtype(w_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported weight dtype code %d", w_dtype);
-  if (N < 1 || K < 1) return mxq_set_error(MXQ_ERR_INVALID, "bad size N=%lld K=%lld", (long long)N, (long long)K);
-  const int64_t kb = (K + 127) / 128, nb = (N + 127) / 128;
-  if (ldw < K || ldq < kb * 128 || ldq % 16 || lds < kb || (qt && (ldqt < nb * 128 || ldqt % 16 || ldst < nb)))
-    return mxq_set_error(MXQ_ERR_INVALID, "bad row strides for N=%lld K=%lld", (long long)N, (long long)K);
-  if (!w || !q || !scale || !aligned16(q) || (qt && (!scale_t || !aligned16(qt))))
-    return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
-  if (nb > 65535 || kb >= (1ll << 31)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 65535 tile rows");
+  const TileOut o = {q, scale, qt, scale_t, ldq, lds, ldqt, ldst, N, K};
+  if (const int rc = check_tiles(o, w, ldw)) return rc;
   with_dtype(w_dtype, [&](auto C) {
-    hipLaunchKernelGGL((fp8_tiles_quant_kernel<decltype(C)::value>), dim3((unsigned)kb, (unsigned)nb), dim3(256), 0,
-                       (hipStream_t)stream, (const char*)w, ldw, q, ldq, scale, lds, qt, ldqt, scale_t, ldst, N, K);
+    hipLaunchKernelGGL((fp8_tiles_quant_kernel<decltype(C)::value>), dim3((unsigned)((K + 127) / 128), (unsigned)((N + 127) / 128)),
+                       dim3(256), 0, (hipStream_t)stream, (const char*)w, ldw, o);
   });
   return mxq_check_launch("fp8_tiles_quant_kernel");
+}
+
+extern "C" int mxq_fp8_prepare_tiles(const uint8_t* w, int64_t ldw, const uint8_t* w_scale, int64_t ldws, uint8_t* q, int64_t ldq,
+                                     uint8_t* scale, int64_t lds, uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst,
+                                     int64_t N, int64_t K, void* stream) {
+  const TileOut o = {q, scale, qt, scale_t, ldq, lds, ldqt, ldst, N, K};
+  if (const int rc = check_tiles(o, w, ldw)) return rc;
+  if (!w_scale || ldws < (K + 127) / 128) return mxq_set_error(MXQ_ERR_INVALID, "null scale or bad row stride");
+  hipLaunchKernelGGL(fp8_tiles_copy_kernel, dim3((unsigned)((K + 127) / 128), (unsigned)((N + 127) / 128)), dim3(256), 0,
+                     (hipStream_t)stream, w, ldw, w_scale, ldws, o);
+  return mxq_check_launch("fp8_tiles_copy_kernel");
 }
 
 // Rows per strip of the gradient pass: whole eights, about four workgroups per CU in all, at least 32 rows.

@@ -74,6 +74,7 @@ SIGNATURES: dict[str, list] = {
     "mxq_fp8_quantize_rows": [_P, _I, _I64, _P, _I64, _P, _I64, _I64, _I64, _P],
     "mxq_fp8_dequantize_rows": [_P, _I64, _P, _I64, _P, _I, _I64, _I64, _P],
     "mxq_fp8_quantize_tiles": [_P, _I, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _P],
+    "mxq_fp8_prepare_tiles": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _P],
     "mxq_fp8_gemm_workspace": [_I64, _I64, _I64, _P],
     "mxq_fp8_gemm": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I, _I64, _I64, _I64, _P, _I64, _P],
     "mxq_fp8_grad_strips": [_I64, _I64, _P],

@@ -179,20 +179,21 @@ def prepare_fp8_weight(weight: torch.Tensor, scale: torch.Tensor | None = None, 
                              f"{scale.dtype}")
         if tuple(scale.shape) != (nb, kb):
             raise ValueError(f"weight scale of shape {tuple(scale.shape)}, expected {(nb, kb)}")
-        _require_gpu(weight, scale)
-        # (byte copies at load: torch's own)
-        qt = _pad(weight.view(torch.uint8).t(), nb * BLOCK).view(_CODES) if transposed else None
-        st = _pad(scale.view(torch.uint8).t(), _ceil(nb, 4)).view(_SCALE) if transposed else None
-        return PreparedFp8Weight(_pad(weight, kb * BLOCK), _pad(scale, _ceil(kb, 4)), qt, st, n, k)
-    code = _float_code(weight, "weight")
-    dev = _require_gpu(weight)
+    else:
+        code = _float_code(weight, "weight")
+    dev = _require_gpu(weight, scale)
     w = _rows_in_place(weight, k)
     q = torch.empty(n, kb * BLOCK, dtype=_CODES, device=dev)
-    s = torch.empty((nb, _ceil(kb, 4)), dtype=_SCALE, device=dev)
-    qt = torch.empty((k, nb * BLOCK), dtype=_CODES, device=dev) if transposed else None
-    st = torch.empty((kb, _ceil(nb, 4)), dtype=_SCALE, device=dev) if transposed else None
-    _launch(dev, "mxq_fp8_quantize_tiles", w.data_ptr(), code, w.stride(0), q.data_ptr(), q.shape[1], s.data_ptr(), s.shape[1],
-            _ptr(qt), nb * BLOCK, _ptr(st), _ceil(nb, 4), n, k)
+    s = torch.empty(nb, _ceil(kb, 4), dtype=_SCALE, device=dev)
+    qt = torch.empty(k, nb * BLOCK, dtype=_CODES, device=dev) if transposed else None
+    st = torch.empty(kb, _ceil(nb, 4), dtype=_SCALE, device=dev) if transposed else None
+    out = (q.data_ptr(), q.shape[1], s.data_ptr(), s.shape[1], _ptr(qt), nb * BLOCK, _ptr(st), _ceil(nb, 4), n, k)
+    ldw = w.stride(0) if n > 1 else k
+    if scale is not None:
+        ws = _rows_in_place(scale, kb)
+        _launch(dev, "mxq_fp8_prepare_tiles", w.data_ptr(), ldw, ws.data_ptr(), ws.stride(0) if nb > 1 else kb, *out)
+    else:
+        _launch(dev, "mxq_fp8_quantize_tiles", w.data_ptr(), code, ldw, *out)
     return PreparedFp8Weight(q, s, qt, st, n, k)
 
 

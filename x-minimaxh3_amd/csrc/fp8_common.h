@@ -34,6 +34,37 @@ int fp8_linear_rows(const void* x, int x_dtype, int64_t ldx, const uint8_t* sx, 
                     const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd, int out_dtype, int64_t M, int64_t N,
                     int64_t K, void* stream);
 
+// Sums to be joined (fp8_join.hip): d [rows, cols] (row stride ldd, of dtype `code`) = slices [splits, rows, ldp] + bias, and
+// out [n] = the columns of in [parts, n]. No slices, no out: nothing to do.
+struct SliceJob {
+  const float* part;
+  const void* bias;
+  void* d;
+  int64_t rows, ldp, ldd;
+  int cols, splits, code;
+};
+struct ColumnJob {
+  const float* in;
+  void* out;
+  int64_t parts, n;
+  int code;
+};
+int fp8_join(const SliceJob& a, const SliceJob& b, const ColumnJob& c, void* stream);
+
+// Microseconds that `s` slices of `n` sums cost a product: the join's launch, and the sums written and read, less where the
+// eight L2s (32 MB) hold them: 3 slices of 100 x 21504 (26 MB) took 3.8 beside the launch, 2 of 1024 x 4096 (34 MB) 13.6.
+inline double slices_cost(int64_t s, int64_t n) {
+  return s > 1 ? 4.0 + (double)n * (double)(s + 1) / (s * n * 4 <= 28000000 ? 2.3e6 : 0.95e6) : 0.0;
+}
+
+// mxq_fp8_gemm and mxq_fp8_wgrad, with the join of their slices, if there is one, left to the caller (`later` not NULL).
+int fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa, const uint8_t* b, int64_t ldb, const uint8_t* sb,
+             int64_t ldsb, const void* bias, void* d, int64_t ldd, int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
+             int64_t workspace_bytes, SliceJob* later, void* stream);
+int fp8_wgrad(const void* dy, int parts, int64_t ldy, const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds, void* dw,
+              int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, SliceJob* later,
+              void* stream);
+
 constexpr int kFp8MinByte = 10;  // 2^-117
 
 // The scale byte of a block from the bits of its (finite) absmax: 448 = 1.75 * 2^8, so a significand above 1.75
@@ -185,6 +216,28 @@ MXQ_DEVICE uint32_t block_scale_byte(const Piece<kCode>& p) {
   uint32_t m = max8(piece_absmax(p));
   if (m >= 0x7F800000u) m = max8(piece_absmax_finite(p));  // (the same for the eight lanes of a block)
   return fp8_scale_byte(m);
+}
+
+// Bias of the four columns from col on (behind the last: the last one's).
+template <int kOut>
+MXQ_DEVICE v4f bias_run(const void* bias, int col, int N) {
+  v4f b = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (!bias) return b;
+  const typename OutT<kOut>::T* p = reinterpret_cast<const typename OutT<kOut>::T*>(bias);
+  if (col + 4 > N) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = OutT<kOut>::load(p + min(col + e, N - 1));
+  } else if constexpr (kOut == MXQ_DTYPE_F32) {
+    b = *reinterpret_cast<const v4f_any*>(p + col);
+  } else {
+    const v2u w = *reinterpret_cast<const v2u_any*>(p + col);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t h = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
+      b[e] = kOut == MXQ_DTYPE_F16 ? f16_to_f32(h) : bf16_to_f32(h);
+    }
+  }
+  return b;
 }
 
 // Orders a wave's LDS accesses: what its lanes wrote, its lanes read.

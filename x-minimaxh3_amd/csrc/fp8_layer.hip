@@ -149,9 +149,10 @@ extern "C" int mxq_fp8_linear_backward(const void* dy, int dy_dtype, int64_t ldy
                                          stream))
       return rc;
   }
+  SliceJob join_x = {}, join_w = {};
   if (dx && M > 0) {
-    if (const int rc = mxq_fp8_gemm(s.dy.q, s.dy.ldq, s.dy.s, s.dy.lds, bt, ldbt, sbt, ldsbt, nullptr, dx, K, dy_dtype, M, K, N, s.gemm,
-                                    s.gemm_bytes, stream))
+    if (const int rc = fp8_gemm(s.dy.q, s.dy.ldq, s.dy.s, s.dy.lds, bt, ldbt, sbt, ldsbt, nullptr, dx, K, dy_dtype, M, K, N, s.gemm,
+                                s.gemm_bytes, &join_x, stream))
       return rc;
   }
   if (dw) {
@@ -161,10 +162,9 @@ extern "C" int mxq_fp8_linear_backward(const void* dy, int dy_dtype, int64_t ldy
       ldq = s.x.ldq;
     }
     const void* y = s.n_parts ? s.parts : dy;
-    if (const int rc = mxq_fp8_wgrad(y, s.n_parts ? s.n_parts : 1, s.n_parts || M == 0 ? s.ldp : ldy, q, M == 0 ? up(K, 16) : ldq, scale,
-                                     M == 0 ? up(K, 128) / 128 : lds, dw, grad_dtype, M, N, K, s.wgrad, s.wgrad_bytes, stream))
+    if (const int rc = fp8_wgrad(y, s.n_parts ? s.n_parts : 1, s.n_parts || M == 0 ? s.ldp : ldy, q, M == 0 ? up(K, 16) : ldq, scale,
+                                     M == 0 ? up(K, 128) / 128 : lds, dw, grad_dtype, M, N, K, s.wgrad, s.wgrad_bytes, &join_w, stream))
       return rc;
   }
-  if (db) return mxq_column_join(s.sums, s.strips, N, db, grad_dtype, stream);
-  return MXQ_OK;
+  return fp8_join(join_x, join_w, {s.sums, db, s.strips, N, grad_dtype}, stream);
 }

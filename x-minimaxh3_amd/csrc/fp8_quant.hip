@@ -290,36 +290,6 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* src, int64
   }
 }
 
-// out[c] = sum over `parts` rows of a float32 [parts, n] table: the columns' last sum. 32 columns (a line) and 32
-// shares of the rows per workgroup: a share's loads go out eight at a time, so there are many shares.
-template <int kCode>
-__global__ __launch_bounds__(1024) void column_join_kernel(const float* in, int64_t parts, int64_t n, void* out) {
-  __shared__ float sm[32][32];
-  const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
-  const int64_t col = (int64_t)blockIdx.x * 32 + c;
-  float v = 0.0f;
-  if (col < n) {
-#pragma unroll 8
-    for (int64_t i = r; i < parts; i += 32) v += in[i * n + col];
-  }
-  sm[r][c] = v;
-  __syncthreads();
-  if (r < 8) {
-    v = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v += sm[r * 4 + k][c];
-  }
-  __syncthreads();
-  if (r < 8) sm[r][c] = v;
-  __syncthreads();
-  if (r == 0 && col < n) {
-    v = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v += sm[k][c];
-    store_out<kCode>(reinterpret_cast<typename OutT<kCode>::T*>(out) + col, v);
-  }
-}
-
 }  // namespace mxq
 
 using namespace mxq;
@@ -459,14 +429,4 @@ extern "C" int mxq_pad_rows(const uint8_t* src, int64_t lds, int64_t width, uint
   hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, (hipStream_t)stream, src, lds,
                      (int)width, dst, (int)ldd, total);
   return mxq_check_launch("pad_rows_kernel");
-}
-
-extern "C" int mxq_column_join(const float* in, int64_t parts, int64_t n, void* out, int out_dtype, void* stream) {
-  if (!float_dtype(out_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported output dtype code %d", out_dtype);
-  if (parts < 0 || n < 1 || n >= (1ll << 27) || !out || (parts && !in)) return mxq_set_error(MXQ_ERR_INVALID, "bad argument");
-  with_dtype(out_dtype, [&](auto C) {
-    hipLaunchKernelGGL((column_join_kernel<decltype(C)::value>), dim3((unsigned)((n + 31) / 32)), dim3(1024), 0,
-                       (hipStream_t)stream, in, parts, n, out);
-  });
-  return mxq_check_launch("column_join_kernel");
 }

@@ -10,7 +10,7 @@
 // read from LDS by ds_read_b64_tr_b16, which hands sixteen lanes the columns of a 4 x 16 patch. A workgroup of eight
 // waves owns a 256 (n) x 256 (k) tile, a wave 64 x 128 of it; a stage is 64 rows of m: dY's 64 x 256 bfloat16 (32 KB) and
 // X's 64 x 256 codes, decoded on the way from registers to LDS (32 KB). Problems of few tiles split M over workgroups,
-// which write float32 sums that wgrad_join_kernel adds in order. 8192 rows, N 5376, K 14336: 1.01 to 1.04 ms, 1.25 PFLOP/s
+// which write float32 sums that fp8_join_kernel adds in order. 8192 rows, N 5376, K 14336: 1.01 to 1.04 ms, 1.25 PFLOP/s
 // at 1.8 GHz, 64 % of the cycles matrix instructions (a library's plain bfloat16 product of row-major operands runs at
 // 1.43 on the same card, with a transposed left operand, which this is, at 0.96).
 
@@ -238,28 +238,14 @@ __global__ __launch_bounds__(kWThreads, 1) void fp8_wgrad_kernel(Wgrad p) {
   }
 }
 
-// D = out(sum over slices), four columns per thread.
-template <int kOut>
-__global__ __launch_bounds__(256) void wgrad_join_kernel(const float* part, int splits, int64_t N, int64_t K, int64_t ldp,
-                                                         char* d) {
-  constexpr int kElem = kOut == MXQ_DTYPE_F32 ? 4 : 2;
-  const int64_t runs = ldp / 4, g = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (g >= N * runs) return;
-  const int64_t row = g / runs;
-  const int col = (int)(g - row * runs) * 4;
-  const v4f y = sum_slices(reinterpret_cast<const v4f*>(part + row * ldp + col), splits, N * runs);
-  const float v[4] = {y[0], y[1], y[2], y[3]};
-  store_run4<kOut>(d + row * K * kElem, col, (int)K - col, v);
-}
-
 struct WgradPlan {
   int splits;
   int64_t rows;
 };
 
-// M slices, by an estimate in microseconds: a round of workgroups takes 4.5 and 1.5 per stage and part, slices cost a join,
-// 4 and its traffic. Measured: N = K = 1024 over 4096 rows (16 tiles) 22 + 9 us in slices, 101 us whole by the estimate;
-// N = K = 5120 over 1024 rows 71 us whole, 400 tiles on 256 CUs.
+// M slices, by an estimate in microseconds: a round of workgroups takes 4.5 and 1.5 per stage and part, slices cost a join.
+// Measured: N = K = 1024 over 4096 rows (16 tiles) 23 + 6 us in slices, 101 us whole by the estimate; N = K = 5120 over
+// 1024 rows 67 us whole, 400 tiles on 256 CUs.
 static WgradPlan plan_wgrad(int64_t M, int64_t N, int64_t K, int parts, int cus) {
   const int64_t tiles = (N + kWTile - 1) / kWTile * ((K + kWTile - 1) / kWTile);
   WgradPlan best = {1, (M + kWRows - 1) / kWRows * kWRows};
@@ -269,7 +255,7 @@ static WgradPlan plan_wgrad(int64_t M, int64_t N, int64_t K, int parts, int cus)
     if (rows == 0 || (M + rows - 1) / rows != s || (s > 1 && tiles * s > 4 * cus)) continue;
     const double rounds = (double)((tiles * s + cus - 1) / cus);
     double cost = rounds * ((double)(rows / kWRows) * parts * 1.5 + 4.5);
-    if (s > 1) cost += 4.0 + (double)(N * K) * (double)(s + 1) / 1.0e6;
+    cost += slices_cost(s, N * K);
     if (cost < best_cost) {
       best_cost = cost;
       best = {(int)s, rows};
@@ -294,9 +280,9 @@ extern "C" int mxq_fp8_wgrad_workspace(int64_t M, int64_t N, int64_t K, int part
   return MXQ_OK;
 }
 
-extern "C" int mxq_fp8_wgrad(const void* dy, int parts, int64_t ldy, const uint8_t* q, int64_t ldq, const uint8_t* scale,
+int mxq::fp8_wgrad(const void* dy, int parts, int64_t ldy, const uint8_t* q, int64_t ldq, const uint8_t* scale,
                              int64_t lds, void* dw, int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
-                             int64_t workspace_bytes, void* stream) {
+                             int64_t workspace_bytes, SliceJob* later, void* stream) {
   if (!float_dtype(out_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported output dtype code %d", out_dtype);
   if (M < 0 || N < 1 || K < 1 || parts < 1 || parts > 3 || M > (1ll << 31) - 1024 || N > (1 << 30) || K > (1 << 30))
     return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld N=%lld K=%lld parts=%d", (long long)M, (long long)N, (long long)K, parts);
@@ -320,17 +306,21 @@ extern "C" int mxq_fp8_wgrad(const void* dy, int parts, int64_t ldy, const uint8
     const int64_t ldp = (K + 3) / 4 * 4;
     p.d = workspace;
     p.ldd = ldp;
-    const int64_t blocks = (N * (ldp / 4) + 255) / 256;
     hipLaunchKernelGGL((fp8_wgrad_kernel<MXQ_DTYPE_F32, true>), dim3(grid), dim3(kWThreads), 0, (hipStream_t)stream, p);
     if (const int rc = mxq_check_launch("fp8_wgrad_kernel")) return rc;
-    with_dtype(out_dtype, [&](auto O) {
-      hipLaunchKernelGGL((wgrad_join_kernel<decltype(O)::value>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream,
-                         (const float*)workspace, plan.splits, N, K, ldp, (char*)dw);
-    });
-    return mxq_check_launch("wgrad_join_kernel");
+    const SliceJob job = {(const float*)workspace, nullptr, dw, N, ldp, K, (int)K, plan.splits, out_dtype};
+    if (!later) return fp8_join(job, {}, {}, stream);
+    *later = job;
+    return MXQ_OK;
   }
   with_dtype(out_dtype, [&](auto O) {
     hipLaunchKernelGGL((fp8_wgrad_kernel<decltype(O)::value, false>), dim3(grid), dim3(kWThreads), 0, (hipStream_t)stream, p);
   });
   return mxq_check_launch("fp8_wgrad_kernel");
+}
+
+extern "C" int mxq_fp8_wgrad(const void* dy, int parts, int64_t ldy, const uint8_t* q, int64_t ldq, const uint8_t* scale,
+                             int64_t lds, void* dw, int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  return fp8_wgrad(dy, parts, ldy, q, ldq, scale, lds, dw, out_dtype, M, N, K, workspace, workspace_bytes, nullptr, stream);
 }

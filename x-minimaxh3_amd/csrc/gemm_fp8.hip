@@ -308,28 +308,6 @@ MXQ_DEVICE uint32_t out_pair(float a, float b) {  // two 16-bit values
   return f32_to_f16_bits(a) | (f32_to_f16_bits(b) << 16);
 }
 
-// Bias of the four columns from col on (behind the last: the last one's).
-template <int kOut>
-MXQ_DEVICE v4f bias_run(const void* bias, int col, int N) {
-  v4f b = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (!bias) return b;
-  const typename OutT<kOut>::T* p = reinterpret_cast<const typename OutT<kOut>::T*>(bias);
-  if (col + 4 > N) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) b[e] = OutT<kOut>::load(p + min(col + e, N - 1));
-  } else if constexpr (kOut == MXQ_DTYPE_F32) {
-    b = *reinterpret_cast<const v4f_any*>(p + col);
-  } else {
-    const v2u w = *reinterpret_cast<const v2u_any*>(p + col);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t h = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-      b[e] = kOut == MXQ_DTYPE_F16 ? f16_to_f32(h) : bf16_to_f32(h);
-    }
-  }
-  return b;
-}
-
 template <class C, int kOut, bool kSplit>
 MXQ_DEVICE void epilogue(const Fp8Gemm& p, char* lds, const v16f (&acc)[C::kBI][C::kBJ], int m0, int n0, int wrow,
                          int wcol, int wave, int lane, void* d) {
@@ -426,21 +404,6 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_kernel(Fp8Gemm p) {
   void* d = p.d;
   if constexpr (kSplit) d = reinterpret_cast<float*>(p.d) + slice * p.M * p.ldd;
   epilogue<C, kOut, kSplit>(p, lds, acc, m0, n0, wrow, wcol, wave, lane, d);
-}
-
-// D = out(sum over slices + bias), four columns per thread; the slices' rows are padded to whole fours.
-template <int kOut>
-__global__ __launch_bounds__(256) void fp8_join_kernel(const float* part, int splits, int64_t M, int64_t N, int64_t ldp,
-                                                       const void* bias, char* d, int64_t ldd) {
-  constexpr int kElem = kOut == MXQ_DTYPE_F32 ? 4 : 2;
-  const int64_t runs = ldp / 4, g = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (g >= M * runs) return;
-  const int64_t row = g / runs;
-  const int col = (int)(g - row * runs) * 4;
-  v4f y = sum_slices(reinterpret_cast<const v4f*>(part + row * ldp + col), splits, M * runs);
-  y += bias_run<kOut>(bias, col, (int)N);
-  const float v[4] = {y[0], y[1], y[2], y[3]};
-  store_run4<kOut>(d + row * ldd * kElem, col, (int)N - col, v);
 }
 
 // ---- few rows (up to 32): a stream of the weight ----
@@ -643,9 +606,10 @@ struct Fp8Plan {
 };
 
 // Tile rows and K slices, by an estimate in microseconds: a round of workgroups takes 5 for its first loads and its
-// epilogue and 1.35 (256 rows) or 0.72 (128 rows) per stage, all of them the weight's bytes; slices cost a join, 4 and its traffic, which the last-level
-// cache holds. Both sides measured: 1501 x 1000 of K = 3001 (48 tiles) takes 14.7 + 5.0 us in slices, 21.9 us whole; 1024 x 5120 of K = 5120 takes 38 us on 160
-// tiles of 128 rows, 2048 rows 60 us on 160 of 256.
+// epilogue and 1.35 (256 rows) or 0.72 (128 rows) per stage, all rounds at least the weight's bytes; slices cost a join.
+// Both sides measured: 1501 x 1000 of K 3001 (48 tiles) takes 14.4 + 5.9 us in slices, 21.9 us whole; 100 x 21504 of K 5376
+// 28.9 + 6.3 and 38.3; 1024 x 4096 of K 5120 26.9 + 10.1 and 36.2; 1024 x 5120 of K 5120 38 us as 160 tiles of 128 rows,
+// 2048 rows 60 us as 160 of 256.
 static Fp8Plan plan_fp8(int64_t M, int64_t N, int64_t kb, int cus) {
   Fp8Plan best = {256, 1, (int)((kb + 3) / 4 * 4), 1e300};
   const double stream = (double)(N * kb) * 128.0 / 4.9e6 + 2.0;
@@ -658,7 +622,7 @@ static Fp8Plan plan_fp8(int64_t M, int64_t N, int64_t kb, int cus) {
       const double stages = (double)(per < kb ? per : kb);
       double cost = rounds * (stages * (tile == 256 ? 1.35 : 0.72) + 5.0);
       if (cost < stream) cost = stream;
-      if (s > 1) cost += 4.0 + (double)(M * N) * (double)(s + 1) / 1.0e6;
+      cost += slices_cost(s, M * N);
       if (cost < best.cost) best = {tile, (int)s, (int)per, cost};
     }
   }
@@ -738,9 +702,9 @@ extern "C" int mxq_fp8_gemm_workspace(int64_t M, int64_t N, int64_t K, int64_t* 
   return MXQ_OK;
 }
 
-extern "C" int mxq_fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa, const uint8_t* b, int64_t ldb,
+int mxq::fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa, const uint8_t* b, int64_t ldb,
                             const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd, int out_dtype,
-                            int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream) {
+                            int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, SliceJob* later, void* stream) {
   if (const int rc = check_product(M, N, K, ldb, ldsb, ldd, out_dtype)) return rc;
   const int64_t kb = (K + 127) / 128;
   if (lda < kb * 128 || lda % 16 || lda > (1ll << 22) + 4096 || ldsa < (kb + 3) / 4 * 4 || ldsa % 4 || ldsa > (1ll << 20))
@@ -771,13 +735,10 @@ extern "C" int mxq_fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, in
     else
       rc = wide ? launch_gemm<128, 0, true, true>(p, stream) : launch_gemm<128, 0, true, false>(p, stream);
     if (rc) return rc;
-    const int64_t blocks = (M * (ldp / 4) + 255) / 256;  // (slices are for few tiles: far below 2^24)
-    with_dtype(out_dtype, [&](auto O) {
-      constexpr int kOut = decltype(O)::value;
-      hipLaunchKernelGGL((fp8_join_kernel<kOut>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream,
-                         (const float*)workspace, plan.splits, M, N, ldp, bias, (char*)d, ldd);
-    });
-    return mxq_check_launch("fp8_join_kernel");
+    const SliceJob job = {(const float*)workspace, bias, d, M, ldp, ldd, (int)N, plan.splits, out_dtype};
+    if (!later) return fp8_join(job, {}, {}, stream);
+    *later = job;
+    return MXQ_OK;
   }
   p.vec = aligned(d, 16) && ldd * dtype_bytes(out_dtype) % 16 == 0;
   return with_dtype(out_dtype, [&](auto O) {
@@ -785,6 +746,12 @@ extern "C" int mxq_fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, in
     constexpr bool kWide = kOut == MXQ_DTYPE_F32;
     return plan.tile == 256 ? launch_gemm<256, kOut, false, kWide>(p, stream) : launch_gemm<128, kOut, false, kWide>(p, stream);
   });
+}
+
+extern "C" int mxq_fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa, const uint8_t* b, int64_t ldb,
+                            const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd, int out_dtype,
+                            int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream) {
+  return fp8_gemm(a, lda, sa, ldsa, b, ldb, sb, ldsb, bias, d, ldd, out_dtype, M, N, K, workspace, workspace_bytes, nullptr, stream);
 }
 
 template <int kOut, int kMT, int kRT, bool kFused>

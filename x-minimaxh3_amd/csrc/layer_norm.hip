@@ -8,7 +8,7 @@
 // chunk, so x (and dy) are read once; the variance is that of the centred values, not a difference of large sums.
 // HBM-bound: 75600 x 5120 bf16 forward 292 us (5.3 TB/s), backward from the input in 8 bits 384 + 8 us (4.9 TB/s). The
 // backward pass also keeps its lanes' columns of dw and db in registers over all the rows a workgroup takes, writes them
-// once per workgroup, and column_join_kernel adds the workgroups' sums in a fixed order: no atomics, the same bits on
+// once per workgroup, and fp8_join_kernel adds the workgroups' sums in a fixed order: no atomics, the same bits on
 // every run. Its x can be the input as it was kept in 8 bits (fp8_common.h), decoded as it is read.
 
 #include "fp8_common.h"

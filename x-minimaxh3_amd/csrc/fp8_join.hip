@@ -7,7 +7,7 @@ using namespace mxq;
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 256;  // (1024: 0.4 us more for small slices, no less for a column's many rows)
 
 // D = out(sum over slices + bias), four columns per thread; the slices' rows are padded to whole fours.
 template <int kOut>
@@ -23,31 +23,22 @@ MXQ_DEVICE void join_slices(const SliceJob& j, int64_t block) {
   store_run4<kOut>(reinterpret_cast<char*>(j.d) + row * j.ldd * kElem, col, j.cols - col, v);
 }
 
-// out[c] = sum over `parts` rows of a float32 [parts, n] table. 32 columns (a line) and 32 shares of the rows per
-// workgroup: a share's loads go out eight at a time, so there are many shares.
+// out[c] = sum over `parts` rows of a float32 [parts, n] table. 32 columns (a line) and 8 shares of the rows per
+// workgroup; a share's loads go out eight at a time.
 template <int kOut>
-MXQ_DEVICE void join_columns(const ColumnJob& j, int64_t block, float (&sm)[32][32]) {
+MXQ_DEVICE void join_columns(const ColumnJob& j, int64_t block, float (&sm)[kThreads / 32][32]) {
   const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
   const int64_t col = block * 32 + c;
   float v = 0.0f;
   if (col < j.n) {
 #pragma unroll 8
-    for (int64_t i = r; i < j.parts; i += 32) v += j.in[i * j.n + col];
+    for (int64_t i = r; i < j.parts; i += kThreads / 32) v += j.in[i * j.n + col];
   }
   sm[r][c] = v;
   __syncthreads();
-  if (r < 8) {
-    v = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v += sm[r * 4 + k][c];
-  }
-  __syncthreads();
-  if (r < 8) sm[r][c] = v;
-  __syncthreads();
   if (r == 0 && col < j.n) {
-    v = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v += sm[k][c];
+    for (int k = 1; k < kThreads / 32; ++k) v += sm[k][c];
     store_out<kOut>(reinterpret_cast<typename OutT<kOut>::T*>(j.out) + col, v);
   }
 }
@@ -61,7 +52,7 @@ MXQ_DEVICE void of_code(int code, F&& f) {
 }
 
 __global__ __launch_bounds__(kThreads) void fp8_join_kernel(SliceJob a, SliceJob b, ColumnJob c, int blocks_c, int blocks_a) {
-  __shared__ float sm[32][32];
+  __shared__ float sm[kThreads / 32][32];
   const int block = blockIdx.x;
   if (block < blocks_c)
     of_code(c.code, [&](auto C) { join_columns<decltype(C)::value>(c, block, sm); });
@@ -78,7 +69,7 @@ int64_t blocks_of(const SliceJob& j) { return j.splits ? (j.rows * (j.ldp / 4) +
 int mxq::fp8_join(const SliceJob& a, const SliceJob& b, const ColumnJob& c, void* stream) {
   const int64_t na = blocks_of(a), nb = blocks_of(b), nc = c.out ? (c.n + 31) / 32 : 0, blocks = na + nb + nc;
   if (blocks == 0) return MXQ_OK;
-  if (blocks >= (1 << 22)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "too many sums to join");
+  if (blocks >= (1 << 24)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "too many sums to join");
   hipLaunchKernelGGL(fp8_join_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, (hipStream_t)stream, a, b, c, (int)nc, (int)na);
   return mxq_check_launch("fp8_join_kernel");
 }

@@ -5,48 +5,38 @@ namespace mxq {
 
 // ---- rows: one scale per 1 x 128 block ----
 // Eight lanes hold a block, 16 elements each, so a wave's loads cover whole lines, a block's maximum stays inside
-// eight lanes and every lane stores 16 codes. HBM-bound: 75600 x 5120 bf16 in 201 us (5.8 TB/s), 8192 x 20480 in 107.
-constexpr int kRowUnroll = 4;
-
+// eight lanes and every lane stores 16 codes. HBM-bound: 75600 x 5120 bf16 in 190 us (6.1 TB/s), 8192 x 20480 in 102.
+// One piece per lane: two to four in flight per lane took longer at every size (720p 197 and 201 us, 333 x 5000 fp16 4.4 and
+// 5.2 us against 4.4), the waves of a CU keep enough loads under way.
 template <int kCode>
 __global__ __launch_bounds__(256) void fp8_rows_quant_kernel(const char* x, int64_t ldx, uint8_t* q, int64_t ldq,
                                                              uint8_t* s, int64_t lds, uint32_t M, uint32_t K, uint32_t kb) {
   constexpr int kElem = kCode == MXQ_DTYPE_F32 ? 4 : 2;
-  const uint32_t total = M * kb;  // below 2^31 (checked by the launcher)
-  const uint32_t piece = threadIdx.x & 7, first = blockIdx.x * (32 * kRowUnroll) + (threadIdx.x >> 3);
-  Piece<kCode> p[kRowUnroll];
-  uint32_t row[kRowUnroll], b[kRowUnroll];
-#pragma unroll
-  for (int u = 0; u < kRowUnroll; ++u) {
-    const uint32_t g = min(first + u * 32, total - 1);
-    row[u] = g / kb;
-    b[u] = g - row[u] * kb;
-    const uint32_t col = b[u] * 128 + piece * 16;
-    p[u] = piece_load<kCode>(x + ((int64_t)row[u] * ldx + col) * kElem, (int)K - (int)col);
-  }
-#pragma unroll
-  for (int u = 0; u < kRowUnroll; ++u) {
-    const uint32_t byte = block_scale_byte(p[u]);
-    const v4u codes = piece_encode(p[u], fp8_scale_f32(byte));
-    if (first + u * 32 < total) {
-      *reinterpret_cast<v4u*>(q + (int64_t)row[u] * ldq + b[u] * 128 + piece * 16) = codes;
-      if (piece == 0) s[(int64_t)row[u] * lds + b[u]] = (uint8_t)byte;
-    }
+  const uint32_t block = blockIdx.x * 32 + (threadIdx.x >> 3), piece = threadIdx.x & 7;
+  const uint32_t row = min(block, M * kb - 1) / kb, b = min(block, M * kb - 1) - row * kb, col = b * 128 + piece * 16;
+  const Piece<kCode> p = piece_load<kCode>(x + ((int64_t)row * ldx + col) * kElem, (int)K - (int)col);
+  const uint32_t byte = block_scale_byte(p);
+  const v4u codes = piece_encode(p, fp8_scale_f32(byte));
+  if (block < M * kb) {
+    *reinterpret_cast<v4u*>(q + (int64_t)row * ldq + col) = codes;
+    if (piece == 0) s[(int64_t)row * lds + b] = (uint8_t)byte;
   }
 }
 
 // ---- the way back ----
 // A lane takes the codes whose values fill one 16-byte store, so that a wave's stores are whole lines. 8192 x 20480 to bf16
 // in 77 us.
+constexpr int kDequantUnroll = 4;  // (8192 x 20480: 76 us, with one 83)
+
 template <int kCode>
 __global__ __launch_bounds__(256) void fp8_rows_dequant_kernel(const uint8_t* q, int64_t ldq, const uint8_t* s, int64_t lds,
                                                                char* out, uint32_t M, uint32_t K, uint32_t pieces) {
   constexpr int kElem = kCode == MXQ_DTYPE_F32 ? 4 : 2, kCodes = 16 / kElem;
   const uint32_t total = M * pieces;
-  uint32_t c[kRowUnroll][2], row[kRowUnroll], col[kRowUnroll], sc[kRowUnroll];
+  uint32_t c[kDequantUnroll][2], row[kDequantUnroll], col[kDequantUnroll], sc[kDequantUnroll];
 #pragma unroll
-  for (int u = 0; u < kRowUnroll; ++u) {
-    const uint32_t g = min(blockIdx.x * (256 * kRowUnroll) + u * 256 + threadIdx.x, total - 1);
+  for (int u = 0; u < kDequantUnroll; ++u) {
+    const uint32_t g = min(blockIdx.x * (256 * kDequantUnroll) + u * 256 + threadIdx.x, total - 1);
     row[u] = g / pieces;
     col[u] = (g - row[u] * pieces) * kCodes;
     const int n = (int)(K - col[u]);
@@ -70,8 +60,8 @@ __global__ __launch_bounds__(256) void fp8_rows_dequant_kernel(const uint8_t* q,
     }
   }
 #pragma unroll
-  for (int u = 0; u < kRowUnroll; ++u) {
-    if (blockIdx.x * (256 * kRowUnroll) + u * 256 + threadIdx.x >= total) return;
+  for (int u = 0; u < kDequantUnroll; ++u) {
+    if (blockIdx.x * (256 * kDequantUnroll) + u * 256 + threadIdx.x >= total) return;
     char* dst = out + ((int64_t)row[u] * K + col[u]) * kElem;
     const int n = (int)(K - col[u]);
     const float scale = fp8_scale_f32(sc[u]);
@@ -306,8 +296,8 @@ extern "C" int mxq_fp8_quantize_rows(const void* x, int x_dtype, int64_t ldx, ui
                          (long long)ldq, (long long)lds, (long long)K);
   if (M == 0) return MXQ_OK;
   if (!x || !q || !scale || !aligned16(q)) return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
-  if (M >= (1ll << 31) / kb - 65536 / kb - 1) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^31 blocks");
-  const unsigned grid = (unsigned)((M * kb + 32 * kRowUnroll - 1) / (32 * kRowUnroll));
+  if (M > (1ll << 29) / kb - 32) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^29 blocks");  // (eight lanes each)
+  const unsigned grid = (unsigned)((M * kb + 31) / 32);
   with_dtype(x_dtype, [&](auto C) {
     hipLaunchKernelGGL((fp8_rows_quant_kernel<decltype(C)::value>), dim3(grid), dim3(256), 0, (hipStream_t)stream,
                        (const char*)x, ldx, q, ldq, scale, lds, (uint32_t)M, (uint32_t)K, (uint32_t)kb);
@@ -327,7 +317,7 @@ extern "C" int mxq_fp8_dequantize_rows(const uint8_t* q, int64_t ldq, const uint
   const int codes = 16 / dtype_bytes(out_dtype);
   const int64_t pieces = (K + codes - 1) / codes;
   if (M >= (1ll << 31) / pieces - 65536 / pieces - 1) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^31 pieces");
-  const unsigned grid = (unsigned)((M * pieces + 256 * kRowUnroll - 1) / (256 * kRowUnroll));
+  const unsigned grid = (unsigned)((M * pieces + 256 * kDequantUnroll - 1) / (256 * kDequantUnroll));
   with_dtype(out_dtype, [&](auto C) {
     hipLaunchKernelGGL((fp8_rows_dequant_kernel<decltype(C)::value>), dim3(grid), dim3(256), 0, (hipStream_t)stream, q, ldq,
                        scale, lds, (char*)out, (uint32_t)M, (uint32_t)K, (uint32_t)pieces);

@@ -200,7 +200,7 @@ __global__ __launch_bounds__(256) void fp8_tiles_copy_kernel(const uint8_t* w, i
 // 2, float32 3: parts p0 = bf16(x), p1 = bf16(x - p0), p2 = bf16(x - p0 - p1), whose sum is x to 16 and 24 bits), and
 // the column sums (the bias's gradient) of a strip of rows, in float32.
 // A workgroup takes 512 columns x `strip` rows: 32 lanes across, 8 rows at a time. 8192 x 5376 bf16 (codes and sums) in
-// 25 us (5.3 TB/s), 1501 x 3001 fp16 with two parts in 11.5 us.
+// 25 us (5.3 TB/s), 1501 x 3001 fp16 with two parts in 9.8 us.
 template <int kCode, int kParts>
 __global__ __launch_bounds__(256) void fp8_grad_pass_kernel(const char* x, int64_t ldx, uint8_t* q, int64_t ldq, uint8_t* s,
                                                             int64_t lds, uint16_t* parts, int64_t ldp, float* sums,
@@ -360,12 +360,13 @@ extern "C" int mxq_fp8_prepare_tiles(const uint8_t* w, int64_t ldw, const uint8_
   return mxq_check_launch("fp8_tiles_copy_kernel");
 }
 
-// Rows per strip of the gradient pass: whole eights, about four workgroups per CU in all, at least 32 rows.
+// Rows per strip of the gradient pass: whole eights, about four workgroups per CU in all, at least 16 rows (1501 x 3001 fp16
+// 9.8 us, at least 32: 12.0; at least 8 gave no more and doubles the sums to join).
 static int64_t grad_strip(int64_t M, int64_t N) {
   const int64_t panels = (N + 511) / 512;
   const int64_t want = panels >= 4 * mxq_cu_count() ? 1 : 4 * mxq_cu_count() / panels;
   int64_t strip = ((M + want - 1) / want + 7) / 8 * 8;
-  if (strip < 32) strip = 32;
+  if (strip < 16) strip = 16;
   const int64_t least = ((M + 65534) / 65535 + 7) / 8 * 8;  // grid.y
   return strip < least ? least : strip;
 }

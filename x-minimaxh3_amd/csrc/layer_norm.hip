@@ -360,12 +360,22 @@ __global__ __launch_bounds__(kThreads) void layer_norm_grad_kernel(NormGrad p) {
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
       const Window c = at(i);
+      if (c.lo == 0 && c.hi == 8) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e >= c.lo && e < c.hi) {
-          out[c.start + e] = dw[i][e];
-          out[p.D + c.start + e] = db[i][e];
+        for (int k = 0; k < 2; ++k) {
+          float* o = out + k * p.D + c.start;
+          const float(&v)[8] = k ? db[i] : dw[i];
+          *reinterpret_cast<v4f_any*>(o) = v4f{v[0], v[1], v[2], v[3]};
+          *reinterpret_cast<v4f_any*>(o + 4) = v4f{v[4], v[5], v[6], v[7]};
         }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e >= c.lo && e < c.hi) {
+            out[c.start + e] = dw[i][e];
+            out[p.D + c.start + e] = db[i][e];
+          }
+      }
     }
   }
 }
@@ -406,13 +416,13 @@ static void with_forward_shape(int D, F&& f) {
   else go(integral_constant<int, 4>{});
 }
 
-// Workgroups of the backward pass: about twenty waves per CU (sixteen of the wide forms), each with an equal share of rows; four rows
-// at least once every CU has a workgroup, since each writes 2 D sums (777 x 1003: 256 workgroups 8.2 us and a join of 3.4,
-// one per row 10.6 and 6.0).
+// Workgroups of the backward pass: about twenty waves per CU (sixteen of the wide forms), each with an equal share of rows; eight rows
+// at least once every CU has a workgroup, since each writes 2 D sums (4000 x 2048 bf16, kernel and join: 12.7 + 6.1 us; at
+// least four rows 13.4 + 8.2, sixteen 15.1 + 4.3; 777 x 1003 fp32: 256 workgroups 7.1 + 3.4, one per row 7.7 + 6.6).
 static int64_t norm_grad_grid(int64_t M, int64_t D, int cus) {
   const int64_t n = (D + 511) / 512, units = n <= 1 ? (M + 3) / 4 : M;
   const int64_t most = cus * (n <= 1 ? 5 : n <= 16 ? (20 / n > 1 ? 20 / n : 1) : 1);
-  const int64_t few = units < cus ? units : units / 4 > cus ? units / 4 : cus;
+  const int64_t few = units < cus ? units : units / 8 > cus ? units / 8 : cus;
   return few < most ? few : most;
 }
 

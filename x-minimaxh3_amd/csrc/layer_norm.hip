@@ -251,10 +251,25 @@ __global__ __launch_bounds__(kThreads) void layer_norm_grad_kernel(NormGrad p) {
   const int waves = kOne ? 1 : blockDim.x >> 6, wave = kOne ? 0 : threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int sub = kOne ? threadIdx.x >> 6 : 0;
   const float inv = 1.0f / (float)p.D;
-  float dw[kChunks][8] = {}, db[kChunks][8] = {}, w[kChunks][8];
+  // (three chunks' weights beside their sums spill: 2000 x 20480 bf16 148 us; read again for every row 115, what still spills
+  // bounds it; six chunks of half as many waves 134)
+  constexpr bool kHoldW = kChunks < 3;
+  float dw[kChunks][8] = {}, db[kChunks][8] = {}, held[kHoldW ? kChunks : 1][8];
   auto at = [&](int i) { return window<kVec>(((i * waves + wave) * 64 + lane) * 8, p.D); };
+  if constexpr (kHoldW) {
 #pragma unroll
-  for (int i = 0; i < kChunks; ++i) param8<kVec>(p.w, p.wcode, at(i), p.D, 1.0f, w[i]);
+    for (int i = 0; i < kChunks; ++i) param8<kVec>(p.w, p.wcode, at(i), p.D, 1.0f, held[i]);
+  }
+  auto weight = [&](int i, float (&v)[8]) {
+    if constexpr (kHoldW) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = held[i][e];
+    } else {
+      uint64_t from = (uint64_t)p.w;
+      __asm__ volatile("" : "+s"(from));  // (or the compiler reads them ahead of the rows and holds them after all)
+      param8<kVec>((const char*)from, p.wcode, at(i), p.D, 1.0f, v);
+    }
+  };
   const int64_t step = (int64_t)gridDim.x * kRows;
   int64_t row = (int64_t)blockIdx.x * kRows + sub;
   // The next row is requested ahead of the present one's arithmetic (kAhead); what a lane keeps of a row is its raw words, from
@@ -307,13 +322,14 @@ __global__ __launch_bounds__(kThreads) void layer_norm_grad_kernel(NormGrad p) {
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      float y[8], x[8];
+      float y[8], x[8], w[8];
+      weight(i, w);
       to_f32(ty[i], 1.0f, y);
       counted<kVec>(at(i), y);  // (y = 0 adds nothing to any sum)
       x_values(tx[i], ts[i], i, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float xh = (x[e] - m) * r, g = y[e] * w[i][e];
+        const float xh = (x[e] - m) * r, g = y[e] * w[e];
         s1 += g;
         s2 = fmaf(g, xh, s2);
         dw[i][e] = fmaf(y[e], xh, dw[i][e]);
@@ -324,7 +340,8 @@ __global__ __launch_bounds__(kThreads) void layer_norm_grad_kernel(NormGrad p) {
     const float rc1 = r * (s1 * inv), a = r * r * (s2 * inv);  // dx = r g - r c1 - (x - m) r^2 c2
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      float v[8], x[8];
+      float v[8], x[8], w[8];
+      weight(i, w);
       // (formed again from the words: the statement keeps the compiler from holding the first pass's values instead)
 #pragma unroll
       for (int k = 0; k < Eight<kCode>::kWords; ++k) __asm__ volatile("" : "+v"(ty[i].w[k]));
@@ -333,7 +350,7 @@ __global__ __launch_bounds__(kThreads) void layer_norm_grad_kernel(NormGrad p) {
       to_f32(ty[i], 1.0f, v);
       x_values(tx[i], ts[i], i, x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e] * w[i][e], r, fmaf(x[e] - m, -a, -rc1));
+      for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e] * w[e], r, fmaf(x[e] - m, -a, -rc1));
       store8<kCode, kVec>(p.dx + row * p.D * kElem, at(i), p.D, v);
     }
   }

@@ -288,7 +288,8 @@ int mxq::fp8_wgrad(const void* dy, int parts, int64_t ldy, const uint8_t* q, int
     return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld N=%lld K=%lld parts=%d", (long long)M, (long long)N, (long long)K, parts);
   const int64_t kb = (K + 127) / 128;
   // (64 rows are one buffer resource)
-  if (ldy >= (1 << 24) || ldq >= (1 << 24) || lds >= (1 << 24) || ldy < (N + 15) / 16 * 16 || ldy % 8 || ldq < (K + 15) / 16 * 16 || ldq % 16 || lds < kb)
+  if (ldy >= (1 << 24) || ldq >= (1 << 24) || lds >= (1 << 24) || ldy < (N + 15) / 16 * 16 || ldy % 8 ||
+      ldq < (K + 15) / 16 * 16 || ldq % 16 || lds < kb)
     return mxq_set_error(MXQ_ERR_INVALID, "bad row strides ldy=%lld ldq=%lld lds=%lld for N=%lld K=%lld", (long long)ldy,
                          (long long)ldq, (long long)lds, (long long)N, (long long)K);
   if (!dw || (M && (!dy || !q || !scale || !wg_aligned(dy, 16) || !wg_aligned(q, 16))))

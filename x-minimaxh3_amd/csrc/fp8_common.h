@@ -247,15 +247,14 @@ MXQ_DEVICE void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// The sum of `n` vectors, `stride` apart, in order; eight loads are in flight.
+// The sum of `n` vectors, `stride` apart, eight in flight at a time and added in pairs.
 MXQ_DEVICE v4f sum_slices(const v4f* p, int n, int64_t stride) {
   v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int s = 0; s < n; s += 8) {
     v4f t[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) t[i] = s + i < n ? p[(s + i) * stride] : v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y += t[i];
+    y += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
   }
   return y;
 }

@@ -7,7 +7,7 @@ using namespace mxq;
 
 namespace {
 
-constexpr int kThreads = 256;  // (1024: 0.4 us more for small slices, no less for a column's many rows)
+constexpr int kThreads = 256, kShares = kThreads / 32;  // (1024: 0.4 us more for small slices, no less for a column's many rows)
 
 // D = out(sum over slices + bias), four columns per thread; the slices' rows are padded to whole fours.
 template <int kOut>
@@ -23,23 +23,32 @@ MXQ_DEVICE void join_slices(const SliceJob& j, int64_t block) {
   store_run4<kOut>(reinterpret_cast<char*>(j.d) + row * j.ldd * kElem, col, j.cols - col, v);
 }
 
+MXQ_DEVICE float sum8(const float (&t)[8]) { return ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7])); }
+
 // out[c] = sum over `parts` rows of a float32 [parts, n] table. 32 columns (a line) and 8 shares of the rows per
-// workgroup; a share's loads go out eight at a time.
+// workgroup; a share's loads go out eight at a time and are added in pairs, as the shares are (one after the other, 256
+// rows of float32 sums were twice as far off).
+static_assert(kShares == 8, "added by sum8");
 template <int kOut>
-MXQ_DEVICE void join_columns(const ColumnJob& j, int64_t block, float (&sm)[kThreads / 32][32]) {
+MXQ_DEVICE void join_columns(const ColumnJob& j, int64_t block, float (&sm)[kShares][32]) {
   const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
   const int64_t col = block * 32 + c;
   float v = 0.0f;
   if (col < j.n) {
-#pragma unroll 8
-    for (int64_t i = r; i < j.parts; i += kThreads / 32) v += j.in[i * j.n + col];
+    for (int64_t i = r; i < j.parts; i += 8 * kShares) {
+      float t[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) t[u] = i + u * kShares < j.parts ? j.in[(i + u * kShares) * j.n + col] : 0.0f;
+      v += sum8(t);
+    }
   }
   sm[r][c] = v;
   __syncthreads();
   if (r == 0 && col < j.n) {
+    float t[8];
 #pragma unroll
-    for (int k = 1; k < kThreads / 32; ++k) v += sm[k][c];
-    store_out<kOut>(reinterpret_cast<typename OutT<kOut>::T*>(j.out) + col, v);
+    for (int k = 0; k < 8; ++k) t[k] = sm[k][c];
+    store_out<kOut>(reinterpret_cast<typename OutT<kOut>::T*>(j.out) + col, sum8(t));
   }
 }
 
@@ -52,7 +61,7 @@ MXQ_DEVICE void of_code(int code, F&& f) {
 }
 
 __global__ __launch_bounds__(kThreads) void fp8_join_kernel(SliceJob a, SliceJob b, ColumnJob c, int blocks_c, int blocks_a) {
-  __shared__ float sm[kThreads / 32][32];
+  __shared__ float sm[kShares][32];
   const int block = blockIdx.x;
   if (block < blocks_c)
     of_code(c.code, [&](auto C) { join_columns<decltype(C)::value>(c, block, sm); });

@@ -422,14 +422,19 @@ def layer_norm_backward(dy: torch.Tensor, x, mean: torch.Tensor, rstd: torch.Ten
 # modules
 # ---------------------------------------------------------------------------------------
 
+def _capturing(device: torch.device) -> bool:
+    """Whether ``device``'s current stream is being captured into a graph."""
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _refuse_capture(device: torch.device) -> None:
     """Autograd keeps one accumulation node per parameter, bound to the stream of its first use, for as long as any graph
     holds it: a backward pass captured while an eager graph of the same parameters lives would join that stream and
     end the process. A training step is captured through the functions, which own no such nodes."""
-    with torch.cuda.device(device):
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("the autograd modules are not captured into graphs; capture fp8_linear, fp8_linear_backward, "
-                               "layer_norm and layer_norm_backward instead")
+    if _capturing(device):
+        raise RuntimeError("the autograd modules are not captured into graphs; capture fp8_linear, fp8_linear_backward, "
+                           "layer_norm and layer_norm_backward instead")
 
 
 class _Fp8LinearFn(torch.autograd.Function):
@@ -488,7 +493,8 @@ class Fp8Linear(torch.nn.Module):
 
     def prepare(self) -> "Fp8Linear":
         """Builds the weight's 8-bit form from its present contents, for calls without weight gradients."""
-        self._prepared, self._prepared_of = prepare_fp8_weight(self.weight), self._state()
+        with torch.inference_mode(False):  # (tensors made in that mode cannot be saved for a backward pass)
+            self._prepared, self._prepared_of = prepare_fp8_weight(self.weight), self._state()
         return self
 
     def _form(self) -> PreparedFp8Weight:

@@ -3,10 +3,17 @@ counted in place of being made, streams are numbers, and the tensors (never fill
 
 from __future__ import annotations
 
+import copy
+import pickle
+
 import pytest
 import torch
 
 BUILD = "mxq_fp8_quantize_tiles"
+
+
+class _Calls(list):
+    pass
 
 
 @pytest.fixture
@@ -14,11 +21,16 @@ def host(monkeypatch):
     """The module's calls into the library as a list of names."""
     from mx_qlinear import fp8
 
-    calls = []
+    calls = _Calls()
     monkeypatch.setattr(fp8, "_launch", lambda dev, name, *args: calls.append(name))
     monkeypatch.setattr(fp8, "_require_gpu", lambda *tensors: torch.device("cpu"))
     monkeypatch.setattr(fp8, "_workspace", lambda *args: 0)
     monkeypatch.setattr(fp8, "_capturing", lambda device: False)
+    calls.stream, calls.follows = 0, []
+    monkeypatch.setattr(fp8, "_raw_stream", lambda index: calls.stream, raising=False)
+    monkeypatch.setattr(fp8, "_event", lambda device: ("built on", calls.stream), raising=False)
+    monkeypatch.setattr(fp8, "_follow", lambda device, event, tensors: calls.follows.append((calls.stream, event, len(tensors))),
+                        raising=False)
     return calls
 
 
@@ -37,3 +49,45 @@ def test_a_form_built_in_inference_mode_serves_a_later_backward_pass(host):
     layer(x).float().sum().backward()
     assert x.grad.shape == x.shape
     assert host.count(BUILD) == 1
+
+
+def test_another_stream_waits_for_the_build(host):
+    """A call on a stream that did not build the form waits for the build and holds the form's four tensors; the builder's
+    own calls do neither."""
+    layer, x = _layer(), torch.zeros(4, 256, dtype=torch.bfloat16)
+    with torch.no_grad():
+        host.stream = 5
+        layer(x)
+        layer(x)
+        assert host.count(BUILD) == 1 and host.follows == []
+        host.stream = 7
+        layer(x)
+        layer(x)
+        assert host.count(BUILD) == 1 and host.follows == [(7, ("built on", 5), 4)] * 2
+        layer.weight.mul_(2)
+        layer(x)
+        assert host.count(BUILD) == 2 and len(host.follows) == 2
+        host.stream = 5
+        layer(x)
+        assert host.follows[2:] == [(5, ("built on", 7), 4)]
+    host.stream = 9
+    layer(x.clone().requires_grad_())  # (the input's gradient alone)
+    assert host.count(BUILD) == 2 and host.follows[3:] == [(9, ("built on", 7), 4)]
+
+
+def test_copies_and_pickles_leave_the_form_behind(host):
+    layer, x = _layer(), torch.zeros(4, 256, dtype=torch.bfloat16)
+    layer(x)
+    for other in (copy.deepcopy(layer), pickle.loads(pickle.dumps(layer))):
+        assert other._prepared is None and layer._prepared is not None
+        assert torch.equal(other.weight, layer.weight)
+        other(x)
+    assert host.count(BUILD) == 3
+    # a pickle of the layer that held the form as an attribute
+    old = layer.__getstate__()
+    del old["_kept"]
+    other = type(layer).__new__(type(layer))
+    other.__setstate__({**old, "_prepared": layer._prepared, "_prepared_of": None})
+    assert other._prepared is None
+    other(x)
+    assert host.count(BUILD) == 4

@@ -488,3 +488,34 @@ def test_the_module_follows_its_weight(dev):
     q, s = mx.quantize_fp8_block128(x)
     want = mx.fp8_linear_backward(torch.ones(40, 96, device=dev, dtype=torch.bfloat16), q, s, mx.prepare_fp8_weight(layer.weight))
     assert torch.equal(xg.grad, want[0])
+
+
+def test_first_calls_on_two_streams(dev):
+    """The layer's hidden form is ordered by the layer: a call on one stream, right behind the call on another that builds
+    the form (held back there), reads the built one; and again behind a change of the weight. Its memory is not given out
+    while the second stream still reads it."""
+    mx = _mx()
+    x = _acts(64, 1024, torch.bfloat16, 1).to(dev)
+    layer = mx.Fp8Linear(1024, 2048, device=dev, dtype=torch.bfloat16).requires_grad_(False)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        want = mx.fp8_linear(x, mx.prepare_fp8_weight(layer.weight), layer.bias)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(a):
+            torch.cuda._sleep(20_000_000)
+            ya = layer(x)
+        with torch.cuda.stream(b):
+            yb = layer(x)
+        torch.cuda.synchronize()
+        assert torch.equal(ya, want) and torch.equal(yb, want)
+        with torch.cuda.stream(b):
+            torch.cuda._sleep(20_000_000)
+            yb = layer(x)
+        with torch.cuda.stream(a):  # (the form's own stream drops it and fills what it gave back)
+            other = layer.weight.clone()
+            layer.prepare()
+            fill = [torch.full_like(t, 127, dtype=torch.uint8) for t in (layer._prepared.q, layer._prepared.qt)]
+        torch.cuda.synchronize()
+        assert torch.equal(yb, want) and torch.equal(other, layer.weight) and len(fill) == 2
+        layer.weight.mul_(-1.5)
+        torch.cuda.synchronize()

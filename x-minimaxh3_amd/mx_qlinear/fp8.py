@@ -14,12 +14,13 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import threading
 from dataclasses import dataclass
 
 import torch
 
 from . import _lib
-from .ops import _OUT_CODES, _bias, _launch, _out_code, _ptr, _require_gpu, _rows, _vector
+from .ops import _OUT_CODES, _bias, _launch, _out_code, _ptr, _raw_stream, _require_gpu, _rows, _vector
 
 BLOCK = 128
 _CODES, _SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
@@ -466,6 +467,47 @@ class _Fp8LinearFn(torch.autograd.Function):
         return (dx.reshape(shape) if want_x else None, dw, db.to(bdtype) if want_b else None, None)
 
 
+def _event(device: torch.device):
+    """An event behind all that ``device``'s current stream has been given."""
+    event = torch.cuda.Event()
+    event.record(torch.cuda.current_stream(device))
+    return event
+
+
+def _follow(device: torch.device, event, tensors) -> None:
+    """Puts ``device``'s current stream behind ``event`` and holds the memory of ``tensors`` until its work on them is done."""
+    stream = torch.cuda.current_stream(device)
+    stream.wait_event(event)
+    for t in tensors:
+        t.record_stream(stream)
+
+
+class _Kept:
+    """A weight's 8-bit form that a layer keeps between calls, and what it was built from. The call that builds it writes
+    memory that its caller does not see, so the order of the streams that use it is kept here: one other than the
+    builder's waits for the build, and the memory is not given out again while it reads."""
+
+    __slots__ = ("form", "of", "stream", "built")
+
+    def __init__(self, form: PreparedFp8Weight, of: tuple):
+        self.form, self.of = form, of
+        self.stream, self.built = _raw_stream(form.device.index), _event(form.device)
+
+    def tensors(self) -> list[torch.Tensor]:
+        f = self.form
+        return [t for t in (f.q, f.scale, f.qt, f.scale_t) if t is not None]
+
+    def use(self) -> PreparedFp8Weight:
+        """The form, for work on the current stream."""
+        device = self.form.device
+        if _raw_stream(device.index) != self.stream:
+            _follow(device, self.built, self.tensors())
+        return self.form
+
+
+_KEPT_LOCK = threading.RLock()  # (calls of one layer from several threads)
+
+
 class Fp8Linear(torch.nn.Module):
     """A linear layer computed in 8-bit floating point, for serving and for training.
 
@@ -483,8 +525,18 @@ class Fp8Linear(torch.nn.Module):
         self.weight = torch.nn.Parameter(torch.empty(out_features, in_features, device=device, dtype=dtype))
         self.bias = torch.nn.Parameter(torch.zeros(out_features, device=device, dtype=dtype)) if bias else None
         torch.nn.init.normal_(self.weight, std=in_features**-0.5)
-        self._prepared: PreparedFp8Weight | None = None
-        self._prepared_of = None
+        self._kept: _Kept | None = None
+
+    @property
+    def _prepared(self) -> PreparedFp8Weight | None:
+        return None if self._kept is None else self._kept.form
+
+    def __getstate__(self):
+        return {**self.__dict__, "_kept": None}  # (copies and pickles build their own)
+
+    def __setstate__(self, state):
+        state = {k: v for k, v in state.items() if k not in ("_prepared", "_prepared_of")}
+        super().__setstate__({"_kept": None, **state})
 
     def _state(self):
         """What changes with the parameter's contents: the parameter, its storage and its count of changes in place."""
@@ -493,17 +545,18 @@ class Fp8Linear(torch.nn.Module):
 
     def prepare(self) -> "Fp8Linear":
         """Builds the weight's 8-bit form from its present contents, for calls without weight gradients."""
-        with torch.inference_mode(False):  # (tensors made in that mode cannot be saved for a backward pass)
-            self._prepared, self._prepared_of = prepare_fp8_weight(self.weight), self._state()
+        with _KEPT_LOCK, torch.inference_mode(False):  # (tensors made in that mode cannot be saved for a backward pass)
+            self._kept = _Kept(prepare_fp8_weight(self.weight), self._state())
         return self
 
     def _form(self) -> PreparedFp8Weight:
-        now, then = self._state(), self._prepared_of
-        if then is not None and then[0][0] is now[0][0] and then[1:] == now[1:]:
-            return self._prepared
-        if self.weight.is_cuda and torch.cuda.is_current_stream_capturing():
-            return prepare_fp8_weight(self.weight)  # (part of the graph, filled by its replays only: not kept)
-        return self.prepare()._prepared
+        with _KEPT_LOCK:
+            now, kept = self._state(), self._kept
+            if kept is not None and kept.of[0][0] is now[0][0] and kept.of[1:] == now[1:]:
+                return kept.use()
+            if self.weight.is_cuda and _capturing(self.weight.device):
+                return prepare_fp8_weight(self.weight)  # (part of the graph, filled by its replays only: not kept)
+            return self.prepare()._kept.use()
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dim() < 1 or x.shape[-1] != self.in_features:

@@ -25,8 +25,9 @@ def host(monkeypatch):
     monkeypatch.setattr(fp8, "_launch", lambda dev, name, *args: calls.append(name))
     monkeypatch.setattr(fp8, "_require_gpu", lambda *tensors: torch.device("cpu"))
     monkeypatch.setattr(fp8, "_workspace", lambda *args: 0)
-    monkeypatch.setattr(fp8, "_capturing", lambda device: False)
-    calls.stream, calls.follows = 0, []
+    monkeypatch.setattr(fp8, "_capturing", lambda device: calls.capturing)
+    monkeypatch.setattr(fp8, "_synchronize", lambda device: calls.append("synchronize"), raising=False)
+    calls.stream, calls.follows, calls.capturing = 0, [], False
     monkeypatch.setattr(fp8, "_raw_stream", lambda index: calls.stream, raising=False)
     monkeypatch.setattr(fp8, "_event", lambda device: ("built on", calls.stream), raising=False)
     monkeypatch.setattr(fp8, "_follow", lambda device, event, tensors: calls.follows.append((calls.stream, event, len(tensors))),
@@ -91,3 +92,70 @@ def test_copies_and_pickles_leave_the_form_behind(host):
     assert other._prepared is None
     other(x)
     assert host.count(BUILD) == 4
+
+
+def _pointers(layer):
+    f = layer._prepared
+    return [t.data_ptr() for t in (f.q, f.scale, f.qt, f.scale_t)]
+
+
+def test_a_captured_call_builds_its_own_form_unless_asked_before(host):
+    """Whether an eager call came first changes nothing: the form is the graph's own, or the one that was asked for."""
+    x = torch.zeros(4, 256, dtype=torch.bfloat16)
+    for eager in (False, True):
+        layer = _layer()
+        if eager:
+            layer(x)
+        kept = layer._prepared
+        host.capturing = True
+        del host[:]
+        layer(x)
+        host.capturing = False
+        assert host.count(BUILD) == 1 and layer._prepared is kept
+    layer.prepare()
+    host.capturing = True
+    del host[:]
+    layer(x)
+    assert host.count(BUILD) == 0 and host.follows == []
+    layer.weight.mul_(2)  # (no longer the weight's)
+    layer(x)
+    assert host.count(BUILD) == 1
+    with pytest.raises(RuntimeError, match="prepare"):
+        layer.prepare()
+
+
+def test_what_a_graph_reads_stays_in_place(host):
+    """The memory of a form that a graph reads is neither given back nor moved: later contents are written into it, between
+    two synchronizations, and a form that no longer fits is held."""
+    layer, x = _layer().prepare(), torch.zeros(4, 256, dtype=torch.bfloat16)
+    host.capturing = True
+    layer(x)
+    host.capturing = False
+    at, form = _pointers(layer), layer._prepared
+    for change in (lambda: layer.weight.mul_(2), lambda: layer.load_state_dict(layer.state_dict()), layer.float,
+                   lambda: setattr(layer, "weight", torch.nn.Parameter(layer.weight.detach() + 1, requires_grad=False))):
+        change()
+        del host[:]
+        layer(x)
+        assert host[:3] == ["synchronize", BUILD, "synchronize"]
+        assert layer._prepared is form and _pointers(layer) == at
+    layer.prepare()
+    assert layer._prepared is form and _pointers(layer) == at
+    layer.weight = torch.nn.Parameter(torch.zeros(100, 256), requires_grad=False)
+    layer.prepare()
+    assert layer._prepared is not form and layer._kept.held == (form,)
+
+
+def test_a_backward_pass_refuses_a_form_that_was_written_over(host):
+    """A form that a graph reads is written in place: a backward pass that saved it before does not run on other contents."""
+    layer = _layer(bias=False).prepare()
+    host.capturing = True
+    layer(torch.zeros(4, 256, dtype=torch.bfloat16))
+    host.capturing = False
+    x = torch.zeros(4, 256, dtype=torch.bfloat16, requires_grad=True)
+    y = layer(x)
+    layer.weight.mul_(2)
+    layer(x.detach())
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        y.float().sum().backward()
+    layer(x).float().sum().backward()

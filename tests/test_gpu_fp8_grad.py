@@ -519,3 +519,59 @@ def test_first_calls_on_two_streams(dev):
         assert torch.equal(yb, want) and torch.equal(other, layer.weight) and len(fill) == 2
         layer.weight.mul_(-1.5)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("eager_first", [False, True])
+@pytest.mark.parametrize("frozen", [False, True])
+def test_replays_of_the_module_follow_its_weight(dev, eager_first, frozen):
+    """Without ``prepare``, a graph's replays read the weight as it is, whether or not an eager call came before."""
+    mx = _mx()
+    x = _acts(40, 512, torch.bfloat16, 1).to(dev)
+    layer = mx.Fp8Linear(512, 384, device=dev, dtype=torch.bfloat16).requires_grad_(not frozen)
+    graph = torch.cuda.CUDAGraph()
+
+    def fresh():
+        return mx.fp8_linear(x, mx.prepare_fp8_weight(layer.weight), layer.bias)
+
+    with torch.no_grad():
+        fresh()
+        if eager_first:
+            layer(x)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            y = layer(x)
+        for i in range(4):
+            graph.replay()
+            assert torch.equal(y, fresh())
+            layer.weight.mul_(-1.25)
+            if i % 2:
+                assert torch.equal(layer(x), fresh())
+
+
+@pytest.mark.parametrize("frozen", [False, True])
+def test_replays_read_the_prepared_form_where_it_is(dev, frozen):
+    """After ``prepare`` a graph reads the layer's form: a changed weight reaches its replays with the next eager call or
+    ``prepare``, in the same memory, whatever else was allocated meanwhile."""
+    mx = _mx()
+    x = _acts(40, 512, torch.bfloat16, 1).to(dev)
+    layer = mx.Fp8Linear(512, 384, device=dev, dtype=torch.bfloat16).requires_grad_(not frozen).prepare()
+    graph, others = torch.cuda.CUDAGraph(), []
+
+    def fresh():
+        return mx.fp8_linear(x, mx.prepare_fp8_weight(layer.weight), layer.bias)
+
+    with torch.no_grad():
+        fresh()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            y = layer(x)
+        for i in range(6):
+            graph.replay()
+            assert torch.equal(y, fresh())
+            layer.weight.mul_(-1.25)
+            if i % 2:
+                layer.prepare()
+            else:
+                assert torch.equal(layer(x), fresh())
+            others += [torch.full_like(t, 127, dtype=torch.uint8) for t in (layer._prepared.q, layer._prepared.qt)]
+            torch.cuda.synchronize()

@@ -180,22 +180,32 @@ def prepare_fp8_weight(weight: torch.Tensor, scale: torch.Tensor | None = None, 
                              f"{scale.dtype}")
         if tuple(scale.shape) != (nb, kb):
             raise ValueError(f"weight scale of shape {tuple(scale.shape)}, expected {(nb, kb)}")
+        code = None
     else:
         code = _float_code(weight, "weight")
     dev = _require_gpu(weight, scale)
+    form = PreparedFp8Weight(
+        torch.empty(n, kb * BLOCK, dtype=_CODES, device=dev), torch.empty(nb, _ceil(kb, 4), dtype=_SCALE, device=dev),
+        torch.empty(k, nb * BLOCK, dtype=_CODES, device=dev) if transposed else None,
+        torch.empty(kb, _ceil(nb, 4), dtype=_SCALE, device=dev) if transposed else None, n, k)
+    _write_form(form, weight, code, scale)
+    return form
+
+
+def _write_form(form: PreparedFp8Weight, weight: torch.Tensor, code: int | None, scale: torch.Tensor | None = None) -> None:
+    """Lays ``weight`` (of dtype ``code``, or codes with ``scale``) out in ``form``'s tensors."""
+    n, k = weight.shape
     w = _rows_in_place(weight, k)
-    q = torch.empty(n, kb * BLOCK, dtype=_CODES, device=dev)
-    s = torch.empty(nb, _ceil(kb, 4), dtype=_SCALE, device=dev)
-    qt = torch.empty(k, nb * BLOCK, dtype=_CODES, device=dev) if transposed else None
-    st = torch.empty(kb, _ceil(nb, 4), dtype=_SCALE, device=dev) if transposed else None
-    out = (q.data_ptr(), q.shape[1], s.data_ptr(), s.shape[1], _ptr(qt), nb * BLOCK, _ptr(st), _ceil(nb, 4), n, k)
+    q, s, qt, st = form.q, form.scale, form.qt, form.scale_t
+    out = (q.data_ptr(), q.shape[1], s.data_ptr(), s.shape[1], _ptr(qt), 0 if qt is None else qt.shape[1], _ptr(st),
+           0 if st is None else st.shape[1], n, k)
     ldw = w.stride(0) if n > 1 else k
     if scale is not None:
+        nb, kb = scale.shape
         ws = _rows_in_place(scale, kb)
-        _launch(dev, "mxq_fp8_prepare_tiles", w.data_ptr(), ldw, ws.data_ptr(), ws.stride(0) if nb > 1 else kb, *out)
+        _launch(form.device, "mxq_fp8_prepare_tiles", w.data_ptr(), ldw, ws.data_ptr(), ws.stride(0) if nb > 1 else kb, *out)
     else:
-        _launch(dev, "mxq_fp8_quantize_tiles", w.data_ptr(), code, ldw, *out)
-    return PreparedFp8Weight(q, s, qt, st, n, k)
+        _launch(form.device, "mxq_fp8_quantize_tiles", w.data_ptr(), code, ldw, *out)
 
 
 # ---------------------------------------------------------------------------------------
@@ -425,6 +435,10 @@ def layer_norm_backward(dy: torch.Tensor, x, mean: torch.Tensor, rstd: torch.Ten
 
 def _capturing(device: torch.device) -> bool:
     """Whether ``device``'s current stream is being captured into a graph."""
+    if device.type != "cuda":
+        return False
+    if torch.cuda.current_device() == device.index:
+        return torch.cuda.is_current_stream_capturing()
     with torch.cuda.device(device):
         return torch.cuda.is_current_stream_capturing()
 
@@ -482,16 +496,30 @@ def _follow(device: torch.device, event, tensors) -> None:
         t.record_stream(stream)
 
 
+def _synchronize(device: torch.device) -> None:
+    torch.cuda.synchronize(device)
+
+
 class _Kept:
     """A weight's 8-bit form that a layer keeps between calls, and what it was built from. The call that builds it writes
     memory that its caller does not see, so the order of the streams that use it is kept here: one other than the
-    builder's waits for the build, and the memory is not given out again while it reads."""
+    builder's waits for the build, and the memory is not given out again while it reads. ``asked``: by the layer's user,
+    who has waited for it. A graph reads only such a form, in place (``captured``); ``held`` are the forms that graphs
+    read and that no longer fit the weight."""
 
-    __slots__ = ("form", "of", "stream", "built")
+    __slots__ = ("form", "of", "asked", "captured", "held", "stream", "built")
 
-    def __init__(self, form: PreparedFp8Weight, of: tuple):
-        self.form, self.of = form, of
-        self.stream, self.built = _raw_stream(form.device.index), _event(form.device)
+    def __init__(self, form: PreparedFp8Weight, of: tuple, asked: bool, held: tuple = ()):
+        self.form, self.captured, self.held = form, False, held
+        self.done(of, asked)
+
+    def done(self, of: tuple, asked: bool) -> None:
+        """The current stream has been given the build."""
+        self.of, self.asked = of, asked
+        self.stream, self.built = _raw_stream(self.form.device.index), _event(self.form.device)
+
+    def fits(self, weight: torch.Tensor) -> bool:
+        return weight.shape == (self.form.out_features, self.form.in_features) and weight.device == self.form.device
 
     def tensors(self) -> list[torch.Tensor]:
         f = self.form
@@ -517,6 +545,9 @@ class Fp8Linear(torch.nn.Module):
     gradient has the form built from the parameter in every forward, and what the backward pass keeps of the input is its
     8-bit pair (:func:`fp8_linear_backward`). The quantizers pass gradients through unchanged. Activations are bf16, fp16
     or fp32.
+
+    Calls without gradients can be captured into a graph. Its replays build the form from the parameter's contents each
+    time, unless :meth:`prepare` was called first: then they read that form.
     """
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None):
@@ -543,20 +574,41 @@ class Fp8Linear(torch.nn.Module):
         w = self.weight
         return (w,), w.data_ptr(), w.dtype, w.device, None if w.is_inference() else w._version
 
+    def _build(self, asked: bool) -> _Kept:
+        """The kept form anew from the parameter's present contents; in the same memory where a graph reads it."""
+        weight, kept = self.weight.detach(), self._kept
+        with torch.inference_mode(False):  # (tensors made in that mode cannot be saved for a backward pass)
+            if kept is None or not kept.captured or not kept.fits(weight):
+                held = () if kept is None else kept.held + ((kept.form,) if kept.captured else ())
+                self._kept = _Kept(prepare_fp8_weight(weight), self._state(), asked, held)
+            else:  # (replays may be under way on any stream, and follow on any)
+                _synchronize(weight.device)
+                _write_form(kept.form, weight, _float_code(weight, "weight"))
+                torch.autograd.graph.increment_version(kept.tensors())  # (backward passes that saved them refuse to run)
+                _synchronize(weight.device)
+                kept.done(self._state(), asked)
+        return self._kept
+
     def prepare(self) -> "Fp8Linear":
-        """Builds the weight's 8-bit form from its present contents, for calls without weight gradients."""
-        with _KEPT_LOCK, torch.inference_mode(False):  # (tensors made in that mode cannot be saved for a backward pass)
-            self._kept = _Kept(prepare_fp8_weight(self.weight), self._state())
+        """Builds the weight's 8-bit form from its present contents, for calls without weight gradients, and waits for it.
+        Calls captured into graphs read this form where it is: later changes of the weight reach their replays with the
+        next ``prepare`` or eager call."""
+        if _capturing(self.weight.device):
+            raise RuntimeError("Fp8Linear.prepare is not captured into graphs: call it before the capture")
+        with _KEPT_LOCK:
+            _synchronize(self._build(True).form.device)
         return self
 
     def _form(self) -> PreparedFp8Weight:
         with _KEPT_LOCK:
             now, kept = self._state(), self._kept
-            if kept is not None and kept.of[0][0] is now[0][0] and kept.of[1:] == now[1:]:
-                return kept.use()
-            if self.weight.is_cuda and _capturing(self.weight.device):
-                return prepare_fp8_weight(self.weight)  # (part of the graph, filled by its replays only: not kept)
-            return self.prepare()._kept.use()
+            current = kept is not None and kept.of[0][0] is now[0][0] and kept.of[1:] == now[1:]
+            if _capturing(self.weight.device):
+                if current and kept.asked:
+                    kept.captured = True
+                    return kept.form
+                return prepare_fp8_weight(self.weight, transposed=False)  # (part of the graph: its replays follow the weight)
+            return (kept if current else self._build(False)).use()
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dim() < 1 or x.shape[-1] != self.in_features:

@@ -38,7 +38,7 @@ def host(monkeypatch):
 def _layer(frozen=True, **kw):
     from mx_qlinear import Fp8Linear
 
-    layer = Fp8Linear(256, 96, dtype=torch.bfloat16, **kw)
+    layer = Fp8Linear(256, 96, **{"dtype": torch.bfloat16, **kw})
     return layer.requires_grad_(not frozen)
 
 
@@ -159,3 +159,121 @@ def test_a_backward_pass_refuses_a_form_that_was_written_over(host):
     with pytest.raises(RuntimeError, match="inplace operation"):
         y.float().sum().backward()
     layer(x).float().sum().backward()
+
+
+@pytest.mark.parametrize("optimizer", [torch.optim.AdamW, torch.optim.SGD])
+def test_a_trainable_weight_is_read_anew_by_every_call(host, optimizer):
+    """A fused optimizer changes the parameter without counting it."""
+    # (float32: of bfloat16 parameters in host memory torch's fused SGD leaves whole vectors as they are)
+    layer, x = _layer(frozen=False, dtype=torch.float32), torch.zeros(4, 256, dtype=torch.bfloat16)
+    step = optimizer(layer.parameters(), lr=0.1, fused=True)
+    with torch.no_grad():
+        layer(x)
+    before, state = layer.weight.detach().clone(), layer._state()
+    layer.weight.grad, layer.bias.grad = torch.ones_like(layer.weight), torch.ones_like(layer.bias)
+    step.step()
+    assert not torch.equal(layer.weight, before)
+    assert layer._state()[1:] == state[1:], "counted after all: the rule can be looser"
+    with torch.no_grad():
+        for calls in (2, 3):
+            layer(x)
+            assert host.count(BUILD) == calls
+        form = layer._form()
+        assert layer._form() is form and host.count(BUILD) == 5  # (the same memory, written anew)
+        assert form.qt is None  # (which only the input's gradient of a frozen layer reads)
+    # asked for, it is kept: up to the next forward with gradients, and train() or eval()
+    for end in (lambda: layer(x), layer.eval, layer.train, lambda: layer.weight.detach().mul_(2),
+                lambda: layer.load_state_dict(layer.state_dict())):
+        layer.prepare()
+        del host[:]
+        with torch.no_grad():
+            layer(x)
+            layer(x)
+        assert host.count(BUILD) == 0
+        end()
+        del host[:]
+        with torch.no_grad():
+            layer(x)
+        assert host.count(BUILD) == 1
+    # frozen after training without a counted change
+    layer.requires_grad_(False)
+    layer(x)
+    layer.requires_grad_(True)
+    layer(x)
+    layer.requires_grad_(False)
+    del host[:]
+    layer(x)
+    layer(x)
+    assert host.count(BUILD) == 1
+
+
+def test_a_frozen_weight_is_read_anew_once_it_may_have_changed(host):
+    layer, x = _layer(), torch.zeros(4, 256, dtype=torch.bfloat16)
+    layer(x)
+    layer(x)
+    assert host.count(BUILD) == 1
+    w = layer.weight
+    # the state before and after a type and back can be the same: a layer of one value, rounded by it
+    for change in (lambda: w.add_(1), lambda: layer.load_state_dict(layer.state_dict()), lambda: layer.float().bfloat16(),
+                   layer.half, layer.eval, lambda: setattr(layer, "weight", torch.nn.Parameter(w.detach() + 1, False))):
+        change()
+        del host[:]
+        layer(x.to(layer.weight.dtype))
+        layer(x.to(layer.weight.dtype))
+        assert host.count(BUILD) == 1
+    layer.prepare()
+    layer.eval()
+    del host[:]
+    layer(x.half())
+    assert host.count(BUILD) == 0
+
+
+def test_a_weight_of_inference_mode_is_read_anew_by_every_call(host):
+    with torch.inference_mode():
+        layer, x = _layer(), torch.zeros(4, 256, dtype=torch.bfloat16)
+        assert layer.weight.is_inference()
+        layer(x)
+        layer.weight.mul_(2)
+        layer(x)
+        assert host.count(BUILD) == 2
+        layer.prepare()
+        layer(x)
+        assert host.count(BUILD) == 3
+        layer.load_state_dict({k: v * 2 for k, v in layer.state_dict().items()})
+        layer(x)
+        assert host.count(BUILD) == 4
+
+
+def test_memory_that_others_read_is_not_written_over(host):
+    """A form that another stream or a backward pass reads is replaced, not written anew."""
+    layer = _layer(bias=False)
+    x = torch.zeros(4, 256, dtype=torch.bfloat16)
+    layer(x)
+    first = layer._prepared
+    layer.weight.mul_(2)
+    layer(x)
+    assert layer._prepared is first
+    y = layer(x.clone().requires_grad_())
+    layer.weight.mul_(2)
+    layer(x)
+    second = layer._prepared
+    assert second is not first
+    y.float().sum().backward()
+    host.stream = 3
+    layer(x)
+    host.stream = 0
+    layer.weight.mul_(2)
+    layer(x)
+    third = layer._prepared
+    assert third is not second
+    host.stream = 3
+    layer.weight.mul_(2)
+    layer(x)
+    assert layer._prepared is not third
+
+
+def test_a_moved_layer_gives_its_form_back(host):
+    layer, x = _layer(), torch.zeros(4, 256, dtype=torch.bfloat16)
+    layer(x)
+    layer.to(torch.float16)
+    assert layer._prepared is None

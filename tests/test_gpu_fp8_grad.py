@@ -575,3 +575,54 @@ def test_replays_read_the_prepared_form_where_it_is(dev, frozen):
                 assert torch.equal(layer(x), fresh())
             others += [torch.full_like(t, 127, dtype=torch.uint8) for t in (layer._prepared.q, layer._prepared.qt)]
             torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("optimizer", [torch.optim.AdamW, torch.optim.SGD])
+def test_evaluation_after_a_fused_step(dev, optimizer):
+    """Train, step with a fused optimizer (which does not count its changes), evaluate: the evaluation has the new weight,
+    also once the layer is frozen, and in a replayed graph."""
+    mx = _mx()
+    x = _acts(40, 256, torch.bfloat16, 1).to(dev)
+    layer = mx.Fp8Linear(256, 96, device=dev, dtype=torch.float32)
+    step, last, graph = optimizer(layer.parameters(), lr=0.05, fused=True), None, torch.cuda.CUDAGraph()
+    with torch.no_grad():
+        layer(x)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            captured = layer(x)
+    for _ in range(3):
+        layer(x).float().square().sum().backward()
+        step.step()
+        step.zero_grad()
+        with torch.no_grad():
+            want = mx.fp8_linear(x, mx.prepare_fp8_weight(layer.weight), layer.bias)
+            assert torch.equal(layer(x), want) and torch.equal(layer(x), want)
+            graph.replay()
+            assert torch.equal(captured, want)
+        assert last is None or not torch.equal(want, last)
+        last = want
+        layer.requires_grad_(False)
+        assert torch.equal(layer(x), want)
+        layer.requires_grad_(True)
+
+
+def test_inference_loads_and_types_and_back(dev):
+    """Contents that change without a count: loaded in inference mode, or rounded by a type and back."""
+    mx = _mx()
+    x = _acts(40, 256, torch.bfloat16, 1).to(dev)
+
+    def right(layer):
+        return torch.equal(layer(x), mx.fp8_linear(x, mx.prepare_fp8_weight(layer.weight), layer.bias))
+
+    with torch.inference_mode():
+        layer = mx.Fp8Linear(256, 96, device=dev, dtype=torch.float32).requires_grad_(False)
+        for _ in range(3):
+            assert right(layer)
+            layer.load_state_dict({k: v * -1.5 for k, v in layer.state_dict().items()})
+    layer = mx.Fp8Linear(256, 96, device=dev, dtype=torch.float32).requires_grad_(False)
+    for _ in range(3):
+        layer.weight.add_(0.001)
+        assert right(layer)
+        layer.bfloat16()
+        layer.float()
+        assert right(layer)

@@ -501,16 +501,17 @@ def _synchronize(device: torch.device) -> None:
 
 
 class _Kept:
-    """A weight's 8-bit form that a layer keeps between calls, and what it was built from. The call that builds it writes
-    memory that its caller does not see, so the order of the streams that use it is kept here: one other than the
-    builder's waits for the build, and the memory is not given out again while it reads. ``asked``: by the layer's user,
-    who has waited for it. A graph reads only such a form, in place (``captured``); ``held`` are the forms that graphs
-    read and that no longer fit the weight."""
+    """A weight's 8-bit form that a layer keeps between calls, and what it was built from (``of``; ``None``: of nothing that
+    still holds). The call that builds it writes memory that its caller does not see, so the order of the streams that use
+    it is kept here: one other than the builder's waits for the build, and the memory is not given out again while it
+    reads. ``asked``: by the layer's user, who has waited for it. A graph reads only such a form, in place (``captured``);
+    ``held`` are the forms that graphs read and that no longer fit the weight. ``shared``: another stream, or a backward
+    pass to come, reads the form."""
 
-    __slots__ = ("form", "of", "asked", "captured", "held", "stream", "built")
+    __slots__ = ("form", "of", "asked", "captured", "shared", "held", "stream", "built")
 
     def __init__(self, form: PreparedFp8Weight, of: tuple, asked: bool, held: tuple = ()):
-        self.form, self.captured, self.held = form, False, held
+        self.form, self.captured, self.shared, self.held = form, False, False, held
         self.done(of, asked)
 
     def done(self, of: tuple, asked: bool) -> None:
@@ -518,8 +519,20 @@ class _Kept:
         self.of, self.asked = of, asked
         self.stream, self.built = _raw_stream(self.form.device.index), _event(self.form.device)
 
-    def fits(self, weight: torch.Tensor) -> bool:
-        return weight.shape == (self.form.out_features, self.form.in_features) and weight.device == self.form.device
+    def forget(self) -> None:
+        self.of, self.asked = None, False
+
+    def holds(self, state: tuple) -> bool:
+        return self.of is not None and self.of[0][0] is state[0][0] and self.of[1:] == state[1:]
+
+    def fits(self, weight: torch.Tensor, transposed: bool) -> bool:
+        f = self.form
+        return (weight.shape == (f.out_features, f.in_features) and weight.device == f.device and
+                (f.qt is not None or not transposed))
+
+    def alone(self) -> bool:
+        """Whether only earlier work of the current stream reads the form."""
+        return not self.shared and self.stream == _raw_stream(self.form.device.index)
 
     def tensors(self) -> list[torch.Tensor]:
         f = self.form
@@ -529,6 +542,7 @@ class _Kept:
         """The form, for work on the current stream."""
         device = self.form.device
         if _raw_stream(device.index) != self.stream:
+            self.shared = True
             _follow(device, self.built, self.tensors())
         return self.form
 
@@ -539,10 +553,11 @@ _KEPT_LOCK = threading.RLock()  # (calls of one layer from several threads)
 class Fp8Linear(torch.nn.Module):
     """A linear layer computed in 8-bit floating point, for serving and for training.
 
-    ``weight`` ``[out_features, in_features]`` and ``bias`` are ordinary parameters (bf16, fp16 or fp32). A weight that needs
-    no gradient is read in its 8-bit form, built by :meth:`prepare` or the first call, and again once the parameter was
-    moved, loaded or changed in place (changes through ``.data`` are not seen: call :meth:`prepare`). One that needs a
-    gradient has the form built from the parameter in every forward, and what the backward pass keeps of the input is its
+    ``weight`` ``[out_features, in_features]`` and ``bias`` are ordinary parameters (bf16, fp16 or fp32). A frozen
+    weight is read in its 8-bit form, built by :meth:`prepare` or the first call, and again once the parameter was moved,
+    loaded or changed in place (changes through ``.data`` are not seen: call :meth:`prepare`). One that needs a gradient, or
+    was made in inference mode, has the form built from the parameter in every call, since fused optimizers and inference
+    mode change it unseen; without gradients :meth:`prepare` saves that. What the backward pass keeps of the input is its
     8-bit pair (:func:`fp8_linear_backward`). The quantizers pass gradients through unchanged. Activations are bf16, fp16
     or fp32.
 
@@ -574,41 +589,74 @@ class Fp8Linear(torch.nn.Module):
         w = self.weight
         return (w,), w.data_ptr(), w.dtype, w.device, None if w.is_inference() else w._version
 
-    def _build(self, asked: bool) -> _Kept:
-        """The kept form anew from the parameter's present contents; in the same memory where a graph reads it."""
+    def _forget(self) -> None:
+        if self._kept is not None:
+            self._kept.forget()
+
+    def _apply(self, fn, recurse: bool = True):
+        out = super()._apply(fn, recurse)
+        with _KEPT_LOCK:  # (a type and back can return the storage and count of before with rounded contents)
+            self._forget()
+            if self._kept is not None and not self._kept.captured:
+                self._kept = None
+        return out
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self._forget()
+
+    def train(self, mode: bool = True):
+        if self.weight.requires_grad or not (self._kept is not None and self._kept.asked):
+            self._forget()
+        return super().train(mode)
+
+    def _build(self, asked: bool, transposed: bool) -> _Kept:
+        """The kept form anew from the parameter's present contents; in the same memory where a graph reads it, or where
+        nothing else can be reading it."""
         weight, kept = self.weight.detach(), self._kept
         with torch.inference_mode(False):  # (tensors made in that mode cannot be saved for a backward pass)
-            if kept is None or not kept.captured or not kept.fits(weight):
+            if kept is None or not kept.fits(weight, transposed) or not (kept.captured or kept.alone()):
                 held = () if kept is None else kept.held + ((kept.form,) if kept.captured else ())
-                self._kept = _Kept(prepare_fp8_weight(weight), self._state(), asked, held)
-            else:  # (replays may be under way on any stream, and follow on any)
-                _synchronize(weight.device)
+                self._kept = _Kept(prepare_fp8_weight(weight, transposed=transposed), self._state(), asked, held)
+            else:
+                if kept.captured:  # (replays may be under way on any stream, and follow on any)
+                    _synchronize(weight.device)
                 _write_form(kept.form, weight, _float_code(weight, "weight"))
                 torch.autograd.graph.increment_version(kept.tensors())  # (backward passes that saved them refuse to run)
-                _synchronize(weight.device)
+                if kept.captured:
+                    _synchronize(weight.device)
                 kept.done(self._state(), asked)
         return self._kept
 
     def prepare(self) -> "Fp8Linear":
         """Builds the weight's 8-bit form from its present contents, for calls without weight gradients, and waits for it.
-        Calls captured into graphs read this form where it is: later changes of the weight reach their replays with the
-        next ``prepare`` or eager call."""
+        The form is taken for the weight's until the parameter is seen to change, moved or loaded, until a forward with
+        gradients of the weight, and, unless it is frozen, until :meth:`train` or :meth:`eval`. Calls captured into graphs
+        read it where it is: later changes of the weight reach their replays with the next ``prepare`` or eager call."""
         if _capturing(self.weight.device):
             raise RuntimeError("Fp8Linear.prepare is not captured into graphs: call it before the capture")
         with _KEPT_LOCK:
-            _synchronize(self._build(True).form.device)
+            _synchronize(self._build(True, True).form.device)
         return self
 
-    def _form(self) -> PreparedFp8Weight:
+    def _form(self, saved: bool = False) -> PreparedFp8Weight:
+        """The form for one call; ``saved``: a backward pass will read it too."""
         with _KEPT_LOCK:
-            now, kept = self._state(), self._kept
-            current = kept is not None and kept.of[0][0] is now[0][0] and kept.of[1:] == now[1:]
-            if _capturing(self.weight.device):
+            kept, weight = self._kept, self.weight
+            # Not every change in place is counted: fused optimizers and changes of inference tensors are not. A form of a
+            # weight that is open to them is the weight's for one call only, unless it was asked for.
+            current = (kept is not None and kept.holds(self._state()) and (kept.form.qt is not None or not saved) and
+                       (kept.asked or not (weight.requires_grad or weight.is_inference())))
+            if _capturing(weight.device):
                 if current and kept.asked:
                     kept.captured = True
                     return kept.form
-                return prepare_fp8_weight(self.weight, transposed=False)  # (part of the graph: its replays follow the weight)
-            return (kept if current else self._build(False)).use()
+                return prepare_fp8_weight(weight, transposed=False)  # (part of the graph: its replays follow the weight)
+            if not current:
+                kept = self._build(False, saved or not weight.requires_grad)
+            form = kept.use()
+            kept.shared |= saved
+            return form
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dim() < 1 or x.shape[-1] != self.in_features:
@@ -616,7 +664,11 @@ class Fp8Linear(torch.nn.Module):
         params = [p for p in (self.weight, self.bias) if p is not None]
         if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, *params))):
             return fp8_linear(x, self._form(), self.bias)
-        prepared = prepare_fp8_weight(self.weight) if self.weight.requires_grad else self._form()
+        if self.weight.requires_grad:
+            self._forget()
+            prepared = prepare_fp8_weight(self.weight)
+        else:
+            prepared = self._form(saved=True)
         return _Fp8LinearFn.apply(x, self.weight, self.bias, prepared)
 
     def extra_repr(self) -> str:

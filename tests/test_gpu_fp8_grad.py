@@ -626,3 +626,22 @@ def test_inference_loads_and_types_and_back(dev):
         layer.bfloat16()
         layer.float()
         assert right(layer)
+
+
+@pytest.mark.parametrize("wtype,btype", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16), (torch.float16, torch.bfloat16)])
+@pytest.mark.parametrize("frozen", [False, True])
+def test_parameters_of_two_types(dev, wtype, btype, frozen):
+    """Each parameter's gradient is rounded once, to its own type."""
+    mx = _mx()
+    layer = mx.Fp8Linear(200, 72, device=dev, dtype=wtype)
+    layer.bias = torch.nn.Parameter(torch.zeros(72, device=dev, dtype=btype))
+    layer.weight.requires_grad_(not frozen)
+    x, dy = _acts(90, 200, torch.bfloat16, 1).to(dev), (_acts(90, 72, torch.bfloat16, 2) * 0.1).to(dev)
+    layer(x).backward(dy)
+    q, s = mx.quantize_fp8_block128(x)
+    _, dw, db = mx.fp8_linear_backward(dy, q, s, mx.prepare_fp8_weight(layer.weight), (False, True, True))
+    assert layer.bias.grad.dtype == btype and torch.equal(layer.bias.grad, db.to(btype))
+    if frozen:
+        assert layer.weight.grad is None
+    else:
+        assert layer.weight.grad.dtype == wtype and torch.equal(layer.weight.grad, dw.to(wtype))

@@ -476,9 +476,11 @@ class _Fp8LinearFn(torch.autograd.Function):
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
         weight = PreparedFp8Weight(q, s, qt, st, n, k)  # (the gradients read the transposed copy only)
         m = q.shape[0]
+        # of two types, both gradients in float32, each then rounded once to its own
+        wanted = {t for t, want in ((wdtype, want_w), (bdtype, want_b)) if want}
         dx, dw, db = fp8_linear_backward(dy.reshape(m, n), q[:, :k], s[:, : -(-k // BLOCK)], weight, (want_x, want_w, want_b),
-                                         wdtype or bdtype or torch.float32)
-        return (dx.reshape(shape) if want_x else None, dw, db.to(bdtype) if want_b else None, None)
+                                         wanted.pop() if len(wanted) == 1 else torch.float32)
+        return (dx.reshape(shape) if want_x else None, dw.to(wdtype) if want_w else None, db.to(bdtype) if want_b else None, None)
 
 
 def _event(device: torch.device):

@@ -645,3 +645,26 @@ def test_parameters_of_two_types(dev, wtype, btype, frozen):
         assert layer.weight.grad is None
     else:
         assert layer.weight.grad.dtype == wtype and torch.equal(layer.weight.grad, dw.to(wtype))
+
+
+@pytest.mark.parametrize("m", [1, 3])
+@pytest.mark.parametrize("far", ["dy", "codes", "scale"])
+def test_backward_of_rows_far_apart(dev, far, m):
+    """Rows further apart than the weight's gradient reads in place: copied, as the forward pass copies them."""
+    mx = _mx()
+    n, k = 48, 384
+    x, w, dy = _acts(m, k, torch.bfloat16, 1), _acts(n, k, torch.float32, 2) * 0.05, (_acts(m, n, torch.bfloat16, 3) * 0.1).to(dev)
+    p = mx.prepare_fp8_weight(w.to(dev))
+    q, s = mx.quantize_fp8_block128(x.to(dev))
+    want = mx.fp8_linear_backward(dy, q, s, p)
+
+    def apart(t):
+        wide = torch.zeros(m, 2**24 + 64, dtype=t.dtype, device=dev)
+        wide[:, : t.shape[1]] = t
+        return wide[:, : t.shape[1]]
+
+    args = {"dy": dy, "codes": q, "scale": s}
+    args[far] = apart(args[far])
+    got = mx.fp8_linear_backward(args["dy"], args["codes"], args["scale"], p)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(mx.fp8_linear_prequantized(args["codes"], args["scale"], p), mx.fp8_linear_prequantized(q, s, p))

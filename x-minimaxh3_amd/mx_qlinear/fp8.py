@@ -25,6 +25,7 @@ from .ops import _OUT_CODES, _bias, _launch, _out_code, _ptr, _raw_stream, _requ
 BLOCK = 128
 _CODES, _SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
 _MAX_STRIDE = 1 << 22  # of an operand's rows; wider ones are copied
+_MAX_GRAD_STRIDE = 1 << 24  # below it, of the rows that the weight's gradient reads
 
 
 def _ceil(n: int, to: int) -> int:
@@ -293,7 +294,7 @@ def fp8_linear_prequantized(q: torch.Tensor, scale: torch.Tensor, weight: Prepar
 def _readable(t: torch.Tensor, width: int) -> bool:
     """Whether every row of ``t`` (1-byte elements) can be read ``width`` wide from 16-byte boundaries."""
     m, ld = t.shape[0], t.stride(0)
-    if t.data_ptr() % 16 or (m > 1 and (ld % 16 or ld < width)):
+    if t.data_ptr() % 16 or (m > 1 and (ld % 16 or not width <= ld < _MAX_GRAD_STRIDE)):
         return False
     return t.untyped_storage().nbytes() - t.storage_offset() >= (m - 1) * ld + width
 
@@ -322,8 +323,10 @@ def fp8_linear_backward(dy: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, 
     dev = _require_gpu(dy, q, scale, weight.q)
     y = _rows_in_place(dy, n)
     ldy = y.stride(0) if m > 1 else n
-    direct = dy.dtype == torch.bfloat16 and n % 16 == 0 and ldy % 8 == 0 and y.data_ptr() % 16 == 0
+    direct = dy.dtype == torch.bfloat16 and n % 16 == 0 and ldy % 8 == 0 and ldy < _MAX_GRAD_STRIDE and y.data_ptr() % 16 == 0
     readable = _readable(q, _ceil(k, 16))
+    if m > 1 and scale.stride(0) >= _MAX_GRAD_STRIDE:
+        scale = scale.contiguous()
     dx = torch.empty(m, k, dtype=dy.dtype, device=dev) if want_x else None
     dw = torch.empty(n, k, dtype=grad_dtype, device=dev) if want_w else None
     db = torch.empty(n, dtype=grad_dtype, device=dev) if want_b else None
@@ -334,9 +337,10 @@ def fp8_linear_backward(dy: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, 
         ws = _room(need, dev)
         bt, st = weight.qt, weight.scale_t
         _launch(dev, "mxq_fp8_linear_backward", y.data_ptr(), code, ldy, direct, q.data_ptr(),
-                q.stride(0) if m > 1 else _ceil(k, 16) if readable else k, scale.data_ptr(), max(scale.stride(0), scale.shape[1]),
-                readable, _ptr(bt), bt.shape[1] if want_x else 0, _ptr(st), st.shape[1] if want_x else 0,
-                dx.data_ptr() if want_x and m else None, _ptr(dw), _ptr(db), gcode, m, n, k, _ptr(ws), need)
+                q.stride(0) if m > 1 else _ceil(k, 16) if readable else k, scale.data_ptr(),
+                scale.stride(0) if m > 1 else scale.shape[1], readable, _ptr(bt), bt.shape[1] if want_x else 0,
+                _ptr(st), st.shape[1] if want_x else 0, dx.data_ptr() if want_x and m else None,
+                _ptr(dw), _ptr(db), gcode, m, n, k, _ptr(ws), need)
     if want_x and len(shape) != 2:
         dx = dx.reshape(shape)
     return dx, dw, db

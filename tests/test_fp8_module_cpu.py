@@ -277,3 +277,26 @@ def test_a_moved_layer_gives_its_form_back(host):
     layer(x)
     layer.to(torch.float16)
     assert layer._prepared is None
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("dual", ["x", "weight", "bias"])
+@pytest.mark.parametrize("name", ["Fp8Linear", "LayerNorm"])
+def test_forward_mode_is_refused(host, name, dual, requires_grad):
+    """A tangent is carried on or refused, never dropped."""
+    import mx_qlinear
+    from torch.autograd import forward_ad
+
+    module = mx_qlinear.Fp8Linear(256, 96) if name == "Fp8Linear" else mx_qlinear.LayerNorm(256)
+    module.requires_grad_(requires_grad)
+    args = {"x": torch.zeros(4, 256), "weight": module.weight, "bias": module.bias}
+    with forward_ad.dual_level():
+        args[dual] = forward_ad.make_dual(args[dual].detach(), torch.ones_like(args[dual]))
+        with pytest.raises(RuntimeError, match="forward mode"):
+            torch.func.functional_call(module, {k: args[k] for k in ("weight", "bias")}, args["x"])
+    params = {"weight": module.weight, "bias": module.bias}
+    args["x"] = torch.zeros(4, 256)
+    start = {**args, **params}[dual].detach().clone()
+    with pytest.raises(RuntimeError, match="forward mode"):
+        torch.func.jvp(lambda t: torch.func.functional_call(module, {**params, dual: t} if dual != "x" else params, t if dual == "x" else args["x"]),
+                       (start,), (torch.ones_like(start),))

@@ -18,6 +18,7 @@ import threading
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _OUT_CODES, _bias, _launch, _out_code, _ptr, _raw_stream, _require_gpu, _rows, _vector
@@ -456,6 +457,15 @@ def _refuse_capture(device: torch.device) -> None:
                            "layer_norm and layer_norm_backward instead")
 
 
+def _refuse_tangents(*tensors: torch.Tensor | None) -> None:
+    """Forward-mode tangents, which the kernels do not carry on (a tensor that has one need not require a gradient)."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # (no level is open: 2 us less of a call's 10)
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("the autograd modules have no forward mode: their inputs and parameters take no tangents")
+
+
 class _Fp8LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, prepared):
@@ -667,6 +677,7 @@ class Fp8Linear(torch.nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dim() < 1 or x.shape[-1] != self.in_features:
             raise ValueError(f"input of shape {tuple(x.shape)} for a layer of {self.in_features} input features")
+        _refuse_tangents(x, self.weight, self.bias)
         params = [p for p in (self.weight, self.bias) if p is not None]
         if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, *params))):
             return fp8_linear(x, self._form(), self.bias)
@@ -716,6 +727,7 @@ class LayerNorm(torch.nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dim() < 1 or x.shape[-1] != self.features:
             raise ValueError(f"input of shape {tuple(x.shape)} for a norm of {self.features} features")
+        _refuse_tangents(x, self.weight, self.bias)
         params = [p for p in (self.weight, self.bias) if p is not None]
         if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, *params))):
             return layer_norm(x, self.weight, self.bias, self.eps)

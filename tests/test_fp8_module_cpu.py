@@ -300,3 +300,17 @@ def test_forward_mode_is_refused(host, name, dual, requires_grad):
     with pytest.raises(RuntimeError, match="forward mode"):
         torch.func.jvp(lambda t: torch.func.functional_call(module, {**params, dual: t} if dual != "x" else params, t if dual == "x" else args["x"]),
                        (start,), (torch.ones_like(start),))
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("name", ["Fp8Linear", "LayerNorm"])
+def test_host_tensors_are_refused_by_name(name, requires_grad):
+    import mx_qlinear
+
+    module = mx_qlinear.Fp8Linear(256, 96) if name == "Fp8Linear" else mx_qlinear.LayerNorm(256)
+    module.requires_grad_(requires_grad)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        module(torch.zeros(4, 256))
+    if name == "Fp8Linear":
+        with pytest.raises(RuntimeError, match="GPU only"):
+            module.prepare()

@@ -337,3 +337,17 @@ def test_weight_from_codes_of_any_layout(dev, n, k):
                 assert torch.equal(p.scale_t.cpu().view(torch.uint8)[:, :nb], scales.t())
             else:
                 assert p.qt is None and p.scale_t is None
+
+
+def test_restoring_more_than_one_launch_counts(dev):
+    """2^31 pieces of 16 bytes and some: what can be put away can be taken out."""
+    mx = _mx()
+    m = 2**26 + 3
+    q = torch.zeros(m, 128, dtype=torch.uint8, device=dev)
+    s = torch.full((m, 1), 127, dtype=torch.uint8, device=dev)
+    at = torch.tensor([0, 1, 2**25, 2**26 - 2050, 2**26 - 2049, 2**26 - 2048, 2**26 - 1, 2**26, m - 1], device=dev)
+    q[at, 7] = 0x40  # 2
+    s[at, 0] = 130
+    out = mx.dequantize_fp8_block128(q.view(torch.float8_e4m3fn), s.view(torch.float8_e8m0fnu), torch.float32)
+    assert bool((out[at, 7] == 16).all())
+    assert sum(int(torch.count_nonzero(part)) for part in out.split(2**24)) == at.numel()

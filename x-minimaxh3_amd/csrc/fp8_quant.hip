@@ -316,12 +316,17 @@ extern "C" int mxq_fp8_dequantize_rows(const uint8_t* q, int64_t ldq, const uint
   if (!q || !scale || !out) return mxq_set_error(MXQ_ERR_INVALID, "null pointer");
   const int codes = 16 / dtype_bytes(out_dtype);
   const int64_t pieces = (K + codes - 1) / codes;
-  if (M >= (1ll << 31) / pieces - 65536 / pieces - 1) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^31 pieces");
-  const unsigned grid = (unsigned)((M * pieces + 256 * kDequantUnroll - 1) / (256 * kDequantUnroll));
-  with_dtype(out_dtype, [&](auto C) {
-    hipLaunchKernelGGL((fp8_rows_dequant_kernel<decltype(C)::value>), dim3(grid), dim3(256), 0, (hipStream_t)stream, q, ldq,
-                       scale, lds, (char*)out, (uint32_t)M, (uint32_t)K, (uint32_t)pieces);
-  });
+  // (pieces are counted in 32 bits, so more of them are several launches)
+  const int64_t most = (1ll << 31) / pieces - 65536 / pieces - 1;
+  for (int64_t row = 0; row < M; row += most) {
+    const int64_t rows = M - row < most ? M - row : most;
+    const unsigned grid = (unsigned)((rows * pieces + 256 * kDequantUnroll - 1) / (256 * kDequantUnroll));
+    with_dtype(out_dtype, [&](auto C) {
+      hipLaunchKernelGGL((fp8_rows_dequant_kernel<decltype(C)::value>), dim3(grid), dim3(256), 0, (hipStream_t)stream,
+                         q + row * ldq, ldq, scale + row * lds, lds, (char*)out + row * K * dtype_bytes(out_dtype), (uint32_t)rows,
+                         (uint32_t)K, (uint32_t)pieces);
+    });
+  }
   return mxq_check_launch("fp8_rows_dequant_kernel");
 }
 

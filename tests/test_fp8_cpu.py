@@ -205,3 +205,25 @@ def test_c_gradient_entries_refuse_before_any_launch():
         _call("mxq_fp8_prepare_tiles", ok, 300, ok, 2, ok, 384, ok, 4, None, 0, None, 0, 100, 300)
     with pytest.raises(ValueError, match="strides"):
         _call("mxq_pad_rows", ok, 100, 100, ok, 104, 4)
+
+
+def test_whole_passes_refuse_before_their_first_launch():
+    """Strides and pointers that only a later step of the pass reads (a launch would fail here with another error)."""
+    ok, room = 1 << 20, 1 << 34
+
+    def forward(ldb=256, sb=ok, ldsb=4, d=ok, ldd=128, b=ok, bias=None, out=2):
+        _call("mxq_fp8_linear", ok, 2, 256, b, ldb, sb, ldsb, bias, d, ldd, out, 100, 128, 256, ok, room)
+
+    for bad in ({"ldb": 128}, {"ldb": 264}, {"sb": None}, {"sb": ok + 1}, {"ldsb": 2}, {"d": None}, {"ldd": 100}, {"b": ok + 4}, {"out": 9}):
+        with pytest.raises(ValueError):
+            forward(**bad)
+
+    def backward(q=ok, ldq=256, scale=ok, lds=2, readable=1, bt=ok, ldbt=128, sbt=ok, ldsbt=4, dy=ok, ldy=128, direct=0, m=100):
+        _call("mxq_fp8_linear_backward", dy, 2, ldy, direct, q, ldq, scale, lds, readable, bt, ldbt, sbt, ldsbt, ok, ok, ok, 0, m, 128,
+              256, ok, room)
+
+    for bad in ({"q": None}, {"q": ok + 8}, {"ldq": 128}, {"ldq": 264}, {"ldq": 1 << 24}, {"scale": None}, {"lds": 1}, {"bt": None},
+                {"bt": ok + 8}, {"ldbt": 64}, {"sbt": None}, {"ldsbt": 1}, {"sbt": ok + 2}, {"readable": 0, "ldq": 128},
+                {"readable": 0, "q": None}, {"dy": None}, {"ldy": 127}, {"direct": 1, "ldy": 1 << 24}):
+        with pytest.raises(ValueError):
+            backward(**bad)

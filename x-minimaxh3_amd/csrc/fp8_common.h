@@ -65,6 +65,12 @@ int fp8_wgrad(const void* dy, int parts, int64_t ldy, const uint8_t* q, int64_t 
               int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, SliceJob* later,
               void* stream);
 
+// Their refusals other than the workspace's, for passes that launch other steps ahead of them.
+int fp8_gemm_check(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa, const uint8_t* b, int64_t ldb, const uint8_t* sb,
+                   int64_t ldsb, const void* d, int64_t ldd, int out_dtype, int64_t M, int64_t N, int64_t K);
+int fp8_wgrad_check(const void* dy, int parts, int64_t ldy, const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds,
+                    const void* dw, int out_dtype, int64_t M, int64_t N, int64_t K);
+
 constexpr int kFp8MinByte = 10;  // 2^-117
 
 // The scale byte of a block from the bits of its (finite) absmax: 448 = 1.75 * 2^8, so a significand above 1.75

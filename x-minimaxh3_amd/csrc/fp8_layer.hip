@@ -115,6 +115,8 @@ extern "C" int mxq_fp8_linear(const void* x, int x_dtype, int64_t ldx, const uin
   if (const int rc = forward_space((uint8_t*)workspace, M, N, K, f)) return rc;
   if (!workspace || workspace_bytes < f.total || reinterpret_cast<uintptr_t>(workspace) % 16)
     return mxq_set_error(MXQ_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)f.total);
+  // (every refusal is ahead of the first launch)
+  if (const int rc = fp8_gemm_check(f.x.q, f.x.ldq, f.x.s, f.x.lds, b, ldb, sb, ldsb, d, ldd, out_dtype, M, N, K)) return rc;
   if (const int rc = mxq_fp8_quantize_rows(x, x_dtype, ldx, f.x.q, f.x.ldq, f.x.s, f.x.lds, M, K, stream)) return rc;
   return mxq_fp8_gemm(f.x.q, f.x.ldq, f.x.s, f.x.lds, b, ldb, sb, ldsb, bias, d, ldd, out_dtype, M, N, K, f.gemm, f.gemm_bytes, stream);
 }
@@ -143,6 +145,20 @@ extern "C" int mxq_fp8_linear_backward(const void* dy, int dy_dtype, int64_t ldy
   if (const int rc = backward_space((uint8_t*)workspace, M, N, K, dy_dtype, direct, readable, needs, s)) return rc;
   if (s.total > 0 && (!workspace || workspace_bytes < s.total || reinterpret_cast<uintptr_t>(workspace) % 16))
     return mxq_set_error(MXQ_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)s.total);
+  // What the last step reads of the input: its own rows, or copies of them. (Every refusal is ahead of the first launch.)
+  const void* wy = s.n_parts ? s.parts : dy;
+  const int64_t ldwy = s.n_parts || M == 0 ? s.ldp : ldy;
+  const bool copied = M > 0 && !readable;
+  const uint8_t* wq = copied ? s.x.q : q;
+  const int64_t ldwq = M == 0 ? up(K, 16) : copied ? s.x.ldq : ldq, ldws = M == 0 ? up(K, 128) / 128 : lds;
+  if (M > 0 && (!dy || ldy < N)) return mxq_set_error(MXQ_ERR_INVALID, "null gradient or bad row stride %lld", (long long)ldy);
+  if (dx && M > 0) {
+    if (const int rc = fp8_gemm_check(s.dy.q, s.dy.ldq, s.dy.s, s.dy.lds, bt, ldbt, sbt, ldsbt, dx, K, dy_dtype, M, K, N)) return rc;
+  }
+  if (dw) {
+    if (copied && (!q || ldq < K)) return mxq_set_error(MXQ_ERR_INVALID, "null codes or bad row stride %lld", (long long)ldq);
+    if (const int rc = fp8_wgrad_check(wy, s.n_parts ? s.n_parts : 1, ldwy, wq, ldwq, scale, ldws, dw, grad_dtype, M, N, K)) return rc;
+  }
   if (M > 0 && (dx || db || s.n_parts)) {
     if (const int rc = mxq_fp8_grad_pass(dy, dy_dtype, ldy, dx ? s.dy.q : nullptr, s.dy.ldq, s.dy.s, s.dy.lds,
                                          s.n_parts ? s.parts : nullptr, s.n_parts, s.ldp, db ? s.sums : nullptr, s.strips, M, N,
@@ -156,14 +172,11 @@ extern "C" int mxq_fp8_linear_backward(const void* dy, int dy_dtype, int64_t ldy
       return rc;
   }
   if (dw) {
-    if (M > 0 && !readable) {
+    if (copied) {
       if (const int rc = mxq_pad_rows(q, ldq, K, s.x.q, s.x.ldq, M, stream)) return rc;
-      q = s.x.q;
-      ldq = s.x.ldq;
     }
-    const void* y = s.n_parts ? s.parts : dy;
-    if (const int rc = fp8_wgrad(y, s.n_parts ? s.n_parts : 1, s.n_parts || M == 0 ? s.ldp : ldy, q, M == 0 ? up(K, 16) : ldq, scale,
-                                     M == 0 ? up(K, 128) / 128 : lds, dw, grad_dtype, M, N, K, s.wgrad, s.wgrad_bytes, &join_w, stream))
+    if (const int rc = fp8_wgrad(wy, s.n_parts ? s.n_parts : 1, ldwy, wq, ldwq, scale, ldws, dw, grad_dtype, M, N, K, s.wgrad,
+                                 s.wgrad_bytes, &join_w, stream))
       return rc;
   }
   return fp8_join(join_x, join_w, {s.sums, db, s.strips, N, grad_dtype}, stream);

@@ -280,9 +280,8 @@ extern "C" int mxq_fp8_wgrad_workspace(int64_t M, int64_t N, int64_t K, int part
   return MXQ_OK;
 }
 
-int mxq::fp8_wgrad(const void* dy, int parts, int64_t ldy, const uint8_t* q, int64_t ldq, const uint8_t* scale,
-                             int64_t lds, void* dw, int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
-                             int64_t workspace_bytes, SliceJob* later, void* stream) {
+int mxq::fp8_wgrad_check(const void* dy, int parts, int64_t ldy, const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds,
+                         const void* dw, int out_dtype, int64_t M, int64_t N, int64_t K) {
   if (!float_dtype(out_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported output dtype code %d", out_dtype);
   if (M < 0 || N < 1 || K < 1 || parts < 1 || parts > 3 || M > (1ll << 31) - 1024 || N > (1 << 30) || K > (1 << 30))
     return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld N=%lld K=%lld parts=%d", (long long)M, (long long)N, (long long)K, parts);
@@ -294,9 +293,17 @@ int mxq::fp8_wgrad(const void* dy, int parts, int64_t ldy, const uint8_t* q, int
                          (long long)ldq, (long long)lds, (long long)N, (long long)K);
   if (!dw || (M && (!dy || !q || !scale || !wg_aligned(dy, 16) || !wg_aligned(q, 16))))
     return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
+  if ((N + kWTile - 1) / kWTile * ((K + kWTile - 1) / kWTile) >= (1ll << 23))  // (so many tiles are not split)
+    return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^23 tiles");
+  return MXQ_OK;
+}
+
+int mxq::fp8_wgrad(const void* dy, int parts, int64_t ldy, const uint8_t* q, int64_t ldq, const uint8_t* scale,
+                             int64_t lds, void* dw, int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
+                             int64_t workspace_bytes, SliceJob* later, void* stream) {
+  if (const int rc = fp8_wgrad_check(dy, parts, ldy, q, ldq, scale, lds, dw, out_dtype, M, N, K)) return rc;
   const WgradPlan plan = plan_wgrad(M, N, K, parts, mxq_cu_count());
   const int64_t tiles_n = (N + kWTile - 1) / kWTile, tiles_k = (K + kWTile - 1) / kWTile;
-  if (tiles_n * tiles_k * plan.splits >= (1ll << 23)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^23 tiles");
   const int64_t need = wgrad_bytes(plan, N, K);
   if (need > 0 && (!workspace || workspace_bytes < need || !wg_aligned(workspace, 16)))
     return mxq_set_error(MXQ_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);

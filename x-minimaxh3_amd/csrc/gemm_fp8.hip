@@ -702,9 +702,12 @@ extern "C" int mxq_fp8_gemm_workspace(int64_t M, int64_t N, int64_t K, int64_t* 
   return MXQ_OK;
 }
 
-int mxq::fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa, const uint8_t* b, int64_t ldb,
-                            const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd, int out_dtype,
-                            int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, SliceJob* later, void* stream) {
+static int64_t tiles_of(const Fp8Plan& plan, int64_t M, int64_t N) {
+  return (M + plan.tile - 1) / plan.tile * ((N + kTileN - 1) / kTileN) * plan.splits;
+}
+
+int mxq::fp8_gemm_check(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa, const uint8_t* b, int64_t ldb,
+                        const uint8_t* sb, int64_t ldsb, const void* d, int64_t ldd, int out_dtype, int64_t M, int64_t N, int64_t K) {
   if (const int rc = check_product(M, N, K, ldb, ldsb, ldd, out_dtype)) return rc;
   const int64_t kb = (K + 127) / 128;
   if (lda < kb * 128 || lda % 16 || lda > (1ll << 22) + 4096 || ldsa < (kb + 3) / 4 * 4 || ldsa % 4 || ldsa > (1ll << 20))
@@ -712,11 +715,22 @@ int mxq::fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa
   if (M == 0) return MXQ_OK;
   if (!a || !sa || !b || !sb || !d || !aligned(a, 16) || !aligned(b, 16) || !aligned(sa, 4) || !aligned(sb, 4))
     return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
+  // (so many tiles are not split; the plan is asked for only where they may be too many)
+  if (tiles_of({128, 1}, M, N) >= (1ll << 23) && tiles_of(plan_fp8(M, N, kb, mxq_cu_count()), M, N) >= (1ll << 23))
+    return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^23 tiles");
+  return MXQ_OK;
+}
+
+int mxq::fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa, const uint8_t* b, int64_t ldb,
+                            const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd, int out_dtype,
+                            int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, SliceJob* later, void* stream) {
+  if (const int rc = fp8_gemm_check(a, lda, sa, ldsa, b, ldb, sb, ldsb, d, ldd, out_dtype, M, N, K)) return rc;
+  if (M == 0) return MXQ_OK;
+  const int64_t kb = (K + 127) / 128;
   if (fp8_rows_pays(M, N, K))
     return fp8_linear_rows(a, MXQ_DTYPE_E4M3, lda, sa, ldsa, b, ldb, sb, ldsb, bias, d, ldd, out_dtype, M, N, K, stream);
   const Fp8Plan plan = plan_fp8(M, N, kb, mxq_cu_count());
   const int64_t tiles_m = (M + plan.tile - 1) / plan.tile, tiles_n = (N + kTileN - 1) / kTileN;
-  if (tiles_m * tiles_n * plan.splits >= (1ll << 23)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^23 tiles");
   const int64_t need = split_bytes(plan, M, N);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return mxq_set_error(MXQ_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);

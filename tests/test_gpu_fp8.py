@@ -351,3 +351,111 @@ def test_restoring_more_than_one_launch_counts(dev):
     out = mx.dequantize_fp8_block128(q.view(torch.float8_e4m3fn), s.view(torch.float8_e8m0fnu), torch.float32)
     assert bool((out[at, 7] == 16).all())
     assert sum(int(torch.count_nonzero(part)) for part in out.split(2**24)) == at.numel()
+
+
+# ---------------------------------------------------------------------------------------
+# the scaled matrix instruction: 16-bit results of more than 16 rows
+# ---------------------------------------------------------------------------------------
+# Its cuts: 64 addends, each by at most 2^-13 of the largest. Where their signs are independent, an element's error has at
+# most the variance 64 (2^-13 max|p|)^2 per 64 columns, and the last rounding, uniform within half a step u, u^2 / 3 y^2.
+
+HALVES = [torch.bfloat16, torch.float16]
+
+
+def _cut_variance(xv, wv):
+    """Sum over 64-long pieces of 64 (2^-13 max|x w|)^2, [M, N]."""
+    out = torch.zeros(xv.shape[0], wv.shape[0], dtype=torch.float64)
+    for k in range(0, xv.shape[1], 64):
+        p = (xv[:, None, k : k + 64].abs() * wv[None, :, k : k + 64].abs()).amax(-1)
+        out += 64 * (2.0**-13 * p) ** 2
+    return out
+
+
+def _check_norm_of_cuts(y, xv, wv):
+    ref = xv @ wv.t()
+    u = _half_step(y.dtype)
+    err = float((y.double().cpu() - ref).square().sum())
+    assert err <= float(u * u / 3 * ref.square().sum() + _cut_variance(xv, wv).sum()) * (1 + 2.0**-6)
+
+
+@pytest.mark.parametrize("out", HALVES)
+@pytest.mark.parametrize("m", [40, 100, 300])
+def test_each_block_has_its_own_scale(dev, out, m):
+    """Rows of one block that is not zero, at far exponents of the row's and the tile's own: the result is that block's product
+    alone, so a scale taken from another stage, row or tile shows whole."""
+    mx = _mx()
+    n, kb = 300, 11
+    g = _gen(m)
+    x = torch.randn(m, kb, 128, generator=g)
+    e = torch.randint(-50, 51, (m, kb), generator=g)
+    f = torch.randint(-50, 51, (-(-n // 128), kb), generator=g)
+    keep = torch.arange(m)[:, None] % kb == torch.arange(kb)
+    # (the tile's exponent is undone by the row's, but for up to 2^5: results stay in float16's range)
+    x = torch.ldexp(x, e[..., None]) * keep[..., None]
+    w = torch.ldexp(torch.randn(n, kb, 128, generator=g), f.repeat_interleave(128, 0)[:n][..., None])
+    for tile in range(f.shape[0]):  # one column tile at a time: its exponents undone
+        rows = slice(tile * 128, min(n, tile * 128 + 128))
+        scale = torch.ldexp(torch.ones(()), (-(e + f[tile]) - 4 + (torch.arange(m)[:, None] % 6))[..., None])
+        xt = (x * scale).view(m, -1)
+        y = mx.fp8_linear(xt.to(dev), mx.prepare_fp8_weight(w.view(n, -1).to(dev)), out_dtype=out).cpu()
+        xv, wv = ob.rows(xt)[0], ob.tiles(w.view(n, -1))[0][rows]
+        check_product(y[:, rows], xv, wv, None, False)
+        _check_norm_of_cuts(y[:, rows], xv, wv)
+
+
+@pytest.mark.parametrize("out", HALVES)
+def test_every_code_and_scale_byte_of_the_scaled_instruction(dev, out):
+    """All codes under all scale bytes (255: NaN) of an activation, and of a weight, times one."""
+    mx = _mx()
+    q = torch.arange(256, dtype=torch.uint8).repeat(256, 1)
+    q[:, [127, 255]] = 0
+    s = torch.arange(256, dtype=torch.uint8)[:, None].repeat(1, 2)
+    byte = torch.arange(256)
+    ref = ob.e4m3_table()[q.long()] * torch.ldexp(torch.ones((), dtype=torch.float64), byte - 127)[:, None]
+    ref[255] = float("nan")
+    fair = ((byte >= 10) & (byte < 247)) | (byte == 255)  # (the scales that the quantizers give of finite values in range)
+    p = mx.prepare_fp8_weight(torch.eye(256).to(dev))
+    y = mx.fp8_linear_prequantized(q.view(torch.float8_e4m3fn).to(dev), s.view(torch.float8_e8m0fnu).to(dev), p, out_dtype=out)
+    assert _same(y.cpu().double()[fair], ref.to(out).double()[fair])
+    # a weight of three tiles of equal rows, each under its byte: row j of the identity picks code j
+    xq, xs = mx.quantize_fp8_block128(torch.eye(128).to(dev))
+    codes = torch.arange(128, dtype=torch.uint8)
+    codes[127] = 0
+    for first in range(10, 241, 33):
+        b = torch.tensor([first, 255, first + 6], dtype=torch.uint8)
+        w = mx.prepare_fp8_weight(codes.repeat(384, 1).view(torch.float8_e4m3fn).to(dev), b[:, None].view(torch.float8_e8m0fnu).to(dev))
+        y = mx.fp8_linear_prequantized(xq, xs, w, out_dtype=out).cpu().double()
+        for t in range(3):
+            v = ob.e4m3_table()[codes.long()] * (float("nan") if t == 1 else 2.0 ** (int(b[t]) - 127))
+            assert _same(y[:, t * 128 : t * 128 + 128], v.to(out).double()[:, None].expand(128, 128))
+
+
+@pytest.mark.parametrize("out", HALVES)
+@pytest.mark.parametrize("m,n,k", [(40, 96, 1152), (130, 200, 2000)])
+def test_outlier_channels(dev, out, m, n, k):
+    """One channel in 200 twenty times larger, as transformers' activations have them."""
+    mx = _mx()
+    g = _gen(k)
+    x = torch.randn(m, k, generator=g)
+    x[:, torch.randperm(k, generator=g)[: k // 200]] *= 20
+    w = torch.randn(n, k, generator=g) * 0.02
+    y = mx.fp8_linear(x.to(out).to(dev), mx.prepare_fp8_weight(w.to(dev)))
+    xv, wv = ob.rows(x.to(out))[0], ob.tiles(w)[0]
+    check_product(y, xv, wv, None, False)
+    _check_norm_of_cuts(y, xv, wv)
+
+
+@pytest.mark.parametrize("out", DTYPES)
+@pytest.mark.parametrize("m", [3, 100, 300])
+def test_small_addends_of_one_sign(dev, out, m):
+    """The worst case of the scaled instruction's cuts: beside one product, 63 of its own sign just below 2^-13 of it. Up to
+    16 rows and float32 results have them; 16-bit results of more rows are within 64 cuts of 2^-13 of the largest."""
+    mx = _mx()
+    x = torch.full((m, 640), 1.875 * 2.0**-6)
+    x[:, ::64] = 256.0
+    w = torch.ones(130, 640)
+    wide = m <= 16 or out == torch.float32
+    y = mx.fp8_linear(x.to(out).to(dev), mx.prepare_fp8_weight(w.to(dev)), out_dtype=out)
+    xv, wv = ob.rows(x)[0], ob.tiles(w)[0]
+    assert torch.equal(xv, x.double())
+    check_product(y, xv, wv, None, wide)

@@ -521,9 +521,12 @@ int mxq_fp8_gemm_workspace(int64_t M, int64_t N, int64_t K, int64_t* bytes);
 /*
  * d [M, N] = out(a b^T + bias): a codes [M, lda] with scales [M, ldsa] (1 x 128), b codes [N, ldb] with scales
  * [ceil(N / 128), ldsb] (128 x 128), both zero behind column K; bias [N] of out_dtype or NULL. Sums are float32.
- * bf16 and fp16 outputs use the e4m3 matrix instructions, which cut addends below 2^-13 of the largest of 64;
- * fp32 outputs and up to 16 rows keep every addend.
+ * bf16 and fp16 outputs use the e4m3 matrix instructions, which cut addends below 2^-13 of the largest of 64 (at worst
+ * 64 * 2^-13 of the largest for every 64 products); fp32 outputs and up to 16 rows keep every addend, and so do others
+ * whose out_dtype has MXQ_FP8_FULL_SUMS added, at half the rate. Of mxq_fp8_linear the same holds, and of
+ * mxq_fp8_linear_backward's dx, whose dy_dtype takes the flag.
  */
+#define MXQ_FP8_FULL_SUMS 256
 int mxq_fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa, const uint8_t* b, int64_t ldb,
                  const uint8_t* sb, int64_t ldsb, const void* bias, void* d, int64_t ldd, int out_dtype, int64_t M,
                  int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);

@@ -459,3 +459,30 @@ def test_small_addends_of_one_sign(dev, out, m):
     xv, wv = ob.rows(x)[0], ob.tiles(w)[0]
     assert torch.equal(xv, x.double())
     check_product(y, xv, wv, None, wide)
+
+
+@pytest.mark.parametrize("out", HALVES)
+@pytest.mark.parametrize("m,n,k", [(5, 40, 300), (31, 40, 300), (33, 300, 1000), (200, 256, 384), (333, 515, 2500), (1025, 1300, 1152),
+                                   (4100, 700, 520), (100, 130, 20000)])
+def test_full_sums(dev, out, m, n, k):
+    """16-bit results with every addend: the float32 result rounded, within float32's own bounds."""
+    mx = _mx()
+    x, w, bias = _acts(m, k, out, m + n), _acts(n, k, torch.float32, n * k) * 0.05, _acts(1, n, out, 3)[0]
+    p = mx.prepare_fp8_weight(w.to(dev))
+    y = mx.fp8_linear(x.to(dev), p, bias.to(dev), full_sums=True)
+    assert y.dtype == out
+    check_product(y, ob.rows(x)[0], ob.tiles(w)[0], bias, True)
+    assert torch.equal(y, mx.fp8_linear(x.to(dev), p, bias.to(dev), out_dtype=torch.float32).to(out))
+    q, s = mx.quantize_fp8_block128(x.to(dev))
+    assert torch.equal(mx.fp8_linear_prequantized(q, s, p, bias.to(dev), out, full_sums=True), y)
+
+
+@pytest.mark.parametrize("out", HALVES)
+@pytest.mark.parametrize("m", [100, 300])
+def test_small_addends_of_one_sign_in_full_sums(dev, out, m):
+    mx = _mx()
+    x = torch.full((m, 640), 1.875 * 2.0**-6)
+    x[:, ::64] = 256.0
+    w = torch.ones(130, 640)
+    y = mx.fp8_linear(x.to(out).to(dev), mx.prepare_fp8_weight(w.to(dev)), full_sums=True)
+    check_product(y, x.double(), ob.tiles(w)[0], None, True)

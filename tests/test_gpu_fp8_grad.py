@@ -668,3 +668,26 @@ def test_backward_of_rows_far_apart(dev, far, m):
     got = mx.fp8_linear_backward(args["dy"], args["codes"], args["scale"], p)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert torch.equal(mx.fp8_linear_prequantized(args["codes"], args["scale"], p), mx.fp8_linear_prequantized(q, s, p))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", [(7, 64, 200), (33, 130, 100), (600, 96, 1000), (2100, 520, 300)])
+def test_full_sums_of_the_inputs_gradient(dev, dtype, m, n, k):
+    """dx with every addend; the other gradients are the same bits; and the module passes it on both ways."""
+    mx = _mx()
+    x, w, dy = _acts(m, k, dtype, 1), _acts(n, k, torch.float32, 2) * 0.05, _acts(m, n, dtype, 3) * 0.01
+    p = mx.prepare_fp8_weight(w.to(dev))
+    q, s = mx.quantize_fp8_block128(x.to(dev))
+    dx, dw, db = mx.fp8_linear_backward(dy.to(dev), q, s, p, full_sums=True)
+    check_product(dx, ob.rows(dy)[0], ob.tiles(w)[0].t(), None, True)
+    plain = mx.fp8_linear_backward(dy.to(dev), q, s, p)
+    assert torch.equal(dw, plain[1]) and torch.equal(db, plain[2])
+    layer = mx.Fp8Linear(k, n, bias=False, device=dev, dtype=dtype, full_sums=True)
+    with torch.no_grad():
+        layer.weight.copy_(w)
+    xg = x.to(dev).requires_grad_()
+    y = layer(xg)
+    y.backward(dy.to(dev))
+    p = mx.prepare_fp8_weight(layer.weight)
+    assert torch.equal(y, mx.fp8_linear(x.to(dev), p, full_sums=True)) and torch.equal(layer(x.to(dev)), y)
+    assert torch.equal(xg.grad, mx.fp8_linear_backward(dy.to(dev), q, s, p, (True, False, False), full_sums=True)[0])

@@ -134,6 +134,8 @@ extern "C" int mxq_fp8_linear_backward(const void* dy, int dy_dtype, int64_t ldy
                                        const uint8_t* scale, int64_t lds, int readable, const uint8_t* bt, int64_t ldbt,
                                        const uint8_t* sbt, int64_t ldsbt, void* dx, void* dw, void* db, int grad_dtype, int64_t M,
                                        int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int dx_dtype = dy_dtype;  // (with MXQ_FP8_FULL_SUMS or without)
+  dy_dtype &= ~MXQ_FP8_FULL_SUMS;
   if (!sizes_ok(M, N, K))
     return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
   if (!float_dtype(dy_dtype) || !float_dtype(grad_dtype))
@@ -153,7 +155,7 @@ extern "C" int mxq_fp8_linear_backward(const void* dy, int dy_dtype, int64_t ldy
   const int64_t ldwq = M == 0 ? up(K, 16) : copied ? s.x.ldq : ldq, ldws = M == 0 ? up(K, 128) / 128 : lds;
   if (M > 0 && (!dy || ldy < N)) return mxq_set_error(MXQ_ERR_INVALID, "null gradient or bad row stride %lld", (long long)ldy);
   if (dx && M > 0) {
-    if (const int rc = fp8_gemm_check(s.dy.q, s.dy.ldq, s.dy.s, s.dy.lds, bt, ldbt, sbt, ldsbt, dx, K, dy_dtype, M, K, N)) return rc;
+    if (const int rc = fp8_gemm_check(s.dy.q, s.dy.ldq, s.dy.s, s.dy.lds, bt, ldbt, sbt, ldsbt, dx, K, dx_dtype, M, K, N)) return rc;
   }
   if (dw) {
     if (copied && (!q || ldq < K)) return mxq_set_error(MXQ_ERR_INVALID, "null codes or bad row stride %lld", (long long)ldq);
@@ -167,7 +169,7 @@ extern "C" int mxq_fp8_linear_backward(const void* dy, int dy_dtype, int64_t ldy
   }
   SliceJob join_x = {}, join_w = {};
   if (dx && M > 0) {
-    if (const int rc = fp8_gemm(s.dy.q, s.dy.ldq, s.dy.s, s.dy.lds, bt, ldbt, sbt, ldsbt, nullptr, dx, K, dy_dtype, M, K, N, s.gemm,
+    if (const int rc = fp8_gemm(s.dy.q, s.dy.ldq, s.dy.s, s.dy.lds, bt, ldbt, sbt, ldsbt, nullptr, dx, K, dx_dtype, M, K, N, s.gemm,
                                 s.gemm_bytes, &join_x, stream))
       return rc;
   }

@@ -12,11 +12,13 @@
 // f8f6f4 applies the scales itself: each lane gives one byte for its row, so a block's scale costs the loop nothing but
 // four words per four stages and wave (a byte per stage, shifted out of a word).
 //
-// Precision of that instruction, measured: within one 64-long product sum, addends below 2^-13 of the largest are
-// cut, and the sum is added to a float32. On the layers' data that is 5e-5 to 2e-4 of the result's root mean square,
-// below bfloat16's and float16's own rounding (1.7e-3, 2.1e-4). For float32 results (kWide) the fragments are
-// converted to bfloat16 with their scales, exactly, and the sums run on v_mfma_f32_32x32x16_bf16, which keeps every
-// addend to float32's precision at half the rate.
+// Precision of that instruction, measured: within one 64-long product sum, addends are cut below 2^-13 of the largest,
+// and the sum is added to a float32. How much that is depends on the data: on the layers' own 5e-5 to 2e-4 of the result's
+// root mean square, beside bfloat16's and float16's rounding of 1.7e-3 and 2.1e-4; at worst, one product beside 63 of its
+// own sign just under 2^-13 of it, 63 * 2^-13 (0.8 %) of the result. 16-bit results take it for its rate. For float32
+// results, and 16-bit ones that are asked for with full sums (kWide), the fragments are converted to bfloat16 with their
+// scales, exactly, and the sums run on v_mfma_f32_32x32x16_bf16, which keeps every addend to float32's precision at half
+// the rate.
 //
 // 75600 x 5120 of K 5120 takes 1.57 to 1.63 ms (2.5 PFLOP/s; 2.67 in the loop, from K 5120 against 10240 at 16384 x 4096):
 // the clock falls to about 1.85 GHz, power bounds it (a library's product 2.81).
@@ -684,7 +686,11 @@ static int64_t split_bytes(const Fp8Plan& plan, int64_t M, int64_t N) {
   return plan.splits > 1 ? plan.splits * M * ((N + 3) / 4 * 4) * 4 : 0;
 }
 
+// (out_dtype may carry MXQ_FP8_FULL_SUMS in what follows)
+static int out_code(int out_dtype) { return out_dtype & ~MXQ_FP8_FULL_SUMS; }
+
 static int check_product(int64_t M, int64_t N, int64_t K, int64_t ldb, int64_t ldsb, int64_t ldd, int out_dtype) {
+  out_dtype = out_code(out_dtype);
   if (!float_dtype(out_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported output dtype code %d", out_dtype);
   if (M < 0 || N < 1 || K < 1 || M > (1ll << 31) - 1024 || N > (1ll << 27) || K > (1ll << 22))
     return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
@@ -736,7 +742,8 @@ int mxq::fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa
     return mxq_set_error(MXQ_ERR_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   Fp8Gemm p = {a, b, sa, sb, bias, d, M, N, lda, ldb, ldsa, ldsb, ldd, (int)kb, (int)tiles_m, (int)tiles_n, plan.splits,
                plan.split_kb, 0};
-  const bool wide = out_dtype == MXQ_DTYPE_F32;
+  const bool wide = out_dtype == MXQ_DTYPE_F32 || (out_dtype & MXQ_FP8_FULL_SUMS);
+  out_dtype = out_code(out_dtype);
   if (plan.splits > 1) {
     const int64_t ldp = (N + 3) / 4 * 4;
     p.d = workspace;
@@ -757,8 +764,10 @@ int mxq::fp8_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa
   p.vec = aligned(d, 16) && ldd * dtype_bytes(out_dtype) % 16 == 0;
   return with_dtype(out_dtype, [&](auto O) {
     constexpr int kOut = decltype(O)::value;
-    constexpr bool kWide = kOut == MXQ_DTYPE_F32;
-    return plan.tile == 256 ? launch_gemm<256, kOut, false, kWide>(p, stream) : launch_gemm<128, kOut, false, kWide>(p, stream);
+    if constexpr (kOut != MXQ_DTYPE_F32) {
+      if (!wide) return plan.tile == 256 ? launch_gemm<256, kOut, false, false>(p, stream) : launch_gemm<128, kOut, false, false>(p, stream);
+    }
+    return plan.tile == 256 ? launch_gemm<256, kOut, false, true>(p, stream) : launch_gemm<128, kOut, false, true>(p, stream);
   });
 }
 
@@ -808,7 +817,7 @@ int mxq::fp8_linear_rows(const void* x, int x_dtype, int64_t ldx, const uint8_t*
     return mxq_set_error(MXQ_ERR_INVALID, "bad row strides of the activations for K=%lld", (long long)K);
   if (!x || !b || !sb || !d || !aligned(b, 16)) return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
   const Fp8Rows p = {x, sx, b, sb, bias, d, M, N, K, ldx, ldsx, ldb, ldsb, ldd, (int)kb, 0, x_dtype};
-  with_dtype(out_dtype, [&](auto O) {
+  with_dtype(out_code(out_dtype), [&](auto O) {
     constexpr int kOut = decltype(O)::value;
     if (fused)
       launch_rows<kOut, 1, true>(p, stream);

@@ -19,6 +19,7 @@ MXQ_ERR_UNSUPPORTED = -2
 MXQ_ERR_HIP = -3
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_E4M3 = 0, 1, 2, 5
+FP8_FULL_SUMS = 256
 ABI_VERSION = 5
 # MXQ_GEMM_WORKSPACE_BYTES: the INT8 GEMMs' tile-queue workspace (counters)
 GEMM_WORKSPACE_BYTES = 4096

@@ -137,7 +137,8 @@ def quantize_fp8_block128(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def dequantize_fp8_block128(q: torch.Tensor, scale: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values of a ``(codes, scale)`` pair, rounded once to ``out_dtype`` (exact in bf16 and fp32)."""
+    """The values of a ``(codes, scale)`` pair, rounded once to ``out_dtype`` (exact in bf16 and fp32). A value that its code
+    rounded past the type's largest is an infinity: float16 inputs from 63488 on, bf16 and fp32 from 1.9375 * 2^127 on."""
     code = _out_code(out_dtype)
     dev = _require_gpu(q, scale)
     shape = q.shape
@@ -227,10 +228,15 @@ def _room(need: int, dev) -> torch.Tensor | None:
     return torch.empty(need, dtype=torch.uint8, device=dev) if need else None
 
 
-def _product(dev, a, sa, m: int, k: int, b, sb, n: int, bias, out_dtype) -> torch.Tensor:
+def _sums(full: bool) -> int:
+    """What an output's type code carries for products that keep every addend."""
+    return _lib.FP8_FULL_SUMS if full else 0
+
+
+def _product(dev, a, sa, m: int, k: int, b, sb, n: int, bias, out_dtype, full_sums: bool) -> torch.Tensor:
     """``[m, n]`` of operands in the products' layout."""
     out = torch.empty(m, n, dtype=out_dtype, device=dev)
-    code = _out_code(out_dtype)
+    code = _out_code(out_dtype) | _sums(full_sums)
     if m == 0:
         return out
     need = _workspace("mxq_fp8_gemm_workspace", dev.index, m, n, k)
@@ -248,16 +254,22 @@ def _check_weight(weight: PreparedFp8Weight, k: int) -> None:
 
 
 def fp8_linear(x: torch.Tensor, weight: PreparedFp8Weight, bias: torch.Tensor | None = None,
-               out_dtype: torch.dtype | None = None) -> torch.Tensor:
+               out_dtype: torch.dtype | None = None, full_sums: bool = False) -> torch.Tensor:
     """``x @ weight.T + bias`` with ``x [..., K]`` quantized as :func:`quantize_fp8_block128` does; ``out_dtype`` defaults
-    to ``x``'s. Up to 16 rows are quantized inside the product's launch."""
+    to ``x``'s. Up to 16 rows are quantized inside the product's launch.
+
+    bf16 and fp16 results of more than 16 rows come from an instruction that cuts each of 64 addends below 2^-13 of the
+    largest of them: beside those types' own rounding little on a layer's usual data (5e-5 to 2e-4 of the results' root
+    mean square), at worst 64 * 2^-13 of the largest for every 64. ``full_sums`` keeps every addend to float32's
+    precision, at half the rate; float32 results and up to 16 rows always do.
+    """
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError("fp8_linear needs a non-empty last dimension")
     _check_weight(weight, x.shape[-1])
     xcode = _float_code(x, "input")
     dev = _require_gpu(x, weight.q, bias)
     out_dtype = out_dtype or x.dtype
-    code = _out_code(out_dtype)
+    code = _out_code(out_dtype) | _sums(full_sums)
     n, k = weight.out_features, weight.in_features
     bias = _bias(bias, n, out_dtype, dev)
     x2 = _rows_in_place(x, k)
@@ -273,7 +285,7 @@ def fp8_linear(x: torch.Tensor, weight: PreparedFp8Weight, bias: torch.Tensor | 
 
 
 def fp8_linear_prequantized(q: torch.Tensor, scale: torch.Tensor, weight: PreparedFp8Weight, bias: torch.Tensor | None = None,
-                            out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+                            out_dtype: torch.dtype = torch.bfloat16, full_sums: bool = False) -> torch.Tensor:
     """:func:`fp8_linear` of an input that is a ``(codes, scale)`` pair already."""
     shape = q.shape
     q, scale, m, k = _pair(q, scale)
@@ -284,7 +296,7 @@ def fp8_linear_prequantized(q: torch.Tensor, scale: torch.Tensor, weight: Prepar
     bias = _bias(bias, n, out_dtype, dev)
     if m:
         q, scale = _operand(q, scale, k)
-    out = _product(dev, q, scale, m, k, weight.q, weight.scale, n, bias, out_dtype)
+    out = _product(dev, q, scale, m, k, weight.q, weight.scale, n, bias, out_dtype, full_sums)
     return out if len(shape) == 2 else out.reshape(*shape[:-1], n)
 
 
@@ -301,12 +313,14 @@ def _readable(t: torch.Tensor, width: int) -> bool:
 
 
 def fp8_linear_backward(dy: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, weight: PreparedFp8Weight,
-                        needs: tuple[bool, bool, bool] = (True, True, True), grad_dtype: torch.dtype = torch.float32):
+                        needs: tuple[bool, bool, bool] = (True, True, True), grad_dtype: torch.dtype = torch.float32,
+                        full_sums: bool = False):
     """Gradients ``(dx, dweight, dbias)`` of :func:`fp8_linear` from the output's gradient ``dy [..., N]``, the input as it
     was kept in 8 bits (the pair ``q [..., K]``, ``scale``) and the prepared weight; ``needs`` says which (``None`` for the
     others). The quantizers pass gradients through unchanged.
 
-    ``dx = dY^ W^`` in ``dy``'s dtype, ``dY^`` being ``dy`` quantized as an activation is; ``dweight = dy^T X^`` and
+    ``dx = dY^ W^`` in ``dy``'s dtype, ``dY^`` being ``dy`` quantized as an activation is (``full_sums`` as in
+    :func:`fp8_linear`); ``dweight = dy^T X^`` and
     ``dbias = sum dy`` in ``grad_dtype``, from ``dy`` itself: with float32 sums of exact products where ``dy`` is bf16,
     fp16 or (to 24 bits) fp32, which go through the matrix instructions as one, two or three bfloat16 parts.
     """
@@ -337,7 +351,7 @@ def fp8_linear_backward(dy: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, 
         need = _workspace("mxq_fp8_linear_backward_workspace", dev.index, m, n, k, code, direct, readable, needs)
         ws = _room(need, dev)
         bt, st = weight.qt, weight.scale_t
-        _launch(dev, "mxq_fp8_linear_backward", y.data_ptr(), code, ldy, direct, q.data_ptr(),
+        _launch(dev, "mxq_fp8_linear_backward", y.data_ptr(), code | _sums(full_sums), ldy, direct, q.data_ptr(),
                 q.stride(0) if m > 1 else _ceil(k, 16) if readable else k, scale.data_ptr(),
                 scale.stride(0) if m > 1 else scale.shape[1], readable, _ptr(bt), bt.shape[1] if want_x else 0,
                 _ptr(st), st.shape[1] if want_x else 0, dx.data_ptr() if want_x and m else None,
@@ -468,15 +482,15 @@ def _refuse_tangents(*tensors: torch.Tensor | None) -> None:
 
 class _Fp8LinearFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, prepared):
+    def forward(ctx, x, weight, bias, prepared, full_sums):
         dev = _require_gpu(x, prepared.q, bias)
         _refuse_capture(dev)
         q, s, m, k = _quantize_rows(x)
         n = prepared.out_features
-        y = _product(dev, q, s, m, k, prepared.q, prepared.scale, n, _bias(bias, n, x.dtype, dev), x.dtype)
+        y = _product(dev, q, s, m, k, prepared.q, prepared.scale, n, _bias(bias, n, x.dtype, dev), x.dtype, full_sums)
         # the input leaves the graph in 8 bits: only the pair is kept
         ctx.save_for_backward(q, s, prepared.qt, prepared.scale_t)
-        ctx.sizes = (x.shape, n, k)
+        ctx.sizes, ctx.full_sums = (x.shape, n, k), full_sums
         ctx.dtypes = (None if weight is None else weight.dtype, None if bias is None else bias.dtype)
         return y.reshape(*x.shape[:-1], n)
 
@@ -493,8 +507,9 @@ class _Fp8LinearFn(torch.autograd.Function):
         # of two types, both gradients in float32, each then rounded once to its own
         wanted = {t for t, want in ((wdtype, want_w), (bdtype, want_b)) if want}
         dx, dw, db = fp8_linear_backward(dy.reshape(m, n), q[:, :k], s[:, : -(-k // BLOCK)], weight, (want_x, want_w, want_b),
-                                         wanted.pop() if len(wanted) == 1 else torch.float32)
-        return (dx.reshape(shape) if want_x else None, dw.to(wdtype) if want_w else None, db.to(bdtype) if want_b else None, None)
+                                         wanted.pop() if len(wanted) == 1 else torch.float32, ctx.full_sums)
+        return (dx.reshape(shape) if want_x else None, dw.to(wdtype) if want_w else None, db.to(bdtype) if want_b else None,
+                None, None)
 
 
 def _event(device: torch.device):
@@ -578,12 +593,13 @@ class Fp8Linear(torch.nn.Module):
     or fp32.
 
     Calls without gradients can be captured into a graph. Its replays build the form from the parameter's contents each
-    time, unless :meth:`prepare` was called first: then they read that form.
+    time, unless :meth:`prepare` was called first: then they read that form. ``full_sums`` as in :func:`fp8_linear`, for
+    the layer's results and its input's gradient.
     """
 
-    def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None):
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None, full_sums: bool = False):
         super().__init__()
-        self.in_features, self.out_features = in_features, out_features
+        self.in_features, self.out_features, self.full_sums = in_features, out_features, full_sums
         self.weight = torch.nn.Parameter(torch.empty(out_features, in_features, device=device, dtype=dtype))
         self.bias = torch.nn.Parameter(torch.zeros(out_features, device=device, dtype=dtype)) if bias else None
         torch.nn.init.normal_(self.weight, std=in_features**-0.5)
@@ -598,7 +614,7 @@ class Fp8Linear(torch.nn.Module):
 
     def __setstate__(self, state):
         state = {k: v for k, v in state.items() if k not in ("_prepared", "_prepared_of")}
-        super().__setstate__({"_kept": None, **state})
+        super().__setstate__({"_kept": None, "full_sums": False, **state})
 
     def _state(self):
         """What changes with the parameter's contents: the parameter, its storage and its count of changes in place."""
@@ -680,13 +696,13 @@ class Fp8Linear(torch.nn.Module):
         _refuse_tangents(x, self.weight, self.bias)
         params = [p for p in (self.weight, self.bias) if p is not None]
         if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, *params))):
-            return fp8_linear(x, self._form(), self.bias)
+            return fp8_linear(x, self._form(), self.bias, full_sums=self.full_sums)
         if self.weight.requires_grad:
             self._forget()
             prepared = prepare_fp8_weight(self.weight)
         else:
             prepared = self._form(saved=True)
-        return _Fp8LinearFn.apply(x, self.weight, self.bias, prepared)
+        return _Fp8LinearFn.apply(x, self.weight, self.bias, prepared, self.full_sums)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"

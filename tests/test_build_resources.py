@@ -49,3 +49,20 @@ def test_gemm_kernels_do_not_spill(tmp_path):
     assert len(gemms) > 20
     # (a few registers around the tile loop; the gated residual epilogue once spilled 67 and then 137)
     assert max(gemms.values()) <= 16, sorted(gemms.items(), key=lambda kv: -kv[1])[:5]
+
+
+@pytest.mark.parametrize("kernel", ["gemm_fp8_kernel", "fp8_wgrad_kernel", "fp8_rows_kernel", "layer_norm_kernel"])
+def test_fp8_kernels_do_not_spill(tmp_path, kernel):
+    """The 8-bit layer's products (the 256-row tile once spilled its accumulators) and the norm's forward pass. Not its
+    gradient, whose forms of two and three chunks a lane spill."""
+    from mx_qlinear import _lib
+
+    if not pathlib.Path(READOBJ).exists():
+        pytest.skip("no llvm-readobj")
+    if not _lib.LIB_PATH.exists():
+        from mx_qlinear import build
+
+        build.build()
+    kernels = {k: v for k, v in _kernels(_lib.LIB_PATH, tmp_path).items() if kernel in k}
+    assert len(kernels) >= 4
+    assert max(kernels.values()) == 0, sorted(kernels.items(), key=lambda kv: -kv[1])[:5]

@@ -531,6 +531,11 @@ def _synchronize(device: torch.device) -> None:
     torch.cuda.synchronize(device)
 
 
+def _state(weight: torch.Tensor) -> tuple:
+    """What changes with a parameter's contents: the parameter, its storage and its count of changes in place."""
+    return (weight,), weight.data_ptr(), weight.dtype, weight.device, None if weight.is_inference() else weight._version
+
+
 class _Kept:
     """A weight's 8-bit form that a layer keeps between calls, and what it was built from (``of``; ``None``: of nothing that
     still holds). The call that builds it writes memory that its caller does not see, so the order of the streams that use
@@ -553,8 +558,9 @@ class _Kept:
     def forget(self) -> None:
         self.of, self.asked = None, False
 
-    def holds(self, state: tuple) -> bool:
-        return self.of is not None and self.of[0][0] is state[0][0] and self.of[1:] == state[1:]
+    def holds(self, weight: torch.Tensor) -> bool:
+        """Whether ``weight`` is what the form was built from, by all that is counted of it."""
+        return self.of is not None and self.of[0][0] is weight and self.of[1:] == _state(weight)[1:]
 
     def fits(self, weight: torch.Tensor, transposed: bool) -> bool:
         f = self.form
@@ -616,10 +622,8 @@ class Fp8Linear(torch.nn.Module):
         state = {k: v for k, v in state.items() if k not in ("_prepared", "_prepared_of")}
         super().__setstate__({"_kept": None, "full_sums": False, **state})
 
-    def _state(self):
-        """What changes with the parameter's contents: the parameter, its storage and its count of changes in place."""
-        w = self.weight
-        return (w,), w.data_ptr(), w.dtype, w.device, None if w.is_inference() else w._version
+    def _state(self) -> tuple:
+        return _state(self.weight)
 
     def _forget(self) -> None:
         if self._kept is not None:
@@ -673,11 +677,12 @@ class Fp8Linear(torch.nn.Module):
 
     def _form(self, saved: bool = False) -> PreparedFp8Weight:
         """The form for one call; ``saved``: a backward pass will read it too."""
+        weight = self.weight
         with _KEPT_LOCK:
-            kept, weight = self._kept, self.weight
+            kept = self._kept
             # Not every change in place is counted: fused optimizers and changes of inference tensors are not. A form of a
             # weight that is open to them is the weight's for one call only, unless it was asked for.
-            current = (kept is not None and kept.holds(self._state()) and (kept.form.qt is not None or not saved) and
+            current = (kept is not None and kept.holds(weight) and (kept.form.qt is not None or not saved) and
                        (kept.asked or not (weight.requires_grad or weight.is_inference())))
             if _capturing(weight.device):
                 if current and kept.asked:
@@ -693,16 +698,16 @@ class Fp8Linear(torch.nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dim() < 1 or x.shape[-1] != self.in_features:
             raise ValueError(f"input of shape {tuple(x.shape)} for a layer of {self.in_features} input features")
-        _refuse_tangents(x, self.weight, self.bias)
-        params = [p for p in (self.weight, self.bias) if p is not None]
-        if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, *params))):
-            return fp8_linear(x, self._form(), self.bias, full_sums=self.full_sums)
-        if self.weight.requires_grad:
+        weight, bias = self.weight, self.bias
+        _refuse_tangents(x, weight, bias)
+        if not torch.is_grad_enabled() or not (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+            return fp8_linear(x, self._form(), bias, full_sums=self.full_sums)
+        if weight.requires_grad:
             self._forget()
-            prepared = prepare_fp8_weight(self.weight)
+            prepared = prepare_fp8_weight(weight)
         else:
             prepared = self._form(saved=True)
-        return _Fp8LinearFn.apply(x, self.weight, self.bias, prepared, self.full_sums)
+        return _Fp8LinearFn.apply(x, weight, bias, prepared, self.full_sums)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
@@ -743,11 +748,11 @@ class LayerNorm(torch.nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dim() < 1 or x.shape[-1] != self.features:
             raise ValueError(f"input of shape {tuple(x.shape)} for a norm of {self.features} features")
-        _refuse_tangents(x, self.weight, self.bias)
-        params = [p for p in (self.weight, self.bias) if p is not None]
-        if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, *params))):
-            return layer_norm(x, self.weight, self.bias, self.eps)
-        return _LayerNormFn.apply(x, self.weight, self.bias, self.eps, self.keep_fp8)
+        weight, bias = self.weight, self.bias
+        _refuse_tangents(x, weight, bias)
+        if not torch.is_grad_enabled() or not (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+            return layer_norm(x, weight, bias, self.eps)
+        return _LayerNormFn.apply(x, weight, bias, self.eps, self.keep_fp8)
 
     def extra_repr(self) -> str:
         return f"{self.features}, eps={self.eps}, bias={self.bias is not None}, keep_fp8={self.keep_fp8}"

@@ -6,7 +6,7 @@
 //
 // A row is held in registers by as many waves as it has chunks of 512 elements (up to sixteen), eight elements per lane and
 // chunk, so x (and dy) are read once; the variance is that of the centred values, not a difference of large sums.
-// HBM-bound: 75600 x 5120 bf16 forward 292 us (5.3 TB/s), backward from the input in 8 bits 384 + 8 us (4.9 TB/s). The
+// HBM-bound: 75600 x 5120 bf16 forward 303 us (5.1 TB/s), backward from the input in 8 bits, with its join, 386 (5.0 TB/s). The
 // backward pass also keeps its lanes' columns of dw and db in registers over all the rows a workgroup takes, writes them
 // once per workgroup, and fp8_join_kernel adds the workgroups' sums in a fixed order: no atomics, the same bits on
 // every run. Its x can be the input as it was kept in 8 bits (fp8_common.h), decoded as it is read.
@@ -419,7 +419,10 @@ static void with_shape(int D, F&& f) {
 }
 
 // The forward pass holds a row from its loads to its stores, so rows under way per CU count: few waves of many chunks
-// (75600 x 5120: two waves of five chunks 297 us, four of three 326, five of two 380, ten of one 458).
+// (75600 x 5120: two waves of five chunks 297 us, four of three 326, five of two 380, ten of one 458). Other widths, 200 M
+// bf16 elements, by one to six chunks: 1024 columns 156 130; 2048 147 132 132 136; 4096 151 133 133 136 135 138; 8192 161
+// 134 135 137 137 137; 12288 - 138 136 139 152 140; 16384 - 143 153 140 162 159; 24576 - - 143 144 171 144. Few rows (256)
+// take the same 8 us in every form.
 template <class F>
 static void with_forward_shape(int D, F&& f) {
   using std::integral_constant;

@@ -314,3 +314,17 @@ def test_host_tensors_are_refused_by_name(name, requires_grad):
     if name == "Fp8Linear":
         with pytest.raises(RuntimeError, match="GPU only"):
             module.prepare()
+
+
+def test_memory_written_anew_on_another_stream_is_still_held(host):
+    """A form that a graph reads can be written anew on a stream that did not allocate it: that stream's calls hold it too."""
+    layer, x = _layer().prepare(), torch.zeros(4, 256, dtype=torch.bfloat16)
+    host.capturing = True
+    layer(x)
+    host.capturing = False
+    host.stream = 7
+    layer.weight.mul_(2)
+    form = layer._prepared
+    layer(x)
+    layer(x)
+    assert layer._prepared is form and host.follows == [(7, ("built on", 7), 4)] * 2

@@ -544,10 +544,11 @@ class _Kept:
     ``held`` are the forms that graphs read and that no longer fit the weight. ``shared``: another stream, or a backward
     pass to come, reads the form."""
 
-    __slots__ = ("form", "of", "asked", "captured", "shared", "held", "stream", "built")
+    __slots__ = ("form", "of", "asked", "captured", "shared", "held", "home", "stream", "built")
 
     def __init__(self, form: PreparedFp8Weight, of: tuple, asked: bool, held: tuple = ()):
         self.form, self.captured, self.shared, self.held = form, False, False, held
+        self.home = _raw_stream(form.device.index)  # (the stream whose memory the form is)
         self.done(of, asked)
 
     def done(self, of: tuple, asked: bool) -> None:
@@ -578,7 +579,8 @@ class _Kept:
     def use(self) -> PreparedFp8Weight:
         """The form, for work on the current stream."""
         device = self.form.device
-        if _raw_stream(device.index) != self.stream:
+        stream = _raw_stream(device.index)
+        if stream != self.stream or stream != self.home:
             self.shared = True
             _follow(device, self.built, self.tensors())
         return self.form

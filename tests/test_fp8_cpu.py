@@ -227,3 +227,15 @@ def test_whole_passes_refuse_before_their_first_launch():
                 {"readable": 0, "q": None}, {"dy": None}, {"ldy": 127}, {"direct": 1, "ldy": 1 << 24}):
         with pytest.raises(ValueError):
             backward(**bad)
+
+
+def test_full_sums_take_the_same_workspace():
+    from mx_qlinear import _lib
+
+    plain, full = ctypes.c_int64(), ctypes.c_int64()
+    for needs in range(1, 8):
+        _lib.call("mxq_fp8_linear_backward_workspace", 700, 300, 500, 1, 0, 1, needs, ctypes.byref(plain))
+        _lib.call("mxq_fp8_linear_backward_workspace", 700, 300, 500, 1 | _lib.FP8_FULL_SUMS, 0, 1, needs, ctypes.byref(full))
+        assert plain.value == full.value
+    with pytest.raises(ValueError):
+        _lib.call("mxq_fp8_linear_backward_workspace", 700, 300, 500, 3 | _lib.FP8_FULL_SUMS, 0, 1, 7, ctypes.byref(full))

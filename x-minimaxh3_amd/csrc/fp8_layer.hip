@@ -123,6 +123,7 @@ extern "C" int mxq_fp8_linear(const void* x, int x_dtype, int64_t ldx, const uin
 
 extern "C" int mxq_fp8_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dy_dtype, int direct, int readable,
                                                  int needs, int64_t* bytes) {
+  dy_dtype &= ~MXQ_FP8_FULL_SUMS;
   if (!sizes_ok(M, N, K) || !float_dtype(dy_dtype) || !bytes) return mxq_set_error(MXQ_ERR_INVALID, "bad argument");
   BackwardSpace s;
   if (const int rc = backward_space(nullptr, M, N, K, dy_dtype, direct, readable, needs, s)) return rc;

@@ -36,6 +36,7 @@ extern "C" {
 #define MXQ_DTYPE_F16 1
 #define MXQ_DTYPE_BF16 2
 #define MXQ_DTYPE_E4M3 5
+#define MXQ_DTYPE_E2M1 8 /* two codes per byte (the 4-bit format below) */
 
 /* Pre-quantization activation codes: CK/backends/_activations.py:19-24. */
 #define MXQ_ACT_NONE 0
@@ -610,6 +611,96 @@ int mxq_fp8_linear_backward(const void* dy, int dy_dtype, int64_t ldy, int direc
                             const uint8_t* scale, int64_t lds, int readable, const uint8_t* bt, int64_t ldbt,
                             const uint8_t* sbt, int64_t ldsbt, void* dx, void* dw, void* db, int grad_dtype, int64_t M,
                             int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * ---- 4-bit floating point in blocks of 32 (MXFP4) ----
+ * e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6; bit 3 the sign), two in a byte, the even column's in the low four bits, with one
+ * E8M0 byte b per 1 x 32 block of a row: the values are code * 2^(b - 127). The quantizer takes the smallest exponent
+ * b - 127 >= -125 with absmax <= 6 * 2^(b - 127) (a block of zeros: b = 127) and rounds x / 2^(b - 127) once, to nearest
+ * even; a block with a NaN or an infinity has b = 255, which makes all its values NaN. Strides of codes are in bytes.
+ * As operands of the products, rows of codes are zero-padded to multiples of 128 bytes (row strides multiples of 16), and the
+ * scale bytes lie in tiles of 512 bytes for 32 rows x 16 blocks: row r, block c of a tile (c = 0 .. 15) at
+ * ((c / 4) % 2) * 256 + r * 8 + (c / 8) * 4 + c % 4, the tiles of 32 rows one after the other (ceil(K / 512) of them), 127 or
+ * any byte but 255 behind a row's last block; MXQ_MXFP4_SCALE_BYTES in all. No counterpart in the reference.
+ */
+#define MXQ_MXFP4_ROW_BYTES(K) (((K) + 255) / 256 * 128)
+#define MXQ_MXFP4_SCALE_BYTES(rows, K) (((rows) + 31) / 32 * (((K) + 511) / 512) * 512)
+
+/*
+ * Codes [M, ldq] and scales of x [M, K] (bf16, fp16 or fp32; row stride ldx): scales [M, lds] with lds a multiple of 4 and at
+ * least ceil(K / 128) * 4, or, with lds = 0, in tiles. Codes are written to whole 128 columns (in tiles: to whole
+ * MXQ_MXFP4_ROW_BYTES), zeros behind column K; ldq a multiple of 16.
+ */
+int mxq_mxfp4_quantize_rows(const void* x, int x_dtype, int64_t ldx, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, int64_t M,
+                            int64_t K, void* stream);
+
+/* The way back: out [M, K] contiguous of out_dtype. Any strides ldq >= ceil(K / 2) and lds >= ceil(K / 32). */
+int mxq_mxfp4_dequantize_rows(const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds, void* out, int out_dtype, int64_t M,
+                              int64_t K, void* stream);
+
+/* Codes and scales of any strides and alignment as operands: q_out [rows, ldqo] (NULL: the scales only) and scale_out in tiles. */
+int mxq_mxfp4_layout(const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds, uint8_t* q_out, int64_t ldqo,
+                     uint8_t* scale_out, int64_t rows, int64_t K, void* stream);
+
+/* Bytes of workspace mxq_mxfp4_gemm needs at this size on the current device (0: none). */
+int mxq_mxfp4_gemm_workspace(int64_t M, int64_t N, int64_t K, int64_t* bytes);
+
+/*
+ * d [M, N] = out(a b^T + bias): operands a [M, lda] with scale tiles sa and b [N, ldb] with sb; bias [N] of out_dtype or NULL.
+ * Sums are float32: a block's 32 products are added exactly, and the blocks' sums to the float32 with what lies below 2^-22
+ * of the largest cut. N and K up to 2^22.
+ */
+int mxq_mxfp4_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, const uint8_t* b, int64_t ldb, const uint8_t* sb,
+                   const void* bias, void* d, int64_t ldd, int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace mxq_mxfp4_linear needs at this size on the current device (0 up to 16 rows). */
+int mxq_mxfp4_linear_workspace(int64_t M, int64_t N, int64_t K, int64_t* bytes);
+
+/* The layer's forward pass in one call: d [M, N] = out(quantize(x) b^T + bias), x [M, ldx] of x_dtype; the rest as above. */
+int mxq_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* b, int64_t ldb, const uint8_t* sb, const void* bias,
+                     void* d, int64_t ldd, int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                     void* stream);
+
+/*
+ * Bytes of workspace mxq_mxfp4_linear_backward needs at this size on the current device. needs: 1 dx, 2 db, added up; direct as
+ * below.
+ */
+int mxq_mxfp4_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dy_dtype, int direct, int needs, int64_t* bytes);
+
+/*
+ * The layer's backward pass in one call, through a frozen weight b [N, ldb] with scale tiles sb: dx [M, K] (contiguous,
+ * dy_dtype) = dy b with the products of dy [M, ldy] as it is exact (one, two or three bfloat16 parts of bf16, fp16 and fp32)
+ * and float32 sums, db [N] = sums of dy's columns (grad_dtype), each NULL to leave it out. direct: the product reads dy itself
+ * (bf16, N % 8 == 0, ldy % 8 == 0, ldy < 2^24, 16-byte aligned) in place of parts of it.
+ */
+int mxq_mxfp4_linear_backward(const void* dy, int dy_dtype, int64_t ldy, int direct, const uint8_t* b, int64_t ldb, const uint8_t* sb,
+                              void* dx, void* db, int grad_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+
+/*
+ * Root-mean-square norm of rows: s = x + r rounded to dtype (x [M, ldx], r [M, ldr]; s is written to sum [M, D] contiguous;
+ * r NULL: s = x and sum is not used), rstd = 1 / sqrt(E[s^2] + eps) with the mean in float64, rounded once, and
+ * y = (s * rstd) * w in float32, w [D] of param_dtype or NULL (1). y_dtype: dtype (y [M, D] contiguous, rounded once; ldq,
+ * scale and lds are not used), MXQ_DTYPE_E4M3 (codes y [M, ldq] and scales [M, lds] by 1 x 128, as mxq_fp8_quantize_rows
+ * makes them of y in float32; ldq a multiple of 8) or MXQ_DTYPE_E2M1 (by 1 x 32, as mxq_mxfp4_quantize_rows; ldq in
+ * bytes, a multiple of 4, at least ceil(D / 128) * 64). rstd fp32 [M] or NULL. D <= 24576.
+ */
+int mxq_rms_norm(const void* x, const void* r, int dtype, int64_t ldx, int64_t ldr, const void* w, int param_dtype, float eps,
+                 void* sum, void* y, int y_dtype, int64_t ldq, uint8_t* scale, int64_t lds, float* rstd, int64_t M, int64_t D,
+                 void* stream);
+
+/* Bytes of workspace mxq_rms_norm_backward needs for dweight at this size on the current device. */
+int mxq_rms_norm_backward_workspace(int64_t M, int64_t D, int64_t* bytes);
+
+/*
+ * Its gradients: dx [M, D] (contiguous, dtype), that of x and of r alike, from dy [M, ldy] of dtype, the normed rows s as
+ * x [M, ldx] of dtype, or as codes with x_dtype MXQ_DTYPE_E4M3 and scales [M, ldxs], and the forward's rstd; dsum [M, ldds]
+ * of dtype (NULL: none), the gradient of sum, is added. dweight fp32 [D] (NULL: none): the sums over rows of dy * s * rstd.
+ */
+int mxq_rms_norm_backward(const void* dy, int dtype, int64_t ldy, const void* x, int x_dtype, int64_t ldx, const uint8_t* x_scale,
+                          int64_t ldxs, const float* rstd, const void* w, int param_dtype, const void* dsum, int64_t ldds, void* dx,
+                          float* dweight, int64_t M, int64_t D, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Measurement helper (no counterpart in the reference; it calibrates the roofline): runs

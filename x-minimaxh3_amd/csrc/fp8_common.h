@@ -292,6 +292,35 @@ MXQ_DEVICE void store_run4(void* row, int64_t col, int n, const float* y) {
   }
 }
 
+// `n` of 16 bytes from s, zeros behind them (n <= 0: nothing is read).
+MXQ_DEVICE v4u bytes_load(const uint8_t* s, int n) {
+  v4u v = {0, 0, 0, 0};
+  if (n >= 16) {
+    v = *reinterpret_cast<const v4u_any*>(s);
+  } else if (n > 0) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t b = s[min(i, n - 1)];
+      v[i >> 2] |= (i < n ? b : 0u) << (8 * (i & 3));
+    }
+  }
+  return v;
+}
+
+inline int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// Consecutive 256-byte aligned pieces of a workspace; with no base, their total size.
+struct Carve {
+  uint8_t* base;
+  int64_t used = 0;
+  template <class T>
+  T* take(int64_t bytes) {
+    uint8_t* p = base ? base + used : nullptr;
+    used += up(bytes, 256);
+    return reinterpret_cast<T*>(p);
+  }
+};
+
 inline int dtype_bytes(int code) { return code == MXQ_DTYPE_F32 ? 4 : 2; }
 inline bool float_dtype(int code) { return code == MXQ_DTYPE_F32 || code == MXQ_DTYPE_F16 || code == MXQ_DTYPE_BF16; }
 

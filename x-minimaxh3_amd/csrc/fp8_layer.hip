@@ -7,20 +7,6 @@ using namespace mxq;
 
 namespace {
 
-int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
-
-// Consecutive 256-byte aligned pieces of a workspace; with no base, their total size.
-struct Carve {
-  uint8_t* base;
-  int64_t used = 0;
-  template <class T>
-  T* take(int64_t bytes) {
-    uint8_t* p = base ? base + used : nullptr;
-    used += up(bytes, 256);
-    return reinterpret_cast<T*>(p);
-  }
-};
-
 struct Pair {  // codes and scales of [rows, cols]
   uint8_t *q, *s;
   int64_t ldq, lds;

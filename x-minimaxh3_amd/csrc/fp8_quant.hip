@@ -86,21 +86,6 @@ __global__ __launch_bounds__(256) void fp8_rows_dequant_kernel(const uint8_t* q,
   }
 }
 
-// `n` of 16 bytes from s, zeros behind them (n <= 0: nothing is read).
-MXQ_DEVICE v4u bytes_load(const uint8_t* s, int n) {
-  v4u v = {0, 0, 0, 0};
-  if (n >= 16) {
-    v = *reinterpret_cast<const v4u_any*>(s);
-  } else if (n > 0) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t b = s[min(i, n - 1)];
-      v[i >> 2] |= (i < n ? b : 0u) << (8 * (i & 3));
-    }
-  }
-  return v;
-}
-
 // ---- weights: one scale per 128 x 128 tile, and the transposed codes that the input's gradient reads ----
 // One workgroup per tile: row t / 8 + 32 i, piece t % 8. The transposed copy goes through a 16 KB byte tile in LDS.
 // HBM-bound: 21504 x 5376 bf16 in 90 us (5.1 TB/s) with the transposed copy, 65 without.

@@ -5,8 +5,9 @@ GEMMs on CDNA4 matrix cores with fused dequant / bias / tanh-GELU / re-quant epi
 W4A8 GEMMs, with the ConvRot (regular Hadamard) rotation and the GELU / SwiGLU input
 activations folded into the quantizer, behind the reference's Comfy-Kitchen function names and its quantized-linear
 module contract; and the 8-bit floating point layer (e4m3 with a power of two per block of 128) with its
-gradients, 8-bit activation checkpoints and the layer norm. All compute runs in hand-written HIP kernels (libmx_qlinear.so, C ABI in
-include/mx_qlinear.h); there is no CPU path.
+gradients, 8-bit activation checkpoints and the layer norm; the microscaled 4-bit layer (e2m1 with a power of two per block
+of 32) with its input's gradient; and the root-mean-square norm behind a residual addition, its output in 16, 8 or 4 bits.
+All compute runs in hand-written HIP kernels (libmx_qlinear.so, C ABI in include/mx_qlinear.h); there is no CPU path.
 """
 
 from .ops import (  # noqa: F401
@@ -54,6 +55,23 @@ from .fp8 import (  # noqa: F401
     layer_norm_backward,
     prepare_fp8_weight,
     quantize_fp8_block128,
+)
+from .mxfp4 import (  # noqa: F401
+    Mxfp4Linear,
+    PreparedMxfp4Weight,
+    dequantize_mxfp4,
+    mxfp4_linear,
+    mxfp4_linear_backward,
+    mxfp4_linear_prequantized,
+    prepare_mxfp4_weight,
+    quantize_mxfp4,
+)
+from .norm import (  # noqa: F401
+    RMSNorm,
+    rms_norm,
+    rms_norm_backward,
+    rms_norm_quantize_fp8,
+    rms_norm_quantize_mxfp4,
 )
 from .checkpoint import (  # noqa: F401
     MappingTensorSource,

@@ -18,7 +18,7 @@ MXQ_ERR_INVALID = -1
 MXQ_ERR_UNSUPPORTED = -2
 MXQ_ERR_HIP = -3
 
-DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_E4M3 = 0, 1, 2, 5
+DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_E4M3, DTYPE_E2M1 = 0, 1, 2, 5, 8
 FP8_FULL_SUMS = 256
 ABI_VERSION = 5
 # MXQ_GEMM_WORKSPACE_BYTES: the INT8 GEMMs' tile-queue workspace (counters)
@@ -92,6 +92,18 @@ SIGNATURES: dict[str, list] = {
     "mxq_fp8_linear_backward_workspace": [_I64, _I64, _I64, _I, _I, _I, _I, _P],
     "mxq_fp8_linear_backward": [_P, _I, _I64, _I, _P, _I64, _P, _I64, _I, _P, _I64, _P, _I64, _P, _P, _P, _I, _I64, _I64, _I64,
                                 _P, _I64, _P],
+    "mxq_mxfp4_quantize_rows": [_P, _I, _I64, _P, _I64, _P, _I64, _I64, _I64, _P],
+    "mxq_mxfp4_dequantize_rows": [_P, _I64, _P, _I64, _P, _I, _I64, _I64, _P],
+    "mxq_mxfp4_layout": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P],
+    "mxq_mxfp4_gemm_workspace": [_I64, _I64, _I64, _P],
+    "mxq_mxfp4_gemm": [_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I, _I64, _I64, _I64, _P, _I64, _P],
+    "mxq_mxfp4_linear_workspace": [_I64, _I64, _I64, _P],
+    "mxq_mxfp4_linear": [_P, _I, _I64, _P, _I64, _P, _P, _P, _I64, _I, _I64, _I64, _I64, _P, _I64, _P],
+    "mxq_mxfp4_linear_backward_workspace": [_I64, _I64, _I64, _I, _I, _I, _P],
+    "mxq_mxfp4_linear_backward": [_P, _I, _I64, _I, _P, _I64, _P, _P, _P, _I, _I64, _I64, _I64, _P, _I64, _P],
+    "mxq_rms_norm": [_P, _P, _I, _I64, _I64, _P, _I, _F, _P, _P, _I, _I64, _P, _I64, _P, _I64, _I64, _P],
+    "mxq_rms_norm_backward_workspace": [_I64, _I64, _P],
+    "mxq_rms_norm_backward": [_P, _I, _I64, _P, _I, _I64, _P, _I64, _P, _P, _I, _P, _I64, _P, _P, _I64, _I64, _P, _I64, _P],
 }
 
 _lib = None

@@ -468,7 +468,8 @@ def _refuse_capture(device: torch.device) -> None:
     end the process. A training step is captured through the functions, which own no such nodes."""
     if _capturing(device):
         raise RuntimeError("the autograd modules are not captured into graphs; capture fp8_linear, fp8_linear_backward, "
-                           "layer_norm and layer_norm_backward instead")
+                           "mxfp4_linear, mxfp4_linear_backward, layer_norm, layer_norm_backward, rms_norm and "
+                           "rms_norm_backward instead")
 
 
 def _refuse_tangents(*tensors: torch.Tensor | None) -> None:

@@ -67,7 +67,7 @@ MXQ_DEVICE v8bf fp4x8_to_bf16(uint32_t q, float scale) {
 }
 
 // mxq_mxfp4_gemm's and the input gradient's refusals other than the workspace's, for passes that launch other steps ahead of
-// them, and the product with the join of its slices, if there is one, left to the caller (`later` not NULL).
+// them; the gradient leaves the join of its slices, if there are any, to the caller.
 int fp4_gemm_check(const uint8_t* a, int64_t lda, const uint8_t* sa, const uint8_t* b, int64_t ldb, const uint8_t* sb, const void* d,
                    int64_t ldd, int out_dtype, int64_t M, int64_t N, int64_t K);
 int fp4_dgrad_check(const void* dy, int64_t ldy, const uint8_t* b, int64_t ldb, const uint8_t* sb, const void* dx, int out_dtype,

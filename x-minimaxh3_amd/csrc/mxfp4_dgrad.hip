@@ -2,78 +2,292 @@
 //
 //   dX[m, k] = sum_n dY[m, n] * W[n, k],   W[n, k] = code[n, k] * 2^(b[n, k / 32] - 127)
 //
-// dY is bfloat16 (float16 and float32 gradients come as two and three bfloat16 parts whose products are summed) and W is
-// decoded to bfloat16, which is exact: the only roundings are those of the float32 sums. The simplest form: a wave per
-// 32 x 32 block of dX, operands straight from memory.
+// dY is bfloat16 [M, N] (float16 and float32 gradients come as two and three bfloat16 parts whose products are summed) and W is
+// decoded to bfloat16, which is exact, so the only roundings are those of the float32 sums: 16-bit matrix instructions
+// (v_mfma_f32_32x32x16_bf16). The 4-bit instructions cannot take W here: their scales go along the summed index, W's across it.
+//
+// dY's rows hold the summed index n, so its fragments (eight consecutive n of one row per lane) are plain 16-byte LDS reads; W
+// has n as its rows, and its fragments come from transposing reads (ds_read_b64_tr_b16), which hand sixteen lanes the columns
+// of a 4 x 16 patch. A workgroup of eight waves owns a 256 (m) x 256 (k) tile, a wave 64 x 128 of it; a stage is 64 of n: dY's
+// 256 x 64 bfloat16 (32 KB) and W's 64 x 256 codes, decoded on the way from registers to LDS (32 KB). Problems of few tiles
+// split N over workgroups, which write float32 sums that fp8_join_kernel adds in order.
 #include "mxfp4_common.h"
 
 namespace mxq {
 
+constexpr int kDTile = 256, kDStage = 64, kDGroup = 4;
+constexpr int kDMB = 2, kDKB = 4;  // 32-row and 32-column blocks of a wave
+constexpr int kDThreads = 512, kDWaves = 8;
+constexpr int kDBytes = kDTile * kDStage * 2;  // of one operand's stage in LDS
+static_assert(2 * kDBytes == 0x10000, "the buffers are one address bit apart");
+
 struct Dgrad {
   const uint16_t* dy;  // part p at dy + p * part_stride
   const uint8_t *b, *sb;
-  void* d;
-  int64_t M, N, K, ldy, part_stride, ldb;
-  int parts, groups;
+  void* d;  // split: float32 sums, slice i at i * M * ldd
+  int64_t M, N, K, ldy, part_stride, ldb, ldd;
+  int parts, groups, tiles_m, tiles_k, splits, split_n;  // split_n: a multiple of kDStage
 };
 
-template <int kOut>
-__global__ __launch_bounds__(64) void mxfp4_dgrad_kernel(Dgrad p) {
-  const int lane = threadIdx.x, lr = lane & 31, h = lane >> 5;
-  const int64_t m0 = (int64_t)blockIdx.x * 32, k0 = (int64_t)blockIdx.y * 32, k = k0 + lr;
-  const int block = (int)(k0 >> 5);
-  v16f acc = {};
-  for (int part = 0; part < p.parts; ++part) {
-    const uint16_t* y = p.dy + part * p.part_stride + min(m0 + lr, p.M - 1) * p.ldy;
-    for (int64_t n0 = 0; n0 < p.N; n0 += 16) {
-      typedef short v8s __attribute__((ext_vector_type(8)));
-      v8s fy, fw;
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef v4s __attribute__((address_space(3)))* lds_v4s;
+typedef v4u __attribute__((address_space(3)))* lds_v4u;
+typedef char __attribute__((address_space(3)))* lds_ptr;  // (pointer arithmetic: constants become the instructions' offsets)
+
+// dY in LDS: rows of 128 bytes (64 n), 16-byte piece c of row r at piece c ^ ((r >> 1) & 7), so that the sixteen lanes a 16-byte
+// read serves at once (sixteen rows, one piece) touch every bank once.
+MXQ_DEVICE int dy_at(int r, int piece) { return r * 128 + ((piece ^ ((r >> 1) & 7)) << 4); }
+
+// W in LDS: rows of 512 bytes (256 bfloat16), 64-byte piece p of row r at piece p ^ (r & 3), so that the sixteen lanes of a
+// transposing read (four rows, 32 bytes) and their neighbours cover all banks.
+MXQ_DEVICE int w_at(int r, int byte) { return r * 512 + ((((byte >> 6) ^ (r & 3)) << 6) | (byte & 63)); }
+
+// A fragment of W: columns c0 + l % 32 (c0 a multiple of 32), rows 8 (l / 32) + {0..7} of the 16 rows from r0 on (a multiple of
+// 16), in two transposing reads of four rows. Lane l of a group of sixteen gives the address of row (l % 16) / 4, columns
+// 4 (l % 4) .. + 3 of a 4 x 16 patch, and receives its column l % 16. The address is that of w_base plus a constant: r & 3, which
+// the swizzle uses, is the lane's own.
+MXQ_DEVICE uint32_t w_base(uint32_t operand, int c0, int lane) {
+  const int r = (lane >> 5) * 8 + ((lane & 15) >> 2);
+  return operand + (uint32_t)w_at(r, (c0 + (lane & 16) + (lane & 3) * 4) * 2);
+}
+template <int kRow>
+MXQ_DEVICE v4s read_transposed(uint32_t base) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)((lds_ptr)(uintptr_t)base + kRow * 512));
+}
+MXQ_DEVICE v8bf join_fragment(const v4s (&f)[2]) {
+  typedef short v8s __attribute__((ext_vector_type(8)));
+  return __builtin_bit_cast(v8bf, v8s{f[0][0], f[0][1], f[0][2], f[0][3], f[1][0], f[1][1], f[1][2], f[1][3]});
+}
+
+MXQ_DEVICE uint32_t dgrad_load_u32(const void* base, int bytes, uint32_t voff) {
+  return __builtin_amdgcn_raw_buffer_load_b32(
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, kRawBufferWord3), (int)voff, 0, 0);
+}
+
+template <int kOut, bool kSplit>
+__global__ __launch_bounds__(kDThreads, 1) void mxfp4_dgrad_kernel(Dgrad p) {
+  __shared__ __attribute__((aligned(131072))) char lds[2 * 2 * kDBytes];  // [buffer][dY, W]
+  const int tiles = p.tiles_m * p.tiles_k, num = tiles * p.splits, per = num / 8, bid = blockIdx.x;
+  int t = bid < per * 8 ? (bid % 8) * per + bid / 8 : bid;  // contiguous ranges over the XCDs
+  const int slice = t / tiles;
+  t -= slice * tiles;
+  // groups of four tile-rows, so that the tiles an XCD runs at once share operand panels in its L2
+  const int group = kDGroup * p.tiles_k, g0 = t / group * kDGroup, rows_g = min(p.tiles_m - g0, kDGroup), in_g = t - g0 * p.tiles_k;
+  const int tk = in_g / rows_g, tm = g0 + in_g - tk * rows_g;
+  const int m0 = tm * kDTile, k0 = tk * kDTile;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int wm = (wave & 3) * 64, wk = (wave >> 2) * 128;  // the wave's part of the tile
+  const int M = (int)p.M, K = (int)p.K, n_first = slice * p.split_n, n_last = min(n_first + p.split_n, (int)p.N);
+  const int stages = (n_last - n_first + kDStage - 1) / kDStage, total = stages * p.parts;
+
+  // A thread's share of a stage, by buffer loads whose offsets point outside for what lies behind the slice's last n or the last
+  // row (they read zeros): of dY the 16-byte piece tid % 8 of rows tid / 8 + 64 j (nothing is read behind column N rounded up to
+  // 8); of W row tid / 8, the words (eight columns) tid % 8 + 8 j with the scale words of the row's blocks 0 .. 3 and 4 .. 7.
+  const int r = tid >> 3, c = tid & 7;
+  const int ldy = (int)p.ldy, ldb = (int)p.ldb, row_tiles = p.groups * (int)kFp4ScaleTile;
+  const uint32_t oy = (uint32_t)(r * ldy + c * 8) * 2, ow = (uint32_t)(r * ldb + c * 4);
+  const uint32_t os = (uint32_t)((r >> 5) * row_tiles + (r & 31) * 8 + ((k0 >> 8) & 1) * 4);
+  v4u y[4];
+  uint32_t w[4], ws[2];
+  // (the position of the next load: n left in the slice and the operands' place)
+  int left = n_last - n_first, parts_left = left > 0 ? p.parts : 0;
+  const uint16_t* py = p.dy + (int64_t)m0 * ldy + n_first;
+  const uint8_t* pw = p.b + (int64_t)n_first * ldb + k0 / 2;
+  const uint8_t* ps = p.sb + (int64_t)(n_first >> 5) * row_tiles + (k0 >> 9) * kFp4ScaleTile;
+  auto load = [&](auto HC) {  // the first or second half of a share
+    constexpr int kH = decltype(HC)::value;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t n = n0 + 8 * h + i, at = min(n, p.N - 1);
-        const uint32_t c = p.b[at * p.ldb + min(k, p.K - 1) / 2] >> (4 * (k & 1));
-        const uint32_t s = p.sb[((at >> 5) * p.groups + (block >> 4)) * kFp4ScaleTile + fp4_scale_at((int)(at & 31), block & 15)];
-        const uint32_t w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c & 15u, fp8_scale_f32(s), 0));
-        fy[i] = n < p.N ? (short)y[n] : (short)0;
-        fw[i] = n < p.N ? (short)(w & 0xFFFFu) : (short)0;
-      }
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, fw), __builtin_bit_cast(v8bf, fy), acc, 0, 0, 0);
+    for (int j = 2 * kH; j < 2 * kH + 2; ++j) {
+      y[j] = buffer_load_x4(py + (int64_t)(64 * j) * ldy, 64 * 2 * ldy, c * 8 < left && m0 + 64 * j + r < M ? oy : kBufferOff);
+      w[j] = dgrad_load_u32(pw, kDStage * ldb, r < left ? ow + 32 * j : kBufferOff);
     }
-  }
-  constexpr int kElem = kOut == MXQ_DTYPE_F32 ? 4 : 2;
-  if (m0 + lr >= p.M) return;
+    ws[kH] = dgrad_load_u32(ps, 2 * row_tiles, r < left ? os + 256 * kH : kBufferOff);
+    if constexpr (kH == 1) {
+      left -= kDStage;
+      py += kDStage;
+      pw += (int64_t)kDStage * ldb;
+      ps += 2 * row_tiles;
+      if (left <= 0) {  // (the slice's end: the next part's first n, or, behind the last part, none: left stays below 1)
+        if (--parts_left > 0) {
+          left = n_last - n_first;
+          py += p.part_stride - (int64_t)stages * kDStage;
+          pw -= (int64_t)stages * kDStage * ldb;
+          ps -= (int64_t)stages * 2 * row_tiles;
+        }
+      }
+    }
+  };
+  const uint32_t at_y = lds_addr(lds) + (uint32_t)dy_at(r, c);  // (row r + 64 j has r's swizzle)
+  // (words c + 8 j: 128 bytes further on, two 64-byte pieces, whose number the swizzle is exclusive with)
+  const uint32_t at_w = lds_addr(lds) + kDBytes + (uint32_t)w_at(r, c * 16);
+  auto put_y = [&](uint32_t buf, auto JC) {
+    constexpr int j = decltype(JC)::value;
+    *(lds_v4u)((lds_ptr)(uintptr_t)(at_y ^ buf) + j * 64 * 128) = y[j];
+  };
+  auto put_w = [&](uint32_t buf, auto JC) {
+    constexpr int j = decltype(JC)::value;
+    const uint32_t byte = (ws[j >> 1] >> (16 * (j & 1) + 8 * (c >> 2))) & 0xFFu;
+    *(lds_v4u)((lds_ptr)(uintptr_t)(at_w ^ buf ^ (j * 128))) = __builtin_bit_cast(v4u, fp4x8_to_bf16(w[j], fp8_scale_f32(byte)));
+  };
+  v16f acc[kDMB][kDKB] = {};
+  // A stage is four steps of 16 n, a step eight slots, each one matrix instruction and a part of the other work, in the order
+  // written (sched_barrier): fragments are read one step ahead; the next stage is written to the other buffer, a half each,
+  // during steps 1 and 2, the one behind it requested as the registers get free, and the barrier passed ahead of the last
+  // step, whose instructions cover the next stage's first reads.
+  constexpr int kSlots = kDMB * kDKB, kReads = kDMB + 2 * kDKB;
+  constexpr int kReadSlots = kSlots * 6 / 8;  // the reads end early: the next step's first instruction waits for them
+  v4u fy[2][kDMB];
+  v4s fw[2][kDKB][2];
+  uint32_t base[kDKB];  // of W's fragments in buffer 0
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int col = (int)k0 + q * 8 + h * 4;
-    if (col >= p.K) continue;
-    const float v[4] = {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
-    store_run4<kOut>(reinterpret_cast<char*>(p.d) + (m0 + lr) * p.K * kElem, col, (int)p.K - col, v);
+  for (int b = 0; b < kDKB; ++b) base[b] = w_base(lds_addr(lds) + kDBytes, wk + b * 32, lane);
+  // dY's fragments: row wm + l % 32 (+ 32 a), piece 2 step + l / 32
+  uint32_t base_y[4];
+#pragma unroll
+  for (int h = 0; h < 4; ++h) base_y[h] = lds_addr(lds) + (uint32_t)dy_at(wm + (lane & 31), 2 * h + (lane >> 5));
+  auto read = [&](uint32_t buf, auto StepC, auto SetC, auto IC) {  // read I of a step, in the order of their use
+    constexpr int kStep = decltype(StepC)::value, kSet = decltype(SetC)::value, kI = decltype(IC)::value;
+    if constexpr (kI == 0 || kI > 2 * kDKB) {
+      constexpr int a = kI == 0 ? 0 : kI - 2 * kDKB;
+      fy[kSet][a] = *(lds_v4u)((lds_ptr)(uintptr_t)(base_y[kStep] ^ buf) + a * 32 * 128);
+    } else {
+      constexpr int b = (kI - 1) / 2, kPart = (kI - 1) & 1;
+      fw[kSet][b][kPart] = read_transposed<kStep * 16 + kPart * 4>(base[b] ^ buf);
+    }
+  };
+  auto publish = [&] {
+    wait_lgkm<0>();
+    __builtin_amdgcn_sched_barrier(0);
+    barrier_no_drain();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  uint32_t buf = 0;  // byte offset of the stage's buffer
+  auto stage = [&] {
+    const uint32_t other = buf ^ (2 * kDBytes);
+    static_for<4>([&](auto H) {
+      constexpr int h = decltype(H)::value, kSet = h & 1;
+      constexpr bool kPut = h == 1 || h == 2;
+      if constexpr (h == 3) publish();
+      static_for<kSlots>([&](auto G) {
+        constexpr int g = decltype(G)::value, a = g / kDKB, b = g % kDKB;
+        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(join_fragment(fw[kSet][b]), __builtin_bit_cast(v8bf, fy[kSet][a]), acc[a][b], 0, 0, 0);
+        static_for<kReads>([&](auto I) {
+          constexpr int i = decltype(I)::value;
+          if constexpr (i * kReadSlots / kReads == g)
+            read(h < 3 ? buf : other, std::integral_constant<int, h < 3 ? h + 1 : 0>{}, std::integral_constant<int, kSet ^ 1>{}, I);
+        });
+        if constexpr (kPut) {
+          constexpr int j = (h - 1) * 2 + g / 4;
+          if constexpr (g % 4 == 0) put_y(other, std::integral_constant<int, j>{});
+          if constexpr (g % 4 == 2) put_w(other, std::integral_constant<int, j>{});
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      if constexpr (kPut) load(std::integral_constant<int, h - 1>{});
+    });
+    buf = other;
+  };
+  // (one loop for all stages: with the last ones peeled off, copies of the accumulators between the loops would spill)
+  static_for<2>(load);
+  static_for<4>([&](auto J) { put_y(0, J); put_w(0, J); });
+  static_for<2>(load);
+  publish();
+  static_for<kReads>([&](auto I) { read(0, std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{}, I); });
+  for (int i = 0; i < total; ++i) stage();
+  // Lane l holds row m = l % 32 of a block and, in register e, column (e / 4) * 8 + (l / 32) * 4 + e % 4. Stored from there, an
+  // instruction would touch 32 bytes of 32 rows; through the wave's 16 KB of LDS (no wave reads a stage any more: the last
+  // barrier is behind the last step's reads) 32 lanes store a row's 128 columns. 16-byte piece c of row r sits at piece c ^ r.
+  constexpr int kElem = kOut == MXQ_DTYPE_F32 ? 4 : 2;
+  char* d = reinterpret_cast<char*>(p.d);
+  if constexpr (kSplit) d += (int64_t)slice * p.M * p.ldd * 4;
+  char* turn = lds + wave * (2 * 2 * kDBytes / kDWaves);
+#pragma unroll
+  for (int a = 0; a < kDMB; ++a) {
+    wave_lds_fence();
+    const int row = lane & 31;
+#pragma unroll
+    for (int b = 0; b < kDKB; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<v4f*>(turn + row * 512 + (((b * 8 + e * 2 + (lane >> 5)) ^ row) << 4)) =
+            v4f{acc[a][b][4 * e], acc[a][b][4 * e + 1], acc[a][b][4 * e + 2], acc[a][b][4 * e + 3]};
+    wave_lds_fence();
+    const int k = k0 + wk + (lane & 31) * 4;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      const int q = u * 2 + (lane >> 5), m = m0 + wm + a * 32 + q;
+      const v4f z = *reinterpret_cast<const v4f*>(turn + q * 512 + (((lane & 31) ^ q) << 4));
+      const float v[4] = {z[0], z[1], z[2], z[3]};
+      if (m < M && k < K) store_run4<kOut>(d + (int64_t)m * p.ldd * kElem, k, K - k, v);
+    }
   }
 }
 
-int64_t fp4_dgrad_workspace(int64_t, int64_t, int64_t, int) { return 0; }
+struct DgradPlan {
+  int splits;
+  int64_t n;
+};
+
+// N slices, by an estimate in microseconds: a round of workgroups takes 4.5 and 1.5 per stage and part, slices cost a join.
+static DgradPlan plan_dgrad(int64_t M, int64_t N, int64_t K, int parts, int cus) {
+  const int64_t tiles = (M + kDTile - 1) / kDTile * ((K + kDTile - 1) / kDTile);
+  DgradPlan best = {1, (N + kDStage - 1) / kDStage * kDStage};
+  double best_cost = 1e300;
+  for (int64_t s = 1; s <= 64; ++s) {
+    const int64_t n = ((N + s - 1) / s + kDStage - 1) / kDStage * kDStage;
+    if ((N + n - 1) / n != s || (s > 1 && tiles * s > 4 * cus)) continue;
+    const double rounds = (double)((tiles * s + cus - 1) / cus);
+    const double cost = rounds * ((double)(n / kDStage) * parts * 1.5 + 4.5) + slices_cost(s, M * K);
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = {(int)s, n};
+    }
+  }
+  return best;
+}
+
+static int64_t dgrad_bytes(const DgradPlan& plan, int64_t M, int64_t K) {
+  return plan.splits > 1 ? plan.splits * M * ((K + 3) / 4 * 4) * 4 : 0;
+}
+
+int64_t fp4_dgrad_workspace(int64_t M, int64_t N, int64_t K, int parts) {
+  return M == 0 ? 0 : dgrad_bytes(plan_dgrad(M, N, K, parts, mxq_cu_count()), M, K);
+}
 
 int fp4_dgrad_check(const void* dy, int64_t ldy, const uint8_t* b, int64_t ldb, const uint8_t* sb, const void* dx, int out_dtype,
                     int64_t M, int64_t N, int64_t K) {
   if (!float_dtype(out_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported output dtype code %d", out_dtype);
   if (M < 0 || N < 1 || K < 1 || M > (1ll << 31) - 1024 || N > (1ll << 22) || K > (1ll << 22))
     return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
-  if (ldy < N || ldb < fp4_row_bytes(K) || ldb % 16 || ldb > (1ll << 22))
+  if (ldy < N || ldy % 8 || ldy >= (1 << 24) || ldb < fp4_row_bytes(K) || ldb % 16 || ldb > (1ll << 22))
     return mxq_set_error(MXQ_ERR_INVALID, "bad row strides ldy=%lld ldb=%lld for N=%lld K=%lld", (long long)ldy, (long long)ldb,
                          (long long)N, (long long)K);
-  if (M > 0 && (!dy || !b || !sb || !dx || reinterpret_cast<uintptr_t>(dy) % 2 || reinterpret_cast<uintptr_t>(b) % 16 ||
+  if (M > 0 && (!dy || !b || !sb || !dx || reinterpret_cast<uintptr_t>(dy) % 16 || reinterpret_cast<uintptr_t>(b) % 16 ||
                 reinterpret_cast<uintptr_t>(sb) % 16))
     return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
+  if ((M + kDTile - 1) / kDTile * ((K + kDTile - 1) / kDTile) >= (1ll << 23))  // (so many tiles are not split)
+    return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^23 tiles");
   return MXQ_OK;
 }
 
 int fp4_dgrad(const void* dy, int parts, int64_t ldy, const uint8_t* b, int64_t ldb, const uint8_t* sb, void* dx, int out_dtype,
-              int64_t M, int64_t N, int64_t K, void*, SliceJob*, void* stream) {
+              int64_t M, int64_t N, int64_t K, void* workspace, SliceJob* later, void* stream) {
   if (const int rc = fp4_dgrad_check(dy, ldy, b, ldb, sb, dx, out_dtype, M, N, K)) return rc;
-  const Dgrad p = {(const uint16_t*)dy, b, sb, dx, M, N, K, ldy, M * ldy, ldb, parts, (int)fp4_groups(K)};
-  const dim3 grid((unsigned)((M + 31) / 32), (unsigned)((K + 31) / 32));
+  const DgradPlan plan = plan_dgrad(M, N, K, parts, mxq_cu_count());
+  const int64_t tiles_m = (M + kDTile - 1) / kDTile, tiles_k = (K + kDTile - 1) / kDTile;
+  Dgrad p = {(const uint16_t*)dy, b, sb, dx, M, N, K, ldy, M * ldy, ldb, K, parts, (int)fp4_groups(K), (int)tiles_m, (int)tiles_k,
+             plan.splits, (int)plan.n};
+  const unsigned grid = (unsigned)(tiles_m * tiles_k * plan.splits);
+  if (plan.splits > 1) {
+    const int64_t ldp = (K + 3) / 4 * 4;
+    p.d = workspace;
+    p.ldd = ldp;
+    hipLaunchKernelGGL((mxfp4_dgrad_kernel<MXQ_DTYPE_F32, true>), dim3(grid), dim3(kDThreads), 0, (hipStream_t)stream, p);
+    *later = {(const float*)workspace, nullptr, dx, M, ldp, K, (int)K, plan.splits, out_dtype};
+    return mxq_check_launch("mxfp4_dgrad_kernel");
+  }
   with_dtype(out_dtype, [&](auto O) {
-    hipLaunchKernelGGL((mxfp4_dgrad_kernel<decltype(O)::value>), grid, dim3(64), 0, (hipStream_t)stream, p);
+    hipLaunchKernelGGL((mxfp4_dgrad_kernel<decltype(O)::value, false>), dim3(grid), dim3(kDThreads), 0, (hipStream_t)stream, p);
   });
   return mxq_check_launch("mxfp4_dgrad_kernel");
 }

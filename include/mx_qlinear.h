@@ -662,6 +662,17 @@ int mxq_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* b, 
                      void* d, int64_t ldd, int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
                      void* stream);
 
+/* Bytes of workspace mxq_mxfp4_linear_prequantized needs at this size on the current device (0 up to 16 rows). */
+int mxq_mxfp4_linear_prequantized_workspace(int64_t M, int64_t N, int64_t K, int direct, int64_t* bytes);
+
+/*
+ * The same of an input that is codes q [M, ldq] and scales [M, lds] already, of any strides and alignment. direct: the product
+ * reads the codes where they are (K % 256 == 0, ldq a multiple of 16 up to 2^22, q 16-byte aligned), else a copy of them.
+ */
+int mxq_mxfp4_linear_prequantized(const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds, int direct, const uint8_t* b,
+                                  int64_t ldb, const uint8_t* sb, const void* bias, void* d, int64_t ldd, int out_dtype, int64_t M,
+                                  int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
+
 /*
  * Bytes of workspace mxq_mxfp4_linear_backward needs at this size on the current device. needs: 1 dx, 2 db, added up; direct as
  * below.

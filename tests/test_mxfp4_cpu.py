@@ -266,6 +266,13 @@ def test_c_products_refuse_before_any_launch():
     few = [*fwd[:10], 3, n, k, None, 0]
     _refused("mxq_mxfp4_linear", few, [(0, None), (1, 4), (2, k - 1), (3, None), (4, 128), (5, None), (7, None), (8, n - 1), (9, 3)])
     _call("mxq_mxfp4_linear", None, 2, k, None, 256, None, None, None, n, 2, 0, n, k, None, 0)
+    _lib.call("mxq_mxfp4_linear_prequantized_workspace", m, n, k, 0, ctypes.byref(need))
+    pre = [OK, 150, OK, 10, 0, OK, 256, OK, None, OK, n, 2, m, n, k, OK, need.value]
+    _refused("mxq_mxfp4_linear_prequantized", pre, [(0, None), (1, 149), (2, None), (3, 9), (4, 1), (5, None), (6, 128), (7, None), (9, None),
+                                                    (10, n - 1), (11, 3), (12, -1), (13, 0), (14, 0), (15, None), (15, OK + 8),
+                                                    (16, need.value - 1)])
+    few = [*pre[:12], 3, n, k, None, 0]
+    _refused("mxq_mxfp4_linear_prequantized", few, [(0, None), (1, 149), (2, None), (3, 9), (5, None), (6, 128), (7, None), (10, n - 1), (11, 3)])
     for dtype, direct, needs in itertools.product((0, 1, 2), (0, 1), (1, 2, 3)):
         _lib.call("mxq_mxfp4_linear_backward_workspace", m, 104, k, dtype, direct if dtype == 2 else 0, needs, ctypes.byref(need))
     _lib.call("mxq_mxfp4_linear_backward_workspace", m, n, k, 0, 0, 3, ctypes.byref(need))

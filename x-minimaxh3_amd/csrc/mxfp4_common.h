@@ -76,10 +76,12 @@ int64_t fp4_dgrad_workspace(int64_t M, int64_t N, int64_t K, int parts);
 int fp4_dgrad(const void* dy, int parts, int64_t ldy, const uint8_t* b, int64_t ldb, const uint8_t* sb, void* dx, int out_dtype,
               int64_t M, int64_t N, int64_t K, void* workspace, SliceJob* later, void* stream);
 
-// The few-row product (mxfp4_rows.hip): up to kFp4FusedRows rows of x_dtype, which it quantizes itself.
+// The few-row product (mxfp4_rows.hip): up to kFp4FusedRows rows of x_dtype, which it quantizes itself, or of codes
+// (MXQ_DTYPE_E2M1) with scales sx, of any strides and alignment.
 constexpr int64_t kFp4FusedRows = 16;
-int fp4_linear_rows(const void* x, int x_dtype, int64_t ldx, const uint8_t* b, int64_t ldb, const uint8_t* sb, const void* bias, void* d,
-                    int64_t ldd, int out_dtype, int64_t M, int64_t N, int64_t K, void* stream);
+int fp4_linear_rows(const void* x, int x_dtype, int64_t ldx, const uint8_t* sx, int64_t ldsx, const uint8_t* b, int64_t ldb,
+                    const uint8_t* sb, const void* bias, void* d, int64_t ldd, int out_dtype, int64_t M, int64_t N, int64_t K,
+                    void* stream);
 
 // Two codes (byte kByte of a word) as float32 (exact).
 template <int kByte>

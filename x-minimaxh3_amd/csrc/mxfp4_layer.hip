@@ -11,12 +11,12 @@ struct Forward {
   void* gemm;
   int64_t ldq, gemm_bytes, total;
 };
-int forward_space(uint8_t* base, int64_t M, int64_t N, int64_t K, Forward& f) {
+int forward_space(uint8_t* base, int64_t M, int64_t N, int64_t K, bool codes, Forward& f) {
   f = {};
   if (M <= kFp4FusedRows) return MXQ_OK;
   Carve c{base};
   f.ldq = fp4_row_bytes(K);
-  f.q = c.take<uint8_t>(M * f.ldq);
+  f.q = c.take<uint8_t>(codes ? M * f.ldq : 0);
   f.s = c.take<uint8_t>(fp4_scale_bytes(M, K));
   if (const int rc = mxq_mxfp4_gemm_workspace(M, N, K, &f.gemm_bytes)) return rc;
   f.gemm = c.take<void>(f.gemm_bytes);
@@ -65,7 +65,7 @@ int check_workspace(const void* workspace, int64_t have, int64_t need) {
 extern "C" int mxq_mxfp4_linear_workspace(int64_t M, int64_t N, int64_t K, int64_t* bytes) {
   if (!sizes_ok(M, N, K) || !bytes) return mxq_set_error(MXQ_ERR_INVALID, "bad argument");
   Forward f;
-  if (const int rc = forward_space(nullptr, M, N, K, f)) return rc;
+  if (const int rc = forward_space(nullptr, M, N, K, true, f)) return rc;
   *bytes = f.total;
   return MXQ_OK;
 }
@@ -79,14 +79,46 @@ extern "C" int mxq_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const u
   if (!float_dtype(x_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported input dtype code %d", x_dtype);
   if (!x || ldx < K) return mxq_set_error(MXQ_ERR_INVALID, "null activations or bad row strides of the activations for K=%lld", (long long)K);
   if (M <= kFp4FusedRows)
-    return fp4_linear_rows(x, x_dtype, ldx, b, ldb, sb, bias, d, ldd, out_dtype, M, N, K, stream);
+    return fp4_linear_rows(x, x_dtype, ldx, nullptr, 0, b, ldb, sb, bias, d, ldd, out_dtype, M, N, K, stream);
   Forward f;
-  if (const int rc = forward_space((uint8_t*)workspace, M, N, K, f)) return rc;
+  if (const int rc = forward_space((uint8_t*)workspace, M, N, K, true, f)) return rc;
   if (const int rc = check_workspace(workspace, workspace_bytes, f.total)) return rc;
   // (every refusal is ahead of the first launch)
   if (const int rc = fp4_gemm_check(f.q, f.ldq, f.s, b, ldb, sb, d, ldd, out_dtype, M, N, K)) return rc;
   if (const int rc = mxq_mxfp4_quantize_rows(x, x_dtype, ldx, f.q, f.ldq, f.s, 0, M, K, stream)) return rc;
   return mxq_mxfp4_gemm(f.q, f.ldq, f.s, b, ldb, sb, bias, d, ldd, out_dtype, M, N, K, f.gemm, f.gemm_bytes, stream);
+}
+
+extern "C" int mxq_mxfp4_linear_prequantized_workspace(int64_t M, int64_t N, int64_t K, int direct, int64_t* bytes) {
+  if (!sizes_ok(M, N, K) || !bytes) return mxq_set_error(MXQ_ERR_INVALID, "bad argument");
+  Forward f;
+  if (const int rc = forward_space(nullptr, M, N, K, !direct, f)) return rc;
+  *bytes = f.total;
+  return MXQ_OK;
+}
+
+extern "C" int mxq_mxfp4_linear_prequantized(const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds, int direct,
+                                             const uint8_t* b, int64_t ldb, const uint8_t* sb, const void* bias, void* d, int64_t ldd,
+                                             int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                                             void* stream) {
+  if (!sizes_ok(M, N, K))
+    return mxq_set_error(MXQ_ERR_INVALID, "bad size M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
+  if (ldq < (K + 1) / 2 || lds < (K + 31) / 32)
+    return mxq_set_error(MXQ_ERR_INVALID, "bad row strides of the activations for K=%lld", (long long)K);
+  if (direct && (K % 256 || ldq % 16 || ldq > (1ll << 22) || reinterpret_cast<uintptr_t>(q) % 16))
+    return mxq_set_error(MXQ_ERR_INVALID, "the product cannot read these codes directly");
+  if (M == 0) return MXQ_OK;
+  if (!q || !scale) return mxq_set_error(MXQ_ERR_INVALID, "null activations");
+  if (M <= kFp4FusedRows)
+    return fp4_linear_rows(q, MXQ_DTYPE_E2M1, ldq, scale, lds, b, ldb, sb, bias, d, ldd, out_dtype, M, N, K, stream);
+  Forward f;
+  if (const int rc = forward_space((uint8_t*)workspace, M, N, K, !direct, f)) return rc;
+  if (const int rc = check_workspace(workspace, workspace_bytes, f.total)) return rc;
+  const uint8_t* a = direct ? q : f.q;
+  const int64_t lda = direct ? ldq : f.ldq;
+  if (const int rc = fp4_gemm_check(a, lda, f.s, b, ldb, sb, d, ldd, out_dtype, M, N, K)) return rc;
+  if (const int rc = mxq_mxfp4_layout(q, ldq, scale, lds, direct ? nullptr : f.q, f.ldq, f.s, M, K, stream)) return rc;
+  return mxq_mxfp4_gemm(a, lda, f.s, b, ldb, sb, bias, d, ldd, out_dtype, M, N, K, f.gemm, f.gemm_bytes, stream);
 }
 
 extern "C" int mxq_mxfp4_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dy_dtype, int direct, int needs, int64_t* bytes) {

@@ -99,6 +99,8 @@ SIGNATURES: dict[str, list] = {
     "mxq_mxfp4_gemm": [_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I, _I64, _I64, _I64, _P, _I64, _P],
     "mxq_mxfp4_linear_workspace": [_I64, _I64, _I64, _P],
     "mxq_mxfp4_linear": [_P, _I, _I64, _P, _I64, _P, _P, _P, _I64, _I, _I64, _I64, _I64, _P, _I64, _P],
+    "mxq_mxfp4_linear_prequantized_workspace": [_I64, _I64, _I64, _I, _P],
+    "mxq_mxfp4_linear_prequantized": [_P, _I64, _P, _I64, _I, _P, _I64, _P, _P, _P, _I64, _I, _I64, _I64, _I64, _P, _I64, _P],
     "mxq_mxfp4_linear_backward_workspace": [_I64, _I64, _I64, _I, _I, _I, _P],
     "mxq_mxfp4_linear_backward": [_P, _I, _I64, _I, _P, _I64, _P, _P, _P, _I, _I64, _I64, _I64, _P, _I64, _P],
     "mxq_rms_norm": [_P, _P, _I, _I64, _I64, _P, _I, _F, _P, _P, _I, _I64, _P, _I64, _P, _I64, _I64, _P],

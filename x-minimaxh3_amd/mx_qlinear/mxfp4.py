@@ -21,7 +21,7 @@ from .ops import _bias, _launch, _out_code, _ptr, _require_gpu
 
 BLOCK = 32
 _CODES, _SCALE = torch.float4_e2m1fn_x2, torch.float8_e8m0fnu
-_MAX_STRIDE = 1 << 22  # bytes, of an operand's rows; wider ones are copied
+_MAX_STRIDE = 1 << 22  # bytes, of rows of codes that the product reads in place
 _MAX_GRAD_STRIDE = 1 << 24  # below it, of the rows that the input's gradient reads in place
 
 
@@ -58,20 +58,6 @@ def _pair(q: torch.Tensor, scale: torch.Tensor, width: int | None, what: str = "
     if scale.stride(1) != 1 or (scale.shape[0] > 1 and scale.stride(0) < kb):
         scale = scale.contiguous()
     return q, scale, q.shape[0], k
-
-
-def _operand(q: torch.Tensor, scale: torch.Tensor, k: int):
-    """A pair as the products read it: code rows of whole 128 bytes, zeros behind column ``k``, and scales in tiles. Codes of
-    whole 256 columns in 16-byte rows pass as they are; others are copied."""
-    m, dev = q.shape[0], q.device
-    ldq = q.stride(0) if m > 1 else q.shape[1]
-    tiles = torch.empty(_scale_bytes(m, k), dtype=torch.uint8, device=dev)
-    in_place = k % 256 == 0 and ldq % 16 == 0 and q.data_ptr() % 16 == 0 and ldq <= _MAX_STRIDE
-    out = None if in_place else torch.empty(m, _row_bytes(k), dtype=torch.uint8, device=dev)
-    if m:
-        _launch(dev, "mxq_mxfp4_layout", q.data_ptr(), ldq, scale.data_ptr(), scale.stride(0) if m > 1 else scale.shape[1], _ptr(out),
-                0 if out is None else out.shape[1], tiles.data_ptr(), m, k)
-    return (q, ldq, tiles) if in_place else (out, out.shape[1], tiles)
 
 
 # ---------------------------------------------------------------------------------------
@@ -211,7 +197,7 @@ def mxfp4_linear(x: torch.Tensor, weight: PreparedMxfp4Weight, bias: torch.Tenso
 
 def mxfp4_linear_prequantized(q: torch.Tensor, scale: torch.Tensor, weight: PreparedMxfp4Weight, bias: torch.Tensor | None = None,
                               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """:func:`mxfp4_linear` of an input that is a ``(codes, scale)`` pair already."""
+    """:func:`mxfp4_linear` of an input that is a ``(codes, scale)`` pair already; up to 16 rows are one launch."""
     if not isinstance(weight, PreparedMxfp4Weight):
         raise TypeError(f"weight must come from prepare_mxfp4_weight, got {type(weight).__name__}")
     lead = q.shape[:-1]
@@ -222,11 +208,13 @@ def mxfp4_linear_prequantized(q: torch.Tensor, scale: torch.Tensor, weight: Prep
     bias = _bias(bias, n, out_dtype, dev)
     out = torch.empty(m, n, dtype=out_dtype, device=dev)
     if m:
-        a, lda, sa = _operand(q, scale, k)
-        need = _workspace("mxq_mxfp4_gemm_workspace", dev.index, m, n, k)
+        ldq = q.stride(0) if m > 1 else q.shape[1]
+        direct = k % 256 == 0 and ldq % 16 == 0 and ldq <= _MAX_STRIDE and q.data_ptr() % 16 == 0
+        need = _workspace("mxq_mxfp4_linear_prequantized_workspace", dev.index, m, n, k, direct)
         ws = _room(need, dev)
-        _launch(dev, "mxq_mxfp4_gemm", a.data_ptr(), lda, sa.data_ptr(), weight.q.data_ptr(), weight.q.shape[1], weight.scale.data_ptr(),
-                _ptr(bias), out.data_ptr(), n, code, m, n, k, _ptr(ws), need)
+        _launch(dev, "mxq_mxfp4_linear_prequantized", q.data_ptr(), ldq, scale.data_ptr(), scale.stride(0) if m > 1 else scale.shape[1],
+                direct, weight.q.data_ptr(), weight.q.shape[1], weight.scale.data_ptr(), _ptr(bias), out.data_ptr(), n, code, m, n, k,
+                _ptr(ws), need)
     return out if len(lead) == 1 else out.reshape(*lead, n)
 
 

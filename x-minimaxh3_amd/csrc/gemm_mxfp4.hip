@@ -37,105 +37,77 @@ struct Fp4Gemm {
   int vec;                   // rows of d are 16-byte aligned
 };
 
-// The 16 bytes (a block) of each of kCount 32-row blocks that a lane feeds the matrix instructions of half stage `half`: row
-// l % 32, pieces 4 (l / 32) + 2 half and the next.
-template <int kCount>
-MXQ_DEVICE void read_frags(uint32_t slot, int row, int lane, int half, v4i (&f)[kCount][2]) {
-  const int lr = lane & 31, c = (lane >> 5) * 4 + half * 2;
-  const uint32_t at = slot + (uint32_t)((row + lr) * kStageK);
-  const uint32_t x0 = at + (uint32_t)((c ^ swizzle(lr)) << 4), x1 = at + (uint32_t)(((c + 1) ^ swizzle(lr)) << 4);
-  static_for<kCount>([&](auto I) {
-    constexpr int i = decltype(I)::value;
-    f[i][0] = lds_read_b128<i * 32 * kStageK>(x0);
-    f[i][1] = lds_read_b128<i * 32 * kStageK>(x1);
-  });
-}
+// A workgroup's tile: four waves, each half of its rows and columns.
+template <int kTM>
+struct Fp4Tile {
+  static constexpr int kBM = kTM, kBI = kTM / 64, kBJ = 4;         // 32-row blocks of a wave
+  static constexpr int kLoadsA = kTM / 32, kLoadsB = kTileN / 32;  // 1 KB loads per wave and chunk
+  static constexpr int kScales = kBI + kBJ;                        // scale loads per wave and two stages
+};
 
 // acc += (b * 2^(sb - 127)) (a * 2^(sa - 127))^T over a block of each half of the lanes; the scales are byte kByte. Written as
-// assembly with the sum in place (see gemm_fp8.hip): two wait states between a vector instruction's write of an operand and
-// its read (s_nop), and mfma_drain before the sums are read.
+// assembly with the sum in place (see gemm_fp8.hip), in the accumulation registers: two wait states between a vector
+// instruction's write of an operand and its read (s_nop), and mfma_drain before the sums are read.
 template <int kByte>
 MXQ_DEVICE void mfma_fp4(v16f& acc, v4i b, v4i a, uint32_t sb, uint32_t sa) {
   if constexpr (kByte == 0)
     __asm__ volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
-                     : "+v"(acc)
+                     : "+a"(acc)
                      : "v"(b), "v"(a), "v"(sb), "v"(sa));
   else if constexpr (kByte == 1)
     __asm__ volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4"
-                     : "+v"(acc)
+                     : "+a"(acc)
                      : "v"(b), "v"(a), "v"(sb), "v"(sa));
   else if constexpr (kByte == 2)
     __asm__ volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[1,1,0] cbsz:4 blgp:4"
-                     : "+v"(acc)
+                     : "+a"(acc)
                      : "v"(b), "v"(a), "v"(sb), "v"(sa));
   else
     __asm__ volatile("s_nop 1\n\tv_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[1,1,0] cbsz:4 blgp:4"
-                     : "+v"(acc)
+                     : "+a"(acc)
                      : "v"(b), "v"(a), "v"(sb), "v"(sa));
 }
 
-// A wave's scale words of a stage: its rows' and its columns'.
-template <class C>
-struct Words {
-  uint32_t a[C::kBI], b[C::kBJ];
-};
-// ... and of two stages, as loaded.
+// A wave's scale words of two stages, its rows' and its columns', as loaded.
 template <class C>
 struct WordPairs {
   v2u a[C::kBI], b[C::kBJ];
 };
-
-// The matrix instructions of a half stage. They compute D^T blocks (B first): lane l holds row l % 32 of D and, in
-// register r, column (r / 4) * 8 + (l / 32) * 4 + r % 4.
-template <class C, int kHalf>
-MXQ_DEVICE void half_stage(const v4i (&fa)[C::kBI][2], const v4i (&fb)[C::kBJ][2], const Words<C>& s, v16f (&acc)[C::kBI][C::kBJ]) {
-  static_for<2>([&](auto T) {
-    constexpr int t = decltype(T)::value;
-#pragma unroll
-    for (int i = 0; i < C::kBI; ++i)
-#pragma unroll
-      for (int j = 0; j < C::kBJ; ++j) mfma_fp4<kHalf * 2 + t>(acc[i][j], fb[j][t], fa[i][t], s.b[j], s.a[i]);
-  });
-}
-
 template <class C>
 struct ScaleSource {
   const uint8_t *a, *b;
-  int bytes_a, bytes_b;
-  uint32_t off_a[C::kBI], off_b[C::kBJ];
+  int bytes_a, bytes_b, row_tiles;
+  uint32_t off_a, off_b;  // of the wave's first 32 rows; the next ones are row_tiles further on
 };
 MXQ_DEVICE v2u buffer_load_x2(const void* base, int bytes, uint32_t voff, int soff) {
   return __builtin_bit_cast(v2u, __builtin_amdgcn_raw_buffer_load_b64(
                                      __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, kRawBufferWord3),
                                      (int)voff, soff, 0));
 }
-template <class C>
-MXQ_DEVICE void load_scales(const ScaleSource<C>& s, int stage, WordPairs<C>& w) {
+// Scale load t: of the 32-row blocks of A, then of B.
+template <class C, int kT>
+MXQ_DEVICE void load_scale(const ScaleSource<C>& s, int stage, WordPairs<C>& w) {
   const int at = (stage >> 1) * (int)kFp4ScaleTile;
-#pragma unroll
-  for (int i = 0; i < C::kBI; ++i) w.a[i] = buffer_load_x2(s.a, s.bytes_a, s.off_a[i], at);
-#pragma unroll
-  for (int j = 0; j < C::kBJ; ++j) w.b[j] = buffer_load_x2(s.b, s.bytes_b, s.off_b[j], at);
+  if constexpr (kT < C::kBI)
+    w.a[kT] = buffer_load_x2(s.a, s.bytes_a, s.off_a, at + kT * s.row_tiles);
+  else
+    w.b[kT - C::kBI] = buffer_load_x2(s.b, s.bytes_b, s.off_b, at + (kT - C::kBI) * s.row_tiles);
 }
 
-// One group's whole main loop over stages [0, n) (kG = 0: waves 0-3, 1: waves 4-7). The operand chunks A_0 B_0 A_1
-// B_1 ... go to slot (chunk index) % 5. Iteration kt has four phases, a workgroup barrier behind each; group g computes
-// in phases 2 q + g and reads in the others:
-//   P0  g0: first half of kt      g1: reads (kt, 0), loads A_kt+2 into B_kt-1's slot
-//   P1  g1: first half            g0: reads (kt, 1), loads A_kt+2
-//   P2  g0: second half           g1: reads (kt, 1)          both then wait for stage kt+1
-//   P3  g1: second half + loads   g0: reads (kt+1, 0), loads B_kt+2 into A_kt's slot
-//       of B_kt+2
-// The scale words of stages 2 g and 2 g + 1 are requested with the B loads of iteration 2 g - 2, so the next iteration's wait
-// covers them.
-template <class C, int kG>
+// The whole main loop of a wave over stages [0, n). The operand chunks A_0 B_0 A_1 B_1 ... go to slot (chunk index) % 5. A stage is
+// four steps, one block of each half of the lanes (pieces 4 (l / 32) + step of a row's 128 bytes); a step is kBI * 4 slots, each
+// one matrix instruction and a part of the other work in the order written (sched_barrier): the fragments of the next step, one
+// ahead; during steps 0 and 1 the loads of A_s+2 into B_s-1's slot; during step 2 of every other stage the scale words of the next
+// two; then, ahead of step 3, whose reads are the next stage's, the wait for that stage and the workgroup's barrier, behind which
+// nobody reads this one; and during step 3 the loads of B_s+2 into A_s's slot.
+template <class C>
 MXQ_DEVICE void main_loop(char* lds, const Chunk<C::kLoadsA>& ca, const Chunk<C::kLoadsB>& cb, const ScaleSource<C>& ss,
                           int n, int wrow, int wcol, int lane, v16f (&acc)[C::kBI][C::kBJ]) {
+  constexpr int kSlots = C::kBI * C::kBJ, kReads = C::kBI + C::kBJ;
+  constexpr int kReadSlots = kSlots * 3 / 4;  // the reads end early: the next step's first instruction waits for them
   const uint32_t base = lds_addr(lds);
-  auto slot_addr = [&](int s) { return base + (uint32_t)(s * kSlot); };
-  Words<C> cur;
-  WordPairs<C> next;
-  load_scales(ss, 0, next);
+  WordPairs<C> cur, next;
+  static_for<C::kScales>([&](auto T) { load_scale<C, decltype(T)::value>(ss, 0, next); });
   __builtin_amdgcn_sched_barrier(0);
   issue_chunk(ca, lds, 0, true);
   issue_chunk(cb, lds + kSlot, 0, true);
@@ -145,109 +117,123 @@ MXQ_DEVICE void main_loop(char* lds, const Chunk<C::kLoadsA>& ca, const Chunk<C:
     wait_vmcnt<C::kLoadsA + C::kLoadsB>();
   else
     wait_vmcnt<0>();
-  auto take = [&](Words<C>& w, bool second) {
+  phase_barrier();
+  // The 16 bytes of row (l % 32) of a 32-row block that a lane feeds step j.
+  uint32_t piece[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) piece[j] = base + (uint32_t)((lane & 31) * kStageK + ((((lane >> 5) * 4 + j) ^ swizzle(lane & 31)) << 4));
+  v4i fa[2][C::kBI], fb[2][C::kBJ];
+  auto read = [&](auto SetC, auto IC, uint32_t at_a, uint32_t at_b) {  // in the order of their use: A_0, B_0 .., A_1 ..
+    constexpr int kSet = decltype(SetC)::value, kI = decltype(IC)::value;
+    if constexpr (kI == 0)
+      fa[kSet][0] = lds_read_b128<0>(at_a);
+    else if constexpr (kI <= C::kBJ)
+      fb[kSet][kI - 1] = lds_read_b128<(kI - 1) * 32 * kStageK>(at_b);
+    else
+      fa[kSet][kI - C::kBJ] = lds_read_b128<(kI - C::kBJ) * 32 * kStageK>(at_a);
+  };
+  const uint32_t row_a = (uint32_t)(wrow * kStageK), row_b = (uint32_t)(wcol * kStageK);
+  static_for<kReads>([&](auto I) { read(std::integral_constant<int, 0>{}, I, piece[0] + row_a, piece[0] + row_b + kSlot); });
+  auto take = [&] {  // the words requested two stages ago
 #pragma unroll
     for (int i = 0; i < C::kBI; ++i) {
-      w.a[i] = second ? next.a[i][1] : next.a[i][0];
-      __asm__ volatile("" : "+v"(w.a[i]));
+      cur.a[i] = next.a[i];
+      __asm__ volatile("" : "+v"(cur.a[i]));
     }
 #pragma unroll
     for (int j = 0; j < C::kBJ; ++j) {
-      w.b[j] = second ? next.b[j][1] : next.b[j][0];
-      __asm__ volatile("" : "+v"(w.b[j]));
+      cur.b[j] = next.b[j];
+      __asm__ volatile("" : "+v"(cur.b[j]));
     }
   };
-  take(cur, false);
-  phase_barrier();
-  v4i fa[C::kBI][2], fb[C::kBJ][2];
-  if constexpr (kG == 0) {
-    read_frags<C::kBI>(slot_addr(0), wrow, lane, 0, fa);
-    read_frags<C::kBJ>(slot_addr(1), wcol, lane, 0, fb);
-    wait_lgkm<0>();
-  }
-  phase_barrier();
+  take();
 
-  int sa = 0;  // slot of A_kt; B_kt is in the next one
-  auto iteration = [&](int kt, auto SteadyC) {
-    constexpr bool kSteady = decltype(SteadyC)::value;  // stage kt + 2 exists
+  int sa = 0;  // slot of A_s; B_s is in the next one
+  // kSecond: the second of two stages; kSteady: stages s + 1 and s + 2 (and the second's next words) exist
+  auto stage = [&](int s, auto SecondC, auto SteadyC) {
+    constexpr int kP = decltype(SecondC)::value;
+    constexpr bool kSteady = decltype(SteadyC)::value;
     const int sb = sa == kRing - 1 ? 0 : sa + 1;
     const int na = sb == kRing - 1 ? 0 : sb + 1;
     const int nb = na == kRing - 1 ? 0 : na + 1;
     const int pa = sa == 0 ? kRing - 1 : sa - 1;
-    const bool more = kSteady || kt + 2 < n;
-    char* slot_pa = lds + pa * kSlot;
-    char* slot_sa = lds + sa * kSlot;
-    auto next_scales = [&] {
-      if ((kt & 1) == 0 && more) load_scales(ss, kt + 2, next);
-    };
-    if constexpr (kG == 0) {
-      half_stage<C, 0>(fa, fb, cur, acc);  // P0
-      phase_barrier();
-      read_frags<C::kBI>(slot_addr(sa), wrow, lane, 1, fa);  // P1
-      read_frags<C::kBJ>(slot_addr(sb), wcol, lane, 1, fb);
-      issue_chunk(ca, slot_pa, kt + 2, more);
+    const bool more = kSteady || s + 2 < n;
+    static_for<4>([&](auto H) {
+      constexpr int h = decltype(H)::value, kSet = h & 1;
+      if constexpr (h == 3) {
+        // stage s + 1 has landed: only A_s+2 and the words (when there are any) were issued after it
+        if constexpr (kSteady)
+          wait_vmcnt<C::kLoadsA + (kP == 0 ? C::kScales : 0)>();
+        else
+          wait_vmcnt<0>();
+      }
       wait_lgkm<0>();
-      phase_barrier();
-      half_stage<C, 1>(fa, fb, cur, acc);  // P2
-    } else {
-      read_frags<C::kBI>(slot_addr(sa), wrow, lane, 0, fa);  // P0
-      read_frags<C::kBJ>(slot_addr(sb), wcol, lane, 0, fb);
-      issue_chunk(ca, slot_pa, kt + 2, more);
-      wait_lgkm<0>();
-      phase_barrier();
-      half_stage<C, 0>(fa, fb, cur, acc);  // P1
-      phase_barrier();
-      read_frags<C::kBI>(slot_addr(sa), wrow, lane, 1, fa);  // P2
-      read_frags<C::kBJ>(slot_addr(sb), wcol, lane, 1, fb);
-      wait_lgkm<0>();
-    }
-    // stage kt + 1 has landed: only A_kt+2 (when it exists) was issued after it
-    if (more)
-      wait_vmcnt<C::kLoadsA>();
-    else
-      wait_vmcnt<0>();
-    // The words requested an iteration ago have landed with it: the next stage's are taken here, ahead of the next request
-    // (behind it, the compiler would wait for that one).
-    Words<C> after;
-    take(after, (kt & 1) == 0);
-    phase_barrier();
-    if constexpr (kG == 0) {
-      // P3 (at the last stage these reads fetch slots nobody uses)
-      read_frags<C::kBI>(slot_addr(na), wrow, lane, 0, fa);
-      read_frags<C::kBJ>(slot_addr(nb), wcol, lane, 0, fb);
-      next_scales();
-      issue_chunk(cb, slot_sa, kt + 2, more);
-      wait_lgkm<0>();
-    } else {
-      next_scales();
-      issue_chunk(cb, slot_sa, kt + 2, more);
-      half_stage<C, 1>(fa, fb, cur, acc);  // P3
-    }
-    phase_barrier();
-    cur = after;
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (h == 3) phase_barrier();
+      const uint32_t at = piece[(h + 1) & 3];
+      const uint32_t at_a = at + row_a + (uint32_t)((h < 3 ? sa : na) * kSlot), at_b = at + row_b + (uint32_t)((h < 3 ? sb : nb) * kSlot);
+      static_for<kSlots>([&](auto G) {
+        constexpr int g = decltype(G)::value, i = g / C::kBJ, j = g % C::kBJ;
+        mfma_fp4<h>(acc[i][j], fb[kSet][j], fa[kSet][i], cur.b[j][kP], cur.a[i][kP]);
+        static_for<kReads>([&](auto I) {
+          if constexpr (decltype(I)::value * kReadSlots / kReads == g) read(std::integral_constant<int, kSet ^ 1>{}, I, at_a, at_b);
+        });
+        if constexpr (h < 2) {
+          constexpr int kHalf = C::kLoadsA / 2;
+          static_for<kHalf>([&](auto T) {
+            if constexpr (decltype(T)::value * kSlots / kHalf == g)
+              if (more) issue_load(ca, lds + pa * kSlot, s + 2, h * kHalf + decltype(T)::value);
+          });
+        } else if constexpr (h == 2 && kP == 0) {
+          static_for<C::kScales>([&](auto T) {
+            if constexpr (decltype(T)::value * kSlots / C::kScales == g)
+              if (more) load_scale<C, decltype(T)::value>(ss, s + 2, next);
+          });
+        } else if constexpr (h == 3) {
+          static_for<C::kLoadsB>([&](auto T) {
+            if constexpr (decltype(T)::value * kSlots / C::kLoadsB == g)
+              if (more) issue_load(cb, lds + sa * kSlot, s + 2, decltype(T)::value);
+          });
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    });
     sa = na;
   };
-  int kt = 0;
-  for (; kt + 2 < n; ++kt) iteration(kt, std::true_type{});
-  do {
-    iteration(kt, std::false_type{});
-  } while (++kt < n);
+  const std::integral_constant<int, 0> first{};
+  const std::integral_constant<int, 1> second{};
+  int s = 0;
+  for (; s + 3 < n; s += 2) {
+    stage(s, first, std::true_type{});
+    stage(s + 1, second, std::true_type{});
+    take();
+  }
+  for (; s < n; s += 2) {
+    stage(s, first, std::false_type{});
+    if (s + 1 < n) stage(s + 1, second, std::false_type{});
+    take();
+  }
+  wait_lgkm<0>();  // (the last step's reads, of slots nobody uses)
+#pragma unroll
+  for (int i = 0; i < C::kBI; ++i) __asm__ volatile("" ::"v"(fa[0][i]));
+#pragma unroll
+  for (int j = 0; j < C::kBJ; ++j) __asm__ volatile("" ::"v"(fb[0][j]));
   mfma_drain();
+  phase_barrier();
 }
 
 template <int kTM, int kOut, bool kSplit>
-__global__ __launch_bounds__(512, 2) void gemm_mxfp4_kernel(Fp4Gemm p) {
-  typedef Tile<kTM> C;
+__global__ __launch_bounds__(256, 1) void gemm_mxfp4_kernel(Fp4Gemm p) {
+  typedef Fp4Tile<kTM> C;
   __shared__ __attribute__((aligned(1024))) char lds[kGemmLds];
   int tm, tn, slice;
   tile_of(blockIdx.x, p, tm, tn, slice);
   const int M = (int)p.M, N = (int)p.N, m0 = tm * kTM, n0 = tn * kTileN;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  // waves w and w + 4 share a SIMD: the two 64-column halves of quadrant w % 4
-  const int wrow = ((wave & 3) >> 1) * C::kWaveM, wcol = (wave & 1) * 128 + (wave >> 2) * 64;
+  const int wrow = (wave >> 1) * (kTM / 2), wcol = (wave & 1) * (kTileN / 2);
   const int first = slice * p.split_stages, n = min(p.split_stages, p.stages - first);
-  const auto ca = make_chunk<C::kLoadsA>(p.a + (int64_t)first * kStageK, p.lda, m0, M, wave, lane);
-  const auto cb = make_chunk<C::kLoadsB>(p.b + (int64_t)first * kStageK, p.ldb, n0, N, wave, lane);
+  const auto ca = make_chunk<C::kLoadsA, 4>(p.a + (int64_t)first * kStageK, p.lda, m0, M, wave, lane);
+  const auto cb = make_chunk<C::kLoadsB, 4>(p.b + (int64_t)first * kStageK, p.ldb, n0, N, wave, lane);
   // (a row of scale tiles holds 32 rows; behind the operands' last one, reads give zeros)
   ScaleSource<C> ss;
   const int row_tiles = p.groups * (int)kFp4ScaleTile, skip = (first >> 1) * (int)kFp4ScaleTile;
@@ -255,15 +241,11 @@ __global__ __launch_bounds__(512, 2) void gemm_mxfp4_kernel(Fp4Gemm p) {
   ss.b = p.sb + (int64_t)(n0 >> 5) * row_tiles + skip;
   ss.bytes_a = ((min(M - m0, kTM) + 31) >> 5) * row_tiles - skip;
   ss.bytes_b = ((min(N - n0, kTileN) + 31) >> 5) * row_tiles - skip;
-#pragma unroll
-  for (int i = 0; i < C::kBI; ++i) ss.off_a[i] = (uint32_t)(((wrow >> 5) + i) * row_tiles + lane * 8);
-#pragma unroll
-  for (int j = 0; j < C::kBJ; ++j) ss.off_b[j] = (uint32_t)(((wcol >> 5) + j) * row_tiles + lane * 8);
+  ss.row_tiles = row_tiles;
+  ss.off_a = (uint32_t)((wrow >> 5) * row_tiles + lane * 8);
+  ss.off_b = (uint32_t)((wcol >> 5) * row_tiles + lane * 8);
   v16f acc[C::kBI][C::kBJ] = {};
-  if (wave < 4)
-    main_loop<C, 0>(lds, ca, cb, ss, n, wrow, wcol, lane, acc);
-  else
-    main_loop<C, 1>(lds, ca, cb, ss, n, wrow, wcol, lane, acc);
+  main_loop<C>(lds, ca, cb, ss, n, wrow, wcol, lane, acc);
   void* d = p.d;
   if constexpr (kSplit) d = reinterpret_cast<float*>(p.d) + slice * p.M * p.ldd;
   epilogue<C, kOut, kSplit>(p, lds, acc, m0, n0, wrow, wcol, wave, lane, d);
@@ -322,7 +304,7 @@ int mxq::fp4_gemm_check(const uint8_t* a, int64_t lda, const uint8_t* sa, const 
 
 template <int kTM, int kOut, bool kSplit>
 static int launch_gemm(const Fp4Gemm& p, void* stream) {
-  hipLaunchKernelGGL((gemm_mxfp4_kernel<kTM, kOut, kSplit>), dim3((unsigned)(p.tiles_m * p.tiles_n * p.splits)), dim3(512), 0,
+  hipLaunchKernelGGL((gemm_mxfp4_kernel<kTM, kOut, kSplit>), dim3((unsigned)(p.tiles_m * p.tiles_n * p.splits)), dim3(256), 0,
                      (hipStream_t)stream, p);
   return mxq_check_launch("gemm_mxfp4_kernel");
 }

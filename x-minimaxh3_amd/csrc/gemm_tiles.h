@@ -33,10 +33,10 @@ struct Chunk {
 
 // (Rows are counted in 32 bits: a buffer resource has to be in scalar registers, and there is no scalar 64-bit minimum.
 // Computed in vector registers, it made every access loop over the lanes' resources.)
-template <int kLoads>
+template <int kLoads, int kWaves = 8>
 MXQ_DEVICE Chunk<kLoads> make_chunk(const uint8_t* p, int64_t ld, int row0, int rows, int wave, int lane) {
   Chunk<kLoads> c;
-  const int valid = min(rows - row0, kLoads * 64);
+  const int valid = min(rows - row0, kLoads * 8 * kWaves);
   c.base = p + row0 * ld;
   c.bytes = valid * (int)ld;
   c.wave = wave;
@@ -48,12 +48,17 @@ MXQ_DEVICE Chunk<kLoads> make_chunk(const uint8_t* p, int64_t ld, int row0, int 
   return c;
 }
 
+// Load t of a chunk.
+template <int kLoads>
+MXQ_DEVICE void issue_load(const Chunk<kLoads>& c, char* slot, int stage, int t) {
+  buffer_load_lds16(c.base, c.bytes, (lptr_t)(slot + (c.wave * kLoads + t) * 1024), c.off[t], stage * kStageK);
+}
+
 template <int kLoads>
 MXQ_DEVICE void issue_chunk(const Chunk<kLoads>& c, char* slot, int stage, bool on) {
   if (on) {
 #pragma unroll
-    for (int t = 0; t < kLoads; ++t)
-      buffer_load_lds16(c.base, c.bytes, (lptr_t)(slot + (c.wave * kLoads + t) * 1024), c.off[t], stage * kStageK);
+    for (int t = 0; t < kLoads; ++t) issue_load(c, slot, stage, t);
   }
 }
 
@@ -105,7 +110,7 @@ MXQ_DEVICE void epilogue(const P& p, char* lds, const v16f (&acc)[C::kBI][C::kBJ
 #pragma unroll
     for (int j = 0; j < C::kBJ; ++j) {
       const int col0 = n0 + wcol + j * 32;
-      if (kElem == 4 || j == 0) wave_lds_fence();  // the piece before has been read
+      if (kElem == 4 || (j & 1) == 0) wave_lds_fence();  // the piece before has been read
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int col = col0 + q * 8 + lh * 4;
@@ -118,13 +123,13 @@ MXQ_DEVICE void epilogue(const P& p, char* lds, const v16f (&acc)[C::kBI][C::kBJ
         } else if constexpr (kElem == 4) {
           *reinterpret_cast<v4f*>(out_stage_at(buf, lr, 2 * q + lh)) = v4f{y[0], y[1], y[2], y[3]};
         } else {
-          *reinterpret_cast<v2u*>(out_stage_at(buf, lr, j * 4 + q) + lh * 8) =
+          *reinterpret_cast<v2u*>(out_stage_at(buf, lr, (j & 1) * 4 + q) + lh * 8) =
               v2u{out_pair<kOut>(y[0], y[1]), out_pair<kOut>(y[2], y[3])};
         }
       }
-      if (lines && (kElem == 4 || j == C::kBJ - 1)) {
+      if (lines && (kElem == 4 || (j & 1) == 1)) {
         wave_lds_fence();
-        const int64_t byte0 = (int64_t)(kElem == 4 ? col0 : n0 + wcol) * kElem;
+        const int64_t byte0 = (int64_t)(kElem == 4 ? col0 : col0 - 32) * kElem;
         v4u v[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) v[t] = *reinterpret_cast<const v4u*>(out_stage_at(buf, t * 8 + (lane >> 3), lane & 7));

@@ -258,18 +258,24 @@ struct Fp4Plan {
   double cost;
 };
 
-// Tile rows and K slices, by an estimate in microseconds: a round of workgroups takes 5 for its first loads and its epilogue and
-// 1.0 (256 rows) or 0.55 (128 rows) per stage, all rounds at least the weight's bytes; slices cost a join.
+// Tile rows and K slices, by an estimate in microseconds: a round of workgroups takes 6 (256 rows) or 4.5 (128 rows) for its first
+// loads and its epilogue and, per stage, 0.94 or 0.64 where few CUs are at work, 1.6 or 1.0 (power) where all are; all rounds
+// take at least the weight's bytes, slices cost a join. Both sides measured, whole and with the layout's launch: 8192 rows, K 20480,
+// N 5120: 378 us of 256 rows, 413 of 128; 1024 rows, K 5120, N 20480: 71.4 and 66.9; 333 rows, K 20480, N 5120: four slices of 128
+// rows 33.9, whole 62.9; 700 rows, K 5120, N 5120: 128 rows whole 24.9, two slices 27.5, 256 rows 35.
 static Fp4Plan plan_fp4(int64_t M, int64_t N, int64_t stages, int cus) {
   Fp4Plan best = {256, 1, (int)((stages + 1) / 2 * 2), 1e300};
   const double stream = (double)(N * stages) * 136.0 / 4.9e6 + 2.0;
   for (int tile = 256; tile >= 128; tile /= 2) {
     const int64_t tiles = (M + tile - 1) / tile * ((N + kTileN - 1) / kTileN);
+    const double alone = tile == 256 ? 0.94 : 0.64, all = tile == 256 ? 1.6 : 1.0, ends = tile == 256 ? 6.0 : 4.5;
     for (int64_t s = 1; s <= 32; ++s) {
       const int64_t per = ((stages + s - 1) / s + 1) / 2 * 2, splits = (stages + per - 1) / per;
       if (splits != s || (s > 1 && tiles * s > 4 * cus)) continue;
-      const double rounds = (double)((tiles * s + cus - 1) / cus);
-      double cost = rounds * ((double)(per < stages ? per : stages) * (tile == 256 ? 1.0 : 0.55) + 5.0);
+      const double n = (double)(per < stages ? per : stages);
+      const int64_t full = tiles * s / cus;
+      const double rest = (double)(tiles * s % cus) / cus;
+      double cost = (double)full * (n * all + ends) + (rest > 0.0 ? n * (alone + (all - alone) * rest) + ends : 0.0);
       if (cost < stream) cost = stream;
       cost += slices_cost(s, M * N);
       if (cost < best.cost) best = {tile, (int)s, (int)per, cost};

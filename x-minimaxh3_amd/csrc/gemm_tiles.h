@@ -79,7 +79,8 @@ MXQ_DEVICE void phase_barrier() {
 
 // ---- epilogue ----
 // A wave passes its output through 4 KB of LDS in pieces of 32 rows x 128 bytes (32-row block i, one or two column
-// blocks), so that eight lanes store a whole line.
+// blocks), so that eight lanes store a whole line, or, where rows are not 16-byte aligned or the tile is an edge's, 16 bytes
+// a lane from any address (lane by lane straight from the sums, 1024 rows x 2049 columns took 8 us longer).
 MXQ_DEVICE char* out_stage_at(char* buf, int r, int c) { return buf + r * 128 + ((c ^ ((r >> 1) & 7)) << 4); }
 
 template <int kOut>
@@ -113,30 +114,43 @@ MXQ_DEVICE void epilogue(const P& p, char* lds, const v16f (&acc)[C::kBI][C::kBJ
       if (kElem == 4 || (j & 1) == 0) wave_lds_fence();  // the piece before has been read
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int col = col0 + q * 8 + lh * 4;
         float y[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = kSplit ? acc[i][j][q * 4 + e] : acc[i][j][q * 4 + e] + bias[kSplit ? 0 : j][q][e];
-        if (!lines) {
-          const int row = row0 + lr;
-          if (row < M) store_run4<kOut>(out + row * p.ldd * kElem, col, N - col, y);
-        } else if constexpr (kElem == 4) {
+        if constexpr (kElem == 4) {
           *reinterpret_cast<v4f*>(out_stage_at(buf, lr, 2 * q + lh)) = v4f{y[0], y[1], y[2], y[3]};
         } else {
           *reinterpret_cast<v2u*>(out_stage_at(buf, lr, (j & 1) * 4 + q) + lh * 8) =
               v2u{out_pair<kOut>(y[0], y[1]), out_pair<kOut>(y[2], y[3])};
         }
       }
-      if (lines && (kElem == 4 || (j & 1) == 1)) {
+      if (kElem == 4 || (j & 1) == 1) {
         wave_lds_fence();
-        const int64_t byte0 = (int64_t)(kElem == 4 ? col0 : col0 - 32) * kElem;
+        constexpr int kRun = 16 / kElem;
+        const int col = (kElem == 4 ? col0 : col0 - 32) + (lane & 7) * kRun;
         v4u v[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) v[t] = *reinterpret_cast<const v4u*>(out_stage_at(buf, t * 8 + (lane >> 3), lane & 7));
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-          __builtin_nontemporal_store(
-              v[t], reinterpret_cast<v4u*>(out + (row0 + t * 8 + (lane >> 3)) * p.ldd * kElem + byte0 + (lane & 7) * 16));
+        for (int t = 0; t < 4; ++t) {
+          const int row = row0 + t * 8 + (lane >> 3);
+          char* to = out + (row * p.ldd + col) * kElem;
+          if (lines) {
+            __builtin_nontemporal_store(v[t], reinterpret_cast<v4u*>(to));
+          } else if (row < M) {
+            const int n = N - col;
+            if (n >= kRun) {
+              *reinterpret_cast<v4u_any*>(to) = v[t];
+            } else {
+#pragma unroll
+              for (int e = 0; e < kRun; ++e)
+                if (e < n) {
+                  if constexpr (kElem == 4) reinterpret_cast<uint32_t*>(to)[e] = v[t][e];
+                  else reinterpret_cast<uint16_t*>(to)[e] = (uint16_t)(v[t][e >> 1] >> (16 * (e & 1)));
+                }
+            }
+          }
+        }
       }
     }
   }

@@ -7,7 +7,6 @@
 // them on the way, which saves the quantizer's launch. How many weight rows a workgroup takes decides (plan_rows): each
 // workgroup quantizes all of x again, and what counts is the CU with the most weight rows.
 #include <algorithm>
-#include <cmath>
 
 #include "mxfp4_common.h"
 
@@ -177,23 +176,28 @@ __global__ __launch_bounds__(512) void mxfp4_rows_kernel(Fp4Rows p) {
   }
 }
 
-// Weight rows (in sixteens) and waves of a workgroup, by an estimate in microseconds: the CU with the most workgroups (rounds)
-// streams its weight rows, 0.09 per sixteen and stage with every CU at work (less where some are idle), and quantizes x for
-// each workgroup, 0.008 per row and stage. Workgroups of four waves share a CU, so that the last round counts half; those of
-// eight take 1 us more to start and end and reach more of a lone CU's rate.
+// Weight rows (in sixteens) and waves of a workgroup, by an estimate in microseconds: the CU with the most workgroups streams their
+// weight rows, 0.090 (four waves) or 0.079 (eight) per sixteen and stage, all CUs together at 5.2 TB/s, and brings x for each
+// workgroup, 0.012 per row and stage, more where four waves are alone on their CU; eight waves take 1 us more to start and end.
+// Measured, bf16, weights from memory, by 16 / 32 / 48 weight rows and four waves, 16 / 32 / 48 / 64 / 80 / 96 / 128 and eight: one row,
+// K 5120, N 5120: 6.4 6.4 8.1, 6.6 6.1 7.8 9.8 11.7 13.2 18.9; N 20480: 13.0 15.1 14.6, 17.4 15.6 16.7 21.5 15.5 16.4 24.3;
+// K 20480, N 5120: 17.9 18.0 23.7, 17.9 16.5 22.1 28.1 34.8 40.0 69.4; 16 rows, K 5120, N 5120: 16.2 14.1 15.5, 14.5 11.3 12.9 14.5
+// 15.9 17.0 23.3; N 20480: 34.1 27.7 25.3, 33.7 26.3 27.4 30.9 19.7 20.8 29.4.
 struct RowsPlan4 {
   int rt, waves;
   double cost;
 };
 static RowsPlan4 plan_rows(int64_t M, int64_t N, int64_t stages, int cus) {
   RowsPlan4 best = {1, 4, 1e300};
+  const double stream = (double)(N * stages) * 136.0 / 5.2e6;
   for (int waves = 4; waves <= 8; waves += 4) {
     for (const int rt : {1, 2, 3, 4, 5, 6, 8}) {
       if (waves == 4 && rt > 3) break;
-      const double groups = (double)((N + 16 * rt - 1) / (16 * rt)), share = groups / cus, rounds = std::ceil(share);
-      const double busy = std::min(1.0, std::max(share, waves == 4 ? 0.78 : 0.7));
-      const double turns = waves == 4 && rounds > 1.0 ? (rounds + share) / 2 : rounds;
-      const double cost = (waves == 4 ? 2.5 : 3.5) + turns * (double)stages * (rt * 0.09 * busy + (double)M * 0.008);
+      const int64_t groups = (N + 16 * rt - 1) / (16 * rt);
+      const double turns = (double)((groups + cus - 1) / cus);
+      const double units = turns * (double)(stages * rt) * (waves == 4 ? 0.090 : 0.079);
+      const double rows = turns * (double)(stages * M) * (waves == 8 ? 0.012 : groups <= cus ? 0.02 : 0.013);
+      const double cost = (waves == 4 ? 2.5 : 3.5) + std::max(units, stream) + rows;
       if (cost < best.cost) best = {rt, waves, cost};
     }
   }

@@ -177,8 +177,8 @@ __global__ __launch_bounds__(512) void mxfp4_rows_kernel(Fp4Rows p) {
 }
 
 // Weight rows (in sixteens) and waves of a workgroup, by an estimate in microseconds: the CU with the most workgroups streams their
-// weight rows, 0.090 (four waves) or 0.079 (eight) per sixteen and stage, all CUs together at 5.2 TB/s, and brings x for each
-// workgroup, 0.012 per row and stage, more where four waves are alone on their CU; eight waves take 1 us more to start and end.
+// weight rows, 0.090 (four waves) or 0.079 (eight) per sixteen and stage, and brings x for each workgroup, 0.012 per row and stage,
+// more where four waves are alone on their CU; all CUs together stream at 5.2 TB/s; eight waves take 1.5 us more to start and end.
 // Measured, bf16, weights from memory, by 16 / 32 / 48 weight rows and four waves, 16 / 32 / 48 / 64 / 80 / 96 / 128 and eight: one row,
 // K 5120, N 5120: 6.4 6.4 8.1, 6.6 6.1 7.8 9.8 11.7 13.2 18.9; N 20480: 13.0 15.1 14.6, 17.4 15.6 16.7 21.5 15.5 16.4 24.3;
 // K 20480, N 5120: 17.9 18.0 23.7, 17.9 16.5 22.1 28.1 34.8 40.0 69.4; 16 rows, K 5120, N 5120: 16.2 14.1 15.5, 14.5 11.3 12.9 14.5
@@ -197,7 +197,7 @@ static RowsPlan4 plan_rows(int64_t M, int64_t N, int64_t stages, int cus) {
       const double turns = (double)((groups + cus - 1) / cus);
       const double units = turns * (double)(stages * rt) * (waves == 4 ? 0.090 : 0.079);
       const double rows = turns * (double)(stages * M) * (waves == 8 ? 0.012 : groups <= cus ? 0.02 : 0.013);
-      const double cost = (waves == 4 ? 2.5 : 3.5) + std::max(units, stream) + rows;
+      const double cost = (waves == 4 ? 2.5 : 4.0) + std::max(units + rows, stream);
       if (cost < best.cost) best = {rt, waves, cost};
     }
   }

@@ -618,18 +618,19 @@ int mxq_fp8_linear_backward(const void* dy, int dy_dtype, int64_t ldy, int direc
  * E8M0 byte b per 1 x 32 block of a row: the values are code * 2^(b - 127). The quantizer takes the smallest exponent
  * b - 127 >= -125 with absmax <= 6 * 2^(b - 127) (a block of zeros: b = 127) and rounds x / 2^(b - 127) once, to nearest
  * even; a block with a NaN or an infinity has b = 255, which makes all its values NaN. Strides of codes are in bytes.
- * As operands of the products, rows of codes are zero-padded to multiples of 128 bytes (row strides multiples of 16), and the
- * scale bytes lie in tiles of 512 bytes for 32 rows x 16 blocks: row r, block c of a tile (c = 0 .. 15) at
+ * As operands of the products, rows of codes are zero-padded to multiples of 128 bytes (an activation's) or 256 (a weight's; row
+ * strides multiples of 16), and the scale bytes lie in tiles of 512 bytes for 32 rows x 16 blocks: row r, block c of a tile (c = 0 .. 15) at
  * ((c / 4) % 2) * 256 + r * 8 + (c / 8) * 4 + c % 4, the tiles of 32 rows one after the other (ceil(K / 512) of them), 127 or
  * any byte but 255 behind a row's last block; MXQ_MXFP4_SCALE_BYTES in all. No counterpart in the reference.
  */
 #define MXQ_MXFP4_ROW_BYTES(K) (((K) + 255) / 256 * 128)
+#define MXQ_MXFP4_WEIGHT_ROW_BYTES(K) (((K) + 511) / 512 * 256)
 #define MXQ_MXFP4_SCALE_BYTES(rows, K) (((rows) + 31) / 32 * (((K) + 511) / 512) * 512)
 
 /*
  * Codes [M, ldq] and scales of x [M, K] (bf16, fp16 or fp32; row stride ldx): scales [M, lds] with lds a multiple of 4 and at
- * least ceil(K / 128) * 4, or, with lds = 0, in tiles. Codes are written to whole 128 columns (in tiles: to whole
- * MXQ_MXFP4_ROW_BYTES), zeros behind column K; ldq a multiple of 16.
+ * least ceil(K / 128) * 4, or, with lds = 0, in tiles. Codes are written to whole 128 columns (with scales in tiles: to whole
+ * 512 columns, or ldq where that is less), zeros behind column K; ldq a multiple of 16.
  */
 int mxq_mxfp4_quantize_rows(const void* x, int x_dtype, int64_t ldx, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, int64_t M,
                             int64_t K, void* stream);
@@ -638,7 +639,10 @@ int mxq_mxfp4_quantize_rows(const void* x, int x_dtype, int64_t ldx, uint8_t* q,
 int mxq_mxfp4_dequantize_rows(const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds, void* out, int out_dtype, int64_t M,
                               int64_t K, void* stream);
 
-/* Codes and scales of any strides and alignment as operands: q_out [rows, ldqo] (NULL: the scales only) and scale_out in tiles. */
+/*
+ * Codes and scales of any strides and alignment as operands: q_out [rows, ldqo] (NULL: the scales only; written to whole 512
+ * columns, or ldqo where that is less) and scale_out in tiles.
+ */
 int mxq_mxfp4_layout(const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds, uint8_t* q_out, int64_t ldqo,
                      uint8_t* scale_out, int64_t rows, int64_t K, void* stream);
 

@@ -181,7 +181,7 @@ def test_prepared_weights(dev, dtype, n, k):
     if k % 2:
         q[:, -1] |= 0xA0  # (what stands behind an odd row is not the weight's)
     c = mx.prepare_mxfp4_weight(q.to(dev).view(CODES), s.to(dev).view(SCALE), in_features=k)
-    want = torch.zeros(n, -(-k // 256) * 128, dtype=torch.uint8)
+    want = torch.zeros(n, -(-k // 512) * 256, dtype=torch.uint8)
     want[:, : -(-k // 2)] = ob.pack(codes)
     places = ob.tiles(b, k)
     for form in (a, c):

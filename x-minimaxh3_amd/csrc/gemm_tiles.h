@@ -14,7 +14,7 @@ constexpr int kGroupRows = 4;  // tile-rows per group of the tile order
 
 template <int kTM>
 struct Tile {
-  static constexpr int kBM = kTM, kWaveM = kTM / 2, kBI = kWaveM / 32, kBJ = 2;
+  static constexpr int kBM = kTM, kBN = kTileN, kWaveM = kTM / 2, kBI = kWaveM / 32, kBJ = 2;
   static constexpr int kLoadsA = kTM / 64, kLoadsB = 4;  // 1 KB loads per wave and chunk
 };
 
@@ -95,7 +95,7 @@ MXQ_DEVICE void epilogue(const P& p, char* lds, const v16f (&acc)[C::kBI][C::kBJ
   constexpr int kElem = kOut == MXQ_DTYPE_F32 ? 4 : 2;
   char* buf = lds + wave * 4096;
   const int M = (int)p.M, N = (int)p.N;
-  const bool lines = p.vec && M - m0 >= C::kBM && N - n0 >= kTileN;
+  const bool lines = p.vec && M - m0 >= C::kBM && N - n0 >= C::kBN;
   const int lr = lane & 31, lh = lane >> 5;
   char* out = reinterpret_cast<char*>(d);
   v4f bias[kSplit ? 1 : C::kBJ][4];  // (read once, ahead of the first piece's stores)

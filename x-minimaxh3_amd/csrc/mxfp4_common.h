@@ -16,10 +16,11 @@
 namespace mxq {
 
 constexpr int kFp4MinByte = 2;  // 2^-125
-constexpr int64_t kFp4Stage = 128;        // bytes of codes (256 columns) that rows are padded to
+constexpr int64_t kFp4Stage = 128;        // bytes of codes (256 columns) that an activation's rows are padded to; a weight's to two
 constexpr int64_t kFp4ScaleTile = 512;    // bytes of a scale tile: 32 rows x 16 blocks
 __host__ MXQ_DEVICE int64_t fp4_groups(int64_t K) { return (K + 511) / 512; }  // scale tiles along K
 inline int64_t fp4_row_bytes(int64_t K) { return (K + 255) / 256 * kFp4Stage; }
+inline int64_t fp4_weight_bytes(int64_t K) { return (K + 511) / 512 * 2 * kFp4Stage; }
 inline int64_t fp4_scale_bytes(int64_t rows, int64_t K) { return (rows + 31) / 32 * fp4_groups(K) * kFp4ScaleTile; }
 
 // The place of a row's block in its tile (both counted within the tile). A stage of the product is 256 columns, half h of

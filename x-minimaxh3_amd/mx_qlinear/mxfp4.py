@@ -26,8 +26,8 @@ _MAX_GRAD_STRIDE = 1 << 24  # below it, of the rows that the input's gradient re
 
 
 def _row_bytes(k: int) -> int:
-    """Bytes of a row of codes as the products read it."""
-    return _ceil(k, 256) // 2
+    """Bytes of a weight's row of codes as the products read it."""
+    return _ceil(k, 512) // 2
 
 
 def _scale_bytes(rows: int, k: int) -> int:
@@ -117,7 +117,7 @@ def dequantize_mxfp4(q: torch.Tensor, scale: torch.Tensor, out_dtype: torch.dtyp
 
 @dataclass(frozen=True)
 class PreparedMxfp4Weight:
-    """A 4-bit weight as the products read it (:func:`prepare_mxfp4_weight`): code rows ``q`` uint8 ``[N, bytes]`` of whole 128
+    """A 4-bit weight as the products read it (:func:`prepare_mxfp4_weight`): code rows ``q`` uint8 ``[N, bytes]`` of whole 256
     bytes and ``scale`` uint8 in tiles of 32 rows x 16 blocks."""
 
     q: torch.Tensor
@@ -282,7 +282,7 @@ class Mxfp4Linear(torch.nn.Module):
     norms, biases): the backward pass gives the input's and the bias's gradients.
 
     The buffers ``qweight`` and ``scale`` are the weight as the products read it (:class:`PreparedMxfp4Weight`), 17/32 byte a
-    weight and nothing beside them; :meth:`from_weight` makes a layer of a float weight or of a ``(codes, scale)`` pair.
+    weight (of whole 512 columns) and nothing beside them; :meth:`from_weight` makes a layer of a float weight or of a ``(codes, scale)`` pair.
     Activations are bf16, fp16 or fp32. Calls without gradients can be captured into a graph.
     """
 

@@ -8,18 +8,25 @@
 //
 // dY's rows hold the summed index n, so its fragments (eight consecutive n of one row per lane) are plain 16-byte LDS reads; W
 // has n as its rows, and its fragments come from transposing reads (ds_read_b64_tr_b16), which hand sixteen lanes the columns
-// of a 4 x 16 patch. A workgroup of eight waves owns a 256 (m) x 256 (k) tile, a wave 64 x 128 of it; a stage is 64 of n: dY's
-// 256 x 64 bfloat16 (32 KB) and W's 64 x 256 codes, decoded on the way from registers to LDS (32 KB). Problems of few tiles
-// split N over workgroups, which write float32 sums that fp8_join_kernel adds in order.
+// of a 4 x 16 patch. A workgroup of eight waves owns a 256 (m) x 256 (k) tile, a wave 64 x 128 of it, or, for problems of few
+// tiles, four waves one of 128 x 128, a wave 64 x 64 of it; a stage is 64 of n: dY's 256 x 64 bfloat16 (32 KB) and W's 64 x 256
+// codes, decoded on the way from registers to LDS (32 KB). Problems of fewer tiles still split N over workgroups, which write
+// float32 sums that fp8_join_kernel adds in order.
 #include "mxfp4_common.h"
 
 namespace mxq {
 
-constexpr int kDTile = 256, kDStage = 64, kDGroup = 4;
-constexpr int kDMB = 2, kDKB = 4;  // 32-row and 32-column blocks of a wave
-constexpr int kDThreads = 512, kDWaves = 8;
-constexpr int kDBytes = kDTile * kDStage * 2;  // of one operand's stage in LDS
-static_assert(2 * kDBytes == 0x10000, "the buffers are one address bit apart");
+constexpr int kDStage = 64, kDGroup = 4;
+
+// A workgroup's tile: kT x kT, four waves along m and two along k (256), or two and two (128).
+template <int kT>
+struct DgradTile {
+  static constexpr int kWaves = kT / 32, kThreads = 64 * kWaves, kWavesM = kT / 64;
+  static constexpr int kMB = 2, kKB = kT / 64;       // 32-row and 32-column blocks of a wave
+  static constexpr int kBytes = kT * kDStage * 2;    // of one operand's stage in LDS
+  static constexpr int kRow = kT * 2;                // of W's rows there
+  static constexpr int kRows = kT / 4;               // rows that the threads' loads take at once
+};
 
 struct Dgrad {
   const uint16_t* dy;  // part p at dy + p * part_stride
@@ -38,21 +45,23 @@ typedef char __attribute__((address_space(3)))* lds_ptr;  // (pointer arithmetic
 // read serves at once (sixteen rows, one piece) touch every bank once.
 MXQ_DEVICE int dy_at(int r, int piece) { return r * 128 + ((piece ^ ((r >> 1) & 7)) << 4); }
 
-// W in LDS: rows of 512 bytes (256 bfloat16), 64-byte piece p of row r at piece p ^ (r & 3), so that the sixteen lanes of a
-// transposing read (four rows, 32 bytes) and their neighbours cover all banks.
-MXQ_DEVICE int w_at(int r, int byte) { return r * 512 + ((((byte >> 6) ^ (r & 3)) << 6) | (byte & 63)); }
+// W in LDS: rows of kRow bytes (a tile's columns in bfloat16), 64-byte piece p of row r at piece p ^ (r & 3), so that the sixteen
+// lanes of a transposing read (four rows, 32 bytes) and their neighbours cover all banks.
+template <int kRow>
+MXQ_DEVICE int w_at(int r, int byte) { return r * kRow + ((((byte >> 6) ^ (r & 3)) << 6) | (byte & 63)); }
 
 // A fragment of W: columns c0 + l % 32 (c0 a multiple of 32), rows 8 (l / 32) + {0..7} of the 16 rows from r0 on (a multiple of
 // 16), in two transposing reads of four rows. Lane l of a group of sixteen gives the address of row (l % 16) / 4, columns
 // 4 (l % 4) .. + 3 of a 4 x 16 patch, and receives its column l % 16. The address is that of w_base plus a constant: r & 3, which
 // the swizzle uses, is the lane's own.
+template <int kRow>
 MXQ_DEVICE uint32_t w_base(uint32_t operand, int c0, int lane) {
   const int r = (lane >> 5) * 8 + ((lane & 15) >> 2);
-  return operand + (uint32_t)w_at(r, (c0 + (lane & 16) + (lane & 3) * 4) * 2);
+  return operand + (uint32_t)w_at<kRow>(r, (c0 + (lane & 16) + (lane & 3) * 4) * 2);
 }
-template <int kRow>
+template <int kOff>
 MXQ_DEVICE v4s read_transposed(uint32_t base) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)((lds_ptr)(uintptr_t)base + kRow * 512));
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)((lds_ptr)(uintptr_t)base + kOff));
 }
 MXQ_DEVICE v8bf join_fragment(const v4s (&f)[2]) {
   typedef short v8s __attribute__((ext_vector_type(8)));
@@ -64,9 +73,12 @@ MXQ_DEVICE uint32_t dgrad_load_u32(const void* base, int bytes, uint32_t voff) {
       __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, kRawBufferWord3), (int)voff, 0, 0);
 }
 
-template <int kOut, bool kSplit>
-__global__ __launch_bounds__(kDThreads, 1) void mxfp4_dgrad_kernel(Dgrad p) {
-  __shared__ __attribute__((aligned(131072))) char lds[2 * 2 * kDBytes];  // [buffer][dY, W]
+template <int kT, int kOut, bool kSplit>
+__global__ __launch_bounds__(DgradTile<kT>::kThreads, kT == 256 ? 1 : 2) void mxfp4_dgrad_kernel(Dgrad p) {
+  typedef DgradTile<kT> C;
+  constexpr int kDMB = C::kMB, kDKB = C::kKB, kDBytes = C::kBytes;
+  // [buffer][dY, W]; the buffers are one address bit apart
+  __shared__ __attribute__((aligned(2 * 2 * C::kBytes))) char lds[2 * 2 * C::kBytes];
   const int tiles = p.tiles_m * p.tiles_k, num = tiles * p.splits, per = num / 8, bid = blockIdx.x;
   int t = bid < per * 8 ? (bid % 8) * per + bid / 8 : bid;  // contiguous ranges over the XCDs
   const int slice = t / tiles;
@@ -74,19 +86,21 @@ __global__ __launch_bounds__(kDThreads, 1) void mxfp4_dgrad_kernel(Dgrad p) {
   // groups of four tile-rows, so that the tiles an XCD runs at once share operand panels in its L2
   const int group = kDGroup * p.tiles_k, g0 = t / group * kDGroup, rows_g = min(p.tiles_m - g0, kDGroup), in_g = t - g0 * p.tiles_k;
   const int tk = in_g / rows_g, tm = g0 + in_g - tk * rows_g;
-  const int m0 = tm * kDTile, k0 = tk * kDTile;
+  const int m0 = tm * kT, k0 = tk * kT;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int wm = (wave & 3) * 64, wk = (wave >> 2) * 128;  // the wave's part of the tile
+  const int wm = (wave % C::kWavesM) * 64, wk = (wave / C::kWavesM) * 32 * kDKB;  // the wave's part of the tile
   const int M = (int)p.M, K = (int)p.K, n_first = slice * p.split_n, n_last = min(n_first + p.split_n, (int)p.N);
   const int stages = (n_last - n_first + kDStage - 1) / kDStage, total = stages * p.parts;
 
   // A thread's share of a stage, by buffer loads whose offsets point outside for what lies behind the slice's last n or the last
-  // row (they read zeros): of dY the 16-byte piece tid % 8 of rows tid / 8 + 64 j (nothing is read behind column N rounded up to
-  // 8); of W row tid / 8, the words (eight columns) tid % 8 + 8 j with the scale words of the row's blocks 0 .. 3 and 4 .. 7.
+  // row (they read zeros): of dY the 16-byte piece tid % 8 of rows tid / 8 + kRows j (nothing is read behind column N rounded up to
+  // 8); of W four words of eight columns, tid % 8 + 8 j of row tid / 8 (256 columns, with the scale words of the row's blocks
+  // 0 .. 3 and 4 .. 7), or tid % 8 + 8 (j % 2) of rows tid / 8 + 32 (j / 2) (128 columns, with the rows' scale words).
+  constexpr int kRows = C::kRows;
   const int r = tid >> 3, c = tid & 7;
   const int ldy = (int)p.ldy, ldb = (int)p.ldb, row_tiles = p.groups * (int)kFp4ScaleTile;
   const uint32_t oy = (uint32_t)(r * ldy + c * 8) * 2, ow = (uint32_t)(r * ldb + c * 4);
-  const uint32_t os = (uint32_t)((r >> 5) * row_tiles + (r & 31) * 8 + ((k0 >> 8) & 1) * 4);
+  const uint32_t os = (uint32_t)((r >> 5) * row_tiles + (r & 31) * 8 + ((k0 >> 8) & 1) * 4 + (kT == 128 ? ((k0 >> 7) & 1) * 256 : 0));
   v4u y[4];
   uint32_t w[4], ws[2];
   // (the position of the next load: n left in the slice and the operands' place)
@@ -96,12 +110,14 @@ __global__ __launch_bounds__(kDThreads, 1) void mxfp4_dgrad_kernel(Dgrad p) {
   const uint8_t* ps = p.sb + (int64_t)(n_first >> 5) * row_tiles + (k0 >> 9) * kFp4ScaleTile;
   auto load = [&](auto HC) {  // the first or second half of a share
     constexpr int kH = decltype(HC)::value;
+    const bool row = r + (kT == 128 ? 32 * kH : 0) < left;
 #pragma unroll
     for (int j = 2 * kH; j < 2 * kH + 2; ++j) {
-      y[j] = buffer_load_x4(py + (int64_t)(64 * j) * ldy, 64 * 2 * ldy, c * 8 < left && m0 + 64 * j + r < M ? oy : kBufferOff);
-      w[j] = dgrad_load_u32(pw, kDStage * ldb, r < left ? ow + 32 * j : kBufferOff);
+      y[j] = buffer_load_x4(py + (int64_t)(kRows * j) * ldy, kRows * 2 * ldy, c * 8 < left && m0 + kRows * j + r < M ? oy : kBufferOff);
+      const uint32_t at = kT == 128 ? (uint32_t)(32 * kH * ldb + 32 * (j & 1)) : (uint32_t)(32 * j);
+      w[j] = dgrad_load_u32(pw, kDStage * ldb, row ? ow + at : kBufferOff);
     }
-    ws[kH] = dgrad_load_u32(ps, 2 * row_tiles, r < left ? os + 256 * kH : kBufferOff);
+    ws[kH] = dgrad_load_u32(ps, 2 * row_tiles, row ? os + (uint32_t)(kT == 128 ? kH * row_tiles : 256 * kH) : kBufferOff);
     if constexpr (kH == 1) {
       left -= kDStage;
       py += kDStage;
@@ -117,20 +133,21 @@ __global__ __launch_bounds__(kDThreads, 1) void mxfp4_dgrad_kernel(Dgrad p) {
       }
     }
   };
-  const uint32_t at_y = lds_addr(lds) + (uint32_t)dy_at(r, c);  // (row r + 64 j has r's swizzle)
+  const uint32_t at_y = lds_addr(lds) + (uint32_t)dy_at(r, c);  // (row r + kRows j has r's swizzle)
   // (words c + 8 j: 128 bytes further on, two 64-byte pieces, whose number the swizzle is exclusive with)
-  const uint32_t at_w = lds_addr(lds) + kDBytes + (uint32_t)w_at(r, c * 16);
+  const uint32_t at_w = lds_addr(lds) + kDBytes + (uint32_t)w_at<C::kRow>(r, c * 16);
   auto put_y = [&](uint32_t buf, auto JC) {
     constexpr int j = decltype(JC)::value;
-    *(lds_v4u)((lds_ptr)(uintptr_t)(at_y ^ buf) + j * 64 * 128) = y[j];
+    *(lds_v4u)((lds_ptr)(uintptr_t)(at_y ^ buf) + j * kRows * 128) = y[j];
   };
   auto put_w = [&](uint32_t buf, auto JC) {
-    constexpr int j = decltype(JC)::value;
+    constexpr int j = decltype(JC)::value, kWord = kT == 128 ? j & 1 : j, kRowOff = kT == 128 ? (j >> 1) * 32 * C::kRow : 0;
     const uint32_t byte = (ws[j >> 1] >> (16 * (j & 1) + 8 * (c >> 2))) & 0xFFu;
-    *(lds_v4u)((lds_ptr)(uintptr_t)(at_w ^ buf ^ (j * 128))) = __builtin_bit_cast(v4u, fp4x8_to_bf16(w[j], fp8_scale_f32(byte)));
+    *(lds_v4u)((lds_ptr)(uintptr_t)(at_w ^ buf ^ (kWord * 128)) + kRowOff) =
+        __builtin_bit_cast(v4u, fp4x8_to_bf16(w[j], fp8_scale_f32(byte)));
   };
   v16f acc[kDMB][kDKB] = {};
-  // A stage is four steps of 16 n, a step eight slots, each one matrix instruction and a part of the other work, in the order
+  // A stage is four steps of 16 n, a step kMB kKB slots, each one matrix instruction and a part of the other work, in the order
   // written (sched_barrier): fragments are read one step ahead; the next stage is written to the other buffer, a half each,
   // during steps 1 and 2, the one behind it requested as the registers get free, and the barrier passed ahead of the last
   // step, whose instructions cover the next stage's first reads.
@@ -140,7 +157,7 @@ __global__ __launch_bounds__(kDThreads, 1) void mxfp4_dgrad_kernel(Dgrad p) {
   v4s fw[2][kDKB][2];
   uint32_t base[kDKB];  // of W's fragments in buffer 0
 #pragma unroll
-  for (int b = 0; b < kDKB; ++b) base[b] = w_base(lds_addr(lds) + kDBytes, wk + b * 32, lane);
+  for (int b = 0; b < kDKB; ++b) base[b] = w_base<C::kRow>(lds_addr(lds) + kDBytes, wk + b * 32, lane);
   // dY's fragments: row wm + l % 32 (+ 32 a), piece 2 step + l / 32
   uint32_t base_y[4];
 #pragma unroll
@@ -152,7 +169,7 @@ __global__ __launch_bounds__(kDThreads, 1) void mxfp4_dgrad_kernel(Dgrad p) {
       fy[kSet][a] = *(lds_v4u)((lds_ptr)(uintptr_t)(base_y[kStep] ^ buf) + a * 32 * 128);
     } else {
       constexpr int b = (kI - 1) / 2, kPart = (kI - 1) & 1;
-      fw[kSet][b][kPart] = read_transposed<kStep * 16 + kPart * 4>(base[b] ^ buf);
+      fw[kSet][b][kPart] = read_transposed<(kStep * 16 + kPart * 4) * C::kRow>(base[b] ^ buf);
     }
   };
   auto publish = [&] {
@@ -176,10 +193,10 @@ __global__ __launch_bounds__(kDThreads, 1) void mxfp4_dgrad_kernel(Dgrad p) {
           if constexpr (i * kReadSlots / kReads == g)
             read(h < 3 ? buf : other, std::integral_constant<int, h < 3 ? h + 1 : 0>{}, std::integral_constant<int, kSet ^ 1>{}, I);
         });
-        if constexpr (kPut) {
-          constexpr int j = (h - 1) * 2 + g / 4;
-          if constexpr (g % 4 == 0) put_y(other, std::integral_constant<int, j>{});
-          if constexpr (g % 4 == 2) put_w(other, std::integral_constant<int, j>{});
+        if constexpr (kPut && g * 4 % kSlots == 0) {  // (four writes a step)
+          constexpr int i = g * 4 / kSlots, j = (h - 1) * 2 + i / 2;
+          if constexpr (i % 2 == 0) put_y(other, std::integral_constant<int, j>{});
+          else put_w(other, std::integral_constant<int, j>{});
         }
         __builtin_amdgcn_sched_barrier(0);
       });
@@ -196,11 +213,13 @@ __global__ __launch_bounds__(kDThreads, 1) void mxfp4_dgrad_kernel(Dgrad p) {
   for (int i = 0; i < total; ++i) stage();
   // Lane l holds row m = l % 32 of a block and, in register e, column (e / 4) * 8 + (l / 32) * 4 + e % 4. Stored from there, an
   // instruction would touch 32 bytes of 32 rows; through the wave's 16 KB of LDS (no wave reads a stage any more: the last
-  // barrier is behind the last step's reads) 32 lanes store a row's 128 columns. 16-byte piece c of row r sits at piece c ^ r.
-  constexpr int kElem = kOut == MXQ_DTYPE_F32 ? 4 : 2;
+  // barrier is behind the last step's reads) kLanes lanes store a row of the wave's columns. 16-byte piece c of row r sits at piece
+  // c ^ (r % kLanes).
+  constexpr int kElem = kOut == MXQ_DTYPE_F32 ? 4 : 2, kLanes = kDKB * 8, kTurn = kLanes * 16;
+  static_assert(2 * 2 * kDBytes / C::kWaves >= 32 * kTurn, "LDS of a wave's block of results");
   char* d = reinterpret_cast<char*>(p.d);
   if constexpr (kSplit) d += (int64_t)slice * p.M * p.ldd * 4;
-  char* turn = lds + wave * (2 * 2 * kDBytes / kDWaves);
+  char* turn = lds + wave * (2 * 2 * kDBytes / C::kWaves);
 #pragma unroll
   for (int a = 0; a < kDMB; ++a) {
     wave_lds_fence();
@@ -209,14 +228,14 @@ __global__ __launch_bounds__(kDThreads, 1) void mxfp4_dgrad_kernel(Dgrad p) {
     for (int b = 0; b < kDKB; ++b)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        *reinterpret_cast<v4f*>(turn + row * 512 + (((b * 8 + e * 2 + (lane >> 5)) ^ row) << 4)) =
+        *reinterpret_cast<v4f*>(turn + row * kTurn + (((b * 8 + e * 2 + (lane >> 5)) ^ (row & (kLanes - 1))) << 4)) =
             v4f{acc[a][b][4 * e], acc[a][b][4 * e + 1], acc[a][b][4 * e + 2], acc[a][b][4 * e + 3]};
     wave_lds_fence();
-    const int k = k0 + wk + (lane & 31) * 4;
+    const int l = lane & (kLanes - 1), k = k0 + wk + l * 4;
 #pragma unroll
-    for (int u = 0; u < 16; ++u) {
-      const int q = u * 2 + (lane >> 5), m = m0 + wm + a * 32 + q;
-      const v4f z = *reinterpret_cast<const v4f*>(turn + q * 512 + (((lane & 31) ^ q) << 4));
+    for (int u = 0; u < kLanes / 2; ++u) {
+      const int q = u * (64 / kLanes) + lane / kLanes, m = m0 + wm + a * 32 + q;
+      const v4f z = *reinterpret_cast<const v4f*>(turn + q * kTurn + ((l ^ (q & (kLanes - 1))) << 4));
       const float v[4] = {z[0], z[1], z[2], z[3]};
       if (m < M && k < K) store_run4<kOut>(d + (int64_t)m * p.ldd * kElem, k, K - k, v);
     }
@@ -224,23 +243,31 @@ __global__ __launch_bounds__(kDThreads, 1) void mxfp4_dgrad_kernel(Dgrad p) {
 }
 
 struct DgradPlan {
-  int splits;
+  int tile, splits;
   int64_t n;
 };
 
-// N slices, by an estimate in microseconds: a round of workgroups takes 4.5 and 1.5 per stage and part, slices cost a join.
+// Tile and N slices, by an estimate in microseconds: a round of workgroups takes 5 and, per stage and part, 1.2 (256) or 0.575 (128)
+// where few CUs are at work, 1.58 or 0.93 (two workgroups a CU) where all are, slices cost a join. Measured, whole and in the best
+// number of slices, 128 / 256: one row, K 5120, N 5120: 52, 15.4 in twelve / 101, 19.8; 700 rows: 54.7, 52.8 in two / 105, 53.9 in
+// four; 2048 rows 128 / 109; 700 rows, K 5120, N 20480: 195, 166 in two / 389, 142 in four; 4096 rows, K 20480, N 5120: 831 / 657;
+// 2048 rows, K 1000, N 3001: 43.7, 34.9 in two / 74.6, 40.6 in four.
 static DgradPlan plan_dgrad(int64_t M, int64_t N, int64_t K, int parts, int cus) {
-  const int64_t tiles = (M + kDTile - 1) / kDTile * ((K + kDTile - 1) / kDTile);
-  DgradPlan best = {1, (N + kDStage - 1) / kDStage * kDStage};
+  DgradPlan best = {256, 1, (N + kDStage - 1) / kDStage * kDStage};
   double best_cost = 1e300;
-  for (int64_t s = 1; s <= 64; ++s) {
-    const int64_t n = ((N + s - 1) / s + kDStage - 1) / kDStage * kDStage;
-    if ((N + n - 1) / n != s || (s > 1 && tiles * s > 4 * cus)) continue;
-    const double rounds = (double)((tiles * s + cus - 1) / cus);
-    const double cost = rounds * ((double)(n / kDStage) * parts * 1.5 + 4.5) + slices_cost(s, M * K);
-    if (cost < best_cost) {
-      best_cost = cost;
-      best = {(int)s, n};
+  for (int tile = 256; tile >= 128; tile /= 2) {
+    const int64_t tiles = (M + tile - 1) / tile * ((K + tile - 1) / tile), at_once = tile == 256 ? cus : 2 * cus;
+    const double alone = tile == 256 ? 1.2 : 0.575, all = tile == 256 ? 1.58 : 0.93;
+    for (int64_t s = 1; s <= 64; ++s) {
+      const int64_t n = ((N + s - 1) / s + kDStage - 1) / kDStage * kDStage;
+      if ((N + n - 1) / n != s || (s > 1 && tiles * s > 4 * cus)) continue;
+      const double units = (double)(n / kDStage * parts), rest = (double)(tiles * s % at_once) / at_once;
+      const double cost = (double)(tiles * s / at_once) * (units * all + 5.0) +
+                          (rest > 0.0 ? units * (alone + (all - alone) * rest) + 5.0 : 0.0) + slices_cost(s, M * K);
+      if (cost < best_cost) {
+        best_cost = cost;
+        best = {tile, (int)s, n};
+      }
     }
   }
   return best;
@@ -265,16 +292,24 @@ int fp4_dgrad_check(const void* dy, int64_t ldy, const uint8_t* b, int64_t ldb, 
   if (M > 0 && (!dy || !b || !sb || !dx || reinterpret_cast<uintptr_t>(dy) % 16 || reinterpret_cast<uintptr_t>(b) % 16 ||
                 reinterpret_cast<uintptr_t>(sb) % 16))
     return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
-  if ((M + kDTile - 1) / kDTile * ((K + kDTile - 1) / kDTile) >= (1ll << 23))  // (so many tiles are not split)
+  if ((M + 127) / 128 * ((K + 127) / 128) >= (1ll << 23))  // (so many tiles are not split)
     return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^23 tiles");
   return MXQ_OK;
+}
+
+template <int kOut, bool kSplit>
+static void launch_dgrad(const Dgrad& p, int tile, unsigned grid, void* stream) {
+  if (tile == 256)
+    hipLaunchKernelGGL((mxfp4_dgrad_kernel<256, kOut, kSplit>), dim3(grid), dim3(DgradTile<256>::kThreads), 0, (hipStream_t)stream, p);
+  else
+    hipLaunchKernelGGL((mxfp4_dgrad_kernel<128, kOut, kSplit>), dim3(grid), dim3(DgradTile<128>::kThreads), 0, (hipStream_t)stream, p);
 }
 
 int fp4_dgrad(const void* dy, int parts, int64_t ldy, const uint8_t* b, int64_t ldb, const uint8_t* sb, void* dx, int out_dtype,
               int64_t M, int64_t N, int64_t K, void* workspace, SliceJob* later, void* stream) {
   if (const int rc = fp4_dgrad_check(dy, ldy, b, ldb, sb, dx, out_dtype, M, N, K)) return rc;
   const DgradPlan plan = plan_dgrad(M, N, K, parts, mxq_cu_count());
-  const int64_t tiles_m = (M + kDTile - 1) / kDTile, tiles_k = (K + kDTile - 1) / kDTile;
+  const int64_t tiles_m = (M + plan.tile - 1) / plan.tile, tiles_k = (K + plan.tile - 1) / plan.tile;
   Dgrad p = {(const uint16_t*)dy, b, sb, dx, M, N, K, ldy, M * ldy, ldb, K, parts, (int)fp4_groups(K), (int)tiles_m, (int)tiles_k,
              plan.splits, (int)plan.n};
   const unsigned grid = (unsigned)(tiles_m * tiles_k * plan.splits);
@@ -282,12 +317,12 @@ int fp4_dgrad(const void* dy, int parts, int64_t ldy, const uint8_t* b, int64_t 
     const int64_t ldp = (K + 3) / 4 * 4;
     p.d = workspace;
     p.ldd = ldp;
-    hipLaunchKernelGGL((mxfp4_dgrad_kernel<MXQ_DTYPE_F32, true>), dim3(grid), dim3(kDThreads), 0, (hipStream_t)stream, p);
+    launch_dgrad<MXQ_DTYPE_F32, true>(p, plan.tile, grid, stream);
     *later = {(const float*)workspace, nullptr, dx, M, ldp, K, (int)K, plan.splits, out_dtype};
     return mxq_check_launch("mxfp4_dgrad_kernel");
   }
   with_dtype(out_dtype, [&](auto O) {
-    hipLaunchKernelGGL((mxfp4_dgrad_kernel<decltype(O)::value, false>), dim3(grid), dim3(kDThreads), 0, (hipStream_t)stream, p);
+    launch_dgrad<decltype(O)::value, false>(p, plan.tile, grid, stream);
   });
   return mxq_check_launch("mxfp4_dgrad_kernel");
 }

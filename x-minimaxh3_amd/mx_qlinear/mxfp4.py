@@ -36,7 +36,7 @@ def _scale_bytes(rows: int, k: int) -> int:
 
 
 def _pair(q: torch.Tensor, scale: torch.Tensor, width: int | None, what: str = "activation"):
-    """A ``(codes, scale)`` pair as 2-D byte tensors with unit column stride: (codes, scale, M, K)."""
+    """A ``(codes, scale)`` pair as 2-D tensors of one-byte elements with unit column stride: (codes, scale, M, K)."""
     if q.dtype != _CODES or scale.dtype != _SCALE:
         raise ValueError(f"a 4-bit {what} is float4_e2m1fn_x2 codes with float8_e8m0fnu scales, got {q.dtype} and {scale.dtype}")
     if q.dim() < 1 or q.shape[-1] == 0:
@@ -49,15 +49,15 @@ def _pair(q: torch.Tensor, scale: torch.Tensor, width: int | None, what: str = "
     if scale.shape != (*q.shape[:-1], kb):
         raise ValueError(f"scale of shape {tuple(scale.shape)} for codes of shape {tuple(q.shape)}: expected "
                          f"{(*q.shape[:-1], kb)}")
-    q, scale = q.view(torch.uint8), scale.view(torch.uint8)
     if q.dim() != 2:
         lead = q.shape[:-1].numel()
-        q, scale = q.reshape(lead, half), scale.reshape(lead, kb)
-    if q.stride(1) != 1 or (q.shape[0] > 1 and q.stride(0) < half):
-        q = q.contiguous()
-    if scale.stride(1) != 1 or (scale.shape[0] > 1 and scale.stride(0) < kb):
+        q, scale = q.view(torch.uint8).reshape(lead, half), scale.reshape(lead, kb)
+    m, (ldq, one), (lds, each) = q.shape[0], q.stride(), scale.stride()
+    if one != 1 or (m > 1 and ldq < half):
+        q = q.view(torch.uint8).contiguous()
+    if each != 1 or (m > 1 and lds < kb):
         scale = scale.contiguous()
-    return q, scale, q.shape[0], k
+    return q, scale, m, k
 
 
 # ---------------------------------------------------------------------------------------
@@ -67,11 +67,11 @@ def _pair(q: torch.Tensor, scale: torch.Tensor, width: int | None, what: str = "
 def _new_pair(m: int, k: int, dev) -> tuple[torch.Tensor, torch.Tensor]:
     """Storage for codes and scales of [m, k]: rows of whole 128 columns."""
     n = -(-k // 128)
-    return torch.empty(m, n * 64, dtype=torch.uint8, device=dev), torch.empty(m, n * 4, dtype=torch.uint8, device=dev)
+    return torch.empty(m, n * 64, dtype=_CODES, device=dev), torch.empty(m, n * 4, dtype=_SCALE, device=dev)
 
 
 def _as_pair(q: torch.Tensor, s: torch.Tensor, lead: tuple[int, ...], k: int) -> tuple[torch.Tensor, torch.Tensor]:
-    return _view(q.view(_CODES), lead, -(-k // 2)), _view(s.view(_SCALE), lead, -(-k // BLOCK))
+    return _view(q, lead, -(-k // 2)), _view(s, lead, -(-k // BLOCK))
 
 
 def quantize_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

@@ -27,27 +27,28 @@ def _rms(what: str, x: torch.Tensor, weight, eps: float, residual, want_rstd: bo
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"residual of {residual.dtype} {tuple(residual.shape)} for an input of {x.dtype} {tuple(x.shape)}")
     dev = _require_gpu(x, residual, weight)
-    d = x.shape[-1]
+    flat, d = x.dim() == 2, x.shape[-1]
     w, _, pcode = _norm_params(d, dev, x.dtype, weight, None)
     x2 = _rows_in_place(x, d)
-    r2 = None if residual is None else _rows_in_place(residual, d)
     m = x2.shape[0]
-    total = None if residual is None else torch.empty(m, d, dtype=x.dtype, device=dev)
+    ldx, r2, ldr, total = x2.stride(0) if m > 1 else d, None, 0, None
+    if residual is not None:
+        r2 = _rows_in_place(residual, d)
+        ldr, total = r2.stride(0) if m > 1 else d, torch.empty(m, d, dtype=x.dtype, device=dev)
     rstd = torch.empty(m, dtype=torch.float32, device=dev) if want_rstd else None
-    s = None
     if target is None:
-        y = torch.empty(m, d, dtype=x.dtype, device=dev)
+        y, s, target, lds = torch.empty(m, d, dtype=x.dtype, device=dev), None, code, 0
     else:
         y, s = fp8._new_pair(m, d, dev) if target == _lib.DTYPE_E4M3 else mxfp4._new_pair(m, d, dev)
+        lds = s.shape[1]
     if m:
-        _launch(dev, "mxq_rms_norm", x2.data_ptr(), _ptr(r2), code, x2.stride(0) if m > 1 else d,
-                0 if r2 is None else r2.stride(0) if m > 1 else d, _ptr(w), pcode, float(eps), _ptr(total), y.data_ptr(),
-                code if target is None else target, y.shape[1], _ptr(s), 0 if s is None else s.shape[1], _ptr(rstd), m, d)
+        _launch(dev, "mxq_rms_norm", x2.data_ptr(), _ptr(r2), code, ldx, ldr, _ptr(w), pcode, float(eps), _ptr(total), y.data_ptr(),
+                target, y.shape[1], _ptr(s), lds, _ptr(rstd), m, d)
     rest = []
     if total is not None:
-        rest.append(total if x.dim() == 2 else total.reshape(x.shape))
-    if rstd is not None:
-        rest.append(rstd if x.dim() == 2 else rstd.reshape(x.shape[:-1]))
+        rest.append(total if flat else total.reshape(x.shape))
+    if want_rstd:
+        rest.append(rstd if flat else rstd.reshape(x.shape[:-1]))
     return (y, s), rest
 
 

@@ -22,6 +22,9 @@ pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 NORMS = [(1, 1), (1, 5120), (3, 7), (5, 8), (4, 100), (2, 511), (9, 512), (3, 513), (65, 1003), (7, 1024), (5, 1500), (4, 2048), (3, 3001),
          (130, 4096), (2, 5376), (3, 6145), (2, 8200), (3, 12288), (2, 20480), (2, 24575), (2, 24576)]
+# A head's columns: rows that share a wave, the last of a workgroup's missing, runs of eight that end in every place.
+NARROW = [(1, 64), (15, 128), (17, 128), (1000, 128), (33, 127), (31, 121), (2, 129), (65, 200), (9, 256), (1003, 256), (5, 257), (18, 9),
+          (35, 2), (4, 130), (7, 252), (5000, 96)]
 
 
 def _mx():
@@ -62,7 +65,7 @@ def check_codes4(q, s, y):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("m,d", NORMS)
+@pytest.mark.parametrize("m,d", NORMS + NARROW)
 def test_forward(dev, dtype, m, d):
     mx = _mx()
     x, r, w = _acts(m, d, dtype, m + d, 2.0), _acts(m, d, dtype, m + d + 1, 2.0), _weight(d, dtype, d)
@@ -162,7 +165,7 @@ def check_backward(dx, dw, dy, s, rstd, weight, dsum):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("m,d", [*NORMS, (700, 64), (2100, 513), (600, 1536)])
+@pytest.mark.parametrize("m,d", [*NORMS, *NARROW, (700, 64), (2100, 513), (600, 1536)])
 def test_backward(dev, dtype, m, d):
     mx = _mx()
     x, w, dy, ds = _acts(m, d, dtype, m + d), _weight(d, dtype, d), _acts(m, d, dtype, m + d + 2) * 0.1, _acts(m, d, dtype, m + d + 3) * 0.1

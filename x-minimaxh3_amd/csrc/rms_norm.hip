@@ -12,6 +12,10 @@
 // A row is held in registers by one or more waves, eight elements per lane and chunk of 512, so x and r are read once. The
 // backward pass also keeps its lanes' columns of dw in registers over all the rows a workgroup takes, and fp8_join_kernel
 // adds the workgroups' sums in a fixed order: no atomics, the same bits on every run.
+//
+// Both passes are bound by HBM. Forward with a residual and 4-bit codes, 75600 x 5120 bf16: 472 us, 5.6 TB/s. Backward there:
+// 500 us, 4.7 TB/s (three streams of one direction each; a second row requested ahead cost registers and time, 125 to 165 us at
+// 19531 x 5120).
 
 #include "mxfp4_common.h"
 #include "norm_common.h"
@@ -20,40 +24,64 @@ namespace mxq {
 
 constexpr int kOutSame = 0, kOutFp8 = 1, kOutFp4 = 2;
 
-// A lane's eight columns from `col` on, `n` of them inside the row (none: nothing is read). kVec: 8 or 0.
+// Eight elements moved down by s (0 to 7) of them, zeros behind.
+template <int kCode>
+MXQ_DEVICE void shift_down(Eight<kCode>& r, int s) {
+  constexpr int kWords = Eight<kCode>::kWords, kBits = 32 * kWords / 8;  // bits of an element
+#pragma unroll
+  for (int b = 4; b >= 1; b /= 2) {
+    const bool on = s & b;
+    const int words = b * kBits / 32, bits = b * kBits % 32;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      const uint32_t lo = i + words < kWords ? r.w[i + words] : 0u, hi = i + words + 1 < kWords ? r.w[i + words + 1] : 0u;
+      const uint32_t v = bits ? __builtin_amdgcn_alignbit(hi, lo, bits) : lo;
+      r.w[i] = on ? v : r.w[i];
+    }
+  }
+}
+
+// A lane's eight columns from `col` on of a row of D, `n` = D - col of them inside it (none: zeros). kVec: n is 8 or more, or none.
+// Else every lane makes the same one access, the row's last eight elements where fewer are left, moved into place (a branch
+// for the lane with some of them made a wave wait once per operand, and its seven loads spilled: 20000 x 5001 bf16 backward
+// 284 us, 178 now). A row below eight elements goes element by element.
 template <int kCode, bool kVec>
 MXQ_DEVICE Eight<kCode> load_run8(const char* row, int col, int n) {
   constexpr int kWords = Eight<kCode>::kWords, kElem = Eight<kCode>::kElem;
   Eight<kCode> r = {};
-  const char* p = row + (int64_t)col * kElem;
-  if (n >= 8) {
-    if constexpr (kWords == 2) {
-      const v2u v = *reinterpret_cast<const v2u_any*>(p);
-      r.w[0] = v[0];
-      r.w[1] = v[1];
-    } else {
+  const int D = col + n;
+  if (!kVec && D < 8) {
+    for (int e = col == 0 ? D - 1 : -1; e >= 0; --e) {
 #pragma unroll
-      for (int i = 0; i < kWords / 4; ++i) {
-        const v4u v = *reinterpret_cast<const v4u_any*>(p + 16 * i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r.w[4 * i + j] = v[j];
+      for (int i = kWords - 1; i >= 0; --i) {
+        const uint32_t below = i ? r.w[i - 1] : 0u;
+        r.w[i] = kElem == 4 ? below : (r.w[i] << (8 * (kElem & 3))) | (below >> (32 - 8 * (kElem & 3)));
       }
+      if constexpr (kElem == 4) r.w[0] = reinterpret_cast<const uint32_t*>(row)[e];
+      else if constexpr (kElem == 1) r.w[0] |= reinterpret_cast<const uint8_t*>(row)[e];
+      else r.w[0] |= reinterpret_cast<const uint16_t*>(row)[e];
     }
-  } else if (!kVec && n > 0) {
+    return r;
+  }
+  if (kVec && n <= 0) return r;
+  const int start = kVec ? col : n > 0 ? min(col, D - 8) : 0;
+  const char* p = row + (int64_t)start * kElem;
+  if constexpr (kWords == 2) {
+    const v2u v = *reinterpret_cast<const v2u_any*>(p);
+    r.w[0] = v[0];
+    r.w[1] = v[1];
+  } else {
 #pragma unroll
-    for (int i = 0; i < 7; ++i) {
-      const int at = min(i, n - 1);
-      if constexpr (kElem == 4) {
-        const uint32_t v = reinterpret_cast<const uint32_t*>(p)[at];
-        r.w[i] = i < n ? v : 0u;
-      } else if constexpr (kElem == 1) {
-        const uint32_t v = reinterpret_cast<const uint8_t*>(p)[at];
-        r.w[i >> 2] |= (i < n ? v : 0u) << (8 * (i & 3));
-      } else {
-        const uint32_t v = reinterpret_cast<const uint16_t*>(p)[at];
-        r.w[i >> 1] |= (i < n ? v : 0u) << (16 * (i & 1));
-      }
+    for (int i = 0; i < kWords / 4; ++i) {
+      const v4u v = *reinterpret_cast<const v4u_any*>(p + 16 * i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.w[4 * i + j] = v[j];
     }
+  }
+  if constexpr (!kVec) {
+    shift_down(r, n > 0 ? col - start : 0);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) r.w[i] = n > 0 ? r.w[i] : 0u;
   }
   return r;
 }
@@ -177,14 +205,41 @@ MXQ_DEVICE void store_fp4(const Rms& p, int64_t row, int col, int lane, const fl
   }
 }
 
-// kOne: a wave per row, four rows per workgroup; else a workgroup per row.
-template <int kCode, int kOut, int kChunks, bool kOne, bool kVec>
-__global__ __launch_bounds__(kOne ? 256 : 1024) void rms_norm_kernel(Rms p) {
+// The sum of a row's lanes, where they are part of one wave: 16, 32 or 64 of them.
+template <int kLanes>
+MXQ_DEVICE double lanes_sum_f64(double v) {
+  if constexpr (kLanes == 64) return wave_sum_f64(v);
+  v = row16_sum_f64(v);
+  if constexpr (kLanes == 32) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+    v = __builtin_bit_cast(double, (uint64_t)lo[0] | ((uint64_t)hi[0] << 32)) +
+        __builtin_bit_cast(double, (uint64_t)lo[1] | ((uint64_t)hi[1] << 32));
+  }
+  return v;
+}
+template <int kLanes>
+MXQ_DEVICE float lanes_sum(float v) {
+  v = sum16(v);
+  if constexpr (kLanes == 32) {
+    const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(q[0]) + __uint_as_float(q[1]);
+  }
+  return v;
+}
+
+// kLanes: what holds a row, 16, 32 or 64 lanes of a workgroup of 256 threads (781250 x 128 bf16, a head's columns: 71 us, 5.6
+// TB/s; 199 us with a wave per row), or 0, a workgroup.
+template <int kCode, int kOut, int kChunks, int kLanes, bool kVec>
+__global__ __launch_bounds__(kLanes ? 256 : 1024) void rms_norm_kernel(Rms p) {
+  constexpr bool kOne = kLanes != 0;
+  constexpr int kGroup = kOne ? kLanes : 64, kRows = 256 / kGroup;
   constexpr int kElem = Eight<kCode>::kElem;
   __shared__ double red[16];
-  const int waves = kOne ? 1 : blockDim.x >> 6, wave = kOne ? 0 : threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, row = kOne ? block * 4 + (threadIdx.x >> 6) : block;
-  if (row >= p.M) return;  // (whole waves; with several per row, whole workgroups)
+  const int waves = kOne ? 1 : blockDim.x >> 6, wave = kOne ? 0 : threadIdx.x >> 6, lane = threadIdx.x & (kGroup - 1);
+  const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, row = kOne ? block * kRows + threadIdx.x / kGroup : block;
+  if (row >= p.M) return;  // (all lanes of a row, which alone exchange values)
   auto col = [&](int i) { return ((i * waves + wave) * 64 + lane) * 8; };
   const char* x = p.x + row * p.ldx * kElem;
   Eight<kCode> s[kChunks];
@@ -215,7 +270,7 @@ __global__ __launch_bounds__(kOne ? 256 : 1024) void rms_norm_kernel(Rms p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) q = fma((double)v[e], (double)v[e], q);
   }
-  q = wave_sum_f64(q);
+  q = lanes_sum_f64<kGroup>(q);
   if constexpr (!kOne) {
     if (lane == 0) red[wave] = q;
     __syncthreads();
@@ -254,38 +309,53 @@ struct RmsGrad {
   int D, wcode;
 };
 
-template <int kCode, int kX, int kChunks, int kThreads, bool kVec>
-__global__ __launch_bounds__(kThreads) void rms_norm_grad_kernel(RmsGrad p) {
-  constexpr bool kOne = kThreads == 256;  // a wave per row, four rows per workgroup; else a workgroup per row
-  constexpr int kElem = Eight<kCode>::kElem, kElemX = Eight<kX>::kElem, kRows = kOne ? 4 : 1;
+// kLanes: as the forward pass.
+template <int kCode, int kX, int kChunks, int kLanes, bool kVec>
+__global__ __launch_bounds__(kLanes ? 256 : 1024) void rms_norm_grad_kernel(RmsGrad p) {
+  constexpr bool kOne = kLanes != 0;
+  constexpr int kGroup = kOne ? kLanes : 64;
+  constexpr int kElem = Eight<kCode>::kElem, kElemX = Eight<kX>::kElem, kRows = kOne ? 256 / kGroup : 1;
   __shared__ float red[2][2][16];
-  const int waves = kOne ? 1 : blockDim.x >> 6, wave = kOne ? 0 : threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int sub = kOne ? threadIdx.x >> 6 : 0;
+  const int waves = kOne ? 1 : blockDim.x >> 6, wave = kOne ? 0 : threadIdx.x >> 6, lane = threadIdx.x & (kGroup - 1);
+  const int sub = kOne ? threadIdx.x / kGroup : 0;
   const float inv = 1.0f / (float)p.D;
+  // Three chunks leave no registers for a row: it is read again behind its sum, from L2 (4882 x 20480 bf16: 155 us, 221 spilled).
+  constexpr bool kTwice = kChunks > 2;
   float dw[kChunks][8] = {};
-  auto col = [&](int i) { return ((i * waves + wave) * 64 + lane) * 8; };
+  auto col = [&](int i) {
+    int c = ((i * waves + wave) * 64 + lane) * 8;
+    if constexpr (kChunks > 1) __asm__ volatile("" : "+v"(c));  // (else every operand's address is held through the loop)
+    return c;
+  };
   const int64_t step = (int64_t)gridDim.x * kRows;
+  // What a lane keeps of a row is its raw words, from which the values are formed again behind the row's sum.
+  Eight<kCode> ty[kChunks], td[kChunks] = {};
+  Eight<kX> tx[kChunks];
+  uint32_t ts[kChunks];
+  auto load = [&](int64_t row, int i, bool ds) {
+    const int c = col(i), n = p.D - c;
+    ty[i] = load_run8<kCode, kVec>(p.dy + row * p.ldy * kElem, c, n);
+    tx[i] = load_run8<kX, kVec>(p.x + row * p.ldx * kElemX, c, n);
+    ts[i] = kX == kCodeFp8 ? (uint32_t)p.xs[row * p.ldxs + (n > 0 ? c >> 7 : 0)] : 0u;
+    if (ds) td[i] = load_run8<kCode, kVec>(p.ds + row * p.ldds * kElem, c, n);
+  };
   int turn = 0;
   for (int64_t row = (int64_t)blockIdx.x * kRows + sub; row < p.M; row += step, turn ^= 1) {
-    Eight<kCode> ry[kChunks], rd[kChunks];
-    Eight<kX> rx[kChunks];
-    uint32_t rs[kChunks];
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const int n = p.D - col(i);
-      ry[i] = load_run8<kCode, kVec>(p.dy + row * p.ldy * kElem, col(i), n);
-      rx[i] = load_run8<kX, kVec>(p.x + row * p.ldx * kElemX, col(i), n);
-      rs[i] = kX == kCodeFp8 ? (uint32_t)p.xs[row * p.ldxs + (n > 0 ? col(i) >> 7 : 0)] : 0u;
-      if (p.ds) rd[i] = load_run8<kCode, kVec>(p.ds + row * p.ldds * kElem, col(i), n);
-    }
+    for (int i = 0; i < kChunks; ++i)
+      if constexpr (!kTwice) load(row, i, p.ds);
     const float r = p.rstd[row];
     float s1 = 0.0f, none = 0.0f;
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
+      if constexpr (kChunks > 1) __builtin_amdgcn_sched_barrier(0);  // one chunk's values at a time
+      if constexpr (kTwice) load(row, i, false);
       float y[8], x[8], w[8];
-      weight8<kVec>(p.w, p.wcode, col(i), p.D - col(i), w);
-      to_f32(ry[i], 1.0f, y);
-      to_f32(rx[i], fp8_scale_f32(rs[i]), x);
+      uint64_t from = (uint64_t)p.w;
+      if constexpr (kChunks > 1) __asm__ volatile("" : "+s"(from));
+      weight8<kVec>((const char*)from, p.wcode, col(i), p.D - col(i), w);
+      to_f32(ty[i], 1.0f, y);
+      to_f32(tx[i], fp8_scale_f32(ts[i]), x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float xh = x[e] * r;
@@ -293,15 +363,31 @@ __global__ __launch_bounds__(kThreads) void rms_norm_grad_kernel(RmsGrad p) {
         dw[i][e] = fmaf(y[e], xh, dw[i][e]);
       }
     }
-    row_sum<kOne>(s1, none, red[turn], wave, waves, lane);
+    if constexpr (kGroup < 64)
+      s1 = lanes_sum<kGroup>(s1);
+    else
+      row_sum<kOne>(s1, none, red[turn], wave, waves, lane);
     const float a = r * r * (s1 * inv);  // dx = r g - x r^2 c + ds
+    int64_t again = row;
+    if constexpr (kTwice) __asm__ volatile("" : "+s"(again));
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
+      if constexpr (kChunks > 1) __builtin_amdgcn_sched_barrier(0);
+      if constexpr (kTwice) load(again, i, p.ds);
       float v[8], x[8], w[8], d[8] = {};
-      weight8<kVec>(p.w, p.wcode, col(i), p.D - col(i), w);
-      to_f32(ry[i], 1.0f, v);
-      to_f32(rx[i], fp8_scale_f32(rs[i]), x);
-      if (p.ds) to_f32(rd[i], 1.0f, d);
+      // (formed again from the words: the statements keep the compiler from holding the first pass's values instead)
+      if constexpr (kChunks > 1) {
+#pragma unroll
+        for (int k = 0; k < Eight<kCode>::kWords; ++k) __asm__ volatile("" : "+v"(ty[i].w[k]));
+#pragma unroll
+        for (int k = 0; k < Eight<kX>::kWords; ++k) __asm__ volatile("" : "+v"(tx[i].w[k]));
+      }
+      uint64_t from = (uint64_t)p.w;
+      if constexpr (kChunks > 1) __asm__ volatile("" : "+s"(from));
+      weight8<kVec>((const char*)from, p.wcode, col(i), p.D - col(i), w);
+      to_f32(ty[i], 1.0f, v);
+      to_f32(tx[i], fp8_scale_f32(ts[i]), x);
+      if (p.ds) to_f32(td[i], 1.0f, d);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e] * w[e], r, -(x[e] * a)) + d[e];
       store_run8<kCode, kVec>(p.dx + row * p.D * kElem, col(i), p.D - col(i), from_f32<kCode>(v));
@@ -309,16 +395,16 @@ __global__ __launch_bounds__(kThreads) void rms_norm_grad_kernel(RmsGrad p) {
   }
   if (!p.sums) return;
   float* out = p.sums + (int64_t)blockIdx.x * p.D;
-  if constexpr (kOne) {  // the workgroup's four waves hold the same columns: their sums in order
-    __shared__ float part[4][64 * 8];
+  if constexpr (kOne) {  // the workgroup's rows hold the same columns: their sums in order
+    __shared__ float part[kRows][kGroup * 8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) part[sub][e * 64 + lane] = dw[0][e];
+    for (int e = 0; e < 8; ++e) part[sub][e * kGroup + lane] = dw[0][e];
     __syncthreads();
+    for (int c = threadIdx.x; c < p.D; c += 256) {
+      float v = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int j = sub * 2 + e;
-      if (lane * 8 + j < p.D)
-        out[lane * 8 + j] = ((part[0][j * 64 + lane] + part[1][j * 64 + lane]) + part[2][j * 64 + lane]) + part[3][j * 64 + lane];
+      for (int g = 0; g < kRows; ++g) v += part[g][c % 8 * kGroup + c / 8];
+      out[c] = v;
     }
   } else {
 #pragma unroll
@@ -337,23 +423,41 @@ __global__ __launch_bounds__(kThreads) void rms_norm_grad_kernel(RmsGrad p) {
   }
 }
 
-// Waves and chunks of the forward pass.
+// Lanes of a row of at most 512 elements.
+static int64_t row_lanes(int64_t D) { return D <= 128 ? 16 : D <= 256 ? 32 : 64; }
+template <class F>
+static void with_lanes(int D, F&& f) {
+  using std::integral_constant;
+  if (D <= 128) f(integral_constant<int, 16>{});
+  else if (D <= 256) f(integral_constant<int, 32>{});
+  else f(integral_constant<int, 64>{});
+}
+// Chunks, lanes (0: a workgroup) and threads of the forward pass.
 template <class F>
 static void with_rms_shape(int D, F&& f) {
   using std::integral_constant;
   const int n = (D + 511) / 512;
-  auto go = [&](auto N) { f(N, std::false_type{}, (n + decltype(N)::value - 1) / decltype(N)::value * 64); };
-  if (n <= 1) f(integral_constant<int, 1>{}, std::true_type{}, 256);
+  auto go = [&](auto N) { f(N, integral_constant<int, 0>{}, (n + decltype(N)::value - 1) / decltype(N)::value * 64); };
+  if (n <= 1) with_lanes(D, [&](auto L) { f(integral_constant<int, 1>{}, L, 256); });
   else if (n <= 4) go(integral_constant<int, 2>{});
   else if (n <= 12) go(integral_constant<int, 4>{});
   else go(integral_constant<int, 6>{});
 }
+// And of the backward pass.
+template <class F>
+static void with_grad_shape(int D, F&& f) {
+  with_shape(D, [&](auto N, auto T, int threads) {
+    if constexpr (decltype(T)::value == 256) with_lanes(D, [&](auto L) { f(N, L, threads); });
+    else f(N, std::integral_constant<int, 0>{}, threads);
+  });
+}
 
 // Workgroups of the backward pass: about twenty waves per CU, each with an equal share of rows, eight rows at least once every
-// CU has a workgroup, since each writes D sums.
+// CU has a workgroup, since each writes D sums. (Two workgroups of eleven or twelve waves: 18600 x 5376 bf16 in 128 us, 154 with
+// one. Four of six instead of three: 33333 x 3000 180 instead of 142.)
 static int64_t rms_grad_grid(int64_t M, int64_t D, int cus) {
-  const int64_t n = (D + 511) / 512, units = n <= 1 ? (M + 3) / 4 : M;
-  const int64_t most = cus * (n <= 1 ? 5 : n <= 16 ? (20 / n > 1 ? 20 / n : 1) : 1);
+  const int64_t n = (D + 511) / 512, rows = n <= 1 ? 256 / row_lanes(D) : 1, units = (M + rows - 1) / rows;
+  const int64_t most = cus * (n <= 1 ? 5 : n <= 10 ? 20 / n : n <= 12 ? 2 : 1);
   const int64_t few = units < cus ? units : units / 8 > cus ? units / 8 : cus;
   return few < most ? few : most;
 }
@@ -389,10 +493,9 @@ extern "C" int mxq_rms_norm(const void* x, const void* r, int dtype, int64_t ldx
     return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");
   const Rms p = {(const char*)x, (const char*)r, (const char*)w, (char*)sum, (char*)y, scale, rstd, M, ldx, ldr, ldq, lds, (int)D,
                  param_dtype, 1.0 / (double)D, (double)eps};
-  with_rms_shape((int)D, [&](auto N, auto One, int threads) {
-    constexpr bool kOne = decltype(One)::value;
-    constexpr int kChunks = decltype(N)::value;
-    const int64_t blocks = kOne ? (M + 3) / 4 : M;
+  with_rms_shape((int)D, [&](auto N, auto L, int threads) {
+    constexpr int kChunks = decltype(N)::value, kLanes = decltype(L)::value, kRows = kLanes ? 256 / kLanes : 1;
+    const int64_t blocks = (M + kRows - 1) / kRows;
     const unsigned wide = (unsigned)(blocks < kRmsGridX ? blocks : kRmsGridX);
     const dim3 grid(wide, (unsigned)((blocks + wide - 1) / wide));
     with_dtype(dtype, [&](auto C) {
@@ -400,11 +503,11 @@ extern "C" int mxq_rms_norm(const void* x, const void* r, int dtype, int64_t ldx
       with_bool(D % 8 == 0, [&](auto V) {
         constexpr bool kVec = decltype(V)::value;
         if (fp8)
-          hipLaunchKernelGGL((rms_norm_kernel<kCode, kOutFp8, kChunks, kOne, kVec>), grid, dim3(threads), 0, (hipStream_t)stream, p);
+          hipLaunchKernelGGL((rms_norm_kernel<kCode, kOutFp8, kChunks, kLanes, kVec>), grid, dim3(threads), 0, (hipStream_t)stream, p);
         else if (fp4)
-          hipLaunchKernelGGL((rms_norm_kernel<kCode, kOutFp4, kChunks, kOne, kVec>), grid, dim3(threads), 0, (hipStream_t)stream, p);
+          hipLaunchKernelGGL((rms_norm_kernel<kCode, kOutFp4, kChunks, kLanes, kVec>), grid, dim3(threads), 0, (hipStream_t)stream, p);
         else
-          hipLaunchKernelGGL((rms_norm_kernel<kCode, kOutSame, kChunks, kOne, kVec>), grid, dim3(threads), 0, (hipStream_t)stream, p);
+          hipLaunchKernelGGL((rms_norm_kernel<kCode, kOutSame, kChunks, kLanes, kVec>), grid, dim3(threads), 0, (hipStream_t)stream, p);
       });
     });
   });
@@ -435,13 +538,13 @@ extern "C" int mxq_rms_norm_backward(const void* dy, int dtype, int64_t ldy, con
   float* sums = dweight ? (float*)workspace : nullptr;
   const RmsGrad p = {(const char*)dy, (const char*)x, (const char*)w, (const char*)dsum, x_scale, rstd, (char*)dx, sums, M, ldy, ldx, ldxs,
                      ldds, (int)D, param_dtype};
-  with_shape((int)D, [&](auto N, auto T, int threads) {
+  with_grad_shape((int)D, [&](auto N, auto L, int threads) {
     with_dtype(dtype, [&](auto C) {
-      constexpr int kCode = decltype(C)::value, kChunks = decltype(N)::value, kThreads = decltype(T)::value;
+      constexpr int kCode = decltype(C)::value, kChunks = decltype(N)::value, kLanes = decltype(L)::value;
       with_bool(D % 8 == 0, [&](auto V) {
         with_bool(kept, [&](auto K) {
           constexpr int kX = decltype(K)::value ? kCodeFp8 : kCode;
-          hipLaunchKernelGGL((rms_norm_grad_kernel<kCode, kX, kChunks, kThreads, decltype(V)::value>), dim3((unsigned)grid),
+          hipLaunchKernelGGL((rms_norm_grad_kernel<kCode, kX, kChunks, kLanes, decltype(V)::value>), dim3((unsigned)grid),
                              dim3(threads), 0, (hipStream_t)stream, p);
         });
       });

@@ -191,6 +191,8 @@ def test_prepared_weights(dev, dtype, n, k):
         assert all(int(got[at]) == byte for at, byte in places.items())
         rows = got.view(-1, -(-k // 512), 2, 32, 8).permute(0, 3, 1, 2, 4).reshape(-1, -(-k // 512) * 16)[:n]
         assert bool((rows != 255).all())
+    again = mx.prepare_mxfp4_weight(w.to(dev))
+    assert torch.equal(a.scale, again.scale) and torch.equal(a.q, again.q)
 
 
 # ---------------------------------------------------------------------------------------
@@ -540,3 +542,88 @@ def test_modules_are_not_captured(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, want)
+
+
+def test_pairs_in_any_order(dev):
+    """Transposed and strided codes and scales, and leading dimensions that no view merges."""
+    mx = _mx()
+    g = _gen(8)
+    q = torch.randint(0, 256, (40, 5, 32), generator=g).to(torch.uint8)
+    s = torch.randint(120, 131, (40, 5, 2), generator=g).to(torch.uint8)
+    wq = torch.randint(0, 256, (48, 32), generator=g).to(torch.uint8)
+    ws = torch.randint(120, 131, (48, 2), generator=g).to(torch.uint8)
+    wv = ob.values(wq, ws, 64)
+    turned = (wq.t().contiguous().to(dev).t().view(CODES), ws.t().contiguous().to(dev).t().view(SCALE))
+    weight = mx.prepare_mxfp4_weight(*turned)
+    plain = mx.prepare_mxfp4_weight(wq.to(dev).view(CODES), ws.to(dev).view(SCALE))
+    assert torch.equal(weight.q, plain.q)
+    assert torch.equal(mx.dequantize_mxfp4(*turned, torch.float32).cpu().double(), wv)
+    for order in ((0, 1, 2), (1, 0, 2)):
+        qv, sv = q.permute(order), s.permute(order)
+        xv = ob.values(qv.reshape(200, 32), sv.reshape(200, 2), 64)
+        pair = (q.to(dev).permute(order).view(CODES), s.to(dev).permute(order).view(SCALE))
+        assert torch.equal(mx.dequantize_mxfp4(*pair, torch.float32).cpu().double(), xv.view(*qv.shape[:2], 64))
+        y = mx.mxfp4_linear_prequantized(*pair, weight, None, torch.float32)
+        assert y.shape == (*qv.shape[:2], 48)
+        check_product(y.reshape(200, 48), xv, wv, None)
+
+
+def test_a_layer_made_in_inference_mode_trains(dev):
+    mx = _mx()
+    w, x0 = _acts(40, 96, torch.bfloat16, 1), _acts(20, 96, torch.bfloat16, 2)
+    with torch.inference_mode():
+        layer = mx.Mxfp4Linear.from_weight(w.to(dev), torch.zeros(40, dtype=torch.bfloat16, device=dev))
+    x = x0.to(dev).requires_grad_()
+    y = layer(x)
+    dy = torch.ones_like(y)
+    y.backward(dy)
+    check_gradients(x.grad, layer.bias.grad, dy.cpu(), ob.rows(w)[0])
+
+
+def test_more_than_2_to_the_32_elements(dev):
+    """Rows on both sides of every power of two that an offset could be cut at, against the same rows by themselves."""
+    mx = _mx()
+    m, k = 135_000, 32_768  # 4.4e9 elements
+    x = torch.empty(m, k, dtype=torch.bfloat16, device=dev)
+    for i in range(0, m, 27_000):
+        x[i:i + 27_000].normal_()
+    at = sorted({0, m - 1, *(min(m - 1, 2**p // w + d) for p in (29, 30, 31, 32) for w in (k // 2, k, 2 * k) for d in (-1, 0, 1))})
+    at = torch.tensor([i for i in at if 0 <= i < m])
+    few = x[at.to(dev)]
+    q, s = mx.quantize_mxfp4(x)
+    del x
+    _, b, codes = ob.rows(few.cpu())
+    assert torch.equal(q.view(torch.uint8)[at.to(dev)].cpu(), ob.pack(codes))
+    assert torch.equal(s.view(torch.uint8)[at.to(dev)].cpu().int(), b)
+    back = mx.dequantize_mxfp4(q, s)
+    assert torch.equal(back[at.to(dev)].cpu().double(), ob.rows(few.cpu())[0])
+    del back
+    w = _acts(40, k, torch.bfloat16, 4)
+    y = mx.mxfp4_linear_prequantized(q, s, mx.prepare_mxfp4_weight(w.to(dev)))
+    check_product(y[at.to(dev)], ob.rows(few.cpu())[0], ob.rows(w)[0], None)
+
+
+def test_products_of_more_than_2_to_the_32_elements(dev):
+    mx = _mx()
+    m, n, k = 135_000, 32_768, 64
+    w = _acts(n, k, torch.bfloat16, 4, 0.5)
+    weight = mx.prepare_mxfp4_weight(w.to(dev))
+    x = torch.randn(m, k, device=dev, dtype=torch.bfloat16)
+    at = sorted({0, m - 1, *(min(m - 1, 2**p // n + d) for p in (29, 30, 31, 32) for d in (-1, 0, 1))})
+    at = torch.tensor([i for i in at if 0 <= i < m])
+    wv = ob.rows(w)[0]
+    y = mx.mxfp4_linear(x, weight)
+    check_product(y[at.to(dev)], ob.rows(x[at.to(dev)].cpu())[0], wv, None)
+    dx, db = mx.mxfp4_linear_backward(y, weight)  # (y as the gradient: 4.4e9 elements)
+    check_gradients(dx[at.to(dev)], None, y[at.to(dev)].cpu(), wv)
+    total, size = torch.zeros(n, dtype=torch.float64, device=dev), torch.zeros(n, dtype=torch.float64, device=dev)
+    for i in range(0, m, 13_500):
+        part = y[i:i + 13_500].double()
+        total += part.sum(0)
+        size += part.abs().sum(0)
+    assert bool(((db.double() - total).abs() <= 2.0**-24 * (m + 2) * size).all())
+    del dx, db, x
+    turned = mx.prepare_mxfp4_weight(_acts(k, n, torch.bfloat16, 5, 0.5).to(dev))  # (and a gradient of as many)
+    dy = torch.randn(m, k, device=dev, dtype=torch.float16)
+    dx, _ = mx.mxfp4_linear_backward(dy, turned)
+    check_gradients(dx[at.to(dev)], None, dy[at.to(dev)].cpu(), ob.rows(_acts(k, n, torch.bfloat16, 5, 0.5))[0])

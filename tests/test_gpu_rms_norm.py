@@ -382,3 +382,35 @@ def test_module_is_not_captured(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("m,d", [(210_000, 20_480), (33_600_000, 128)])
+def test_more_than_2_to_the_32_elements(dev, m, d):
+    """Rows on both sides of every power of two that an offset could be cut at."""
+    mx = _mx()
+    x = torch.empty(m, d, dtype=torch.bfloat16, device=dev)
+    for i in range(0, m, m // 5):
+        x[i:i + m // 5].normal_()
+    at = sorted({0, m - 1, *(min(m - 1, 2**p // d + e) for p in (29, 30, 31, 32) for e in (-1, 0, 1))})
+    at = torch.tensor([i for i in at if 0 <= i < m])
+    w = _weight(d, torch.bfloat16, 3)
+    y, s, rstd = mx.rms_norm(x, w.to(dev), 1e-6, residual=x, return_rstd=True)
+    few = (2 * x[at.to(dev)].float()).to(torch.bfloat16).cpu()
+    assert torch.equal(s[at.to(dev)].cpu(), few)
+    r = rstd[at.to(dev)].cpu()
+    check_rstd(r, few, 1e-6)
+    want = ob.normed(few, r, w)
+    assert torch.equal(y[at.to(dev)].cpu(), want.to(torch.bfloat16))
+    del y
+    q, sc = mx.rms_norm_quantize_mxfp4(x, w.to(dev), 1e-6, residual=x)[:2]
+    check_codes4(q.view(torch.uint8)[at.to(dev)].view(torch.float4_e2m1fn_x2), sc.view(torch.uint8)[at.to(dev)].view(torch.float8_e8m0fnu),
+                 want)
+    del q, sc
+    dx, dw = mx.rms_norm_backward(x, s, rstd, w.to(dev), x)
+    check_backward(dx[at.to(dev)], None, x[at.to(dev)].cpu(), few, r, w, x[at.to(dev)].cpu())
+    total, size = torch.zeros(d, dtype=torch.float64, device=dev), torch.zeros(d, dtype=torch.float64, device=dev)
+    for i in range(0, m, m // 20):
+        part = x[i:i + m // 20].double() * s[i:i + m // 20].double() * rstd[i:i + m // 20, None].double()
+        total += part.sum(0)
+        size += part.abs().sum(0)
+    assert bool(((dw.double() - total).abs() <= 2.0**-24 * (m + 4) * size).all())

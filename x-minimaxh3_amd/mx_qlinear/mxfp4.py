@@ -4,7 +4,9 @@ The format is e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two i
 bits, with a power of two (an E8M0 byte) per 1 x 32 block of a row, for activations and weights alike: what gfx950's 4-bit
 matrix instructions read. Block scales are the smallest 2^e (e >= -125) with ``absmax <= 6 * 2^e``, so no value is cut off;
 codes are ``x / 2^e`` rounded once to nearest even. e2m1 has no NaN: a block with a NaN or an infinity has the scale byte
-255 and is NaN throughout. Pairs of other making are taken too: any code and scale byte.
+255 and is NaN throughout. Pairs of other making are taken too: any code and scale byte (the input's gradient may count weights
+below 2^-126, which only the bytes 0 and 1 make, as zeros, and takes one that is past float32's range, 6 * 2^126 and more, as
+an infinity).
 
 No counterpart in the reference. Every function runs the HIP kernels of libmx_qlinear.so on the tensors' GPU and current
 stream; there is no CPU path.
@@ -146,8 +148,10 @@ def prepare_mxfp4_weight(weight: torch.Tensor, scale: torch.Tensor | None = None
     else:
         q, s, _, k = _pair(weight, scale, in_features, "weight")
     dev = _require_gpu(weight, scale)
-    out = torch.empty(n, _row_bytes(k), dtype=torch.uint8, device=dev)
-    tiles = torch.empty(_scale_bytes(n, k), dtype=torch.uint8, device=dev)
+    with torch.inference_mode(False):  # (tensors made in that mode cannot be saved for a backward pass)
+        out = torch.empty(n, _row_bytes(k), dtype=torch.uint8, device=dev)
+        # (the places of a last tile's missing rows, which no product uses: the same bytes for the same weight)
+        tiles = (torch.empty if n % 32 == 0 else torch.zeros)(_scale_bytes(n, k), dtype=torch.uint8, device=dev)
     if scale is None:
         w = _rows_in_place(weight, k)
         _launch(dev, "mxq_mxfp4_quantize_rows", w.data_ptr(), code, w.stride(0) if n > 1 else k, out.data_ptr(), out.shape[1],
@@ -303,7 +307,8 @@ class Mxfp4Linear(torch.nn.Module):
         if bias is not None:
             if bias.shape != (form.out_features,):
                 raise ValueError(f"bias of shape {tuple(bias.shape)}, expected ({form.out_features},)")
-            layer.bias = torch.nn.Parameter(bias.detach().clone())
+            with torch.inference_mode(False):
+                layer.bias = torch.nn.Parameter(bias.detach().clone())
         return layer
 
     def prepared(self) -> PreparedMxfp4Weight:

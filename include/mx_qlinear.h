@@ -658,7 +658,7 @@ int mxq_mxfp4_gemm(const uint8_t* a, int64_t lda, const uint8_t* sa, const uint8
                    const void* bias, void* d, int64_t ldd, int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
                    int64_t workspace_bytes, void* stream);
 
-/* Bytes of workspace mxq_mxfp4_linear needs at this size on the current device (0 up to 16 rows). */
+/* Bytes of workspace mxq_mxfp4_linear needs at this size on the current device (0 for up to 16 rows of no long K). */
 int mxq_mxfp4_linear_workspace(int64_t M, int64_t N, int64_t K, int64_t* bytes);
 
 /* The layer's forward pass in one call: d [M, N] = out(quantize(x) b^T + bias), x [M, ldx] of x_dtype; the rest as above. */
@@ -666,7 +666,8 @@ int mxq_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* b, 
                      void* d, int64_t ldd, int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
                      void* stream);
 
-/* Bytes of workspace mxq_mxfp4_linear_prequantized needs at this size on the current device (0 up to 16 rows). */
+/* Bytes of workspace mxq_mxfp4_linear_prequantized needs at this size on the current device (0 for up to 16 rows of no long
+ * K). */
 int mxq_mxfp4_linear_prequantized_workspace(int64_t M, int64_t N, int64_t K, int direct, int64_t* bytes);
 
 /*

@@ -201,7 +201,7 @@ def test_prepared_weights(dev, dtype, n, k):
 
 PRODUCTS = [(1, 1, 1), (1, 16, 32), (1, 100, 5000), (2, 33, 257), (7, 300, 520), (15, 17, 1000), (16, 2049, 640), (17, 64, 33),
             (31, 129, 31), (33, 257, 255), (64, 96, 4096), (100, 520, 1025), (130, 130, 5120), (257, 300, 256), (300, 1000, 777),
-            (600, 260, 2048), (1100, 513, 100)]
+            (600, 260, 2048), (1100, 513, 100), (5, 33, 20480), (16, 70, 9000), (16, 40, 20480)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -11,9 +11,10 @@ struct Forward {
   void* gemm;
   int64_t ldq, gemm_bytes, total;
 };
-int forward_space(uint8_t* base, int64_t M, int64_t N, int64_t K, bool codes, Forward& f) {
+// codes: the call makes its own copy of the codes.
+int forward_space(uint8_t* base, int64_t M, int64_t N, int64_t K, bool pair, bool codes, Forward& f) {
   f = {};
-  if (M <= kFp4FusedRows) return MXQ_OK;
+  if (fp4_few_rows(M, N, K, pair)) return MXQ_OK;
   Carve c{base};
   f.ldq = fp4_row_bytes(K);
   f.q = c.take<uint8_t>(codes ? M * f.ldq : 0);
@@ -65,7 +66,7 @@ int check_workspace(const void* workspace, int64_t have, int64_t need) {
 extern "C" int mxq_mxfp4_linear_workspace(int64_t M, int64_t N, int64_t K, int64_t* bytes) {
   if (!sizes_ok(M, N, K) || !bytes) return mxq_set_error(MXQ_ERR_INVALID, "bad argument");
   Forward f;
-  if (const int rc = forward_space(nullptr, M, N, K, true, f)) return rc;
+  if (const int rc = forward_space(nullptr, M, N, K, false, true, f)) return rc;
   *bytes = f.total;
   return MXQ_OK;
 }
@@ -78,10 +79,10 @@ extern "C" int mxq_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const u
   if (M == 0) return MXQ_OK;
   if (!float_dtype(x_dtype)) return mxq_set_error(MXQ_ERR_INVALID, "unsupported input dtype code %d", x_dtype);
   if (!x || ldx < K) return mxq_set_error(MXQ_ERR_INVALID, "null activations or bad row strides of the activations for K=%lld", (long long)K);
-  if (M <= kFp4FusedRows)
+  if (fp4_few_rows(M, N, K, false))
     return fp4_linear_rows(x, x_dtype, ldx, nullptr, 0, b, ldb, sb, bias, d, ldd, out_dtype, M, N, K, stream);
   Forward f;
-  if (const int rc = forward_space((uint8_t*)workspace, M, N, K, true, f)) return rc;
+  if (const int rc = forward_space((uint8_t*)workspace, M, N, K, false, true, f)) return rc;
   if (const int rc = check_workspace(workspace, workspace_bytes, f.total)) return rc;
   // (every refusal is ahead of the first launch)
   if (const int rc = fp4_gemm_check(f.q, f.ldq, f.s, b, ldb, sb, d, ldd, out_dtype, M, N, K)) return rc;
@@ -92,7 +93,7 @@ extern "C" int mxq_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const u
 extern "C" int mxq_mxfp4_linear_prequantized_workspace(int64_t M, int64_t N, int64_t K, int direct, int64_t* bytes) {
   if (!sizes_ok(M, N, K) || !bytes) return mxq_set_error(MXQ_ERR_INVALID, "bad argument");
   Forward f;
-  if (const int rc = forward_space(nullptr, M, N, K, !direct, f)) return rc;
+  if (const int rc = forward_space(nullptr, M, N, K, true, !direct, f)) return rc;
   *bytes = f.total;
   return MXQ_OK;
 }
@@ -109,10 +110,10 @@ extern "C" int mxq_mxfp4_linear_prequantized(const uint8_t* q, int64_t ldq, cons
     return mxq_set_error(MXQ_ERR_INVALID, "the product cannot read these codes directly");
   if (M == 0) return MXQ_OK;
   if (!q || !scale) return mxq_set_error(MXQ_ERR_INVALID, "null activations");
-  if (M <= kFp4FusedRows)
+  if (fp4_few_rows(M, N, K, true))
     return fp4_linear_rows(q, MXQ_DTYPE_E2M1, ldq, scale, lds, b, ldb, sb, bias, d, ldd, out_dtype, M, N, K, stream);
   Forward f;
-  if (const int rc = forward_space((uint8_t*)workspace, M, N, K, !direct, f)) return rc;
+  if (const int rc = forward_space((uint8_t*)workspace, M, N, K, true, !direct, f)) return rc;
   if (const int rc = check_workspace(workspace, workspace_bytes, f.total)) return rc;
   const uint8_t* a = direct ? q : f.q;
   const int64_t lda = direct ? ldq : f.ldq;

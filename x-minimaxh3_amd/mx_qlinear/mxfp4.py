@@ -176,8 +176,8 @@ def _check_weight(weight: PreparedMxfp4Weight, k: int) -> None:
 def mxfp4_linear(x: torch.Tensor, weight: PreparedMxfp4Weight, bias: torch.Tensor | None = None,
                  out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``x @ weight.T + bias`` with ``x [..., K]`` quantized as :func:`quantize_mxfp4` does; ``out_dtype`` defaults to ``x``'s.
-    Up to 16 rows are quantized inside the product's launch. Sums are float32: a block's 32 products are added exactly, and
-    the blocks' sums with what lies below 2^-22 of the largest cut."""
+    Up to 16 rows, or fewer of a long ``K``, are quantized inside the product's launch. Sums are float32: a block's 32
+    products are added exactly, and the blocks' sums with what lies below 2^-22 of the largest cut."""
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError("mxfp4_linear needs a non-empty last dimension")
     _check_weight(weight, x.shape[-1])
@@ -201,7 +201,8 @@ def mxfp4_linear(x: torch.Tensor, weight: PreparedMxfp4Weight, bias: torch.Tenso
 
 def mxfp4_linear_prequantized(q: torch.Tensor, scale: torch.Tensor, weight: PreparedMxfp4Weight, bias: torch.Tensor | None = None,
                               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """:func:`mxfp4_linear` of an input that is a ``(codes, scale)`` pair already; up to 16 rows are one launch."""
+    """:func:`mxfp4_linear` of an input that is a ``(codes, scale)`` pair already; up to 16 rows, or fewer of a long
+    ``K``, are one launch."""
     if not isinstance(weight, PreparedMxfp4Weight):
         raise TypeError(f"weight must come from prepare_mxfp4_weight, got {type(weight).__name__}")
     lead = q.shape[:-1]

@@ -82,11 +82,11 @@ int fp4_dgrad(const void* dy, int parts, int64_t ldy, const uint8_t* b, int64_t 
 constexpr int64_t kFp4FusedRows = 16;
 // Where a layer's call takes it. Every workgroup brings all of x, M K elements, while the weight, N K, streams; tiles of 128 rows
 // cost a launch, a join and idle rows instead, about the same for one row and sixteen. Measured, few-row kernel / tiles in us, x
-// in bf16: K 5120, N 5120, 16 rows 12.2 / 13.0; K 20480, N 5120, 6 rows 23.3 / 23.7, 8 25.5 / 23.6, 16 31.2 / 24.0; K 20480, N
-// 20480, 16 rows 55.0 / 57.6; K 40960, N 1024, 4 rows 19.6 / 15.7, 16 39.2 / 16.0. Pairs, which need no quantizing: K 20480,
-// N 5120, 12 rows 22.9 / 24.1, 16 25.4 / 23.9; K 40960, N 1024, 16 rows 31.0 / 16.4.
+// in bf16: K 5120, N 5120, 16 rows 11.4 / 12.4; K 20480, N 5120, 6 rows 20.0 / 22.8, 8 22.6 / 22.9, 16 28.6 / 23.1; K 14336, N 5376,
+// 8 rows 17.8 / 18.5, 16 23.1 / 18.7; K 20480, N 20480, 16 rows 54.2 / 56.9; K 40960, N 1024, 2 rows 17.7 / 15.7, 16 42.7 / 16.5.
+// Pairs, which need no quantizing: K 20480, N 5120, 12 rows 20.8 / 23.4, 16 22.9 / 23.3; K 40960, N 1024, 16 rows 29.2 / 16.8.
 inline bool fp4_few_rows(int64_t M, int64_t N, int64_t K, bool pair) {
-  return M <= kFp4FusedRows && M * K <= (pair ? 2 : 1) * (80000 + 12 * N);
+  return M <= kFp4FusedRows && M * K <= (pair ? 2 : 1) * (90000 + 12 * N);
 }
 int fp4_linear_rows(const void* x, int x_dtype, int64_t ldx, const uint8_t* sx, int64_t ldsx, const uint8_t* b, int64_t ldb,
                     const uint8_t* sb, const void* bias, void* d, int64_t ldd, int out_dtype, int64_t M, int64_t N, int64_t K,

@@ -1,11 +1,12 @@
 // The 4-bit layer of few rows (up to 16; mxfp4_common.h): a stream of the weight.
 //
-// A workgroup's four or eight waves take 16 kRT weight rows and share K. Weight fragments go from memory straight to registers (a
+// A workgroup's four or eight waves take up to 16 kRT weight rows and share K. Weight fragments go from memory straight to registers (a
 // lane: row l % 16, blocks l / 16 and 4 + l / 16 of a stage of 256 columns), a stage ahead of the one at work, and are multiplied by
 // v_mfma_scale_f32_16x16x128_f8f6f4 as they are, each lane giving the scale byte of its own block. The activations come in their
 // own type or as a pair; each wave brings its own K range of them, a chunk of stages at a time, into its part of LDS, quantizing
 // them on the way, which saves the quantizer's launch. How many weight rows a workgroup takes decides (plan_rows): each
-// workgroup quantizes all of x again, and what counts is the CU with the most weight rows.
+// workgroup quantizes all of x again, and what counts is the CU with the most weight rows. Missing rows of a block of sixteen are
+// not read.
 #include <algorithm>
 
 #include "mxfp4_common.h"
@@ -21,6 +22,7 @@ struct Fp4Rows {
   int64_t M, N, K, ldx, ldsx, ldb, ldd;
   int x_code, groups, stages;
   int chunk_log2;  // stages per chunk
+  int rows;        // weight rows of a workgroup: a multiple of 4, 16 kRT at most
 };
 
 // LDS of a wave's chunk: rows of codes, 16 bytes apart in banks, then eight scale bytes per row and stage.
@@ -95,9 +97,9 @@ __global__ __launch_bounds__(512) void mxfp4_rows_kernel(Fp4Rows p) {
   const int kW = blockDim.x >> 6;
   extern __shared__ __align__(16) uint8_t rows_lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
-  const int N = (int)p.N, M = (int)p.M, n0 = blockIdx.x * (16 * kRT);
+  const int N = (int)p.N, M = (int)p.M, n0 = blockIdx.x * p.rows;
   const int per = (p.stages + kW - 1) / kW, first = wave * per, last = min(first + per, p.stages);
-  const int rows = min(N - n0, 16 * kRT), row_tiles = p.groups * (int)kFp4ScaleTile;
+  const int rows = min(N - n0, p.rows), row_tiles = p.groups * (int)kFp4ScaleTile;
   const uint8_t* wb = p.b + (int64_t)n0 * p.ldb;
   const uint8_t* sb = p.sb + (int64_t)(n0 >> 5) * row_tiles;
   const int wbytes = rows * (int)p.ldb, sbytes = (((n0 & 31) + rows + 31) >> 5) * row_tiles;
@@ -168,7 +170,7 @@ __global__ __launch_bounds__(512) void mxfp4_rows_kernel(Fp4Rows p) {
     const int col = n0 + r * 16 + g * 4;
     v4f y = part[r * 64 + lane];
     for (int k = 1; k < kW; ++k) y += part[(k * kRT + r) * 64 + lane];
-    if (lr < M && col < N) {
+    if (lr < M && col < n0 + rows) {
       y += bias_run<kOut>(p.bias, col, N);
       const float v[4] = {y[0], y[1], y[2], y[3]};
       store_run4<kOut>(reinterpret_cast<char*>(p.d) + lr * p.ldd * kElem, col, N - col, v);
@@ -176,29 +178,29 @@ __global__ __launch_bounds__(512) void mxfp4_rows_kernel(Fp4Rows p) {
   }
 }
 
-// Weight rows (in sixteens) and waves of a workgroup, by an estimate in microseconds: the CU with the most workgroups streams their
-// weight rows, 0.090 (four waves) or 0.079 (eight) per sixteen and stage, and brings x for each workgroup, 0.012 per row and stage,
-// more where four waves are alone on their CU; all CUs together stream at 5.2 TB/s; eight waves take 1.5 us more to start and end.
-// Measured, bf16, weights from memory, by 16 / 32 / 48 weight rows and four waves, 16 / 32 / 48 / 64 / 80 / 96 / 128 and eight: one row,
-// K 5120, N 5120: 6.4 6.4 8.1, 6.6 6.1 7.8 9.8 11.7 13.2 18.9; N 20480: 13.0 15.1 14.6, 17.4 15.6 16.7 21.5 15.5 16.4 24.3;
-// K 20480, N 5120: 17.9 18.0 23.7, 17.9 16.5 22.1 28.1 34.8 40.0 69.4; 16 rows, K 5120, N 5120: 16.2 14.1 15.5, 14.5 11.3 12.9 14.5
-// 15.9 17.0 23.3; N 20480: 34.1 27.7 25.3, 33.7 26.3 27.4 30.9 19.7 20.8 29.4.
+// Weight rows (a multiple of 4: mostly what gives every CU its share and no more) and waves of a workgroup, by an estimate in
+// microseconds: the CU with the most workgroups streams their weight rows, 0.090 (four waves) or 0.079 (eight) per sixteen and stage,
+// half of it for a block's missing rows too, and brings x for each workgroup, 0.013 per row and stage, 0.025 where four waves are
+// alone on their CU; all CUs together stream at 5.2 TB/s; eight waves take longer to start and to add up. Measured, bf16, weights from
+// memory, by rows and waves: one row, K 5120, N 5120: 20/4 6.1, 32/4 6.5, 20/8 6.0, 32/8 6.2, 64/8 9.9; N 20480: 16/4 13.0, 32/4 15.2,
+// 80/8 15.6; K 20480, N 5120: 16/4 17.8, 20/4 15.8, 32/4 17.9, 16/8 18.0, 20/8 14.6, 32/8 16.4; K 14336, N 5376: 16/4 12.5, 24/8 11.9,
+// 32/8 12.5; four rows, K 20480, N 5120: 20/4 22.1, 20/8 18.4, 32/8 20.4; K 5376, N 21504: 28/4 15.7, 44/4 16.1, 84/8 17.7; 16 rows,
+// K 5120, N 20480: 16/4 33.9, 48/4 25.3, 80/8 19.7.
 struct RowsPlan4 {
-  int rt, waves;
+  int rows, waves;
   double cost;
 };
 static RowsPlan4 plan_rows(int64_t M, int64_t N, int64_t stages, int cus) {
-  RowsPlan4 best = {1, 4, 1e300};
+  RowsPlan4 best = {16, 4, 1e300};
   const double stream = (double)(N * stages) * 136.0 / 5.2e6;
   for (int waves = 4; waves <= 8; waves += 4) {
-    for (const int rt : {1, 2, 3, 4, 5, 6, 8}) {
-      if (waves == 4 && rt > 3) break;
-      const int64_t groups = (N + 16 * rt - 1) / (16 * rt);
-      const double turns = (double)((groups + cus - 1) / cus);
-      const double units = turns * (double)(stages * rt) * (waves == 4 ? 0.090 : 0.079);
-      const double rows = turns * (double)(stages * M) * (waves == 8 ? 0.012 : groups <= cus ? 0.02 : 0.013);
-      const double cost = (waves == 4 ? 2.5 : 4.0) + std::max(units + rows, stream);
-      if (cost < best.cost) best = {rt, waves, cost};
+    for (int rows = 12; rows <= (waves == 4 ? 48 : 128); rows += 4) {
+      const int64_t groups = (N + rows - 1) / rows;
+      const double turns = (double)((groups + cus - 1) / cus), blocks = (double)((rows + 15) / 16);
+      const double units = turns * (double)stages * (rows / 32.0 + blocks / 2.0) * (waves == 4 ? 0.090 : 0.079);
+      const double x = turns * (double)(stages * M) * (waves == 8 ? 0.014 : groups <= cus ? 0.025 : 0.013);
+      const double cost = (waves == 4 ? 2.5 : 3.0 + 0.35 * blocks) + std::max(units + x, stream);
+      if (cost < best.cost) best = {rows, waves, cost};
     }
   }
   return best;
@@ -211,7 +213,7 @@ static void launch_rows(Fp4Rows p, int waves, void* stream) {
   p.chunk_log2 = 1;
   while (p.chunk_log2 < 6 && (1 << p.chunk_log2) < per && waves * fp4_chunk_bytes(M, p.chunk_log2 + 1) <= 36 * 1024) ++p.chunk_log2;
   const int bytes = std::max(kRT * 1024 * waves, waves * fp4_chunk_bytes(M, p.chunk_log2));
-  hipLaunchKernelGGL((mxfp4_rows_kernel<kOut, kRT>), dim3((unsigned)((p.N + 16 * kRT - 1) / (16 * kRT))), dim3(64 * waves), bytes,
+  hipLaunchKernelGGL((mxfp4_rows_kernel<kOut, kRT>), dim3((unsigned)((p.N + p.rows - 1) / p.rows)), dim3(64 * waves), bytes,
                      (hipStream_t)stream, p);
 }
 
@@ -219,11 +221,12 @@ int fp4_linear_rows(const void* x, int x_dtype, int64_t ldx, const uint8_t* sx, 
                     const uint8_t* sb, const void* bias, void* d, int64_t ldd, int out_dtype, int64_t M, int64_t N, int64_t K,
                     void* stream) {
   if (const int rc = fp4_gemm_check(b, ldb, sb, b, ldb, sb, d, ldd, out_dtype, M, N, K)) return rc;
-  const Fp4Rows p = {x, sx, b, sb, bias, d, M, N, K, ldx, ldsx, ldb, ldd, x_dtype, (int)fp4_groups(K), (int)(fp4_row_bytes(K) / kFp4Stage), 0};
+  Fp4Rows p = {x, sx, b, sb, bias, d, M, N, K, ldx, ldsx, ldb, ldd, x_dtype, (int)fp4_groups(K), (int)(fp4_row_bytes(K) / kFp4Stage), 0, 0};
   const RowsPlan4 plan = plan_rows(M, N, p.stages, mxq_cu_count());
+  p.rows = plan.rows;
   with_dtype(out_dtype, [&](auto O) {
     constexpr int kOut = decltype(O)::value;
-    switch (plan.rt) {
+    switch ((plan.rows + 15) / 16) {
       case 1: return launch_rows<kOut, 1>(p, plan.waves, stream);
       case 2: return launch_rows<kOut, 2>(p, plan.waves, stream);
       case 3: return launch_rows<kOut, 3>(p, plan.waves, stream);

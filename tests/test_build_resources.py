@@ -66,3 +66,24 @@ def test_fp8_kernels_do_not_spill(tmp_path, kernel):
     kernels = {k: v for k, v in _kernels(_lib.LIB_PATH, tmp_path).items() if kernel in k}
     assert len(kernels) >= 4
     assert max(kernels.values()) == 0, sorted(kernels.items(), key=lambda kv: -kv[1])[:5]
+
+
+@pytest.mark.parametrize("kernel,least,most", [("gemm_mxfp4_kernel", 12, 1), ("mxfp4_dgrad_kernel", 8, 0), ("mxfp4_rows_kernel", 12, 0),
+                                               ("mxfp4_quant_kernel", 6, 0), ("mxfp4_dequant_kernel", 3, 0), ("rms_norm_kernel", 50, 0),
+                                               ("rms_norm_grad_kernel", 40, 24)])
+def test_mxfp4_and_rms_norm_kernels_do_not_spill(tmp_path, kernel, least, most):
+    """The 4-bit layer's kernels (the 256-row product keeps one register of its tile loop in memory) and the rms norm's (of its
+    gradient only the rows beyond 16384 elements, three chunks a lane, spill)."""
+    from mx_qlinear import _lib
+
+    if not pathlib.Path(READOBJ).exists():
+        pytest.skip("no llvm-readobj")
+    if not _lib.LIB_PATH.exists():
+        from mx_qlinear import build
+
+        build.build()
+    kernels = {k: v for k, v in _kernels(_lib.LIB_PATH, tmp_path).items() if kernel in k}
+    assert len(kernels) >= least
+    assert max(kernels.values()) <= most, sorted(kernels.items(), key=lambda kv: -kv[1])[:5]
+    if kernel == "rms_norm_grad_kernel":
+        assert max(v for k, v in kernels.items() if "Li3ELi0E" not in k) == 0

@@ -193,8 +193,9 @@ struct RowsPlan4 {
 static RowsPlan4 plan_rows(int64_t M, int64_t N, int64_t stages, int cus) {
   RowsPlan4 best = {16, 4, 1e300};
   const double stream = (double)(N * stages) * 136.0 / 5.2e6;
+  // (more than 96 rows in eight waves spill)
   for (int waves = 4; waves <= 8; waves += 4) {
-    for (int rows = 12; rows <= (waves == 4 ? 48 : 128); rows += 4) {
+    for (int rows = 12; rows <= (waves == 4 ? 48 : 96); rows += 4) {
       const int64_t groups = (N + rows - 1) / rows;
       const double turns = (double)((groups + cus - 1) / cus), blocks = (double)((rows + 15) / 16);
       const double units = turns * (double)stages * (rows / 32.0 + blocks / 2.0) * (waves == 4 ? 0.090 : 0.079);
@@ -232,8 +233,7 @@ int fp4_linear_rows(const void* x, int x_dtype, int64_t ldx, const uint8_t* sx, 
       case 3: return launch_rows<kOut, 3>(p, plan.waves, stream);
       case 4: return launch_rows<kOut, 4>(p, plan.waves, stream);
       case 5: return launch_rows<kOut, 5>(p, plan.waves, stream);
-      case 6: return launch_rows<kOut, 6>(p, plan.waves, stream);
-      default: return launch_rows<kOut, 8>(p, plan.waves, stream);
+      default: return launch_rows<kOut, 6>(p, plan.waves, stream);
     }
   });
   return mxq_check_launch("mxfp4_rows_kernel");

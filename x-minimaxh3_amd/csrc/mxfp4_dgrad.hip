@@ -12,6 +12,10 @@
 // tiles, four waves one of 128 x 128, a wave 64 x 64 of it; a stage is 64 of n: dY's 256 x 64 bfloat16 (32 KB) and W's 64 x 256
 // codes, decoded on the way from registers to LDS (32 KB). Problems of fewer tiles still split N over workgroups, which write
 // float32 sums that fp8_join_kernel adds in order.
+//
+// 8192 rows, N 14336, K 5376 take 0.98 ms (1.28 PFLOP/s), 16384 rows, N and K 8192 1.65 (1.34): the rate of a library's plain
+// bfloat16 product (1.25 to 1.33 for 8192 cubed). The matrix cores are busy 58 % of the time in the first, whose 2.6 rounds of tiles
+// run as three. Four waves of 128 x 128, with two thirds of the LDS reads, ran 5 % slower.
 #include "mxfp4_common.h"
 
 namespace mxq {

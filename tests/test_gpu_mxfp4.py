@@ -627,3 +627,29 @@ def test_products_of_more_than_2_to_the_32_elements(dev):
     dy = torch.randn(m, k, device=dev, dtype=torch.float16)
     dx, _ = mx.mxfp4_linear_backward(dy, turned)
     check_gradients(dx[at.to(dev)], None, dy[at.to(dev)].cpu(), ob.rows(_acts(k, n, torch.bfloat16, 5, 0.5))[0])
+
+
+def test_module_gives_the_gradients_asked_for(dev):
+    """Only the bias's, only the input's, none of either, and those of no rows."""
+    mx = _mx()
+    w, bias = _acts(40, 96, torch.bfloat16, 1), _acts(1, 40, torch.bfloat16, 2)[0]
+    layer = mx.Mxfp4Linear.from_weight(w.to(dev), bias.to(dev))
+    x0, dy = _acts(20, 96, torch.bfloat16, 3), _acts(20, 40, torch.bfloat16, 4)
+    want_x, want_b = mx.mxfp4_linear_backward(dy.to(dev), layer.prepared(), grad_dtype=torch.bfloat16)
+    for of_x in (False, True):
+        for of_b in (False, True):
+            x = x0.to(dev).requires_grad_(of_x)
+            layer.bias.requires_grad_(of_b).grad = None
+            y = layer(x)
+            assert y.requires_grad == (of_x or of_b)
+            if y.requires_grad:
+                y.backward(dy.to(dev))
+            assert (x.grad is None) == (not of_x) and (not of_x or torch.equal(x.grad, want_x))
+            assert (layer.bias.grad is None) == (not of_b) and (not of_b or torch.equal(layer.bias.grad, want_b))
+    x = x0[:0].to(dev).requires_grad_()
+    layer.bias.grad = None
+    layer(x).sum().backward()
+    assert x.grad.shape == (0, 96) and bool((layer.bias.grad == 0).all())
+    with torch.no_grad():
+        x = x0.to(dev).requires_grad_()
+        assert not layer(x).requires_grad

@@ -414,3 +414,31 @@ def test_more_than_2_to_the_32_elements(dev, m, d):
         total += part.sum(0)
         size += part.abs().sum(0)
     assert bool(((dw.double() - total).abs() <= 2.0**-24 * (m + 4) * size).all())
+
+
+@pytest.mark.parametrize("keep", [False, True])
+def test_module_gives_the_gradients_asked_for(dev, keep):
+    """Every choice of input, residual and weight; the sum's output alone; no rows."""
+    mx = _mx()
+    m, d = 19, 264
+    x0, r0, dy, ds = (_acts(m, d, torch.bfloat16, i) for i in range(4))
+    norm = mx.RMSNorm(d, keep_fp8=keep, device=dev, dtype=torch.bfloat16)
+    got = {}
+    for choice in range(1, 8):
+        x, r = x0.to(dev).requires_grad_(bool(choice & 1)), r0.to(dev).requires_grad_(bool(choice & 2))
+        norm.weight.requires_grad_(bool(choice & 4)).grad = None
+        y, s = norm(x, r)
+        torch.autograd.backward([y, s], [dy.to(dev), ds.to(dev)]) if choice & 3 else y.backward(dy.to(dev))
+        for name, t, on in (("x", x, choice & 1), ("r", r, choice & 2), ("w", norm.weight, choice & 4)):
+            assert (t.grad is None) == (not on)
+            if on:
+                assert torch.equal(got.setdefault(name, t.grad.clone()), t.grad)
+    assert torch.equal(got["x"], got["r"])
+    x, r = x0.to(dev).requires_grad_(), r0.to(dev).requires_grad_()
+    norm.weight.grad = None
+    norm(x, r)[1].backward(ds.to(dev))
+    assert torch.equal(x.grad.cpu(), ds) and torch.equal(r.grad.cpu(), ds) and (norm.weight.grad is None or bool((norm.weight.grad == 0).all()))
+    x = x0[:0].to(dev).requires_grad_()
+    norm.weight.grad = None
+    norm(x).sum().backward()
+    assert x.grad.shape == (0, d) and bool((norm.weight.grad == 0).all())

@@ -9,8 +9,8 @@
 // dY's rows hold the summed index n, so its fragments (eight consecutive n of one row per lane) are plain 16-byte LDS reads; W
 // has n as its rows, and its fragments come from transposing reads (ds_read_b64_tr_b16), which hand sixteen lanes the columns
 // of a 4 x 16 patch. A workgroup of eight waves owns a 256 (m) x 256 (k) tile, a wave 64 x 128 of it, or, for problems of few
-// tiles, four waves one of 128 x 128, a wave 64 x 64 of it; a stage is 64 of n: dY's 256 x 64 bfloat16 (32 KB) and W's 64 x 256
-// codes, decoded on the way from registers to LDS (32 KB). Problems of fewer tiles still split N over workgroups, which write
+// tiles, four waves one of 128 x 128, or, of up to 64 rows, 64 x 256, a wave 64 x 64 of it; a stage is 64 of n: of the large tile,
+// dY's 256 x 64 bfloat16 (32 KB) and W's 64 x 256 codes, decoded on the way from registers to LDS (32 KB). Problems of fewer tiles still split N over workgroups, which write
 // float32 sums that fp8_join_kernel adds in order.
 //
 // 8192 rows, N 14336, K 5376 take 0.98 ms (1.28 PFLOP/s), 16384 rows, N and K 8192 1.65 (1.34): the rate of a library's plain
@@ -22,14 +22,16 @@ namespace mxq {
 
 constexpr int kDStage = 64, kDGroup = 4;
 
-// A workgroup's tile: kT x kT, four waves along m and two along k (256), or two and two (128).
-template <int kT>
+// A workgroup's tile: kTM x kTK, waves of 64 x 128 (256 x 256) or 64 x 64.
+template <int kTM, int kTK>
 struct DgradTile {
-  static constexpr int kWaves = kT / 32, kThreads = 64 * kWaves, kWavesM = kT / 64;
-  static constexpr int kMB = 2, kKB = kT / 64;       // 32-row and 32-column blocks of a wave
-  static constexpr int kBytes = kT * kDStage * 2;    // of one operand's stage in LDS
-  static constexpr int kRow = kT * 2;                // of W's rows there
-  static constexpr int kRows = kT / 4;               // rows that the threads' loads take at once
+  static constexpr int kWavesM = kTM / 64, kMB = 2, kKB = kTM == 256 ? 4 : 2;  // 32-row and 32-column blocks of a wave
+  static constexpr int kWaves = kWavesM * (kTK / (kKB * 32)), kThreads = 64 * kWaves;
+  static constexpr int kBytesY = kTM * kDStage * 2, kBytesW = kTK * kDStage * 2;  // of an operand's stage in LDS
+  static constexpr int kRow = kTK * 2;                                            // of W's rows there
+  static constexpr int kRows = kThreads / 8;                                      // rows that the threads' loads take at once
+  // a thread's loads of a stage: 16-byte pieces of dY, words of W (kWords in each of its rows), scale words
+  static constexpr int kLoadsY = kTM / kRows, kWords = kTK / 64, kLoadsW = kDStage / kRows * kWords, kLoadsS = kLoadsW / 2;
 };
 
 struct Dgrad {
@@ -77,12 +79,13 @@ MXQ_DEVICE uint32_t dgrad_load_u32(const void* base, int bytes, uint32_t voff) {
       __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, kRawBufferWord3), (int)voff, 0, 0);
 }
 
-template <int kT, int kOut, bool kSplit>
-__global__ __launch_bounds__(DgradTile<kT>::kThreads, kT == 256 ? 1 : 2) void mxfp4_dgrad_kernel(Dgrad p) {
-  typedef DgradTile<kT> C;
-  constexpr int kDMB = C::kMB, kDKB = C::kKB, kDBytes = C::kBytes;
-  // [buffer][dY, W]; the buffers are one address bit apart
-  __shared__ __attribute__((aligned(2 * 2 * C::kBytes))) char lds[2 * 2 * C::kBytes];
+template <int kTM, int kTK, int kOut, bool kSplit>
+__global__ __launch_bounds__((DgradTile<kTM, kTK>::kThreads), kTM == 256 ? 1 : 2) void mxfp4_dgrad_kernel(Dgrad p) {
+  typedef DgradTile<kTM, kTK> C;
+  constexpr int kDMB = C::kMB, kDKB = C::kKB, kBytesY = C::kBytesY, kBytesW = C::kBytesW, kLds = 2 * (kBytesY + kBytesW);
+  // W's two buffers, then dY's, an operand's one address bit apart
+  static_assert(kBytesY <= kBytesW, "alignment of dY's buffers");
+  __shared__ __attribute__((aligned(2 * C::kBytesW))) char lds[kLds];
   const int tiles = p.tiles_m * p.tiles_k, num = tiles * p.splits, per = num / 8, bid = blockIdx.x;
   int t = bid < per * 8 ? (bid % 8) * per + bid / 8 : bid;  // contiguous ranges over the XCDs
   const int slice = t / tiles;
@@ -90,7 +93,7 @@ __global__ __launch_bounds__(DgradTile<kT>::kThreads, kT == 256 ? 1 : 2) void mx
   // groups of four tile-rows, so that the tiles an XCD runs at once share operand panels in its L2
   const int group = kDGroup * p.tiles_k, g0 = t / group * kDGroup, rows_g = min(p.tiles_m - g0, kDGroup), in_g = t - g0 * p.tiles_k;
   const int tk = in_g / rows_g, tm = g0 + in_g - tk * rows_g;
-  const int m0 = tm * kT, k0 = tk * kT;
+  const int m0 = tm * kTM, k0 = tk * kTK;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int wm = (wave % C::kWavesM) * 64, wk = (wave / C::kWavesM) * 32 * kDKB;  // the wave's part of the tile
   const int M = (int)p.M, K = (int)p.K, n_first = slice * p.split_n, n_last = min(n_first + p.split_n, (int)p.N);
@@ -98,15 +101,14 @@ __global__ __launch_bounds__(DgradTile<kT>::kThreads, kT == 256 ? 1 : 2) void mx
 
   // A thread's share of a stage, by buffer loads whose offsets point outside for what lies behind the slice's last n or the last
   // row (they read zeros): of dY the 16-byte piece tid % 8 of rows tid / 8 + kRows j (nothing is read behind column N rounded up to
-  // 8); of W four words of eight columns, tid % 8 + 8 j of row tid / 8 (256 columns, with the scale words of the row's blocks
-  // 0 .. 3 and 4 .. 7), or tid % 8 + 8 (j % 2) of rows tid / 8 + 32 (j / 2) (128 columns, with the rows' scale words).
-  constexpr int kRows = C::kRows;
+  // 8); of W the words of eight columns tid % 8 + 8 j of rows tid / 8 (+ kRows), with those rows' scale words, one per 128 columns.
+  constexpr int kRows = C::kRows, kWords = C::kWords, kLoadsY = C::kLoadsY, kLoadsW = C::kLoadsW, kLoadsS = C::kLoadsS;
   const int r = tid >> 3, c = tid & 7;
   const int ldy = (int)p.ldy, ldb = (int)p.ldb, row_tiles = p.groups * (int)kFp4ScaleTile;
   const uint32_t oy = (uint32_t)(r * ldy + c * 8) * 2, ow = (uint32_t)(r * ldb + c * 4);
-  const uint32_t os = (uint32_t)((r >> 5) * row_tiles + (r & 31) * 8 + ((k0 >> 8) & 1) * 4 + (kT == 128 ? ((k0 >> 7) & 1) * 256 : 0));
-  v4u y[4];
-  uint32_t w[4], ws[2];
+  const uint32_t os = (uint32_t)((r >> 5) * row_tiles + (r & 31) * 8 + ((k0 >> 8) & 1) * 4 + (kTK == 128 ? ((k0 >> 7) & 1) * 256 : 0));
+  v4u y[kLoadsY];
+  uint32_t w[kLoadsW], ws[kLoadsS];
   // (the position of the next load: n left in the slice and the operands' place)
   int left = n_last - n_first, parts_left = left > 0 ? p.parts : 0;
   const uint16_t* py = p.dy + (int64_t)m0 * ldy + n_first;
@@ -114,14 +116,19 @@ __global__ __launch_bounds__(DgradTile<kT>::kThreads, kT == 256 ? 1 : 2) void mx
   const uint8_t* ps = p.sb + (int64_t)(n_first >> 5) * row_tiles + (k0 >> 9) * kFp4ScaleTile;
   auto load = [&](auto HC) {  // the first or second half of a share
     constexpr int kH = decltype(HC)::value;
-    const bool row = r + (kT == 128 ? 32 * kH : 0) < left;
 #pragma unroll
-    for (int j = 2 * kH; j < 2 * kH + 2; ++j) {
+    for (int j = kH * kLoadsY / 2; j < (kH + 1) * kLoadsY / 2; ++j)
       y[j] = buffer_load_x4(py + (int64_t)(kRows * j) * ldy, kRows * 2 * ldy, c * 8 < left && m0 + kRows * j + r < M ? oy : kBufferOff);
-      const uint32_t at = kT == 128 ? (uint32_t)(32 * kH * ldb + 32 * (j & 1)) : (uint32_t)(32 * j);
-      w[j] = dgrad_load_u32(pw, kDStage * ldb, row ? ow + at : kBufferOff);
+#pragma unroll
+    for (int j = kH * kLoadsW / 2; j < (kH + 1) * kLoadsW / 2; ++j) {
+      const int down = j / kWords * kRows;
+      w[j] = dgrad_load_u32(pw, kDStage * ldb, r + down < left ? ow + (uint32_t)(down * ldb + 32 * (j % kWords)) : kBufferOff);
     }
-    ws[kH] = dgrad_load_u32(ps, 2 * row_tiles, row ? os + (uint32_t)(kT == 128 ? kH * row_tiles : 256 * kH) : kBufferOff);
+#pragma unroll
+    for (int j = kH * kLoadsS / 2; j < (kH + 1) * kLoadsS / 2; ++j) {
+      const int down = j / (kWords / 2) * kRows;
+      ws[j] = dgrad_load_u32(ps, 2 * row_tiles, r + down < left ? os + (uint32_t)((down >> 5) * row_tiles + 256 * (j % (kWords / 2))) : kBufferOff);
+    }
     if constexpr (kH == 1) {
       left -= kDStage;
       py += kDStage;
@@ -137,17 +144,19 @@ __global__ __launch_bounds__(DgradTile<kT>::kThreads, kT == 256 ? 1 : 2) void mx
       }
     }
   };
-  const uint32_t at_y = lds_addr(lds) + (uint32_t)dy_at(r, c);  // (row r + kRows j has r's swizzle)
+  const uint32_t lds_y = lds_addr(lds) + 2 * kBytesW;
+  const uint32_t at_y = lds_y + (uint32_t)dy_at(r, c);  // (row r + kRows j has r's swizzle)
   // (words c + 8 j: 128 bytes further on, two 64-byte pieces, whose number the swizzle is exclusive with)
-  const uint32_t at_w = lds_addr(lds) + kDBytes + (uint32_t)w_at<C::kRow>(r, c * 16);
-  auto put_y = [&](uint32_t buf, auto JC) {
+  const uint32_t at_w = lds_addr(lds) + (uint32_t)w_at<C::kRow>(r, c * 16);
+  // (odd: the second of an operand's buffers, all bits set, or none)
+  auto put_y = [&](uint32_t odd, auto JC) {
     constexpr int j = decltype(JC)::value;
-    *(lds_v4u)((lds_ptr)(uintptr_t)(at_y ^ buf) + j * kRows * 128) = y[j];
+    *(lds_v4u)((lds_ptr)(uintptr_t)(at_y ^ (odd & kBytesY)) + j * kRows * 128) = y[j];
   };
-  auto put_w = [&](uint32_t buf, auto JC) {
-    constexpr int j = decltype(JC)::value, kWord = kT == 128 ? j & 1 : j, kRowOff = kT == 128 ? (j >> 1) * 32 * C::kRow : 0;
+  auto put_w = [&](uint32_t odd, auto JC) {
+    constexpr int j = decltype(JC)::value, kWord = j % kWords, kRowOff = j / kWords * kRows * C::kRow;
     const uint32_t byte = (ws[j >> 1] >> (16 * (j & 1) + 8 * (c >> 2))) & 0xFFu;
-    *(lds_v4u)((lds_ptr)(uintptr_t)(at_w ^ buf ^ (kWord * 128)) + kRowOff) =
+    *(lds_v4u)((lds_ptr)(uintptr_t)(at_w ^ (odd & kBytesW) ^ (kWord * 128)) + kRowOff) =
         __builtin_bit_cast(v4u, fp4x8_to_bf16(w[j], fp8_scale_f32(byte)));
   };
   v16f acc[kDMB][kDKB] = {};
@@ -161,19 +170,19 @@ __global__ __launch_bounds__(DgradTile<kT>::kThreads, kT == 256 ? 1 : 2) void mx
   v4s fw[2][kDKB][2];
   uint32_t base[kDKB];  // of W's fragments in buffer 0
 #pragma unroll
-  for (int b = 0; b < kDKB; ++b) base[b] = w_base<C::kRow>(lds_addr(lds) + kDBytes, wk + b * 32, lane);
+  for (int b = 0; b < kDKB; ++b) base[b] = w_base<C::kRow>(lds_addr(lds), wk + b * 32, lane);
   // dY's fragments: row wm + l % 32 (+ 32 a), piece 2 step + l / 32
   uint32_t base_y[4];
 #pragma unroll
-  for (int h = 0; h < 4; ++h) base_y[h] = lds_addr(lds) + (uint32_t)dy_at(wm + (lane & 31), 2 * h + (lane >> 5));
-  auto read = [&](uint32_t buf, auto StepC, auto SetC, auto IC) {  // read I of a step, in the order of their use
+  for (int h = 0; h < 4; ++h) base_y[h] = lds_y + (uint32_t)dy_at(wm + (lane & 31), 2 * h + (lane >> 5));
+  auto read = [&](uint32_t odd, auto StepC, auto SetC, auto IC) {  // read I of a step, in the order of their use
     constexpr int kStep = decltype(StepC)::value, kSet = decltype(SetC)::value, kI = decltype(IC)::value;
     if constexpr (kI == 0 || kI > 2 * kDKB) {
       constexpr int a = kI == 0 ? 0 : kI - 2 * kDKB;
-      fy[kSet][a] = *(lds_v4u)((lds_ptr)(uintptr_t)(base_y[kStep] ^ buf) + a * 32 * 128);
+      fy[kSet][a] = *(lds_v4u)((lds_ptr)(uintptr_t)(base_y[kStep] ^ (odd & kBytesY)) + a * 32 * 128);
     } else {
       constexpr int b = (kI - 1) / 2, kPart = (kI - 1) & 1;
-      fw[kSet][b][kPart] = read_transposed<(kStep * 16 + kPart * 4) * C::kRow>(base[b] ^ buf);
+      fw[kSet][b][kPart] = read_transposed<(kStep * 16 + kPart * 4) * C::kRow>(base[b] ^ (odd & kBytesW));
     }
   };
   auto publish = [&] {
@@ -182,9 +191,9 @@ __global__ __launch_bounds__(DgradTile<kT>::kThreads, kT == 256 ? 1 : 2) void mx
     barrier_no_drain();
     __builtin_amdgcn_sched_barrier(0);
   };
-  uint32_t buf = 0;  // byte offset of the stage's buffer
+  uint32_t buf = 0;  // the stage's buffers
   auto stage = [&] {
-    const uint32_t other = buf ^ (2 * kDBytes);
+    const uint32_t other = ~buf;
     static_for<4>([&](auto H) {
       constexpr int h = decltype(H)::value, kSet = h & 1;
       constexpr bool kPut = h == 1 || h == 2;
@@ -197,10 +206,15 @@ __global__ __launch_bounds__(DgradTile<kT>::kThreads, kT == 256 ? 1 : 2) void mx
           if constexpr (i * kReadSlots / kReads == g)
             read(h < 3 ? buf : other, std::integral_constant<int, h < 3 ? h + 1 : 0>{}, std::integral_constant<int, kSet ^ 1>{}, I);
         });
-        if constexpr (kPut && g * 4 % kSlots == 0) {  // (four writes a step)
-          constexpr int i = g * 4 / kSlots, j = (h - 1) * 2 + i / 2;
-          if constexpr (i % 2 == 0) put_y(other, std::integral_constant<int, j>{});
-          else put_w(other, std::integral_constant<int, j>{});
+        if constexpr (kPut) {  // (half of dY's and of W's writes a step)
+          constexpr int kPutsY = kLoadsY / 2, kPuts = kPutsY + kLoadsW / 2;
+          static_for<kPuts>([&](auto I) {
+            constexpr int i = decltype(I)::value;
+            if constexpr (i * kSlots / kPuts == g) {
+              if constexpr (i % 2 == 0 && i / 2 < kPutsY) put_y(other, std::integral_constant<int, (h - 1) * kPutsY + i / 2>{});
+              else put_w(other, std::integral_constant<int, (h - 1) * (kLoadsW / 2) + i - (i / 2 + 1 < kPutsY ? i / 2 + 1 : kPutsY)>{});
+            }
+          });
         }
         __builtin_amdgcn_sched_barrier(0);
       });
@@ -210,7 +224,8 @@ __global__ __launch_bounds__(DgradTile<kT>::kThreads, kT == 256 ? 1 : 2) void mx
   };
   // (one loop for all stages: with the last ones peeled off, copies of the accumulators between the loops would spill)
   static_for<2>(load);
-  static_for<4>([&](auto J) { put_y(0, J); put_w(0, J); });
+  static_for<kLoadsY>([&](auto J) { put_y(0, J); });
+  static_for<kLoadsW>([&](auto J) { put_w(0, J); });
   static_for<2>(load);
   publish();
   static_for<kReads>([&](auto I) { read(0, std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{}, I); });
@@ -220,10 +235,10 @@ __global__ __launch_bounds__(DgradTile<kT>::kThreads, kT == 256 ? 1 : 2) void mx
   // barrier is behind the last step's reads) kLanes lanes store a row of the wave's columns. 16-byte piece c of row r sits at piece
   // c ^ (r % kLanes).
   constexpr int kElem = kOut == MXQ_DTYPE_F32 ? 4 : 2, kLanes = kDKB * 8, kTurn = kLanes * 16;
-  static_assert(2 * 2 * kDBytes / C::kWaves >= 32 * kTurn, "LDS of a wave's block of results");
+  static_assert(kLds / C::kWaves >= 32 * kTurn, "LDS of a wave's block of results");
   char* d = reinterpret_cast<char*>(p.d);
   if constexpr (kSplit) d += (int64_t)slice * p.M * p.ldd * 4;
-  char* turn = lds + wave * (2 * 2 * kDBytes / C::kWaves);
+  char* turn = lds + wave * (kLds / C::kWaves);
 #pragma unroll
   for (int a = 0; a < kDMB; ++a) {
     wave_lds_fence();
@@ -247,27 +262,31 @@ __global__ __launch_bounds__(DgradTile<kT>::kThreads, kT == 256 ? 1 : 2) void mx
 }
 
 struct DgradPlan {
-  int tile, splits;
+  int tile, splits;  // tile: its rows
   int64_t n;
 };
 
-// Tile and N slices, by an estimate in microseconds: a round of workgroups takes 5 and, per stage and part, 1.2 (256) or 0.575 (128)
-// where few CUs are at work, 1.58 or 0.93 (two workgroups a CU) where all are, slices cost a join. Measured, whole and in the best
-// number of slices, 128 / 256: one row, K 5120, N 5120: 52, 15.4 in twelve / 101, 19.8; 700 rows: 54.7, 52.8 in two / 105, 53.9 in
-// four; 2048 rows 128 / 109; 700 rows, K 5120, N 20480: 195, 166 in two / 389, 142 in four; 4096 rows, K 20480, N 5120: 831 / 657;
-// 2048 rows, K 1000, N 3001: 43.7, 34.9 in two / 74.6, 40.6 in four.
+static int tile_width(int rows) { return rows == 128 ? 128 : 256; }
+
+// Tile and N slices, by an estimate in microseconds: a round of workgroups takes 5 and, per stage and part, 1.2 (256 x 256), 0.575
+// (128 x 128) or 0.8 (64 x 256) where few CUs are at work, 1.58, 0.93 or 1.1 (two workgroups a CU) where all are, slices cost a join.
+// Measured, whole and in the best number of slices, 128 / 256: one row, K 5120, N 5120: 52, 15.4 in twelve / 101, 19.8; 700 rows: 54.7,
+// 52.8 in two / 105, 53.9 in four; 2048 rows 128 / 109; 700 rows, K 5120, N 20480: 195, 166 in two / 389, 142 in four; 4096 rows, K
+// 20480, N 5120: 831 / 657; 2048 rows, K 1000, N 3001: 43.7, 34.9 in two / 74.6, 40.6 in four. In slices, 64 / 128: 40 rows, K 5120,
+// N 5120: 17.5 / 17.9; K 5120, N 20480: 29.0 / 35.2, one row 24.4 / 32.4, 64 in fp32 67.4 / 89.7; K 2048, N 2048: 10.8 / 10.3.
 static DgradPlan plan_dgrad(int64_t M, int64_t N, int64_t K, int parts, int cus) {
   DgradPlan best = {256, 1, (N + kDStage - 1) / kDStage * kDStage};
   double best_cost = 1e300;
-  for (int tile = 256; tile >= 128; tile /= 2) {
-    const int64_t tiles = (M + tile - 1) / tile * ((K + tile - 1) / tile), at_once = tile == 256 ? cus : 2 * cus;
-    const double alone = tile == 256 ? 1.2 : 0.575, all = tile == 256 ? 1.58 : 0.93;
+  for (const int tile : {256, 128, 64}) {
+    if (tile == 64 && M > 64) break;
+    const int64_t tiles = (M + tile - 1) / tile * ((K + tile_width(tile) - 1) / tile_width(tile)), at_once = tile == 256 ? cus : 2 * cus;
+    const double alone = tile == 256 ? 1.2 : tile == 128 ? 0.575 : 0.8, all = tile == 256 ? 1.58 : tile == 128 ? 0.93 : 1.1;
     for (int64_t s = 1; s <= 64; ++s) {
       const int64_t n = ((N + s - 1) / s + kDStage - 1) / kDStage * kDStage;
       if ((N + n - 1) / n != s || (s > 1 && tiles * s > 4 * cus)) continue;
       const double units = (double)(n / kDStage * parts), rest = (double)(tiles * s % at_once) / at_once;
       const double cost = (double)(tiles * s / at_once) * (units * all + 5.0) +
-                          (rest > 0.0 ? units * (alone + (all - alone) * rest) + 5.0 : 0.0) + slices_cost(s, M * K);
+                          (rest > 0.0 ? units * (alone + (all - alone) * rest) + 5.0 : 0.0) + slices_cost(s, M * K) + 0.1 * s;
       if (cost < best_cost) {
         best_cost = cost;
         best = {tile, (int)s, n};
@@ -301,19 +320,22 @@ int fp4_dgrad_check(const void* dy, int64_t ldy, const uint8_t* b, int64_t ldb, 
   return MXQ_OK;
 }
 
+template <int kTM, int kTK, int kOut, bool kSplit>
+static void launch_tile(const Dgrad& p, unsigned grid, void* stream) {
+  hipLaunchKernelGGL((mxfp4_dgrad_kernel<kTM, kTK, kOut, kSplit>), dim3(grid), dim3(DgradTile<kTM, kTK>::kThreads), 0, (hipStream_t)stream, p);
+}
 template <int kOut, bool kSplit>
 static void launch_dgrad(const Dgrad& p, int tile, unsigned grid, void* stream) {
-  if (tile == 256)
-    hipLaunchKernelGGL((mxfp4_dgrad_kernel<256, kOut, kSplit>), dim3(grid), dim3(DgradTile<256>::kThreads), 0, (hipStream_t)stream, p);
-  else
-    hipLaunchKernelGGL((mxfp4_dgrad_kernel<128, kOut, kSplit>), dim3(grid), dim3(DgradTile<128>::kThreads), 0, (hipStream_t)stream, p);
+  if (tile == 256) launch_tile<256, 256, kOut, kSplit>(p, grid, stream);
+  else if (tile == 128) launch_tile<128, 128, kOut, kSplit>(p, grid, stream);
+  else launch_tile<64, 256, kOut, kSplit>(p, grid, stream);
 }
 
 int fp4_dgrad(const void* dy, int parts, int64_t ldy, const uint8_t* b, int64_t ldb, const uint8_t* sb, void* dx, int out_dtype,
               int64_t M, int64_t N, int64_t K, void* workspace, SliceJob* later, void* stream) {
   if (const int rc = fp4_dgrad_check(dy, ldy, b, ldb, sb, dx, out_dtype, M, N, K)) return rc;
   const DgradPlan plan = plan_dgrad(M, N, K, parts, mxq_cu_count());
-  const int64_t tiles_m = (M + plan.tile - 1) / plan.tile, tiles_k = (K + plan.tile - 1) / plan.tile;
+  const int64_t tiles_m = (M + plan.tile - 1) / plan.tile, tiles_k = (K + tile_width(plan.tile) - 1) / tile_width(plan.tile);
   Dgrad p = {(const uint16_t*)dy, b, sb, dx, M, N, K, ldy, M * ldy, ldb, K, parts, (int)fp4_groups(K), (int)tiles_m, (int)tiles_k,
              plan.splits, (int)plan.n};
   const unsigned grid = (unsigned)(tiles_m * tiles_k * plan.splits);

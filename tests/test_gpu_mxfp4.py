@@ -319,7 +319,7 @@ def test_nan_and_infinities_stay_in_their_rows(dev, m):
 # the input's gradient
 # ---------------------------------------------------------------------------------------
 
-BACKWARD = [(1, 1, 1), (1, 520, 300), (3, 7, 33), (16, 64, 1000), (33, 130, 100), (70, 257, 511), (300, 96, 1000), (257, 1000, 256),
+BACKWARD = [(40, 2100, 1300), (64, 5000, 260), (33, 130, 4097), (1, 1, 1), (1, 520, 300), (3, 7, 33), (16, 64, 1000), (33, 130, 100), (70, 257, 511), (300, 96, 1000), (257, 1000, 256),
             (600, 513, 130), (130, 2050, 257), (1100, 72, 40)]
 PARTS = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}
 

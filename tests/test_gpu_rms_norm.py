@@ -208,6 +208,54 @@ def test_backward_layouts(dev, dtype):
     check_backward(dx, dw, base[:1, :77].expand(4, 77), base[:4, :77], rstd[:4], None, None)
 
 
+def check_far_backward(dx, dw, dy, s, rstd, weight, dsum, steps):
+    """dx = r g - (xh r) c + ds with c = E[g xh], whose magnitudes are T1 = |r g|, T2 = |xh| r E|g xh| and |ds|. The sum of c has at
+    most D roundings of its partial sums, each at most E|g xh|; six more steps (xh, g, the three products, the sum) are each
+    half a step of float32 of the terms; ``steps`` are those of an rstd that is not the kernel's own."""
+    ref, refw = ob.rms_norm_backward(dy, s, rstd, weight, dsum)
+    u, (m, d) = torch.finfo(dx.dtype).eps / 2, dy.shape
+    r = rstd.double()[:, None]
+    xh = s.double().abs() * r
+    g = dy.double().abs() * (1 if weight is None else weight.double().abs())
+    t2 = xh * r * (g * xh).mean(1, keepdim=True)
+    terms = r * g + t2 + (0 if dsum is None else dsum.double().abs())
+    bound = u * ref.abs() + 2.0**-24 * ((d + 8) * t2 + (6 + steps) * terms) + torch.finfo(dx.dtype).tiny
+    err = (dx.double().cpu() - ref).abs()
+    assert bool((err <= bound * (1 + u)).all()), f"rows at worst {(err / bound).amax(1).tolist()} of the bound"
+    if dw is not None:
+        bound = 2.0**-24 * (m + 4) * (dy.double().abs() * xh).sum(0) + 2.0**-140
+        assert bool(((dw.double().cpu() - refw).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [5, 128, 200, 300, 1003, 5120, 9000, 20480])
+def test_backward_of_far_rows(dev, dtype, d):
+    """Rows of every magnitude that the forward pass takes, one of each in a tensor, by themselves and kept in 8 bits: rstd
+    squared is beyond float32 in half of them, the gradient is not. dy has a share along the row, so that the term with
+    rstd squared is of the size of the other."""
+    mx = _mx()
+    sizes = torch.tensor([1e-30, 1e-20, 1e-19, 1e-10, 1.0, 1e10, 1e19, 1e20, 1e22, 1e24, 1e30, 1e36])[:, None]
+    unit = _acts(12, d, torch.float32, d, 0.0)
+    x, w = (unit * sizes).to(dtype), _weight(d, dtype, d + 1)
+    dy = (0.1 * _acts(12, d, torch.float32, d + 2, 0.0) + 0.2 * unit).to(dtype)
+    rstd = x.double().square().mean(1).rsqrt().float()
+    for ds in (None, (dy.float() * rstd[:, None]).to(dtype)):
+        on = None if ds is None else ds.to(dev)
+        dx, dw = mx.rms_norm_backward(dy.to(dev), x.to(dev), rstd.to(dev), w.to(dev), on)
+        check_far_backward(dx, dw, dy, x, rstd, w, ds, 0)
+        q, s = mx.quantize_fp8_block128(x.to(dev))
+        dx, dw = mx.rms_norm_backward(dy.to(dev), (q, s), rstd.to(dev), w.to(dev), on)
+        check_far_backward(dx, dw, dy, o8.values(q, s), rstd, w, ds, 0)
+    # through the module: its own rstd is one rounding off, a step of float32 in T1 and three in T2
+    for keep in (False, True):
+        norm = mx.RMSNorm(d, 0.0, keep_fp8=keep, device=dev, dtype=dtype)
+        norm.weight.data.copy_(w)
+        xx = x.to(dev).requires_grad_()
+        norm(xx).backward(dy.to(dev))
+        kept = o8.values(*mx.quantize_fp8_block128(x.to(dev))) if keep else x
+        check_far_backward(xx.grad, None, dy, kept, rstd, w, None, 8)
+
+
 def test_backward_against_differences(dev):
     """float32 central differences of sum(y dy) + sum(s ds): steps of 2^-7 leave 2^-14 |x| of curvature and 2^-24 / 2^-7 of
     rounding, each times the row's sums of magnitudes."""

@@ -66,14 +66,19 @@ MXQ_DEVICE void row_sum(float& a, float& b, float (&red)[2][16], int wave, int w
   b = lane_value(v, 32);
 }
 
-// The backward passes' term x r^2 c as (x p) a, p the power of two in r: r^2 by itself leaves float32's range for rows whose
-// magnitude is beyond 2^63 or below 2^-64, where dx does not (a row of 10^24: r^2 = 0, and the whole term was lost). Scaling by
-// powers of two is exact, so rows whose r^2 is in range have the bits of x * (r * r * c).
-MXQ_DEVICE void projection(float r, float c, float& p, float& a) {
-  const uint32_t e = max(__float_as_uint(r) >> 23 & 0xFFu, 1u);  // (a subnormal r counts as one of 2^-126)
-  p = __uint_as_float(e << 23);
-  const float s = __builtin_ldexpf(r, 127 - (int)e);
-  a = s * s * c * p;
+// p, the power of two in r, and q = r^2 / p, for the backward passes' term x r^2 c = (x p) (q c): r^2 by itself leaves float32's
+// range for rows whose magnitude is beyond 2^63 or below 2^-64, where dx does not (a row of 10^24: r^2 = 0, and the whole term
+// was lost). Scaling by powers of two is exact, so rows whose r^2 is in range have the bits of r g - x (r r c). kUniform: into
+// scalar registers (r is the workgroup's one row's).
+struct RowFactors {
+  float p, q;
+};
+template <bool kUniform>
+MXQ_DEVICE RowFactors row_factors(float r) {
+  const int e = __builtin_amdgcn_frexp_expf(r);  // (0 for infinities and NaN, which q keeps)
+  const float p = __builtin_ldexpf(0.5f, e), q = r * __builtin_ldexpf(r, 1 - e);
+  if constexpr (kUniform) return {lane_value(p, 0), lane_value(q, 0)};
+  return {p, q};
 }
 
 // Chunks per lane and waves per row of the backward pass: up to 512 elements one wave, up to 8192 a chunk per lane of as

@@ -368,12 +368,8 @@ __global__ __launch_bounds__(kLanes ? 256 : 1024) void rms_norm_grad_kernel(RmsG
       s1 = lanes_sum<kGroup>(s1);
     else
       row_sum<kOne>(s1, none, red[turn], wave, waves, lane);
-    float power, a;  // dx = r g - x r^2 c + ds
-    projection(r, s1 * inv, power, a);
-    if constexpr (!kOne) {  // (a workgroup's one row: scalar registers)
-      power = lane_value(power, 0);
-      a = lane_value(a, 0);
-    }
+    const RowFactors f = row_factors<!kOne>(r);  // (here: ahead of the sum, the row's loads would be waited for)
+    float a = f.q * (s1 * inv);
     int64_t again = row;
     if constexpr (kTwice) __asm__ volatile("" : "+s"(again));
 #pragma unroll
@@ -395,7 +391,7 @@ __global__ __launch_bounds__(kLanes ? 256 : 1024) void rms_norm_grad_kernel(RmsG
       to_f32(tx[i], fp8_scale_f32(ts[i]), x);
       if (p.ds) to_f32(td[i], 1.0f, d);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e] * w[e], r, -(x[e] * power * a)) + d[e];
+      for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e] * w[e], r, -(x[e] * f.p * a)) + d[e];
       store_run8<kCode, kVec>(p.dx + row * p.D * kElem, col(i), p.D - col(i), from_f32<kCode>(v));
     }
   }

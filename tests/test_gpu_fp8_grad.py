@@ -222,6 +222,25 @@ def test_layer_norm_backward(dev, dtype, m, d):
     assert torch.equal(only[0], got[0]) and only[1] is None and only[2] is None
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [5, 300, 513, 1000, 5120, 9000, 20480])
+def test_layer_norm_backward_of_far_rows(dev, dtype, d):
+    """Rows of every magnitude, one of each in a tensor: rstd squared is beyond float32 in most of them, the gradient is not. dy
+    has a share along the row, so that the term with rstd squared is of the size of the others."""
+    mx = _mx()
+    sizes = torch.tensor([1e-30, 1e-20, 1e-19, 1e-10, 1.0, 1e10, 1e19, 1e20, 1e22, 1e24, 1e30, 1e36])[:, None]
+    unit = torch.randn(12, d, generator=_gen(d))
+    x = (unit * sizes).to(dtype)
+    _, w, _, noise = _norm_inputs(12, d, dtype, d + 1)
+    dy = (noise.float() + 0.2 * unit).to(dtype)
+    _, mean, rstd = ob.layer_norm(x, None, None, 0.0)
+    mean, rstd = mean.float(), rstd.float()
+    args = (mean.to(dev), rstd.to(dev), w.to(dev))
+    _check_norm_grad(mx.layer_norm_backward(dy.to(dev), x.to(dev), *args), dy, x, mean, rstd, w)
+    pair = mx.quantize_fp8_block128(x.to(dev))
+    _check_norm_grad(mx.layer_norm_backward(dy.to(dev), pair, *args), dy, ob.rows(x)[0], mean, rstd, w)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_layer_norm_parameters_and_strides(dev, dtype):
     mx = _mx()

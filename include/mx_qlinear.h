@@ -679,6 +679,17 @@ int mxq_mxfp4_linear_prequantized(const uint8_t* q, int64_t ldq, const uint8_t* 
                                   int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
+ * The kernel that the 4-bit layer's forward pass takes at this size on the current device (pair: of an input that is codes and
+ * scales already): plan[0] weight rows of a workgroup of the few-row kernel, plan[1] its waves, or 0 and 0 and the product's
+ * plan[2] tile rows, plan[3] tile columns, plan[4] K slices. plan holds 5 entries, M is 1 or more. Host only; tests and tuning
+ * read it.
+ */
+int mxq_mxfp4_linear_plan(int64_t M, int64_t N, int64_t K, int pair, int64_t* plan);
+
+/* The same of the input's gradient: plan[0] tile rows, plan[1] tile columns, plan[2] N slices (3 entries). */
+int mxq_mxfp4_linear_backward_plan(int64_t M, int64_t N, int64_t K, int dy_dtype, int64_t* plan);
+
+/*
  * Bytes of workspace mxq_mxfp4_linear_backward needs at this size on the current device. needs: 1 dx, 2 db, added up; direct as
  * below.
  */

@@ -451,6 +451,11 @@ static Fp4Plan plan_fp4(int64_t M, int64_t N, int64_t stages, int cus) {
   return best;
 }
 
+Fp4TileForm fp4_gemm_form(int64_t M, int64_t N, int64_t K) {
+  const Fp4Plan plan = plan_fp4(M, N, fp4_row_bytes(K) / kFp4Stage, mxq_cu_count());
+  return {plan.tile ? plan.tile : 128, plan.tile ? 256 : 128, plan.splits};
+}
+
 }  // namespace mxq
 
 using namespace mxq;

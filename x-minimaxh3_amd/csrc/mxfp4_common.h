@@ -92,6 +92,18 @@ int fp4_linear_rows(const void* x, int x_dtype, int64_t ldx, const uint8_t* sx, 
                     const uint8_t* sb, const void* bias, void* d, int64_t ldd, int out_dtype, int64_t M, int64_t N, int64_t K,
                     void* stream);
 
+// What the passes choose on the current device: weight rows and waves of the few-row kernel's workgroups; rows and columns of a
+// product's or a gradient's tile and the slices of the summed index.
+struct Fp4RowsForm {
+  int rows, waves;
+};
+struct Fp4TileForm {
+  int rows, cols, slices;
+};
+Fp4RowsForm fp4_rows_form(int64_t M, int64_t N, int64_t K);
+Fp4TileForm fp4_gemm_form(int64_t M, int64_t N, int64_t K);
+Fp4TileForm fp4_dgrad_form(int64_t M, int64_t N, int64_t K, int parts);
+
 // Two codes (byte kByte of a word) as float32 (exact).
 template <int kByte>
 MXQ_DEVICE v2f fp4x2_to_f32(uint32_t q, float scale) {

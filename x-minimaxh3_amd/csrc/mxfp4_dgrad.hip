@@ -296,6 +296,11 @@ static DgradPlan plan_dgrad(int64_t M, int64_t N, int64_t K, int parts, int cus)
   return best;
 }
 
+Fp4TileForm fp4_dgrad_form(int64_t M, int64_t N, int64_t K, int parts) {
+  const DgradPlan plan = plan_dgrad(M, N, K, parts, mxq_cu_count());
+  return {plan.tile, tile_width(plan.tile), plan.splits};
+}
+
 static int64_t dgrad_bytes(const DgradPlan& plan, int64_t M, int64_t K) {
   return plan.splits > 1 ? plan.splits * M * ((K + 3) / 4 * 4) * 4 : 0;
 }

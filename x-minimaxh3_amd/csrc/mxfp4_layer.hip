@@ -160,3 +160,25 @@ extern "C" int mxq_mxfp4_linear_backward(const void* dy, int dy_dtype, int64_t l
   }
   return fp8_join(join, {}, {s.sums, db, s.strips, N, grad_dtype}, stream);
 }
+
+extern "C" int mxq_mxfp4_linear_plan(int64_t M, int64_t N, int64_t K, int pair, int64_t* plan) {
+  if (!sizes_ok(M, N, K) || M == 0 || !plan) return mxq_set_error(MXQ_ERR_INVALID, "bad argument");
+  const bool few = fp4_few_rows(M, N, K, pair != 0);
+  const Fp4RowsForm r = few ? fp4_rows_form(M, N, K) : Fp4RowsForm{0, 0};
+  const Fp4TileForm t = few ? Fp4TileForm{0, 0, 0} : fp4_gemm_form(M, N, K);
+  plan[0] = r.rows;
+  plan[1] = r.waves;
+  plan[2] = t.rows;
+  plan[3] = t.cols;
+  plan[4] = t.slices;
+  return MXQ_OK;
+}
+
+extern "C" int mxq_mxfp4_linear_backward_plan(int64_t M, int64_t N, int64_t K, int dy_dtype, int64_t* plan) {
+  if (!sizes_ok(M, N, K) || M == 0 || !float_dtype(dy_dtype) || !plan) return mxq_set_error(MXQ_ERR_INVALID, "bad argument");
+  const Fp4TileForm t = fp4_dgrad_form(M, N, K, parts_of(dy_dtype));
+  plan[0] = t.rows;
+  plan[1] = t.cols;
+  plan[2] = t.slices;
+  return MXQ_OK;
+}

@@ -207,6 +207,11 @@ static RowsPlan4 plan_rows(int64_t M, int64_t N, int64_t stages, int cus) {
   return best;
 }
 
+Fp4RowsForm fp4_rows_form(int64_t M, int64_t N, int64_t K) {
+  const RowsPlan4 plan = plan_rows(M, N, fp4_row_bytes(K) / kFp4Stage, mxq_cu_count());
+  return {plan.rows, plan.waves};
+}
+
 template <int kOut, int kRT>
 static void launch_rows(Fp4Rows p, int waves, void* stream) {
   // chunks of a wave's whole K range where all rows' take up to 36 KB of LDS, down to two stages

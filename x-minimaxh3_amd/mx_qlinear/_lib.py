@@ -103,6 +103,8 @@ SIGNATURES: dict[str, list] = {
     "mxq_mxfp4_linear_prequantized": [_P, _I64, _P, _I64, _I, _P, _I64, _P, _P, _P, _I64, _I, _I64, _I64, _I64, _P, _I64, _P],
     "mxq_mxfp4_linear_backward_workspace": [_I64, _I64, _I64, _I, _I, _I, _P],
     "mxq_mxfp4_linear_backward": [_P, _I, _I64, _I, _P, _I64, _P, _P, _P, _I, _I64, _I64, _I64, _P, _I64, _P],
+    "mxq_mxfp4_linear_plan": [_I64, _I64, _I64, _I, _P],
+    "mxq_mxfp4_linear_backward_plan": [_I64, _I64, _I64, _I, _P],
     "mxq_rms_norm": [_P, _P, _I, _I64, _I64, _P, _I, _F, _P, _P, _I, _I64, _P, _I64, _P, _I64, _I64, _P],
     "mxq_rms_norm_backward_workspace": [_I64, _I64, _P],
     "mxq_rms_norm_backward": [_P, _I, _I64, _P, _I, _I64, _P, _I64, _P, _P, _I, _P, _I64, _P, _P, _I64, _I64, _P, _I64, _P],
@@ -176,6 +178,21 @@ def gemm_workspace_bytes(m: int, n: int, k: int, table: int = 0) -> int:
     out = ctypes.c_int64()
     call("mxq_int8_gemm_workspace", m, n, k, int(table), ctypes.byref(out))
     return out.value
+
+
+def mxfp4_plan(m: int, n: int, k: int, pair: bool = False) -> dict:
+    """The kernel of the 4-bit layer's forward pass (mxq_mxfp4_linear_plan): weight rows and waves of a workgroup of the few-row
+    kernel, or tile rows, tile columns and K slices of the product (zeros for the other one's)."""
+    out = (ctypes.c_int64 * 5)()
+    call("mxq_mxfp4_linear_plan", m, n, k, int(pair), out)
+    return {"rows": out[0], "waves": out[1], "tile": (out[2], out[3]), "slices": out[4]}
+
+
+def mxfp4_backward_plan(m: int, n: int, k: int, dtype: int) -> dict:
+    """The tile and N slices of its input's gradient (mxq_mxfp4_linear_backward_plan) for gradients of type code ``dtype``."""
+    out = (ctypes.c_int64 * 3)()
+    call("mxq_mxfp4_linear_backward_plan", m, n, k, dtype, out)
+    return {"tile": (out[0], out[1]), "slices": out[2]}
 
 
 def call(name: str, *args) -> None:

@@ -409,6 +409,28 @@ def test_weights_of_all_scale_bytes_pass_gradients(dev):
         assert _same(dx.double(), wv.to(dtype).double())
 
 
+@pytest.mark.parametrize("m,k", [(1, 4992), (300, 4992), (1100, 4992)])
+def test_weights_past_float32_pass_gradients(dev, m, k):
+    """Every code under the bytes 250 to 254 (and 2), a layer of one output: below 2^128 the value itself, from there on, which
+    begins with code 4 under byte 253, an infinity; in fp16 and fp32 gradients, whose other parts are zeros, NaN as well."""
+    mx = _mx()
+    wq = torch.arange(256, dtype=torch.uint8).repeat(k // 512 + 1)[None, :k // 2].contiguous()
+    ws = torch.tensor([2, 250, 251, 252, 253, 254], dtype=torch.uint8).repeat_interleave(8).repeat(k // 32)[None, :k // 32].contiguous()
+    wv = ob.values(wq, ws, k)
+    over = wv.abs() >= 2.0**128
+    assert bool(((ws == 253).repeat_interleave(32, 1) & over).any()) and not bool(((ws < 253).repeat_interleave(32, 1) & over).any())
+    weight = mx.prepare_mxfp4_weight(wq.to(dev).view(CODES), ws.to(dev).view(SCALE))
+    for dtype in DTYPES:
+        dx = mx.mxfp4_linear_backward(torch.ones(m, 1, dtype=dtype, device=dev), weight, (True, False))[0].double().cpu()
+        want = wv.float().to(dtype).double().expand(m, k)
+        on = over.expand(m, k)
+        assert torch.equal(dx[~on], want[~on])
+        if dtype == torch.bfloat16:
+            assert torch.equal(dx[on], want[on])
+        else:
+            assert not bool(torch.isfinite(dx[on]).any())
+
+
 # ---------------------------------------------------------------------------------------
 # graphs, streams, the module
 # ---------------------------------------------------------------------------------------

@@ -5,8 +5,8 @@ bits, with a power of two (an E8M0 byte) per 1 x 32 block of a row, for activati
 matrix instructions read. Block scales are the smallest 2^e (e >= -125) with ``absmax <= 6 * 2^e``, so no value is cut off;
 codes are ``x / 2^e`` rounded once to nearest even. e2m1 has no NaN: a block with a NaN or an infinity has the scale byte
 255 and is NaN throughout. Pairs of other making are taken too: any code and scale byte (the input's gradient may count weights
-below 2^-126, which only the bytes 0 and 1 make, as zeros, and takes one that is past float32's range, 6 * 2^126 and more, as
-an infinity).
+below 2^-126, which only the bytes 0 and 1 make, as zeros, and takes one that is past float32's range, 2^128 and more, as an
+infinity, with fp16 and fp32 gradients also as NaN; the quantizer makes one of an element from 3.5 * 2^126 on).
 
 No counterpart in the reference. Every function runs the HIP kernels of libmx_qlinear.so on the tensors' GPU and current
 stream; there is no CPU path.

@@ -464,6 +464,19 @@ def test_more_than_2_to_the_32_elements(dev, m, d):
     assert bool(((dw.double() - total).abs() <= 2.0**-24 * (m + 4) * size).all())
 
 
+def test_weight_of_another_shape_is_refused(dev):
+    """Under the name of the function's own norm."""
+    mx = _mx()
+    x, stat, w = torch.zeros(4, 64, device=dev), torch.ones(4, device=dev), torch.ones(63, device=dev)
+    for call in (lambda: mx.rms_norm(x, w), lambda: mx.rms_norm_quantize_fp8(x, w), lambda: mx.rms_norm_quantize_mxfp4(x, w),
+                 lambda: mx.rms_norm_backward(x, x, stat, w)):
+        with pytest.raises(ValueError, match=r"^rms norm weight of shape \(63,\), expected \(64,\)"):
+            call()
+    for call in (lambda: mx.layer_norm(x, w), lambda: mx.layer_norm_backward(x, x, stat, stat, w)):
+        with pytest.raises(ValueError, match="^layer norm weight of shape"):
+            call()
+
+
 @pytest.mark.parametrize("keep", [False, True])
 def test_module_gives_the_gradients_asked_for(dev, keep):
     """Every choice of input, residual and weight; the sum's output alone; no rows."""

@@ -365,13 +365,13 @@ def fp8_linear_backward(dy: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, 
 # layer norm
 # ---------------------------------------------------------------------------------------
 
-def _norm_params(d: int, dev, dtype, weight, bias):
+def _norm_params(d: int, dev, dtype, weight, bias, what: str = "layer norm"):
     """Weight and bias as the kernels read them: both of x's dtype or both float32."""
     target = dtype
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None:
             if t.shape != (d,):
-                raise ValueError(f"layer norm {name} of shape {tuple(t.shape)}, expected ({d},)")
+                raise ValueError(f"{what} {name} of shape {tuple(t.shape)}, expected ({d},)")
             if t.dtype != dtype:
                 target = torch.float32
     return (None if weight is None else _vector(weight, target, dev), None if bias is None else _vector(bias, target, dev),

@@ -28,7 +28,7 @@ def _rms(what: str, x: torch.Tensor, weight, eps: float, residual, want_rstd: bo
         raise ValueError(f"residual of {residual.dtype} {tuple(residual.shape)} for an input of {x.dtype} {tuple(x.shape)}")
     dev = _require_gpu(x, residual, weight)
     flat, d = x.dim() == 2, x.shape[-1]
-    w, _, pcode = _norm_params(d, dev, x.dtype, weight, None)
+    w, _, pcode = _norm_params(d, dev, x.dtype, weight, None, "rms norm")
     x2 = _rows_in_place(x, d)
     m = x2.shape[0]
     ldx, r2, ldr, total = x2.stride(0) if m > 1 else d, None, 0, None
@@ -107,7 +107,7 @@ def rms_norm_backward(dy: torch.Tensor, x, rstd: torch.Tensor, weight: torch.Ten
     if rstd.dtype != torch.float32 or rstd.numel() != m:
         raise ValueError(f"rstd must be float32 with one entry per row ({m}), got {rstd.dtype} {tuple(rstd.shape)}")
     dev = _require_gpu(dy, x2, xs, rstd, weight, dsum)
-    w, _, pcode = _norm_params(d, dev, dy.dtype, weight, None)
+    w, _, pcode = _norm_params(d, dev, dy.dtype, weight, None, "rms norm")
     s2 = None if dsum is None else _rows_in_place(dsum, d)
     dx = torch.empty(m, d, dtype=dy.dtype, device=dev)
     dw = torch.empty(d, dtype=torch.float32, device=dev) if needs_params else None

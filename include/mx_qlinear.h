@@ -707,7 +707,7 @@ int mxq_mxfp4_linear_backward(const void* dy, int dy_dtype, int64_t ldy, int dir
 
 /*
  * Root-mean-square norm of rows: s = x + r rounded to dtype (x [M, ldx], r [M, ldr]; s is written to sum [M, D] contiguous;
- * r NULL: s = x and sum is not used), rstd = 1 / sqrt(E[s^2] + eps) with the mean in float64, rounded once, and
+ * r NULL: s = x and sum is not used), rstd = 1 / sqrt(E[s^2] + eps) with the mean and the sum in float64, rounded once, and
  * y = (s * rstd) * w in float32, w [D] of param_dtype or NULL (1). y_dtype: dtype (y [M, D] contiguous, rounded once; ldq,
  * scale and lds are not used), MXQ_DTYPE_E4M3 (codes y [M, ldq] and scales [M, lds] by 1 x 128, as mxq_fp8_quantize_rows
  * makes them of y in float32; ldq a multiple of 8) or MXQ_DTYPE_E2M1 (by 1 x 32, as mxq_mxfp4_quantize_rows; ldq in

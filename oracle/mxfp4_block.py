@@ -87,9 +87,10 @@ def tiles(scale: torch.Tensor, k: int) -> dict[int, int]:
 
 
 def rms_norm(x, weight, eps, residual=None):
-    """(y float32, s in x's dtype, rstd float32) with the roundings of the definition: s to x's dtype, rstd once from float64,
-    s * rstd and the product with the weight to float32."""
+    """(y float32, s in x's dtype, rstd float32) with the roundings of the definition: s to x's dtype, eps to float32, rstd once
+    from float64, s * rstd and the product with the weight to float32."""
     s = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+    eps = float(torch.tensor(eps, dtype=torch.float32))
     rstd = (1.0 / (s.double().square().mean(1) + eps).sqrt()).float()
     return normed(s, rstd, weight), s, rstd
 

@@ -464,6 +464,26 @@ def test_more_than_2_to_the_32_elements(dev, m, d):
     assert bool(((dw.double() - total).abs() <= 2.0**-24 * (m + 4) * size).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [5, 128, 1003, 5120])
+def test_eps_is_float32(dev, dtype, d):
+    """Rows of zeros, whose rstd is eps's alone, and rows whose mean square is of its size. 1e-5 as float32 lies 2.5e-8 below
+    itself, which moves the first row's rstd by a step."""
+    mx = _mx()
+    x = (_acts(65, d, torch.float32, d, 0.0) * 3e-3).to(dtype)
+    x[0] = 0.0
+    moved = 0
+    for eps in (1e-5, 1e-6, 3e-5):
+        y, rstd = mx.rms_norm(x.to(dev), None, eps, return_rstd=True)
+        want, _, ref = ob.rms_norm(x, None, eps)
+        assert float(rstd[0]) == float(torch.tensor(eps, dtype=torch.float32).double().rsqrt().float())
+        assert torch.equal(rstd.cpu(), ref) and torch.equal(y.cpu(), want.to(dtype))
+        q, s = mx.rms_norm_quantize_mxfp4(x.to(dev), None, eps)
+        check_codes4(q, s, want)
+        moved += int((rstd.cpu() != (1.0 / (x.double().square().mean(1) + eps).sqrt()).float()).sum())
+    assert moved > 0
+
+
 def test_weight_of_another_shape_is_refused(dev):
     """Under the name of the function's own norm."""
     mx = _mx()

@@ -5,9 +5,10 @@
 //   dx = rstd * (g - xh * E[g * xh]) + ds,  g = dy * w, xh = s * rstd        dw = sum over rows of dy * xh
 //
 // y leaves in the rows' type, or quantized as the 8-bit layer (fp8_common.h, 1 x 128) or the 4-bit layer (mxfp4_common.h,
-// 1 x 32) reads it, straight from the registers that hold the row. E[s^2] is summed in float64 and rstd rounded once from
-// there, then s * rstd and the product with w are one float32 rounding each: y is the same to the last bit in every
-// implementation of the formula, and so are the codes made of it, where a last bit decides at the border of two.
+// 1 x 32) reads it, straight from the registers that hold the row. eps is a float32; E[s^2] is summed in float64 and rstd rounded
+// once from there, then s * rstd and the product with w are one float32 rounding each: with eps rounded to float32 first, y is
+// the same to the last bit in an implementation of the formula in float64 (but for an rstd closer to a border of float32 than float64's
+// own rounding), and so are the codes made of it, where a last bit decides at the border of two.
 //
 // A row is held in registers by one or more waves, eight elements per lane and chunk of 512, so x and r are read once. The
 // backward pass also keeps its lanes' columns of dw in registers over all the rows a workgroup takes, and fp8_join_kernel

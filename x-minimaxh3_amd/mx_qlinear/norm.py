@@ -1,7 +1,7 @@
 """Root-mean-square norm behind a residual addition, with outputs that the 8-bit and the 4-bit layer read, and its gradients.
 
-``s = x + residual`` rounded to ``x``'s dtype, ``rstd = 1 / sqrt(E[s^2] + eps)`` with the mean in float64 and rounded once to
-float32, ``y = (s * rstd) * weight`` in float32; ``y`` is rounded once to ``x``'s dtype, or quantized. The norm under the
+``s = x + residual`` rounded to ``x``'s dtype, ``rstd = 1 / sqrt(E[s^2] + eps)`` with ``eps`` as float32, the mean in float64 and
+rounded once to float32, ``y = (s * rstd) * weight`` in float32; ``y`` is rounded once to ``x``'s dtype, or quantized. The norm under the
 reference's rms_adaln (h3serve/native_engine/model/kernels.py:7594-7640), with a learned weight in place of the modulation.
 
 Every function runs the HIP kernels of libmx_qlinear.so on the tensors' GPU and current stream; there is no CPU path.
@@ -54,7 +54,8 @@ def _rms(what: str, x: torch.Tensor, weight, eps: float, residual, want_rstd: bo
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-5, residual: torch.Tensor | None = None,
              return_rstd: bool = False):
-    """``y = s * rstd * weight`` over the last dimension (at most 24576) with ``s = x + residual`` (``s = x`` without one).
+    """``y = s * rstd * weight`` over the last dimension (at most 24576) with ``s = x + residual`` (``s = x`` without one); ``eps``
+    counts as float32 (1e-5: 9.99999975e-6).
     Returns ``y``; with ``residual`` also ``s``, the residual stream behind the addition, and with ``return_rstd`` the rows'
     float32 ``rstd``, which :func:`rms_norm_backward` takes: ``(y[, s][, rstd])``."""
     (y, _), rest = _rms("rms_norm", x, weight, eps, residual, return_rstd, None)

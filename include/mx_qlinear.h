@@ -697,8 +697,8 @@ int mxq_mxfp4_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int dy_
 
 /*
  * The layer's backward pass in one call, through a frozen weight b [N, ldb] with scale tiles sb: dx [M, K] (contiguous,
- * dy_dtype) = dy b with the products of dy [M, ldy] as it is exact (one, two or three bfloat16 parts of bf16, fp16 and fp32)
- * and float32 sums, db [N] = sums of dy's columns (grad_dtype), each NULL to leave it out. direct: the product reads dy itself
+ * dy_dtype) = dy b with the products of dy [M, ldy] as it is exact (one, two or three bfloat16 parts of bf16, fp16 and fp32; of
+ * fp32 from 2^-103 up to (2 - 2^-8) 2^127, from where on a value is an infinity) and float32 sums, db [N] = sums of dy's columns (grad_dtype), each NULL to leave it out. direct: the product reads dy itself
  * (bf16, N % 8 == 0, ldy % 8 == 0, ldy < 2^24, 16-byte aligned) in place of parts of it.
  */
 int mxq_mxfp4_linear_backward(const void* dy, int dy_dtype, int64_t ldy, int direct, const uint8_t* b, int64_t ldb, const uint8_t* sb,

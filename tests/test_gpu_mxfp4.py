@@ -409,6 +409,23 @@ def test_weights_of_all_scale_bytes_pass_gradients(dev):
         assert _same(dx.double(), wv.to(dtype).double())
 
 
+def test_range_of_float32_gradients(dev):
+    """Through a weight of ones every value of 24 bits comes back from 2^-103 to bfloat16's largest and half a step; from there on it
+    is an infinity."""
+    mx = _mx()
+    weight = mx.prepare_mxfp4_weight(torch.ones(1, 32, device=dev))
+    g = _gen(3)
+    mant = 1 + torch.randint(0, 1 << 23, (231, 8), generator=g).double() * 2.0**-23
+    mant[:, 0], mant[:, 1] = 2 - 2.0**-23, 1 + 2.0**-23
+    dy = mant * torch.exp2(torch.arange(-103, 128).double())[:, None] * torch.tensor([1, 1, 1, 1, -1, -1, -1, 1.0], dtype=torch.float64)
+    edge = (2 - 2.0**-8) * 2.0**127
+    dy[-1, 2], dy[-1, 3] = edge, edge - 2.0**104
+    dy = dy.float().reshape(-1, 1)
+    dx = mx.mxfp4_linear_backward(dy.to(dev), weight, (True, False))[0].cpu()
+    want = torch.where(dy.double().abs() >= edge, torch.copysign(torch.full_like(dy, float("inf")), dy), dy)
+    assert torch.equal(dx, want.expand(-1, 32)) and bool(torch.isinf(want).any())
+
+
 @pytest.mark.parametrize("m,k", [(1, 4992), (300, 4992), (1100, 4992)])
 def test_weights_past_float32_pass_gradients(dev, m, k):
     """Every code under the bytes 250 to 254 (and 2), a layer of one output: below 2^128 the value itself, from there on, which

@@ -229,8 +229,8 @@ def mxfp4_linear_backward(dy: torch.Tensor, weight: PreparedMxfp4Weight, needs: 
     ``needs`` says which (``None`` for the other). The quantizer passes gradients through unchanged.
 
     ``dx = dy W^`` in ``dy``'s dtype and ``dbias = sum dy`` in ``grad_dtype``, from ``dy`` as it is: float32 sums of products
-    that are exact where ``dy`` is bf16, fp16 or (to 24 bits) fp32, which go through the matrix instructions as one, two or
-    three bfloat16 parts.
+    that are exact where ``dy`` is bf16, fp16 or (to 24 bits, from 2^-103 up) fp32, which go through the matrix instructions as
+    one, two or three bfloat16 parts; an fp32 value that bfloat16 rounds to an infinity, ``(2 - 2^-8) 2^127`` and more, is one.
     """
     if not isinstance(weight, PreparedMxfp4Weight):
         raise TypeError(f"weight must come from prepare_mxfp4_weight, got {type(weight).__name__}")

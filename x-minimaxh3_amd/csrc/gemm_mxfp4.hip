@@ -473,7 +473,8 @@ int mxq::fp4_gemm_check(const uint8_t* a, int64_t lda, const uint8_t* sa, const 
   if (lda < bytes || lda % 16 || lda > (1ll << 22))
     return mxq_set_error(MXQ_ERR_INVALID, "bad row strides of the activations for K=%lld", (long long)K);
   if (M == 0) return MXQ_OK;
-  // (so many tiles are not split; of 256 rows, as the plan may take them, there are half as many)
+  // (counted in tiles of 256 x 256; of the plan's other tiles there are up to four times as many, fewer than 2^24 workgroups of 256
+  // threads, and a launch takes less than 2^32 threads. So many tiles are not split.)
   if ((M + 255) / 256 * ((N + kTileN - 1) / kTileN) >= (1ll << 22)) return mxq_set_error(MXQ_ERR_UNSUPPORTED, "more than 2^22 tiles");
   if (!a || !sa || !b || !sb || !d || !aligned(a, 16) || !aligned(b, 16) || !aligned(sa, 16) || !aligned(sb, 16))
     return mxq_set_error(MXQ_ERR_INVALID, "null or misaligned pointer");

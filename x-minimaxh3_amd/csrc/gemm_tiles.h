@@ -1,5 +1,5 @@
-// What the block-scaled matrix products (gemm_fp8.hip, gemm_mxfp4.hip) share: tiles of a workgroup of eight waves, operand chunks
-// of 128 bytes a row on their way into a ring of LDS slots, the tile order and the epilogue.
+// What the block-scaled matrix products share, gemm_fp8.hip's workgroups of eight waves (Tile) and gemm_mxfp4.hip's of four: operand
+// chunks of 128 bytes a row on their way into a ring of LDS slots, the tile order and the epilogue.
 #pragma once
 
 #include "fp8_common.h"

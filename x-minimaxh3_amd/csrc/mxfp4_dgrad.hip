@@ -2,9 +2,9 @@
 //
 //   dX[m, k] = sum_n dY[m, n] * W[n, k],   W[n, k] = code[n, k] * 2^(b[n, k / 32] - 127)
 //
-// dY is bfloat16 [M, N] (float16 and float32 gradients come as two and three bfloat16 parts whose products are summed) and W is
-// decoded to bfloat16, which is exact, so the only roundings are those of the float32 sums: 16-bit matrix instructions
-// (v_mfma_f32_32x32x16_bf16). The 4-bit instructions cannot take W here: their scales go along the summed index, W's across it.
+// dY is bfloat16 [M, N] (float16 and float32 gradients come as two and three bfloat16 parts whose products are summed; a float32
+// value that bfloat16 rounds to an infinity, from (2 - 2^-8) 2^127 on, is one) and W is decoded to bfloat16, which is exact, so the
+// only roundings are those of the float32 sums: 16-bit matrix instructions (v_mfma_f32_32x32x16_bf16). The 4-bit instructions cannot take W here: their scales go along the summed index, W's across it.
 //
 // dY's rows hold the summed index n, so its fragments (eight consecutive n of one row per lane) are plain 16-byte LDS reads; W
 // has n as its rows, and its fragments come from transposing reads (ds_read_b64_tr_b16), which hand sixteen lanes the columns
@@ -13,8 +13,8 @@
 // dY's 256 x 64 bfloat16 (32 KB) and W's 64 x 256 codes, decoded on the way from registers to LDS (32 KB). Problems of fewer tiles still split N over workgroups, which write
 // float32 sums that fp8_join_kernel adds in order.
 //
-// 8192 rows, N 14336, K 5376 take 0.98 ms (1.28 PFLOP/s), 16384 rows, N and K 8192 1.65 (1.34): the rate of a library's plain
-// bfloat16 product (1.25 to 1.33 for 8192 cubed). The matrix cores are busy 58 % of the time in the first, whose 2.6 rounds of tiles
+// 8192 rows, N 14336, K 5376 take 0.963 ms (1.31 PFLOP/s), 16384 rows, N and K 8192 1.65 (1.34): the rate of a library's plain
+// bfloat16 product (1.25 to 1.34 for 8192 cubed). The matrix cores are busy 58 % of the time in the first, whose 2.6 rounds of tiles
 // run as three. Four waves of 128 x 128, with two thirds of the LDS reads, ran 5 % slower.
 #include "mxfp4_common.h"
 

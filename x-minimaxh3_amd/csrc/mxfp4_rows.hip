@@ -180,8 +180,8 @@ __global__ __launch_bounds__(512) void mxfp4_rows_kernel(Fp4Rows p) {
 
 // Weight rows (a multiple of 4: mostly what gives every CU its share and no more) and waves of a workgroup, by an estimate in
 // microseconds: the CU with the most workgroups streams their weight rows, 0.090 (four waves) or 0.079 (eight) per sixteen and stage,
-// half of it for a block's missing rows too, and brings x for each workgroup, 0.013 per row and stage, 0.025 where four waves are
-// alone on their CU; all CUs together stream at 5.2 TB/s; eight waves take longer to start and to add up. Measured, bf16, weights from
+// half of it for a block's missing rows too, and brings x for each workgroup, per row and stage 0.013 (four waves; 0.025 where they
+// are alone on their CU) or 0.014 (eight); all CUs together stream at 5.2 TB/s; eight waves take longer to start and to add up. Measured, bf16, weights from
 // memory, by rows and waves: one row, K 5120, N 5120: 20/4 6.1, 32/4 6.5, 20/8 6.0, 32/8 6.2, 64/8 9.9; N 20480: 16/4 13.0, 32/4 15.2,
 // 80/8 15.6; K 20480, N 5120: 16/4 17.8, 20/4 15.8, 32/4 17.9, 16/8 18.0, 20/8 14.6, 32/8 16.4; K 14336, N 5376: 16/4 12.5, 24/8 11.9,
 // 32/8 12.5; four rows, K 20480, N 5120: 20/4 22.1, 20/8 18.4, 32/8 20.4; K 5376, N 21504: 28/4 15.7, 44/4 16.1, 84/8 17.7; 16 rows,

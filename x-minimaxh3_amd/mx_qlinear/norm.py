@@ -75,7 +75,8 @@ def rms_norm_quantize_fp8(x: torch.Tensor, weight: torch.Tensor | None = None, e
 def rms_norm_quantize_mxfp4(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-5,
                             residual: torch.Tensor | None = None, return_rstd: bool = False):
     """:func:`rms_norm` with ``y`` quantized from float32 as :func:`quantize_mxfp4` does: ``(codes, scale[, s][, rstd])``, a pair
-    for :func:`mxfp4_linear_prequantized` in one launch."""
+    for :func:`mxfp4_linear_prequantized` in one launch (of more than 16 rows, or fewer of a long ``K``, each product lays the
+    scales out for itself first, and copies the codes where ``K`` is not a multiple of 256)."""
     (q, s), rest = _rms("rms_norm_quantize_mxfp4", x, weight, eps, residual, return_rstd, _lib.DTYPE_E2M1)
     return (*mxfp4._as_pair(q, s, tuple(x.shape[:-1]), x.shape[-1]), *rest)
 

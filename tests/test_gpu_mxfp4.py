@@ -479,6 +479,35 @@ def test_captured_and_replayed(dev, m):
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
+@pytest.mark.parametrize("m", [3, 40])
+def test_deterministic_mode(dev, m):
+    """Every function and both modules under torch.use_deterministic_algorithms: the same bits."""
+    mx = _mx()
+    x, r, w = _acts(m, 300, torch.bfloat16, 1).to(dev), _acts(m, 300, torch.bfloat16, 2).to(dev), _acts(70, 300, torch.bfloat16, 3).to(dev)
+
+    def run():
+        weight = mx.prepare_mxfp4_weight(w)
+        q, s = mx.quantize_mxfp4(x)
+        nq, ns, total, rstd = mx.rms_norm_quantize_mxfp4(x, None, 1e-6, residual=r, return_rstd=True)
+        n8, s8 = mx.rms_norm_quantize_fp8(x)
+        y = mx.mxfp4_linear(x, weight)
+        norm, layer = mx.RMSNorm(300, keep_fp8=True, device=dev, dtype=torch.bfloat16), mx.Mxfp4Linear.from_weight(w)
+        xx = x.clone().requires_grad_()
+        layer(norm(xx)).backward(y)
+        return [t.view(torch.uint8) if t.dtype in (CODES, SCALE, torch.float8_e4m3fn) else t for t in
+                (weight.q, weight.scale, q, s, nq, ns, total, rstd, n8, s8, y, mx.dequantize_mxfp4(q, s),
+                 mx.mxfp4_linear_prequantized(q, s, weight), *mx.mxfp4_linear_backward(y, weight),
+                 *mx.rms_norm_backward(x, total, rstd, None, r), xx.grad, norm.weight.grad)]
+
+    want = run()
+    torch.use_deterministic_algorithms(True)
+    try:
+        got = run()
+    finally:
+        torch.use_deterministic_algorithms(False)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_two_streams_at_once(dev):
     """Calls of different inputs on two streams share no memory."""
     mx = _mx()

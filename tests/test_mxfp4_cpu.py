@@ -211,6 +211,19 @@ def test_module_buffers():
     assert p.q is other.qweight and (p.out_features, p.in_features) == (70, 1000)
 
 
+def test_storage_in_deterministic_mode():
+    """torch fills new tensors in that mode, which it cannot do in the codes' type."""
+    from mx_qlinear import mxfp4
+
+    torch.use_deterministic_algorithms(True)
+    try:
+        q, s = mxfp4._new_pair(3, 130, "cpu")
+    finally:
+        torch.use_deterministic_algorithms(False)
+    for t, want in zip((q, s), mxfp4._new_pair(3, 130, "cpu")):
+        assert (t.dtype, t.shape, t.stride()) == (want.dtype, want.shape, want.stride())
+
+
 # ---------------------------------------------------------------------------------------
 # the C entries
 # ---------------------------------------------------------------------------------------

@@ -69,7 +69,11 @@ def _pair(q: torch.Tensor, scale: torch.Tensor, width: int | None, what: str = "
 def _new_pair(m: int, k: int, dev) -> tuple[torch.Tensor, torch.Tensor]:
     """Storage for codes and scales of [m, k]: rows of whole 128 columns."""
     n = -(-k // 128)
-    return torch.empty(m, n * 64, dtype=_CODES, device=dev), torch.empty(m, n * 4, dtype=_SCALE, device=dev)
+    if torch.are_deterministic_algorithms_enabled():  # (it then fills what it allocates, which it cannot in the codes' type)
+        q = torch.empty(m, n * 64, dtype=torch.uint8, device=dev).view(_CODES)
+    else:
+        q = torch.empty(m, n * 64, dtype=_CODES, device=dev)
+    return q, torch.empty(m, n * 4, dtype=_SCALE, device=dev)
 
 
 def _as_pair(q: torch.Tensor, s: torch.Tensor, lead: tuple[int, ...], k: int) -> tuple[torch.Tensor, torch.Tensor]:

@@ -479,6 +479,20 @@ def test_captured_and_replayed(dev, m):
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
+def test_module_with_a_float64_bias(dev):
+    """As a model cast to float64 has it: taken, and its gradient is float32's."""
+    mx = _mx()
+    w, x, dy = _acts(70, 300, torch.float32, 1), _acts(9, 300, torch.float32, 2), _acts(9, 70, torch.float32, 3)
+    grads = []
+    for dtype in (torch.float32, torch.float64):
+        layer = mx.Mxfp4Linear.from_weight(w.to(dev), torch.ones(70, device=dev)).to(dtype)
+        xx = x.to(dev).requires_grad_()
+        layer(xx).backward(dy.to(dev))
+        assert layer.bias.grad.dtype == dtype
+        grads.append((xx.grad, layer.bias.grad.double()))
+    assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][1], grads[1][1])
+
+
 @pytest.mark.parametrize("m", [3, 40])
 def test_deterministic_mode(dev, m):
     """Every function and both modules under torch.use_deterministic_algorithms: the same bits."""

@@ -19,7 +19,7 @@ from dataclasses import dataclass
 import torch
 
 from .fp8 import _ceil, _float_code, _refuse_capture, _refuse_tangents, _room, _rows_in_place, _view, _workspace
-from .ops import _bias, _launch, _out_code, _ptr, _require_gpu
+from .ops import _OUT_CODES, _bias, _launch, _out_code, _ptr, _require_gpu
 
 BLOCK = 32
 _CODES, _SCALE = torch.float4_e2m1fn_x2, torch.float8_e8m0fnu
@@ -281,9 +281,10 @@ class _Mxfp4LinearFn(torch.autograd.Function):
         _refuse_capture(dy.device)
         qweight, scale = ctx.saved_tensors
         want_x, want_b = ctx.needs_input_grad[0], ctx.needs_input_grad[3]
+        # (a float64 bias's gradient is summed in float32)
         dx, db = mxfp4_linear_backward(dy, PreparedMxfp4Weight(qweight, scale, *ctx.sizes), (want_x, want_b),
-                                       ctx.bias_dtype if want_b else torch.float32)
-        return dx, None, None, db, None
+                                       ctx.bias_dtype if ctx.bias_dtype in _OUT_CODES else torch.float32)
+        return dx, None, None, db.to(ctx.bias_dtype) if want_b else None, None
 
 
 class Mxfp4Linear(torch.nn.Module):

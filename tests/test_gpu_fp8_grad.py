@@ -328,6 +328,22 @@ def test_gradients_against_differences(dev):
 # modules
 # ---------------------------------------------------------------------------------------
 
+def test_layer_with_a_float64_bias(dev):
+    """Taken beside a frozen weight, and its gradient is float32's."""
+    mx = _mx()
+    layer = mx.Fp8Linear(300, 70, device=dev)
+    layer.weight.requires_grad_(False)
+    x, dy = _acts(9, 300, torch.float32, 2).to(dev), _acts(9, 70, torch.float32, 3).to(dev)
+    grads = []
+    for dtype in (torch.float32, torch.float64):
+        layer.bias = torch.nn.Parameter(torch.ones(70, device=dev, dtype=dtype))
+        xx = x.clone().requires_grad_()
+        layer(xx).backward(dy)
+        assert layer.bias.grad.dtype == dtype
+        grads.append((xx.grad, layer.bias.grad.double()))
+    assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][1], grads[1][1])
+
+
 @pytest.mark.parametrize("keep", [False, True])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_norm_and_layer_trained_together(dev, dtype, keep):

@@ -505,10 +505,11 @@ class _Fp8LinearFn(torch.autograd.Function):
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
         weight = PreparedFp8Weight(q, s, qt, st, n, k)  # (the gradients read the transposed copy only)
         m = q.shape[0]
-        # of two types, both gradients in float32, each then rounded once to its own
+        # of two types (or a float64 bias's alone), in float32, each then rounded once to its own
         wanted = {t for t, want in ((wdtype, want_w), (bdtype, want_b)) if want}
+        own = wanted.pop() if len(wanted) == 1 else None
         dx, dw, db = fp8_linear_backward(dy.reshape(m, n), q[:, :k], s[:, : -(-k // BLOCK)], weight, (want_x, want_w, want_b),
-                                         wanted.pop() if len(wanted) == 1 else torch.float32, ctx.full_sums)
+                                         own if own in _OUT_CODES else torch.float32, ctx.full_sums)
         return (dx.reshape(shape) if want_x else None, dw.to(wdtype) if want_w else None, db.to(bdtype) if want_b else None,
                 None, None)
 

@@ -278,3 +278,63 @@ def test_nothing_is_written_behind_the_rows(dev, dtype, m, n, k):
     assert torch.equal(out[1:m + 1, :n], want)
     out[1:m + 1, :n] = 7.0
     assert bool((out == 7.0).all())
+
+
+def _far(dev, t, stride, offset=0):
+    """``t [rows, cols]`` as rows ``stride`` elements apart, ``offset`` from the start of their memory."""
+    raw = t.view(torch.uint8) if t.dtype in (CODES, SCALE) else t
+    base = torch.empty((t.shape[0] - 1) * stride + t.shape[1] + offset, dtype=raw.dtype, device=dev)
+    far = base.as_strided(t.shape, (stride, 1), offset)
+    far.copy_(raw)
+    return far.view(t.dtype) if t.dtype in (CODES, SCALE) else far
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 7, 16, 40, 300])
+@pytest.mark.parametrize("stride", [(1 << 22) - 16, 1 << 22, (1 << 22) + 16, (1 << 24) + 3])
+def test_rows_far_apart(dev, m, stride):
+    """Inputs and pairs whose rows are at and beyond the strides that the products read in place: the same bits as of contiguous
+    rows."""
+    mx = _mx()
+    n, k = 520, 1024
+    weight = _prepare(*_weight(dev, n, k, 1), k)
+    x = _rows(dev, m, k, BF16, 2)
+    pair = mx.quantize_mxfp4(x)
+    far = _far(dev, x, stride)
+    assert torch.equal(mx.mxfp4_linear(far, weight), mx.mxfp4_linear(x, weight))
+    for a, b in zip(mx.quantize_mxfp4(far), pair):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    want = mx.mxfp4_linear_prequantized(*pair, weight)
+    for off in (0, 5):
+        q, s = _far(dev, pair[0], stride, off), _far(dev, pair[1], stride, off)
+        assert torch.equal(mx.mxfp4_linear_prequantized(q, s, weight), want)
+        assert torch.equal(mx.dequantize_mxfp4(q, s), mx.dequantize_mxfp4(*pair))
+    w, r = _rows(dev, 1, k, BF16, 3)[0], _far(dev, _rows(dev, m, k, BF16, 4), stride, 1)
+    y, total, rstd = mx.rms_norm(far, w, residual=r, return_rstd=True)
+    for a, b in zip((y, total, rstd), mx.rms_norm(x, w, residual=r.contiguous(), return_rstd=True)):
+        assert torch.equal(a, b)
+    kept = mx.quantize_fp8_block128(x)
+    q8 = torch.empty((m - 1) * stride + k, dtype=torch.float8_e4m3fn, device=dev).as_strided((m, k), (stride, 1)).copy_(kept[0])
+    for x_far, x_near in ((far, x), ((q8, kept[1]), kept)):
+        for a, b in zip(mx.rms_norm_backward(r, x_far, rstd, w, far), mx.rms_norm_backward(r.contiguous(), x_near, rstd, w, x)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m,n,k", [(40, 1032, 20001), (70, 520, 300), (130, 64, 40001)])
+def test_gradient_rows_far_apart(dev, dtype, m, n, k):
+    """Up to the largest stride that is read in place (2^24 - 8), at it and beyond, in each of the tiles."""
+    mx = _mx()
+    weight = _prepare(*_weight(dev, n, k, 1), k)
+    dy = _rows(dev, m, n, dtype, 2)
+    want = mx.mxfp4_linear_backward(dy, weight)
+    for stride in ((1 << 24) - 8, 1 << 24, (1 << 24) + 3):
+        for a, b in zip(mx.mxfp4_linear_backward(_far(dev, dy, stride), weight), want):
+            assert torch.equal(a, b)
+
+
+def test_far_gradients_take_each_tile():
+    lib = _lib()
+    assert {lib.mxfp4_backward_plan(m, n, k, TYPE_CODE[BF16])["tile"] for m, n, k in
+            ((40, 1032, 20001), (70, 520, 300), (130, 64, 40001))} == {(64, 256), (128, 128), (256, 256)}

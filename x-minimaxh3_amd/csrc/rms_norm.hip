@@ -14,8 +14,8 @@
 // backward pass also keeps its lanes' columns of dw in registers over all the rows a workgroup takes, and fp8_join_kernel
 // adds the workgroups' sums in a fixed order: no atomics, the same bits on every run.
 //
-// Both passes are bound by HBM. Forward with a residual and 4-bit codes, 75600 x 5376 bf16: 472 us, 5.6 TB/s. Backward, 75600 x 5120
-// bf16, of an input kept in 8 bits and with a gradient added: 500 us, 5.4 TB/s. (One chunk a lane keeps the row's values behind its
+// Both passes are bound by HBM. Forward with a residual and 4-bit codes, 75600 x 5376 bf16: 478 us, 5.6 TB/s. Backward, 75600 x 5120
+// bf16, of an input kept in 8 bits and with a gradient added: 509 us, 5.3 TB/s. (One chunk a lane keeps the row's values behind its
 // sum; forming them anew from the words, as two and three do to save registers, took 165 us for 126 at 19531 x 5120, and a second
 // row requested ahead another 16.)
 
